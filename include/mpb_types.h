@@ -70,6 +70,29 @@ enum mpb_red_op {
   MPB_R_ARGMIN_REC = 8
 };
 
+// Form of the gated scan (mpb_gated_scan): the gate is the decay itself, or
+// the decay is its sigmoid and the input is weighted with one minus it.
+enum mpb_scan_mode {
+  MPB_SCAN_LINEAR = 0,
+  MPB_SCAN_SIGMOID = 1
+};
+
+// Extent of a branch's gate (mpb_gated_residual_norm): none, a value for
+// every element, for every row, for every channel.
+enum mpb_gate_kind {
+  MPB_GATE_NONE = 0,
+  MPB_GATE_FULL = 1,
+  MPB_GATE_ROW = 2,
+  MPB_GATE_CHANNEL = 3
+};
+
+// What the gate goes through: itself, its sigmoid, gate * sigmoid(gate).
+enum mpb_activation {
+  MPB_ACT_LINEAR = 0,
+  MPB_ACT_SIGMOID = 1,
+  MPB_ACT_SILU = 2
+};
+
 // Status codes returned by every extended entry point.
 enum mpb_status {
   MPB_OK = 0,

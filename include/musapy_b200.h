@@ -191,6 +191,92 @@ int mpb_cumsum(int ndim, const int64_t* shape, const int64_t* strides, const voi
  * its scratch: MPB_OK, or MPB_ERR_TIMEOUT when a bounded wait gave up. */
 int mpb_cumsum_status(const void* scratch, mpb_stream_t stream);
 
+/* ------------------------------------------- recurrent block operators */
+
+/* The operators below are new: musapy has no counterpart. Element types are
+ * MPB_F32, MPB_F16 and MPB_BF16, arithmetic is in float, outputs are
+ * C-contiguous, the innermost stride of every input is 1 and the other
+ * strides are given in elements. */
+
+/* Gated linear recurrence over time. x is (B, T, D) with strides x_sb, x_st
+ * over sequences and steps; gate is (B, T, H), H a divisor of D (channel d
+ * has gate d / (D / H)), of x's type or MPB_F32; h0 (B, D) floats or NULL for
+ * zero. mode MPB_SCAN_LINEAR: h[t] = g h[t-1] + x[t]; MPB_SCAN_SIGMOID:
+ * h[t] = s h[t-1] + (1 - s) x[t], s = sigmoid(g). Writes h (B, T, D) in x's
+ * type and, when state is not NULL, h[T-1] (h0 when T == 0) in float; state
+ * may be h0 itself. Scratch: mpb_gated_scan_scratch_bytes(..., backward = 0). */
+size_t mpb_gated_scan_scratch_bytes(int64_t B, int64_t T, int64_t D, int64_t H, int x_dtype, int gate_dtype,
+                                    int backward);
+int mpb_gated_scan(int64_t B, int64_t T, int64_t D, int64_t H, const void* x, int x_dtype, int64_t x_sb, int64_t x_st,
+                   const void* gate, int gate_dtype, int64_t g_sb, int64_t g_st, const float* h0, int mode, void* h,
+                   float* state, void* scratch, size_t scratch_bytes, mpb_stream_t stream);
+
+/* Gradients of mpb_gated_scan from dh (B, T, D), the gradient of every h[t],
+ * and dstate (B, D) or NULL, that of the last state in float. h is the
+ * forward pass's output as it stored it, h0 what it started from. Writes dx
+ * (B, T, D), dgate (B, T, H, summed over a gate's channels in a fixed order,
+ * in the gate's type) and dh0 (B, D) in float when not NULL. */
+int mpb_gated_scan_backward(int64_t B, int64_t T, int64_t D, int64_t H, const void* dh, int64_t dh_sb, int64_t dh_st,
+                            const void* x, int x_dtype, int64_t x_sb, int64_t x_st, const void* gate, int gate_dtype,
+                            int64_t g_sb, int64_t g_st, const void* h, int64_t h_sb, int64_t h_st, const float* h0,
+                            const float* dstate, int mode, void* dx, void* dgate, float* dh0, void* scratch,
+                            size_t scratch_bytes, mpb_stream_t stream);
+
+/* One step of B running sequences: x (B, D), gate (B, H); updates state
+ * (B, D) in place and writes the new state in x's type to h (B, D). */
+int mpb_gated_scan_step(int64_t B, int64_t D, int64_t H, const void* x, int x_dtype, int64_t x_sb, const void* gate,
+                        int gate_dtype, int64_t g_sb, int mode, float* state, void* h, mpb_stream_t stream);
+
+/* Norms before and after a block with its gate, dropout and residual scale,
+ * over R rows of D: n = z rms(z) w_post; y = x + scale * drop(act(gate) n);
+ * u = y rms(y) w_pre, rms(v) = (mean v^2 + eps)^(-1/2). x, z, gate in
+ * `dtype` with row strides x_sr, z_sr, g_sr; gate_kind says the gate's extent
+ * (mpb_gate_kind), activation what it goes through (mpb_activation); the
+ * weights are D floats. dropout > 0 drops elements of the branch as
+ * mpb_dropout does, by their index in (R, D). Writes y and u (R, D) and
+ * rstd (2, R): the two rms factors. z == NULL: the plain norm u = x rms(x)
+ * w_pre, no y, rstd (1, R). */
+int mpb_gated_residual_norm(int64_t R, int64_t D, int dtype, const void* x, int64_t x_sr, const void* z, int64_t z_sr,
+                            const void* gate, int64_t g_sr, int gate_kind, int activation, const float* w_post,
+                            const float* w_pre, double scale, double eps, double dropout, uint64_t seed,
+                            uint64_t offset, void* y, void* u, float* rstd, mpb_stream_t stream);
+
+/* Gradients of mpb_gated_residual_norm from dy and du (each may be NULL for
+ * zero), with y and rstd as the forward pass left them and the same gate,
+ * scale, dropout, seed and offset. Writes dx, dz (R, D), dgate (the gate's
+ * extent, its type) and the weights' gradients (D floats), summed in a fixed
+ * order. z == NULL: the plain norm's gradients (y is its input; dz, dgate and
+ * dw_post unused). */
+size_t mpb_gated_residual_norm_scratch_bytes(int64_t R, int64_t D, int dtype, int branch, int gate_kind);
+int mpb_gated_residual_norm_backward(int64_t R, int64_t D, int dtype, const void* dy, int64_t dy_sr, const void* du,
+                                     int64_t du_sr, const void* y, int64_t y_sr, const void* z, int64_t z_sr,
+                                     const void* gate, int64_t g_sr, int gate_kind, int activation,
+                                     const float* w_post, const float* w_pre, const float* rstd, double scale,
+                                     double dropout, uint64_t seed, uint64_t offset, void* dx, void* dz, void* dgate,
+                                     float* dw_post, float* dw_pre, void* scratch, size_t scratch_bytes,
+                                     mpb_stream_t stream);
+
+/* Dropout of n contiguous elements: element i is dropped when its 16 bits of
+ * a Philox-4x32-10 stream (counter {i / 8, offset}, key seed, half i % 8) are
+ * below k = floor(p * 65536 + 1/2), else multiplied by 65536 / (65536 - k).
+ * The gradient is the same call on the output's gradient. */
+int mpb_dropout(int64_t n, const void* x, int dtype, double p, uint64_t seed, uint64_t offset, void* y,
+                mpb_stream_t stream);
+
+/* Clipped policy loss with a KL term over N tokens of V logits (row stride
+ * l_sr) and, when dlogits is not NULL, its gradient times grad_scale. targets
+ * are N MPB_I32 or MPB_I64 indices; old_logp, advantages, ref_logp (NULL: no
+ * KL term) N floats; mask N bytes or NULL. Writes the mean loss over the mask,
+ * logp, kl (N floats), clipped (N bytes) and dlogits (N, V) in `dtype`;
+ * tokens outside the mask give zeros whatever their logits and target hold;
+ * a target outside [0, V) gives NaN. */
+size_t mpb_policy_loss_scratch_bytes(int64_t N, int64_t V, int dtype);
+int mpb_policy_loss(int64_t N, int64_t V, const void* logits, int dtype, int64_t l_sr, const void* targets,
+                    int targets_dtype, const float* old_logp, const float* advantages, const float* ref_logp,
+                    const void* mask, double clip_low, double clip_high, double kl_coef, double grad_scale, float* loss,
+                    float* logp, float* kl, void* clipped, void* dlogits, void* scratch, size_t scratch_bytes,
+                    mpb_stream_t stream);
+
 /* ---------------------------------------------------------------- creation */
 
 /* Fills `out` (n contiguous elements of `dtype`) with start + i*step, each

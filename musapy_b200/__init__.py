@@ -5,7 +5,10 @@ rebuilt for NVIDIA B200 (sm_100a).
 (python/musapy/__init__.py:3-110): add/sub/mul/div/pow, sin/cos/exp/log/abs/
 sign/neg, clamp, eq/ne/lt/gt/le/ge, sum/prod/max/min/mean/argmax/argmin/
 cumsum, ``Array.astype`` and the dunders, plus the array creation and view
-helpers those ops need. Every op runs on the CUDA kernels of
+helpers those ops need. The operators of a recurrent block (blocks.py) come
+beside them: gated_scan, gated_scan_backward, gated_scan_step, rms_norm,
+rms_norm_backward, gated_residual_norm, gated_residual_norm_backward, dropout
+and policy_loss. Every op runs on the CUDA kernels of
 ``_lib/libmusapy_b200.so``; there is no CPU execution path.
 """
 from . import dtypes as _dtype_mod
@@ -30,6 +33,18 @@ from .array import (
     slice,
     squeeze,
     transpose,
+)
+from .blocks import (
+    PolicyLoss,
+    dropout,
+    gated_residual_norm,
+    gated_residual_norm_backward,
+    gated_scan,
+    gated_scan_backward,
+    gated_scan_step,
+    policy_loss,
+    rms_norm,
+    rms_norm_backward,
 )
 from .dtypes import (
     Dtype,

@@ -21,6 +21,9 @@
 //                        compute_dtype) -> bytes
 //   reduce(op, shape, strides, a, in_dtype, axes_mask, out, out_dtype,
 //          compute_dtype, nan_first_rule, scratch, scratch_bytes, stream)
+//   gated_scan, gated_scan_backward, gated_scan_step, gated_residual_norm,
+//   gated_residual_norm_backward, dropout, policy_loss: the arguments of the
+//   mpb_* function of that name, in its order; *_scratch_bytes -> bytes
 // Pointers and streams are ints (0 or None for none); a_strides / b_strides
 // may be None where the C-ABI accepts a null array.
 #define PY_SSIZE_T_CLEAN
@@ -216,6 +219,163 @@ PyObject* py_reduce(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return PyLong_FromLong(rc);
 }
 
+// Reads a call's arguments one after the other; the first that does not
+// convert leaves its Python error and the reader false.
+class Args {
+ public:
+  Args(PyObject* const* a, Py_ssize_t n, Py_ssize_t want, const char* fn) : a_(a), ok_(nargs(n, want, fn)) {}
+  explicit operator bool() const { return ok_; }
+  template <class T = void>
+  T* p() {
+    void* v = nullptr;
+    ok_ = ok_ && ptr(*a_++, &v);
+    return static_cast<T*>(v);
+  }
+  int i() {
+    int v = 0;
+    ok_ = ok_ && i32(*a_++, &v);
+    return v;
+  }
+  int64_t l() {
+    if (!ok_) return 0;
+    const long long v = PyLong_AsLongLong(*a_++);
+    ok_ = !(v == -1 && PyErr_Occurred());
+    return v;
+  }
+  uint64_t u() {
+    uint64_t v = 0;
+    ok_ = ok_ && u64(*a_++, &v);
+    return v;
+  }
+  double d() {
+    if (!ok_) return 0.0;
+    const double v = PyFloat_AsDouble(*a_++);
+    ok_ = !(v == -1.0 && PyErr_Occurred());
+    return v;
+  }
+
+ private:
+  PyObject* const* a_;
+  bool ok_;
+};
+
+// The braces of these initialisers fix the order in which the arguments are read.
+PyObject* py_gated_scan_scratch_bytes(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 7, "gated_scan_scratch_bytes");
+  struct { int64_t B, T, D, H; int xd, gd, back; } v{a.l(), a.l(), a.l(), a.l(), a.i(), a.i(), a.i()};
+  if (!a) return nullptr;
+  return PyLong_FromSize_t(mpb_gated_scan_scratch_bytes(v.B, v.T, v.D, v.H, v.xd, v.gd, v.back));
+}
+
+PyObject* py_gated_scan(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 19, "gated_scan");
+  struct {
+    int64_t B, T, D, H;
+    void* x; int xd; int64_t xb, xt;
+    void* g; int gd; int64_t gb, gt;
+    float* h0; int mode; void* h; float* state; void* scratch; int64_t bytes; void* stream;
+  } v{a.l(), a.l(), a.l(), a.l(), a.p(), a.i(), a.l(), a.l(), a.p(), a.i(), a.l(), a.l(), a.p<float>(), a.i(), a.p(),
+      a.p<float>(), a.p(), a.l(), a.p()};
+  if (!a) return nullptr;
+  return PyLong_FromLong(mpb_gated_scan(v.B, v.T, v.D, v.H, v.x, v.xd, v.xb, v.xt, v.g, v.gd, v.gb, v.gt, v.h0, v.mode,
+                                        v.h, v.state, v.scratch, (size_t)v.bytes, (mpb_stream_t)v.stream));
+}
+
+PyObject* py_gated_scan_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 27, "gated_scan_backward");
+  struct {
+    int64_t B, T, D, H;
+    void* dh; int64_t db, dt;
+    void* x; int xd; int64_t xb, xt;
+    void* g; int gd; int64_t gb, gt;
+    void* h; int64_t hb, ht;
+    float *h0, *dstate; int mode; void *dx, *dg; float* dh0; void* scratch; int64_t bytes; void* stream;
+  } v{a.l(), a.l(), a.l(), a.l(), a.p(), a.l(), a.l(), a.p(), a.i(), a.l(), a.l(), a.p(), a.i(), a.l(), a.l(),
+      a.p(), a.l(), a.l(), a.p<float>(), a.p<float>(), a.i(), a.p(), a.p(), a.p<float>(), a.p(), a.l(), a.p()};
+  if (!a) return nullptr;
+  return PyLong_FromLong(mpb_gated_scan_backward(v.B, v.T, v.D, v.H, v.dh, v.db, v.dt, v.x, v.xd, v.xb, v.xt, v.g, v.gd,
+                                                 v.gb, v.gt, v.h, v.hb, v.ht, v.h0, v.dstate, v.mode, v.dx, v.dg, v.dh0,
+                                                 v.scratch, (size_t)v.bytes, (mpb_stream_t)v.stream));
+}
+
+PyObject* py_gated_scan_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 13, "gated_scan_step");
+  struct {
+    int64_t B, D, H; void* x; int xd; int64_t xb; void* g; int gd; int64_t gb; int mode; float* state; void *h, *stream;
+  } v{a.l(), a.l(), a.l(), a.p(), a.i(), a.l(), a.p(), a.i(), a.l(), a.i(), a.p<float>(), a.p(), a.p()};
+  if (!a) return nullptr;
+  return PyLong_FromLong(mpb_gated_scan_step(v.B, v.D, v.H, v.x, v.xd, v.xb, v.g, v.gd, v.gb, v.mode, v.state, v.h,
+                                             (mpb_stream_t)v.stream));
+}
+
+PyObject* py_gated_residual_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 22, "gated_residual_norm");
+  struct {
+    int64_t R, D; int dt;
+    void* x; int64_t xr; void* z; int64_t zr; void* g; int64_t gr; int kind, act;
+    float *post, *pre; double scale, eps, drop; uint64_t seed, off; void *y, *u; float* rstd; void* stream;
+  } v{a.l(), a.l(), a.i(), a.p(), a.l(), a.p(), a.l(), a.p(), a.l(), a.i(), a.i(), a.p<float>(), a.p<float>(), a.d(),
+      a.d(), a.d(), a.u(), a.u(), a.p(), a.p(), a.p<float>(), a.p()};
+  if (!a) return nullptr;
+  return PyLong_FromLong(mpb_gated_residual_norm(v.R, v.D, v.dt, v.x, v.xr, v.z, v.zr, v.g, v.gr, v.kind, v.act, v.post,
+                                                 v.pre, v.scale, v.eps, v.drop, v.seed, v.off, v.y, v.u, v.rstd,
+                                                 (mpb_stream_t)v.stream));
+}
+
+PyObject* py_gated_residual_norm_scratch_bytes(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 5, "gated_residual_norm_scratch_bytes");
+  struct { int64_t R, D; int dt, branch, kind; } v{a.l(), a.l(), a.i(), a.i(), a.i()};
+  if (!a) return nullptr;
+  return PyLong_FromSize_t(mpb_gated_residual_norm_scratch_bytes(v.R, v.D, v.dt, v.branch, v.kind));
+}
+
+PyObject* py_gated_residual_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 30, "gated_residual_norm_backward");
+  struct {
+    int64_t R, D; int dt;
+    void* dy; int64_t dyr; void* du; int64_t dur; void* y; int64_t yr; void* z; int64_t zr; void* g; int64_t gr;
+    int kind, act; float *post, *pre, *rstd; double scale, drop; uint64_t seed, off; void *dx, *dz, *dg;
+    float *dpost, *dpre; void* scratch; int64_t bytes; void* stream;
+  } v{a.l(), a.l(), a.i(), a.p(), a.l(), a.p(), a.l(), a.p(), a.l(), a.p(), a.l(), a.p(), a.l(), a.i(), a.i(),
+      a.p<float>(), a.p<float>(), a.p<float>(), a.d(), a.d(), a.u(), a.u(), a.p(), a.p(), a.p(), a.p<float>(),
+      a.p<float>(), a.p(), a.l(), a.p()};
+  if (!a) return nullptr;
+  return PyLong_FromLong(mpb_gated_residual_norm_backward(
+      v.R, v.D, v.dt, v.dy, v.dyr, v.du, v.dur, v.y, v.yr, v.z, v.zr, v.g, v.gr, v.kind, v.act, v.post, v.pre, v.rstd,
+      v.scale, v.drop, v.seed, v.off, v.dx, v.dz, v.dg, v.dpost, v.dpre, v.scratch, (size_t)v.bytes,
+      (mpb_stream_t)v.stream));
+}
+
+PyObject* py_dropout(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 8, "dropout");
+  struct { int64_t n; void* x; int dt; double p; uint64_t seed, off; void *y, *stream; } v{
+      a.l(), a.p(), a.i(), a.d(), a.u(), a.u(), a.p(), a.p()};
+  if (!a) return nullptr;
+  return PyLong_FromLong(mpb_dropout(v.n, v.x, v.dt, v.p, v.seed, v.off, v.y, (mpb_stream_t)v.stream));
+}
+
+PyObject* py_policy_loss_scratch_bytes(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 3, "policy_loss_scratch_bytes");
+  struct { int64_t N, V; int dt; } v{a.l(), a.l(), a.i()};
+  if (!a) return nullptr;
+  return PyLong_FromSize_t(mpb_policy_loss_scratch_bytes(v.N, v.V, v.dt));
+}
+
+PyObject* py_policy_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 23, "policy_loss");
+  struct {
+    int64_t N, V; void* z; int dt; int64_t sr; void* t; int tdt; float *old, *adv, *ref; void* mask;
+    double lo, hi, kl, gs; float *loss, *logp, *klo; void *clipped, *grad, *scratch; int64_t bytes; void* stream;
+  } v{a.l(), a.l(), a.p(), a.i(), a.l(), a.p(), a.i(), a.p<float>(), a.p<float>(), a.p<float>(), a.p(), a.d(), a.d(),
+      a.d(), a.d(), a.p<float>(), a.p<float>(), a.p<float>(), a.p(), a.p(), a.p(), a.l(), a.p()};
+  if (!a) return nullptr;
+  return PyLong_FromLong(mpb_policy_loss(v.N, v.V, v.z, v.dt, v.sr, v.t, v.tdt, v.old, v.adv, v.ref, v.mask, v.lo, v.hi,
+                                         v.kl, v.gs, v.loss, v.logp, v.klo, v.clipped, v.grad, v.scratch,
+                                         (size_t)v.bytes, (mpb_stream_t)v.stream));
+}
+
+#define MPB_METHOD(name, doc) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, doc}
+
 PyMethodDef kMethods[] = {
     {"elementwise", (PyCFunction)(void (*)(void))py_elementwise, METH_FASTCALL,
      "mpb_elementwise with shapes and strides as tuples"},
@@ -224,6 +384,16 @@ PyMethodDef kMethods[] = {
     {"reduce_scratch_bytes", (PyCFunction)(void (*)(void))py_reduce_scratch_bytes, METH_FASTCALL,
      "mpb_reduce_scratch_bytes with shapes and strides as tuples"},
     {"reduce", (PyCFunction)(void (*)(void))py_reduce, METH_FASTCALL, "mpb_reduce with shapes and strides as tuples"},
+    MPB_METHOD(gated_scan, "mpb_gated_scan"),
+    MPB_METHOD(gated_scan_backward, "mpb_gated_scan_backward"),
+    MPB_METHOD(gated_scan_step, "mpb_gated_scan_step"),
+    MPB_METHOD(gated_scan_scratch_bytes, "mpb_gated_scan_scratch_bytes"),
+    MPB_METHOD(gated_residual_norm, "mpb_gated_residual_norm"),
+    MPB_METHOD(gated_residual_norm_backward, "mpb_gated_residual_norm_backward"),
+    MPB_METHOD(gated_residual_norm_scratch_bytes, "mpb_gated_residual_norm_scratch_bytes"),
+    MPB_METHOD(dropout, "mpb_dropout"),
+    MPB_METHOD(policy_loss, "mpb_policy_loss"),
+    MPB_METHOD(policy_loss_scratch_bytes, "mpb_policy_loss_scratch_bytes"),
     {nullptr, nullptr, 0, nullptr},
 };
 
