@@ -15,9 +15,9 @@ import torch
 
 from . import dtypes as _dt
 from . import errors
-from ._lib import NATIVE, check
+from ._lib import LIB, NATIVE, check
 from .array import Array
-from .ops import _alias, _check_out, _launch, _out, _same_device, contiguous, full
+from .ops import _CHECK_SCAN_STATUS, _alias, _check_out, _launch, _out, _same_device, _stream, contiguous, full
 
 _MODES = {"linear": 0, "sigmoid": 1}
 _ACTIVATIONS = {"linear": 0, "sigmoid": 1, "silu": 2}
@@ -115,6 +115,12 @@ def _scan_inputs(name: str, x, gate, time: bool):
     return _unit_inner(x), _unit_inner(gate), B, T, D, H
 
 
+def _scan_status(name: str, scratch, T: int, dev: int) -> None:
+    """With ``ops.set_scan_status_check(True)`` (it synchronises): did a wait between the pieces of a sequence give up?"""
+    if scratch is not None and _CHECK_SCAN_STATUS[0]:
+        check(LIB.mpb_gated_scan_status(scratch.data_ptr(), T, _stream(dev)), name)
+
+
 def gated_scan(x, gate, h0=None, mode="linear", return_state=False, out=None):
     """Gated linear recurrence over time: ``h[t] = a[t] h[t-1] + b[t]``.
 
@@ -146,6 +152,7 @@ def gated_scan(x, gate, h0=None, mode="linear", return_state=False, out=None):
         check(NATIVE.gated_scan(B, T, D, H, x._ptr, x._dtype.code, xb, xt, gate._ptr, gate._dtype.code, gb, gt,
                                 _ptr(h0), m, h._ptr, _ptr(state), _sptr(scratch), nbytes,
                                 _launch(name, dev, *ins, h, state)), name)
+        _scan_status(name, scratch, T, dev)
     return (h, state) if return_state else h
 
 
@@ -176,6 +183,7 @@ def gated_scan_backward(dh, x, gate, h, h0=None, dstate=None, mode="linear"):
                                          gate._dtype.code, *_btd(gate), h._ptr, *_btd(h), _ptr(h0), _ptr(dstate), m,
                                          dx._ptr, dgate._ptr, dh0._ptr, _sptr(scratch), nbytes,
                                          _launch(name, dev, *ins, dx, dgate, dh0)), name)
+        _scan_status(name, scratch, T, dev)
     return dx, dgate, dh0
 
 
