@@ -222,10 +222,10 @@ int mpb_gated_scan_backward(int64_t B, int64_t T, int64_t D, int64_t H, const vo
                             const float* dstate, int mode, void* dx, void* dgate, float* dh0, void* scratch,
                             size_t scratch_bytes, mpb_stream_t stream);
 
-/* Synchronises `stream` and reads the status word that a scan over T steps
- * left in its scratch: MPB_OK, or MPB_ERR_TIMEOUT when a bounded wait between
+/* Synchronises `stream` and reads the status word that a scan left in its
+ * scratch (NULL: it had none): MPB_OK, or MPB_ERR_TIMEOUT when a bounded wait between
  * the pieces of a long sequence gave up (the results from there on are NaN). */
-int mpb_gated_scan_status(const void* scratch, int64_t T, mpb_stream_t stream);
+int mpb_gated_scan_status(const void* scratch, mpb_stream_t stream);
 
 /* One step of B running sequences: x (B, D), gate (B, H); updates state
  * (B, D) in place and writes the new state in x's type to h (B, D). */

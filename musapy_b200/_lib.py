@@ -98,7 +98,7 @@ def _load() -> ctypes.CDLL:
     L.mpb_cumsum_status.restype = ctypes.c_int
     L.mpb_cumsum_status.argtypes = [c_vp, c_vp]
     L.mpb_gated_scan_status.restype = ctypes.c_int
-    L.mpb_gated_scan_status.argtypes = [c_vp, ctypes.c_int64, c_vp]
+    L.mpb_gated_scan_status.argtypes = [c_vp, c_vp]
     L.mpb_launch_count.restype = ctypes.c_ulonglong
     L.mpb_launch_count.argtypes = []
     L.mpb_shard_arg_combine.restype = ctypes.c_int

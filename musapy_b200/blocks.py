@@ -115,10 +115,10 @@ def _scan_inputs(name: str, x, gate, time: bool):
     return _unit_inner(x), _unit_inner(gate), B, T, D, H
 
 
-def _scan_status(name: str, scratch, T: int, dev: int) -> None:
+def _scan_status(name: str, scratch, dev: int) -> None:
     """With ``ops.set_scan_status_check(True)`` (it synchronises): did a wait between the pieces of a sequence give up?"""
     if scratch is not None and _CHECK_SCAN_STATUS[0]:
-        check(LIB.mpb_gated_scan_status(scratch.data_ptr(), T, _stream(dev)), name)
+        check(LIB.mpb_gated_scan_status(scratch.data_ptr(), _stream(dev)), name)
 
 
 def gated_scan(x, gate, h0=None, mode="linear", return_state=False, out=None):
@@ -152,7 +152,7 @@ def gated_scan(x, gate, h0=None, mode="linear", return_state=False, out=None):
         check(NATIVE.gated_scan(B, T, D, H, x._ptr, x._dtype.code, xb, xt, gate._ptr, gate._dtype.code, gb, gt,
                                 _ptr(h0), m, h._ptr, _ptr(state), _sptr(scratch), nbytes,
                                 _launch(name, dev, *ins, h, state)), name)
-        _scan_status(name, scratch, T, dev)
+        _scan_status(name, scratch, dev)
     return (h, state) if return_state else h
 
 
@@ -183,7 +183,7 @@ def gated_scan_backward(dh, x, gate, h, h0=None, dstate=None, mode="linear"):
                                          gate._dtype.code, *_btd(gate), h._ptr, *_btd(h), _ptr(h0), _ptr(dstate), m,
                                          dx._ptr, dgate._ptr, dh0._ptr, _sptr(scratch), nbytes,
                                          _launch(name, dev, *ins, dx, dgate, dh0)), name)
-        _scan_status(name, scratch, T, dev)
+        _scan_status(name, scratch, dev)
     return dx, dgate, dh0
 
 

@@ -2,7 +2,9 @@
 // a counter (philox.cuh), so the backward pass is the same call on the
 // gradient with the same seed and offset. No counterpart in the reference.
 //
-// Bound: memory (one read and one write per element).
+// A thread takes eight elements, one counter, per step: one 16-byte load and
+// store of a 16-bit type, two of float. Bound: memory (one read and one write
+// per element).
 #include "common.cuh"
 #include "internal.h"
 #include "musapy_b200.h"
@@ -13,11 +15,59 @@ namespace mpb {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kUnroll = 2;  // counters per thread and step, their loads first
 
-// A thread takes eight elements, one counter, per step.
+template <class T>
+struct Eight {
+  static constexpr int kWords = (int)sizeof(T) / 2;
+  union {
+    uint4 w[kWords];
+    T v[8];
+  };
+  MPB_D Eight() {}
+};
+
+// Each element's 16-bit half is compared with the threshold; what stays is
+// scaled in float and rounded once.
+template <class T>
+MPB_D void drop_eight(Eight<T>& x, const uint4& w, const Dropper& d) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float v = to_f(x.v[j]) * d.up;
+    x.v[j] = Cvt<T>::from(half_of(w, j) >= d.drop ? v : 0.0f);
+  }
+}
+
 template <class T>
 __global__ void __launch_bounds__(kThreads) k_dropout(const T* __restrict__ x, T* __restrict__ y, int64_t n,
                                                       Dropper d) {
+  const int64_t whole = n / 8, stride = (int64_t)gridDim.x * kThreads;
+  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  for (int64_t b = at; b < whole; b += stride * kUnroll) {
+    Eight<T> v[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (b + u * stride < whole)
+#pragma unroll
+        for (int k = 0; k < Eight<T>::kWords; ++k)
+          v[u].w[k] = ld_stream16((const char*)x + ((b + u * stride) * Eight<T>::kWords + k) * 16);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (b + u * stride < whole) {
+        drop_eight(v[u], philox(d, (uint64_t)(b + u * stride)), d);
+#pragma unroll
+        for (int k = 0; k < Eight<T>::kWords; ++k)
+          st_stream16((char*)y + ((b + u * stride) * Eight<T>::kWords + k) * 16, v[u].w[k]);
+      }
+  }
+  const int64_t i = whole * 8 + at;  // the last elements, fewer than eight
+  if (i < n) y[i] = keeps(d, (uint64_t)i) ? Cvt<T>::from(to_f(x[i]) * d.up) : Cvt<T>::from(0.0f);
+}
+
+// Addresses that no 16-byte access may use: a thread still takes one counter per step.
+template <class T>
+__global__ void __launch_bounds__(kThreads) k_dropout_any(const T* __restrict__ x, T* __restrict__ y, int64_t n,
+                                                          Dropper d) {
   const int64_t blocks = (n + 7) / 8;
   for (int64_t b = (int64_t)blockIdx.x * kThreads + threadIdx.x; b < blocks; b += (int64_t)gridDim.x * kThreads) {
     const uint4 w = philox(d, (uint64_t)b);
@@ -32,7 +82,9 @@ __global__ void __launch_bounds__(kThreads) k_dropout(const T* __restrict__ x, T
 template <class T>
 int launch_dropout(const void* x, void* y, int64_t n, const Dropper& d, cudaStream_t s) {
   const int64_t want = ((n + 7) / 8 + kThreads - 1) / kThreads, cap = (int64_t)sm_count() * 64;
-  k_dropout<T><<<(unsigned)(want < cap ? want : cap), kThreads, 0, s>>>((const T*)x, (T*)y, n, d);
+  const unsigned grid = (unsigned)(want < cap ? want : cap);
+  if (((uintptr_t)x | (uintptr_t)y) % 16 == 0) k_dropout<T><<<grid, kThreads, 0, s>>>((const T*)x, (T*)y, n, d);
+  else k_dropout_any<T><<<grid, kThreads, 0, s>>>((const T*)x, (T*)y, n, d);
   return launch_check("dropout");
 }
 

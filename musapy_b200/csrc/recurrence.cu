@@ -16,21 +16,29 @@
 // of a shared gate sums over its channels in a fixed order. The state runs in
 // float whatever the element type.
 //
-// One pass over the data, in tiles of 32 lanes x V channels by S x 16 steps.
-// A warp holds 16 steps of its channels in registers and folds them to the
-// map c -> A c + B that they apply to the state; the block joins the maps of
-// its S warps, gets the state that enters the tile, and each warp then runs
-// its steps once more from the state that enters them and writes. Where T
-// takes several tiles they form a chain: a tile publishes its map, then its
-// outgoing state, and takes its incoming state from the nearest earlier tile
-// that has published one, applying the maps between them in time order. A
-// state passes through the same operations wherever the look-back found it, so
-// results do not depend on timing. Tiles are handed out by a ticket, all
-// chains' first tiles first, so that a tile waits only for tiles that already
-// run, and every wait is bounded. The backward pass is the same walk with time
-// reversed, over the map u -> a (u + dh).
+// One pass over the data, in tiles of 32 lanes x V channels by S warps x 16
+// (backward 8) steps. A warp folds its steps to the map c -> A c + B that they
+// apply to the state; the block joins the maps of its warps, and each warp
+// then runs its steps once more from the state that enters them and writes.
+// Each thread copies the words it will use itself into shared memory some
+// tiles ahead (cp.async), so the copies of the next tiles are in flight while
+// a tile is computed, and no barrier guards them.
+//
+// Along time either a block walks a chain (the tiles of 32 V channels of a
+// sequence) and carries the state, or, where there are too few chains to
+// occupy the GPU that way, the tiles of a chain run at the same time: a tile
+// publishes its map, then its outgoing state, and takes its incoming state
+// from the nearest earlier tile that has published one, applying the maps
+// between them in time order. A state passes through the same operations
+// wherever the look-back found it, so results do not depend on timing. Words
+// are published without flags or fences: zero means not there yet, and a zero
+// value is written as -0. Tiles are handed out by a ticket, all chains' first
+// tiles first, so that a tile waits only for tiles that already run, and every
+// wait is bounded. The backward pass is the same walk with time reversed, over
+// the map u -> a (u + dh).
 //
 // Bound: memory.
+#include "async_copy.cuh"
 #include "common.cuh"
 #include "internal.h"
 #include "musapy_b200.h"
@@ -40,9 +48,10 @@
 namespace mpb {
 namespace {
 
-constexpr int kSteps = 16;               // steps per warp and tile
-constexpr int kWarps = 8;                // warps of a full tile
-constexpr uint32_t kMap = 1, kState = 2; // what a tile has published
+constexpr int kWarps = 8;       // warps of a full tile
+constexpr int kFwd = 16;        // steps per warp and tile, forward
+constexpr int kBwd = 8;         // backward: four inputs instead of two
+constexpr int kRing = 96 << 10; // shared memory of a block for tiles under way, two blocks per SM
 
 struct ScanArgs {
   int64_t B, T, D, H, P;  // P = D / H channels per gate
@@ -59,25 +68,39 @@ struct ScanArgs {
   uint32_t chains, chunks;    // B * groups, tiles per chain
   FastDiv by_groups, by_groups_per, by_lanes_per, by_chains;
   int steps;                  // of a tile
+  int walk;                   // a block takes whole chains
   // scratch
-  uint32_t *ticket, *status, *flags;
-  float *map_a, *map_b, *out_state;  // (tiles, channels of a group)
-  float* part;                       // (B, T, H, groups_per)
+  uint32_t *ticket, *status;
+  uint64_t* maps;    // (tiles, channels of a group): {A, B}
+  uint32_t* states;  // (tiles, channels of a group): the state after the tile
+  float* part;       // (B, T, H, groups_per)
 };
 
-template <class G, bool SIG>
-MPB_D void gate_of(G g, float& a, float& om) {
-  if (SIG) {
-    sigmoid2(to_f(g), a, om);
+// The decay a and what the input is weighted with, om, of a gate.
+template <bool SIG, class F>
+MPB_D void gate_of(F g, F& a, F& om) {
+  if constexpr (SIG) {
+    sigmoid2(g, a, om);
   } else {
-    a = to_f(g);
-    om = 1.0f;
+    a = om = g;
+  }
+}
+// Of a gate's pack; one that the lane's channels share is evaluated once.
+template <bool SIG, int V, class P>
+MPB_D void gates_of(const P& g, Floats<V>& a, Floats<V>& om) {
+  if constexpr (sizeof(P::v) == sizeof(g.v[0]) && V == 2) {
+    float sa, so;
+    gate_of<SIG>(to_f(g.v[0]), sa, so);
+    a = vset<V>(sa);
+    om = vset<V>(so);
+  } else {
+    gate_of<SIG>(unpack(g), a, om);
   }
 }
 
-// The state after the map (a, b). A zero state stays out of the product: the
-// product of a tile's gates may have overflowed although no state did.
-MPB_D float apply(float a, float b, float c) { return c == 0.0f ? b : fmaf(a, c, b); }
+// The product of a warp's decays, kept finite: gates above one may overflow it
+// where no state does, and an infinity would turn a state of zero into NaN.
+MPB_D float finite(float a) { return fminf(fmaxf(a, -3.0e38f), 3.0e38f); }
 
 // Where a lane works.
 struct Lane {
@@ -112,202 +135,441 @@ MPB_D Lane place(const ScanArgs& p, uint32_t chain, int lane) {
   return l;
 }
 
-MPB_D uint32_t ld_flag(const uint32_t* p) {
+MPB_D uint32_t ld_word(const uint32_t* p) {
   uint32_t v;
   asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
-MPB_D void st_flag(uint32_t* p, uint32_t v) {
+MPB_D uint64_t ld_word(const uint64_t* p) {
+  uint64_t v;
+  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+  return v;
+}
+MPB_D void st_word(uint32_t* p, uint32_t v) {
   asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+MPB_D void st_word(uint64_t* p, uint64_t v) {
+  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
 }
 MPB_D unsigned long long now_ns() {
   unsigned long long t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
+constexpr unsigned long long kPatience = 2000000000ull;  // ns a wait lasts at most
 
-// Warp 0 of a tile: the state that enters it, per lane and channel. `first`
-// is the state before the chain; (a, b) is the tile's own map, published when
-// the tile before has no state yet.
+// A value as a word that is never zero, and back (+0 for -0).
+MPB_D uint32_t state_word(float v) {
+  const uint32_t w = __float_as_uint(v);
+  return w ? w : 0x80000000u;
+}
+MPB_D uint64_t map_word(float a, float b) {
+  const uint64_t w = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+  return w ? w : 0x80000000ull;
+}
+
+// A word some other tile publishes, when it is there; false when the wait ran out.
+template <class W>
+MPB_D bool await(const W* p, W& w) {
+  w = ld_word(p);
+  if (w) return true;
+  const unsigned long long t0 = now_ns();
+  do {
+    w = ld_word(p);
+    if (w) return true;
+  } while (now_ns() - t0 < kPatience);
+  return false;
+}
+
+// Warp 0 of a tile: the state that enters it, per lane and channel (carry
+// holds the one before the chain). (a, b) is the tile's own map, published
+// when the tile before has no state yet; early: that tile's words as seen
+// before this tile's data came.
 template <int V>
 MPB_D void look_back(const ScanArgs& p, uint32_t chain, uint32_t chunk, int lane, const float (&a)[V],
-                     const float (&b)[V], float (&carry)[V]) {
+                     const float (&b)[V], uint32_t (&early)[V], float (&carry)[V]) {
   constexpr int C = 32 * V;
-  const uint32_t tile = chunk * p.chains + chain;
+  if (chunk == 0) return;
   auto at = [&](uint32_t k) { return (size_t)(k * p.chains + chain) * C + lane * V; };
-  uint32_t back = 0;  // distance - 1 of the nearest tile with a state
-  bool found = chunk == 0 || ld_flag(p.flags + tile - p.chains) == kState;
-  found = __all_sync(0xffffffffu, found);
-  if (!found) {
+  bool there = true;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      __stcg(p.map_a + at(chunk) + v, a[v]);
-      __stcg(p.map_b + at(chunk) + v, b[v]);
+  for (int v = 0; v < V; ++v) {
+    if (!early[v]) early[v] = ld_word(p.states + at(chunk - 1) + v);
+    there = there && early[v];
+  }
+  if (__all_sync(0xffffffffu, there)) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) carry[v] = __uint_as_float(early[v]) + 0.0f;
+    return;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) st_word(p.maps + at(chunk) + v, map_word(a[v], b[v]));
+  // lane i looks at the first channel of the tile i + 1 before this one;
+  // before the chain's first tile stands the initial state
+  uint32_t back;
+  bool ok = true;
+  const unsigned long long t0 = now_ns();
+  for (;;) {
+    const bool before = (uint32_t)lane >= chunk;
+    const size_t q = before ? 0 : (size_t)((chunk - 1 - lane) * p.chains + chain) * C;
+    const uint32_t states = __ballot_sync(0xffffffffu, before || ld_word(p.states + q) != 0);
+    const uint32_t nothing = __ballot_sync(0xffffffffu, !before && ld_word(p.maps + q) == 0);
+    if (states) {
+      back = __ffs(states) - 1;
+      if ((nothing & ((1u << back) - 1)) == 0) break;
     }
-    __threadfence();
-    __syncwarp();
-    if (lane == 0) st_flag(p.flags + tile, kMap);
-    const unsigned long long t0 = now_ns();
-    for (;;) {
-      // lane i looks at the tile i + 1 before this one; before the chain's
-      // first tile stands the initial state
-      const uint32_t f = (uint32_t)lane < chunk ? ld_flag(p.flags + tile - (lane + 1) * p.chains) : kState;
-      const uint32_t states = __ballot_sync(0xffffffffu, f == kState);
-      const uint32_t nothing = __ballot_sync(0xffffffffu, f == 0);
-      if (states) {
-        back = __ffs(states) - 1;
-        if ((nothing & ((1u << back) - 1)) == 0) break;
-      }
-      const bool late = now_ns() - t0 > 2000000000ull;
-      if (__any_sync(0xffffffffu, late)) {  // give up: what follows is marked and NaN
-        if (lane == 0) st_flag(p.status, MPB_ERR_TIMEOUT);
-#pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = NAN;
-        return;
-      }
+    if (__any_sync(0xffffffffu, now_ns() - t0 > kPatience)) {
+      ok = false;
+      back = 0;
+      break;
     }
   }
-  __threadfence();
-  __syncwarp();
-  if (chunk > back)
+  // the other channels' words of those tiles are there or about to be
+  if (chunk > back && ok)
 #pragma unroll
-    for (int v = 0; v < V; ++v) carry[v] = __ldcg(p.out_state + at(chunk - 1 - back) + v);
+    for (int v = 0; v < V; ++v) {
+      uint32_t w = 0;
+      ok = ok && await(p.states + at(chunk - 1 - back) + v, w);
+      carry[v] = __uint_as_float(w) + 0.0f;
+    }
   for (uint32_t k = chunk - back; k < chunk; ++k)
 #pragma unroll
-    for (int v = 0; v < V; ++v) carry[v] = apply(__ldcg(p.map_a + at(k) + v), __ldcg(p.map_b + at(k) + v), carry[v]);
+    for (int v = 0; v < V; ++v) {
+      uint64_t w = 0;
+      ok = ok && await(p.maps + at(k) + v, w);
+      carry[v] = fmaf(__uint_as_float((uint32_t)w), carry[v], __uint_as_float((uint32_t)(w >> 32)));
+    }
+  if (!ok) {  // gave up: what follows is marked and NaN
+    st_word(p.status, MPB_ERR_TIMEOUT);
+#pragma unroll
+    for (int v = 0; v < V; ++v) carry[v] = NAN;
+  }
 }
 
-// Joins the maps of the block's warps (a, b: this warp's), gets the state
-// `carry` that enters the tile (in: the one before the chain) and returns the
-// state that enters the warp's steps.
 template <int V>
-MPB_D void join(const ScanArgs& p, uint32_t chain, uint32_t chunk, int warp, int lane, const float (&a)[V],
-                const float (&b)[V], float (&carry)[V]) {
+struct Shared {
+  __align__(8) float a[2][kWarps][32 * V];  // the warps' maps, of this tile and of the one before
+  __align__(8) float b[2][kWarps][32 * V];
+  __align__(8) float carry[32 * V];
+  uint32_t tiles[4];
+};
+
+// The state after warp w's steps.
+template <int V>
+MPB_D Floats<V> through(const Shared<V>& sh, int side, int w, int lane, Floats<V> c) {
+  return vfma(*reinterpret_cast<const Floats<V>*>(&sh.a[side][w][lane * V]), c,
+              *reinterpret_cast<const Floats<V>*>(&sh.b[side][w][lane * V]));
+}
+
+// Joins the maps of the block's warps (a, b: this warp's). carry: the state
+// that enters the tile (look-back: before the chain) and, on return, the one
+// that leaves it (walk). Returns in `in` the state that enters the warp's steps.
+template <int V, bool WALK>
+MPB_D void join(const ScanArgs& p, Shared<V>& sh, int side, uint32_t chain, uint32_t chunk, int warp, int lane,
+                Floats<V> a, Floats<V> b, uint32_t (&early)[V], Floats<V>& carry, Floats<V>& in) {
   constexpr int C = 32 * V;
-  __shared__ float sa[kWarps][C], sb[kWarps][C], sc[C];
   const int warps = blockDim.x >> 5;
-  if (warps == 1 && p.chunks == 1) return;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    sa[warp][lane * V + v] = a[v];
-    sb[warp][lane * V + v] = b[v];
-  }
-  __syncthreads();
-  if (p.chunks > 1) {
-    if (warp == 0) {
-      float ta[V], tb[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        ta[v] = a[v], tb[v] = b[v];
-        for (int w = 1; w < warps; ++w) {
-          const float aw = sa[w][lane * V + v];
-          tb[v] = apply(aw, sb[w][lane * V + v], tb[v]);
-          ta[v] *= aw;
-        }
-      }
-      look_back<V>(p, chain, chunk, lane, ta, tb, carry);
-      const uint32_t tile = chunk * p.chains + chain;
-      if (chunk + 1 < p.chunks) {
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          __stcg(p.out_state + (size_t)tile * C + lane * V + v, apply(ta[v], tb[v], carry[v]));
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) st_flag(p.flags + tile, kState);
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) sc[lane * V + v] = carry[v];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < V; ++v) carry[v] = sc[lane * V + v];
-  }
-  for (int w = 0; w < warp; ++w)
-#pragma unroll
-    for (int v = 0; v < V; ++v) carry[v] = apply(sa[w][lane * V + v], sb[w][lane * V + v], carry[v]);
-}
-
-// The block's tile: the next ticket, or its index where no tile waits for another.
-MPB_D void take_tile(const ScanArgs& p, uint32_t& chain, uint32_t& chunk) {
-  uint32_t tile = blockIdx.x;
-  if (p.chunks > 1) {
-    __shared__ uint32_t mine;
-    if (threadIdx.x == 0) mine = atomicAdd(p.ticket, 1u);
-    __syncthreads();
-    tile = mine;
-  }
-  p.by_chains.divmod(tile, chunk, chain);
-}
-
-template <class X, class G, bool SIG, int V, bool SHARED>
-__global__ void __launch_bounds__(kWarps * 32, 2) k_gscan(ScanArgs p) {
-  using XP = Pack<X, V>;
-  using GP = Pack<G, SHARED ? 1 : V>;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t chain, chunk;
-  take_tile(p, chain, chunk);
-  const Lane l = place<V, SHARED>(p, chain, lane);
-  const int64_t t0 = (int64_t)chunk * p.steps + warp * kSteps;
-  const int n = l.in ? (int)(p.T - t0 < kSteps ? p.T - t0 : kSteps) : 0;
-  const X* x = (const X*)p.x + l.b * p.x_sb + t0 * p.x_st + l.ch;
-  const G* g = (const G*)p.gate + l.b * p.g_sb + t0 * p.g_st + l.gate;
-  XP xw[kSteps];
-  GP gw[kSteps];
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i)
-    if (i < n) {
-      xw[i].w = *reinterpret_cast<const typename XP::W*>(x + i * p.x_st);
-      gw[i].w = *reinterpret_cast<const typename GP::W*>(g + i * p.g_st);
-    }
-  float carry[V], a[kSteps][V], b[kSteps][V], ma[V], mb[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    carry[v] = l.in && p.h0 ? p.h0[l.b * p.D + l.ch + v] : 0.0f;
-    ma[v] = 1.0f;
-    mb[v] = 0.0f;
-  }
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i)
+  if (warps > 1 || !WALK) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      a[i][v] = 1.0f;
-      b[i][v] = 0.0f;
-      if (i < n) {
-        float om;
-        gate_of<G, SIG>(gw[i].v[SHARED ? 0 : v], a[i][v], om);
-        b[i][v] = SIG ? om * to_f(xw[i].v[v]) : to_f(xw[i].v[v]);
-      }
-      ma[v] *= a[i][v];
-      mb[v] = fmaf(a[i][v], mb[v], b[i][v]);
+      sh.a[side][warp][lane * V + v] = finite(vget(a, v));
+      sh.b[side][warp][lane * V + v] = vget(b, v);
     }
-  join<V>(p, chain, chunk, warp, lane, ma, mb, carry);
-  X* h = (X*)p.h + (l.b * p.T + t0) * p.D + l.ch;
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i)
-    if (i < n) {
-      XP out;
+    __syncthreads();
+  }
+  if (!WALK) {
+    if (warp == 0) {
+      float ta[V], tb[V], c[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        carry[v] = fmaf(a[i][v], carry[v], b[i][v]);
-        out.v[v] = Cvt<X>::from(carry[v]);
-      }
-      *reinterpret_cast<typename XP::W*>(h + i * p.D) = out.w;
-    }
-  if (p.state && n > 0 && t0 + n == p.T)
+        c[v] = vget(carry, v);
+        ta[v] = finite(vget(a, v)), tb[v] = vget(b, v);
 #pragma unroll
-    for (int v = 0; v < V; ++v) p.state[l.b * p.D + l.ch + v] = carry[v];
+        for (int w = 1; w < kWarps; ++w) {
+          const float aw = sh.a[side][w][lane * V + v];
+          tb[v] = fmaf(aw, tb[v], sh.b[side][w][lane * V + v]);
+          ta[v] = finite(ta[v] * aw);
+        }
+      }
+      look_back<V>(p, chain, chunk, lane, ta, tb, early, c);
+      if (chunk + 1 < p.chunks) {
+        const size_t at = (size_t)(chunk * p.chains + chain) * C + lane * V;
+#pragma unroll
+        for (int v = 0; v < V; ++v) st_word(p.states + at + v, state_word(fmaf(ta[v], c[v], tb[v])));
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) sh.carry[lane * V + v] = c[v];
+    }
+    __syncthreads();
+    in = *reinterpret_cast<const Floats<V>*>(&sh.carry[lane * V]);
+    for (int w = 0; w < warp; ++w) in = through<V>(sh, side, w, lane, in);
+    return;
+  }
+  in = carry;
+  if (warps == 1) return;  // the warp's own steps end the tile: the caller carries on from them
+  if (warps == kWarps) {
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w == warp) in = carry;
+      carry = through<V>(sh, side, w, lane, carry);
+    }
+  } else {
+    for (int w = 0; w < warps; ++w) {
+      if (w == warp) in = carry;
+      carry = through<V>(sh, side, w, lane, carry);
+    }
+  }
 }
 
-// Sums over the `lanes` (a power of two) neighbours of a lane of kSteps values
-// each: every round gives half of the values to the partner and takes its
-// half of the others', so 16 shuffles do for 16 values over 32 lanes. On
-// return val[0..left) of a lane are the sums of the steps first..first + left,
-// the same in the lanes that differ in bits above log2(kSteps).
-MPB_D void sum_over_lanes(float (&val)[kSteps], int lane, int lanes, int& first, int& left) {
-  first = 0;
-  left = kSteps;
+// cp.async of the word that holds the element(s): 4 bytes for one 32-bit or
+// two 16-bit elements, 8 for two 32-bit ones. Of a single 16-bit element the
+// aligned word around it is taken (an address of 2 modulo 4 is never the start
+// of an allocation; at 0 modulo 4 only the element's two bytes are read).
+template <int BYTES>
+MPB_D void copy_word(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 8) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+  } else if constexpr (BYTES == 4) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+  } else {
+    const uintptr_t q = (uintptr_t)src;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(q & ~(uintptr_t)3),
+                 "r"((q & 2) ? 4 : 2)
+                 : "memory");
+  }
+}
+MPB_D void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+MPB_D void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// p + st as one 64-bit add (the compiler would multiply for every step).
+template <class T>
+MPB_D T* ahead_by(T* p, int64_t st) {
+  uint64_t q = (uint64_t)p;
+  asm("add.s64 %0, %0, %1;" : "+l"(q) : "l"(st));
+  return (T*)q;
+}
+
+// Stores through a pointer that ahead_by has moved: it is global memory.
+template <class T, int N>
+MPB_D void put_global(char* p, const Pack<T, N>& v) {
+  if constexpr (sizeof(T) * N == 8) {
+    asm volatile("st.global.v2.u32 [%0], {%1, %2};" ::"l"(p), "r"(v.w.x), "r"(v.w.y) : "memory");
+  } else if constexpr (sizeof(T) * N == 4) {
+    asm volatile("st.global.u32 [%0], %1;" ::"l"(p), "r"(*reinterpret_cast<const uint32_t*>(&v.w)) : "memory");
+  } else {
+    asm volatile("st.global.u16 [%0], %1;" ::"l"(p), "h"(v.w) : "memory");
+  }
+}
+
+// One input of a tile: N elements of T per step, in words of shared memory
+// [step][thread].
+template <class T, int N>
+struct Column {
+  static constexpr int kElems = (int)sizeof(T) * N;        // bytes used
+  static constexpr int kWord = kElems < 4 ? 4 : kElems;    // bytes kept
+  static constexpr uint32_t bytes(int steps) { return (uint32_t)steps * kWarps * 32 * kWord; }
+  // n of STEPS steps, st bytes apart
+  template <int STEPS>
+  static MPB_D void copy(uint32_t base, const char* src, int64_t st, int n) {
+    base += threadIdx.x * kWord;
+    if (n >= STEPS) {
 #pragma unroll
-  for (int half = kSteps / 2, bit = 1; half > 0; half >>= 1, bit <<= 1) {
+      for (int i = 0; i < STEPS; ++i) {
+        copy_word<kElems>(base + i * kWarps * 32 * kWord, src);
+        src = ahead_by(src, st);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        if (i < n) copy_word<kElems>(base + i * kWarps * 32 * kWord, src);
+        src = ahead_by(src, st);
+      }
+    }
+  }
+  // half: of a single 16-bit element, bit 1 of its address
+  static MPB_D Pack<T, N> get(const char* base, int i, uint32_t half) {
+    Pack<T, N> v;
+    const char* q = base + (i * kWarps * 32 + threadIdx.x) * kWord;
+    if constexpr (kElems < 4) q += half & 2;
+    v.w = *reinterpret_cast<const typename Pack<T, N>::W*>(q);
+    return v;
+  }
+};
+
+// What the tiles of a block are, in order. Walk: the chunks of chain blockIdx,
+// then of chain blockIdx + grid, ... Look-back: the tickets it took.
+template <bool WALK>
+struct Order {
+  uint32_t chain, chunk;
+  MPB_D void first() {
+    chain = blockIdx.x;
+    chunk = 0;
+  }
+  // The tile number `it` of the block (walk: the one it stands at); false when there is none.
+  MPB_D bool here(const ScanArgs& p, const uint32_t* tiles, int it) {
+    if (WALK) return chain < p.chains;
+    const uint32_t t = tiles[it & 3];
+    p.by_chains.divmod(t, chunk, chain);
+    return t < p.chains * p.chunks;
+  }
+  MPB_D void next(const ScanArgs& p) {
+    if (WALK && ++chunk == p.chunks) {
+      chunk = 0;
+      chain += gridDim.x;
+    }
+  }
+};
+
+// Where a thread's words of a tile lie: placed anew for every tile of a
+// look-back, but along a chain only moved on.
+template <bool WALK, int PER, int N>
+struct Place {
+  const char* at[N];
+  int left;  // steps from the warp's first one to the end of the sequence; 0 on an idle lane
+  template <class F>
+  MPB_D void go(const ScanArgs& p, const Order<WALK>& o, int warp, const int64_t (&st)[N], F place_at) {
+    if (!WALK || o.chunk == 0) {
+      place_at(o, *this);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) at[k] += st[k] * p.steps;
+      left -= p.steps;
+    }
+  }
+  MPB_D int steps() const { return left < PER ? left : PER; }
+};
+
+template <class X, class G, int V, bool SHARED>
+struct FwdTile {
+  using CX = Column<X, V>;
+  using CG = Column<G, SHARED ? 1 : V>;
+  static constexpr uint32_t kG = CX::bytes(kFwd), kBytes = kG + CG::bytes(kFwd);
+  static constexpr int kStages = kRing / kBytes < 3 ? kRing / kBytes : 3;
+  static_assert(kStages >= 2, "a tile is copied while another is computed");
+};
+
+template <class X, class G, bool SIG, int V, bool SHARED, bool WALK>
+__global__ void __launch_bounds__(kWarps * 32, 2) k_gscan(ScanArgs p) {
+  using Tile = FwdTile<X, G, V, SHARED>;
+  constexpr int NST = Tile::kStages;
+  extern __shared__ __align__(16) char ring[];
+  __shared__ Shared<V> sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t base = smem_u32(ring);
+  Order<WALK> cur, ahead;
+  cur.first();
+  ahead.first();
+  if (WALK) {
+    if (p.status && blockIdx.x == 0 && threadIdx.x == 0) *p.status = MPB_OK;  // nothing waits
+  } else {
+    if (threadIdx.x < NST) sh.tiles[threadIdx.x] = atomicAdd(p.ticket, 1u);
+    __syncthreads();
+  }
+  const int64_t in_st[2] = {p.x_st * (int64_t)sizeof(X), p.g_st * (int64_t)sizeof(G)};
+  const int64_t out_st[1] = {p.D * (int64_t)sizeof(X)};
+  Place<WALK, kFwd, 2> from;
+  Place<WALK, kFwd, 1> to;
+  auto copy = [&](int it, int s) {  // the block's tile number `it` into stage s
+    if (ahead.here(p, sh.tiles, it)) {
+      from.go(p, ahead, warp, in_st, [&](const Order<WALK>& o, auto& f) {
+        const Lane l = place<V, SHARED>(p, o.chain, lane);
+        const int64_t t0 = (int64_t)o.chunk * p.steps + warp * kFwd;
+        f.at[0] = (const char*)((const X*)p.x + l.b * p.x_sb + t0 * p.x_st + l.ch);
+        f.at[1] = (const char*)((const G*)p.gate + l.b * p.g_sb + t0 * p.g_st + l.gate);
+        f.left = l.in ? (int)(p.T - t0) : 0;
+      });
+      Tile::CX::template copy<kFwd>(base + s * Tile::kBytes, from.at[0], in_st[0], from.left);
+      Tile::CG::template copy<kFwd>(base + s * Tile::kBytes + Tile::kG, from.at[1], in_st[1], from.left);
+      ahead.next(p);
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < NST - 1; ++s) copy(s, s);
+  int stage = 0;
+  Floats<V> carry = vset<V>(0.0f);
+  size_t state_at = 0;
+  uint32_t half_x = 0, half_g = 0;  // bit 1 of the addresses of single 16-bit elements at step 0
+  for (int it = 0; cur.here(p, sh.tiles, it); ++it) {
+    copy(it + NST - 1, stage == 0 ? NST - 1 : stage - 1);
+    to.go(p, cur, warp, out_st, [&](const Order<WALK>& o, auto& f) {
+      const Lane l = place<V, SHARED>(p, o.chain, lane);
+      const int64_t t0 = (int64_t)o.chunk * p.steps + warp * kFwd;
+      f.at[0] = (const char*)((const X*)p.h + (l.b * p.T + t0) * p.D + l.ch);
+      f.left = l.in ? (int)(p.T - t0) : 0;
+      state_at = (size_t)(l.b * p.D + l.ch);
+      half_x = (uint32_t)(uintptr_t)((const X*)p.x + l.b * p.x_sb + l.ch);
+      half_g = (uint32_t)(uintptr_t)((const G*)p.gate + l.b * p.g_sb + l.gate);
+      if (o.chunk == 0 || !WALK)
+#pragma unroll
+        for (int v = 0; v < V; ++v) vput(carry, v, o.chunk == 0 && l.in && p.h0 ? p.h0[state_at + v] : 0.0f);
+    });
+    const uint32_t t0 = cur.chunk * p.steps + warp * kFwd;
+    auto half = [&](uint32_t at0, int64_t st, int i) { return at0 + (t0 + i) * (uint32_t)st; };
+    uint32_t early[V];
+    if (!WALK) {
+      if (threadIdx.x == 0) sh.tiles[(it + NST) & 3] = atomicAdd(p.ticket, 1u);
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        early[v] = warp == 0 && cur.chunk > 0
+                       ? ld_word(p.states + (size_t)((cur.chunk - 1) * p.chains + cur.chain) * 32 * V + lane * V + v)
+                       : 0;
+    }
+    copies_wait<NST - 1>();
+    const char* mine = ring + stage * Tile::kBytes;
+    // Steps after the last are computed from whatever the ring holds: nothing
+    // follows them in the chain, and they are not written.
+    Floats<V> a[kFwd], b[kFwd], ma = vset<V>(1.0f), mb = vset<V>(0.0f), in;
+#pragma unroll
+    for (int i = 0; i < kFwd; ++i) {
+      const Floats<V> x = unpack(Tile::CX::get(mine, i, half(half_x, in_st[0], i)));
+      Floats<V> om;
+      gates_of<SIG, V>(Tile::CG::get(mine + Tile::kG, i, half(half_g, in_st[1], i)), a[i], om);
+      b[i] = SIG ? vmul(om, x) : x;
+      ma = vmul(ma, a[i]);
+      mb = vfma(a[i], mb, b[i]);
+    }
+    join<V, WALK>(p, sh, it & 1, cur.chain, cur.chunk, warp, lane, ma, mb, early, carry, in);
+    const int n = to.steps();
+    char* h = const_cast<char*>(to.at[0]);
+    if (__all_sync(0xffffffffu, n == kFwd)) {
+#pragma unroll
+      for (int i = 0; i < kFwd; ++i) {
+        in = vfma(a[i], in, b[i]);
+        put_global(h, pack<X>(in));
+        h = ahead_by(h, out_st[0]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kFwd; ++i)
+        if (i < n) {
+          in = vfma(a[i], in, b[i]);
+          put_global(h, pack<X>(in));
+          h = ahead_by(h, out_st[0]);
+        }
+    }
+    if (p.state && n > 0 && n == to.left)
+#pragma unroll
+      for (int v = 0; v < V; ++v) p.state[state_at + v] = vget(in, v);
+    if (WALK && blockDim.x == 32) carry = in;
+    cur.next(p);
+    stage = stage + 1 == NST ? 0 : stage + 1;
+  }
+}
+
+// Sums over the `lanes` (a power of two) neighbours of a lane of kBwd values
+// each: every round gives half of the values to the partner and takes its
+// half of the others', so 9 shuffles do for 8 values over 32 lanes. On
+// return val[0..left) of a lane are the sums of the steps first..first + left,
+// the same in the lanes that differ in bits from log2(kBwd) on.
+MPB_D void sum_over_lanes(float (&val)[kBwd], int lane, int lanes, int& first, int& left) {
+  first = 0;
+  left = kBwd;
+#pragma unroll
+  for (int half = kBwd / 2, bit = 1; half > 0; half >>= 1, bit <<= 1) {
     if (bit < lanes) {
       const bool up = lane & bit;
 #pragma unroll
@@ -320,111 +582,180 @@ MPB_D void sum_over_lanes(float (&val)[kSteps], int lane, int lanes, int& first,
     }
   }
 #pragma unroll
-  for (int bit = kSteps; bit < 32; bit <<= 1)
+  for (int bit = kBwd; bit < 32; bit <<= 1)
     if (bit < lanes) val[0] += __shfl_xor_sync(0xffffffffu, val[0], bit);
 }
 
 template <class X, class G, bool SIG, int V, bool SHARED>
+struct BwdTile {
+  using CX = Column<X, V>;
+  using CG = Column<G, SHARED ? 1 : V>;
+  static constexpr uint32_t kH = CX::bytes(kBwd), kX = 2 * kH, kG = SIG ? 3 * kH : kX, kBytes = kG + CG::bytes(kBwd);
+  static constexpr int kStages = kRing / kBytes < 3 ? kRing / kBytes : 3;
+  static_assert(kStages >= 2, "a tile is copied while another is computed");
+};
+
+// As k_gscan, from the last step to the first. The gate is taken from shared
+// memory twice rather than kept (backward moves twice the bytes per element,
+// so the second exponential fits beside them).
+template <class X, class G, bool SIG, int V, bool SHARED, bool WALK>
 __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd(ScanArgs p) {
-  using XP = Pack<X, V>;
-  using GP = Pack<G, SHARED ? 1 : V>;
+  using Tile = BwdTile<X, G, SIG, V, SHARED>;
+  constexpr int NST = Tile::kStages;
+  extern __shared__ __align__(16) char ring[];
+  __shared__ Shared<V> sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t chain, chunk;
-  take_tile(p, chain, chunk);
-  const Lane l = place<V, SHARED>(p, chain, lane);
-  const int64_t r0 = (int64_t)chunk * p.steps + warp * kSteps;  // steps counted from the end
-  const int64_t t0 = p.T - 1 - r0;
-  const int n = l.in ? (int)(p.T - r0 < kSteps ? p.T - r0 : kSteps) : 0;
-  const X* dh = (const X*)p.dh + l.b * p.dh_sb + t0 * p.dh_st + l.ch;
-  const X* x = (const X*)p.x + l.b * p.x_sb + t0 * p.x_st + l.ch;
-  const X* hs = (const X*)p.hsaved + l.b * p.h_sb + (t0 - 1) * p.h_st + l.ch;
-  const G* g = (const G*)p.gate + l.b * p.g_sb + t0 * p.g_st + l.gate;
-  XP dw[kSteps], xw[kSteps], hw[kSteps];
-  GP gw[kSteps];
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i)
-    if (i < n) {
-      dw[i].w = *reinterpret_cast<const typename XP::W*>(dh - i * p.dh_st);
-      gw[i].w = *reinterpret_cast<const typename GP::W*>(g - i * p.g_st);
-    }
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i)
-    if (i < n) {
-      if (SIG) xw[i].w = *reinterpret_cast<const typename XP::W*>(x - i * p.x_st);
-      if (t0 - i > 0) hw[i].w = *reinterpret_cast<const typename XP::W*>(hs - i * p.h_st);
-    }
-  float carry[V], ma[V], mb[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    carry[v] = l.in && p.dstate ? p.dstate[l.b * p.D + l.ch + v] : 0.0f;
-    ma[v] = 1.0f;
-    mb[v] = 0.0f;
+  const uint32_t base = smem_u32(ring);
+  Order<WALK> cur, ahead;
+  cur.first();
+  ahead.first();
+  if (WALK) {
+    if (p.status && blockIdx.x == 0 && threadIdx.x == 0) *p.status = MPB_OK;  // nothing waits
+  } else {
+    if (threadIdx.x < NST) sh.tiles[threadIdx.x] = atomicAdd(p.ticket, 1u);
+    __syncthreads();
   }
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i)
-    if (i < n)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float a, om;
-        gate_of<G, SIG>(gw[i].v[SHARED ? 0 : v], a, om);
-        ma[v] *= a;
-        mb[v] = a * (mb[v] + to_f(dw[i].v[v]));
-      }
-  join<V>(p, chain, chunk, warp, lane, ma, mb, carry);
-  X* dx = (X*)p.dx + (l.b * p.T + t0) * p.D + l.ch;
-  G* dg = (G*)p.dgate + (l.b * p.T + t0) * p.H + l.gate;
-  float sum[kSteps];
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    sum[i] = 0.0f;
-    if (i < n) {
-      XP out;
-      GP gout;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float a, om;
-        gate_of<G, SIG>(gw[i].v[SHARED ? 0 : v], a, om);
-        const float s = to_f(dw[i].v[v]) + carry[v];
-        float low = t0 - i > 0 ? to_f(hw[i].v[v]) : (p.h0 ? p.h0[l.b * p.D + l.ch + v] : 0.0f);
-        if (SIG) low -= to_f(xw[i].v[v]);
-        out.v[v] = Cvt<X>::from(SIG ? om * s : s);
-        if (SHARED) {
-          sum[i] = fmaf(s, low, sum[i]);
-        } else {
-          gout.v[v] = Cvt<G>::from(SIG ? s * low * (a * om) : s * low);
-        }
-        carry[v] = a * s;
-      }
-      *reinterpret_cast<typename XP::W*>(dx - i * p.D) = out.w;
-      if (!SHARED) *reinterpret_cast<typename GP::W*>(dg - i * p.H) = gout.w;
+  const int64_t in_st[4] = {-p.dh_st * (int64_t)sizeof(X), -p.h_st * (int64_t)sizeof(X), -p.x_st * (int64_t)sizeof(X),
+                            -p.g_st * (int64_t)sizeof(G)};
+  const int64_t out_st[2] = {-p.D * (int64_t)sizeof(X), -p.H * (int64_t)sizeof(G)};
+  Place<WALK, kBwd, 4> from;
+  Place<WALK, kBwd, 2> to;
+  auto copy = [&](int it, int s) {  // the block's tile number `it` into stage s
+    if (ahead.here(p, sh.tiles, it)) {
+      from.go(p, ahead, warp, in_st, [&](const Order<WALK>& o, auto& f) {
+        const Lane l = place<V, SHARED>(p, o.chain, lane);
+        const int64_t r0 = (int64_t)o.chunk * p.steps + warp * kBwd, t0 = p.T - 1 - r0;
+        f.at[0] = (const char*)((const X*)p.dh + l.b * p.dh_sb + t0 * p.dh_st + l.ch);
+        f.at[1] = (const char*)((const X*)p.hsaved + l.b * p.h_sb + (t0 - 1) * p.h_st + l.ch);
+        f.at[2] = (const char*)((const X*)p.x + l.b * p.x_sb + t0 * p.x_st + l.ch);
+        f.at[3] = (const char*)((const G*)p.gate + l.b * p.g_sb + t0 * p.g_st + l.gate);
+        f.left = l.in ? (int)(p.T - r0) : 0;
+      });
+      const uint32_t q = base + s * Tile::kBytes;
+      Tile::CX::template copy<kBwd>(q, from.at[0], in_st[0], from.left);
+      Tile::CX::template copy<kBwd>(q + Tile::kH, from.at[1], in_st[1], from.left - 1);  // h[-1] is h0
+      if (SIG) Tile::CX::template copy<kBwd>(q + Tile::kX, from.at[2], in_st[2], from.left);
+      Tile::CG::template copy<kBwd>(q + Tile::kG, from.at[3], in_st[3], from.left);
+      ahead.next(p);
     }
-  }
-  if (p.dh0 && n > 0 && r0 + n == p.T)
+    copies_commit();
+  };
 #pragma unroll
-    for (int v = 0; v < V; ++v) p.dh0[l.b * p.D + l.ch + v] = carry[v];
-  if (!SHARED) return;
-  // a head's lanes: a power of two of them, or the whole warp (idle lanes add zeros)
-  const int lanes = p.heads_per > 1 ? (int)p.lanes_per : 32;
-  int first, left;
-  sum_over_lanes(sum, lane, lanes, first, left);
-  // lanes that hold the same sums: the one with the upper bits clear writes
-  const int at = p.heads_per > 1 ? lane & (lanes - 1) : lane;
-  const uint32_t group = chain - (uint32_t)l.b * p.groups;
-  const int64_t head = p.groups_per > 1 ? (int64_t)p.by_groups_per.div(group)
-                                        : (int64_t)group * p.heads_per + (p.heads_per > 1 ? lane / lanes : 0);
-  if (at >= kSteps || head >= p.H) return;
-  const int64_t bt = (int64_t)p.by_groups.div(chain) * p.T;
+  for (int s = 0; s < NST - 1; ++s) copy(s, s);
+  int stage = 0;
+  Floats<V> carry = vset<V>(0.0f);
+  size_t state_at = 0;
+  uint32_t half0[4] = {};  // bit 1 of the addresses of single 16-bit elements at the sequence's last step
+  for (int it = 0; cur.here(p, sh.tiles, it); ++it) {
+    copy(it + NST - 1, stage == 0 ? NST - 1 : stage - 1);
+    to.go(p, cur, warp, out_st, [&](const Order<WALK>& o, auto& f) {
+      const Lane l = place<V, SHARED>(p, o.chain, lane);
+      const int64_t r0 = (int64_t)o.chunk * p.steps + warp * kBwd, t0 = p.T - 1 - r0;
+      f.at[0] = (const char*)((const X*)p.dx + (l.b * p.T + t0) * p.D + l.ch);
+      f.at[1] = (const char*)((const G*)p.dgate + (l.b * p.T + t0) * p.H + l.gate);
+      f.left = l.in ? (int)(p.T - r0) : 0;
+      state_at = (size_t)(l.b * p.D + l.ch);
+      half0[0] = (uint32_t)(uintptr_t)((const X*)p.dh + l.b * p.dh_sb + (p.T - 1) * p.dh_st + l.ch);
+      half0[1] = (uint32_t)(uintptr_t)((const X*)p.hsaved + l.b * p.h_sb + (p.T - 2) * p.h_st + l.ch);
+      half0[2] = (uint32_t)(uintptr_t)((const X*)p.x + l.b * p.x_sb + (p.T - 1) * p.x_st + l.ch);
+      half0[3] = (uint32_t)(uintptr_t)((const G*)p.gate + l.b * p.g_sb + (p.T - 1) * p.g_st + l.gate);
+      if (o.chunk == 0 || !WALK)
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int64_t t = t0 - (first + i);
-    if (i >= left || t < 0 || r0 + first + i >= p.T) continue;
-    if (p.groups_per > 1) {
-      p.part[((bt + t) * p.H + head) * p.groups_per + (group - (uint32_t)head * p.groups_per)] = sum[i];
+        for (int v = 0; v < V; ++v) vput(carry, v, o.chunk == 0 && l.in && p.dstate ? p.dstate[state_at + v] : 0.0f);
+    });
+    const uint32_t r0 = cur.chunk * p.steps + warp * kBwd;  // steps counted from the end
+    auto half = [&](int k, int i) { return half0[k] + (r0 + i) * (uint32_t)in_st[k]; };
+    uint32_t early[V];
+    if (!WALK) {
+      if (threadIdx.x == 0) sh.tiles[(it + NST) & 3] = atomicAdd(p.ticket, 1u);
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        early[v] = warp == 0 && cur.chunk > 0
+                       ? ld_word(p.states + (size_t)((cur.chunk - 1) * p.chains + cur.chain) * 32 * V + lane * V + v)
+                       : 0;
+    }
+    copies_wait<NST - 1>();
+    const char* mine = ring + stage * Tile::kBytes;
+    Floats<V> ma = vset<V>(1.0f), mb = vset<V>(0.0f), in;
+    auto gate_at = [&](int i, Floats<V>& a, Floats<V>& om) {
+      gates_of<SIG, V>(Tile::CG::get(mine + Tile::kG, i, half(3, i)), a, om);
+    };
+#pragma unroll
+    for (int i = 0; i < kBwd; ++i) {
+      Floats<V> a, om;
+      gate_at(i, a, om);
+      ma = vmul(ma, a);
+      mb = vmul(a, vadd(mb, unpack(Tile::CX::get(mine, i, half(0, i)))));
+    }
+    join<V, WALK>(p, sh, it & 1, cur.chain, cur.chunk, warp, lane, ma, mb, early, carry, in);
+    const int n = to.steps();
+    char *dx = const_cast<char*>(to.at[0]), *dg = const_cast<char*>(to.at[1]);
+    float sum[kBwd];
+    auto step = [&](int i, Floats<V> low) {  // low: h[t - 1]
+      Floats<V> a, om;
+      gate_at(i, a, om);
+      const Floats<V> s = vadd(unpack(Tile::CX::get(mine, i, half(0, i))), in);
+      if constexpr (SIG) low = vfma(unpack(Tile::CX::get(mine + Tile::kX, i, half(2, i))), vset<V>(-1.0f), low);
+      put_global(dx, pack<X>(SIG ? vmul(om, s) : s));
+      dx = ahead_by(dx, out_st[0]);
+      in = vmul(a, s);
+      const Floats<V> da = vmul(s, low);
+      if constexpr (SHARED) {
+        sum[i] = V == 2 ? vget(da, 0) + vget(da, 1) : vget(da, 0);
+      } else {
+        put_global(dg, pack<G>(SIG ? vmul(da, vmul(a, om)) : da));
+        dg = ahead_by(dg, out_st[1]);
+      }
+    };
+    if (__all_sync(0xffffffffu, to.left > kBwd)) {
+#pragma unroll
+      for (int i = 0; i < kBwd; ++i) step(i, unpack(Tile::CX::get(mine + Tile::kH, i, half(1, i))));
     } else {
-      float a, om;
-      gate_of<G, SIG>(((const G*)p.gate)[(int64_t)p.by_groups.div(chain) * p.g_sb + t * p.g_st + head], a, om);
-      ((G*)p.dgate)[(bt + t) * p.H + head] = Cvt<G>::from(SIG ? sum[i] * (a * om) : sum[i]);
+#pragma unroll
+      for (int i = 0; i < kBwd; ++i) {
+        sum[i] = 0.0f;
+        if (i < n) {
+          Floats<V> low = unpack(Tile::CX::get(mine + Tile::kH, i, half(1, i)));
+          if (to.left - 1 == i)  // the first step of the sequence
+#pragma unroll
+            for (int v = 0; v < V; ++v) vput(low, v, p.h0 ? p.h0[state_at + v] : 0.0f);
+          step(i, low);
+        }
+      }
     }
+    if (p.dh0 && n > 0 && n == to.left)
+#pragma unroll
+      for (int v = 0; v < V; ++v) p.dh0[state_at + v] = vget(in, v);
+    if (SHARED) {
+      // a head's lanes: a power of two of them, or the whole warp (idle lanes add zeros)
+      const int lanes = p.heads_per > 1 ? (int)p.lanes_per : 32;
+      int first, left;
+      sum_over_lanes(sum, lane, lanes, first, left);
+      // of the lanes that hold the same sums the one with the upper bits clear writes
+      const int at = p.heads_per > 1 ? lane & (lanes - 1) : lane;
+      const uint32_t b = p.by_groups.div(cur.chain), group = cur.chain - b * p.groups;
+      const int64_t head = p.groups_per > 1 ? (int64_t)p.by_groups_per.div(group)
+                                            : (int64_t)group * p.heads_per + (p.heads_per > 1 ? lane / lanes : 0);
+      if (at < kBwd && head < p.H) {
+        const int64_t bt = (int64_t)b * p.T;
+#pragma unroll
+        for (int i = 0; i < kBwd; ++i) {
+          const int64_t t = p.T - 1 - (int64_t)r0 - (first + i);
+          if (i < left && t >= 0) {
+            if (p.groups_per > 1) {
+              p.part[((bt + t) * p.H + head) * p.groups_per + (group - (uint32_t)head * p.groups_per)] = sum[i];
+            } else {
+              float a, om;
+              gate_of<SIG>(to_f(((const G*)p.gate)[(int64_t)b * p.g_sb + t * p.g_st + head]), a, om);
+              ((G*)p.dgate)[(bt + t) * p.H + head] = Cvt<G>::from(SIG ? sum[i] * (a * om) : sum[i]);
+            }
+          }
+        }
+      }
+    }
+    if (WALK && blockDim.x == 32) carry = in;
+    cur.next(p);
+    stage = stage + 1 == NST ? 0 : stage + 1;
   }
 }
 
@@ -437,7 +768,7 @@ __global__ void __launch_bounds__(256) k_gscan_heads(ScanArgs p) {
   float s = 0.0f;
   for (uint32_t k = 0; k < p.groups_per; ++k) s += p.part[i * p.groups_per + k];
   float a, om;
-  gate_of<G, SIG>(((const G*)p.gate)[b * p.g_sb + t * p.g_st + head], a, om);
+  gate_of<SIG>(to_f(((const G*)p.gate)[b * p.g_sb + t * p.g_st + head]), a, om);
   ((G*)p.dgate)[i] = Cvt<G>::from(SIG ? s * (a * om) : s);
 }
 
@@ -456,21 +787,20 @@ __global__ void __launch_bounds__(256) k_gscan_step(ScanArgs p, FastDiv by_d, Fa
   by_d.divmod(blockIdx.x * 256 + threadIdx.x, b, d);
   if (b >= p.B) return;
   d *= V;
-  XP xw, out;
+  XP xw;
   GP gw;
   xw.w = *reinterpret_cast<const typename XP::W*>((const X*)p.x + b * p.x_sb + d);
   gw.w = *reinterpret_cast<const typename GP::W*>((const G*)p.gate + b * p.g_sb + (SHARED ? by_p.div(d) : d));
   float* s = p.state + b * p.D + d;
+  Floats<V> h, a, om;
+  const Floats<V> x = unpack(xw);
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    float a, om;
-    gate_of<G, SIG>(gw.v[SHARED ? 0 : v], a, om);
-    const float x = to_f(xw.v[v]);
-    const float h = fmaf(a, s[v], SIG ? om * x : x);
-    s[v] = h;
-    out.v[v] = Cvt<X>::from(h);
-  }
-  *reinterpret_cast<typename XP::W*>((X*)p.h + b * p.D + d) = out.w;
+  for (int v = 0; v < V; ++v) vput(h, v, s[v]);
+  gates_of<SIG, V>(gw, a, om);
+  h = vfma(a, h, SIG ? vmul(om, x) : x);
+#pragma unroll
+  for (int v = 0; v < V; ++v) s[v] = vget(h, v);
+  *reinterpret_cast<typename XP::W*>((X*)p.h + b * p.D + d) = pack<X>(h).w;
 }
 
 // ------------------------------------------------------------------- host
@@ -489,8 +819,13 @@ bool pairs(const ScanArgs& p, int x_dt, int g_dt, bool backward) {
   return ok;
 }
 
-// The channel groups and tiles for V channels per lane.
-void lay_out(ScanArgs& p, int V) {
+// From this many chains on a block walks a chain: a block per SM. 256 chains
+// ((8, 4096, 2048) bf16) take 112 us walked and 143 us by look-back; 32 ((1, 65536,
+// 1000) f32) take 960 us walked and 696 us by look-back.
+constexpr uint32_t kWalkFrom = 148;
+
+// The channel groups and tiles for V channels per lane and `per` steps per warp.
+void lay_out(ScanArgs& p, int V, int per) {
   const int64_t C = 32 * V;
   if (p.H == p.D) {
     p.groups = (uint32_t)((p.D + C - 1) / C);
@@ -503,10 +838,11 @@ void lay_out(ScanArgs& p, int V) {
     p.heads_per = (lanes & (lanes - 1)) == 0 && lanes < 32 ? (uint32_t)(32 / lanes) : 1;
     p.groups = (uint32_t)(p.groups_per > 1 ? p.H * p.groups_per : (p.H + p.heads_per - 1) / p.heads_per);
   }
-  const int64_t warps = (p.T + kSteps - 1) / kSteps;
-  p.steps = (int)(warps < kWarps ? warps : kWarps) * kSteps;
+  const int64_t warps = (p.T + per - 1) / per;
+  p.steps = (int)(warps < kWarps ? warps : kWarps) * per;
   p.chains = (uint32_t)(p.B * p.groups);
   p.chunks = (uint32_t)((p.T + p.steps - 1) / p.steps);
+  p.walk = p.chunks == 1 || p.chains >= kWalkFrom;
   p.by_groups = FastDiv(p.groups);
   p.by_groups_per = FastDiv(p.groups_per);
   p.by_lanes_per = FastDiv(p.lanes_per);
@@ -515,34 +851,31 @@ void lay_out(ScanArgs& p, int V) {
 
 size_t align16(size_t n) { return (n + 15) & ~(size_t)15; }
 
-// Scratch: {ticket, status}, flags (cleared by the call), maps and states of the tiles, sums of wide heads.
+// Scratch: {ticket, status}, states and maps of the tiles (cleared by the call), sums of wide heads.
 size_t scratch_of(ScanArgs& p, int V, bool backward, void* base, size_t* cleared) {
-  size_t at = 0;
+  size_t at = 16;
   char* q = (char*)base;
   *cleared = 0;
-  if (p.chunks > 1) {
-    const size_t tiles = (size_t)p.chains * p.chunks, data = align16(tiles * 32 * V * sizeof(float));
+  if (!p.walk) {
+    const size_t words = (size_t)p.chains * p.chunks * 32 * V;
     p.ticket = (uint32_t*)q;
     p.status = (uint32_t*)(q + 4);
-    p.flags = (uint32_t*)(q + 16);
-    at = *cleared = align16(16 + tiles * sizeof(uint32_t));
-    p.map_a = (float*)(q + at);
-    p.map_b = (float*)(q + at + data);
-    p.out_state = (float*)(q + at + 2 * data);
-    at += 3 * data;
+    p.maps = (uint64_t*)(q + 16);
+    p.states = (uint32_t*)(q + 16 + words * 8);
+    at = *cleared = align16(16 + words * 12);
   }
   if (backward && p.groups_per > 1) {
     p.part = (float*)(q + at);
     at += align16((size_t)(p.B * p.T * p.H) * p.groups_per * sizeof(float));
   }
-  return at;
+  return at > 16 ? at : 0;
 }
 
 // Enough for either V: the choice needs addresses and strides.
 size_t scratch_need(ScanArgs p, bool backward) {
   size_t most = 0, cleared;
   for (int V = 1; V <= 2; ++V) {
-    lay_out(p, V);
+    lay_out(p, V, backward ? kBwd : kFwd);
     const size_t n = scratch_of(p, V, backward, nullptr, &cleared);
     most = n > most ? n : most;
   }
@@ -550,44 +883,60 @@ size_t scratch_need(ScanArgs p, bool backward) {
 }
 
 int prepare(const char* what, ScanArgs& p, int V, bool backward, void* scratch, cudaStream_t s) {
-  lay_out(p, V);
+  lay_out(p, V, backward ? kBwd : kFwd);
   size_t cleared;
+  if (scratch_need(p, backward)) p.status = (uint32_t*)((char*)scratch + 4);
   scratch_of(p, V, backward, scratch, &cleared);
   if (cleared) return cuda_check(cudaMemsetAsync(scratch, 0, cleared, s), what);
   return MPB_OK;
 }
 
+// The block's shared memory for tiles under way needs the opt-in above 48 KB, once per kernel and device.
+template <auto kernel>
+int launch_tiles(const char* what, const ScanArgs& p, int per, int smem, cudaStream_t s) {
+  static bool set[64] = {};
+  int dev = 0;
+  if (int rc = cuda_check(cudaGetDevice(&dev), what)) return rc;
+  if (dev < 0 || dev >= 64 || !set[dev]) {
+    if (int rc = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what)) return rc;
+    if (dev >= 0 && dev < 64) set[dev] = true;
+  }
+  const uint32_t most = (uint32_t)sm_count() * 2, tiles = p.walk ? p.chains : p.chains * p.chunks;
+  kernel<<<tiles < most ? tiles : most, (unsigned)(p.steps / per) * 32, smem, s>>>(p);
+  return launch_check(what);
+}
+
+template <class X, class G, bool SIG, int V, bool SHARED>
+int launch_fwd_v(const ScanArgs& p, cudaStream_t s) {
+  using Tile = FwdTile<X, G, V, SHARED>;
+  constexpr int smem = Tile::kStages * Tile::kBytes;
+  return p.walk ? launch_tiles<k_gscan<X, G, SIG, V, SHARED, true>>("gated_scan", p, kFwd, smem, s)
+                : launch_tiles<k_gscan<X, G, SIG, V, SHARED, false>>("gated_scan", p, kFwd, smem, s);
+}
+
+template <class X, class G, bool SIG, int V, bool SHARED>
+int launch_bwd_v(const ScanArgs& p, cudaStream_t s) {
+  using Tile = BwdTile<X, G, SIG, V, SHARED>;
+  constexpr int smem = Tile::kStages * Tile::kBytes;
+  return p.walk ? launch_tiles<k_gscan_bwd<X, G, SIG, V, SHARED, true>>("gated_scan_backward", p, kBwd, smem, s)
+                : launch_tiles<k_gscan_bwd<X, G, SIG, V, SHARED, false>>("gated_scan_backward", p, kBwd, smem, s);
+}
+
 template <class X, class G, bool SIG>
 int launch_fwd(ScanArgs& p, int V, void* scratch, cudaStream_t s) {
   if (int rc = prepare("gated_scan", p, V, false, scratch, s)) return rc;
-  const unsigned grid = p.chains * p.chunks, block = (unsigned)p.steps / kSteps * 32;
-  const bool shared = p.H != p.D;
   constexpr int W = sizeof(X) == 2 ? 2 : 1;
-  if (V == 2) {
-    if (shared) k_gscan<X, G, SIG, W, true><<<grid, block, 0, s>>>(p);
-    else k_gscan<X, G, SIG, W, false><<<grid, block, 0, s>>>(p);
-  } else {
-    if (shared) k_gscan<X, G, SIG, 1, true><<<grid, block, 0, s>>>(p);
-    else k_gscan<X, G, SIG, 1, false><<<grid, block, 0, s>>>(p);
-  }
-  return launch_check("gated_scan");
+  if (p.H != p.D) return V == 2 ? launch_fwd_v<X, G, SIG, W, true>(p, s) : launch_fwd_v<X, G, SIG, 1, true>(p, s);
+  return V == 2 ? launch_fwd_v<X, G, SIG, W, false>(p, s) : launch_fwd_v<X, G, SIG, 1, false>(p, s);
 }
 
 template <class X, class G, bool SIG>
 int launch_bwd(ScanArgs& p, int V, void* scratch, cudaStream_t s) {
   if (int rc = prepare("gated_scan_backward", p, V, true, scratch, s)) return rc;
-  const unsigned grid = p.chains * p.chunks, block = (unsigned)p.steps / kSteps * 32;
-  const bool shared = p.H != p.D;
   constexpr int W = sizeof(X) == 2 ? 2 : 1;
-  if (V == 2) {
-    if (shared) k_gscan_bwd<X, G, SIG, W, true><<<grid, block, 0, s>>>(p);
-    else k_gscan_bwd<X, G, SIG, W, false><<<grid, block, 0, s>>>(p);
-  } else {
-    if (shared) k_gscan_bwd<X, G, SIG, 1, true><<<grid, block, 0, s>>>(p);
-    else k_gscan_bwd<X, G, SIG, 1, false><<<grid, block, 0, s>>>(p);
-  }
-  if (int rc = launch_check("gated_scan_backward")) return rc;
-  if (!shared || p.groups_per == 1) return MPB_OK;
+  if (p.H == p.D) return V == 2 ? launch_bwd_v<X, G, SIG, W, false>(p, s) : launch_bwd_v<X, G, SIG, 1, false>(p, s);
+  if (int rc = V == 2 ? launch_bwd_v<X, G, SIG, W, true>(p, s) : launch_bwd_v<X, G, SIG, 1, true>(p, s)) return rc;
+  if (p.groups_per == 1) return MPB_OK;
   k_gscan_heads<G, SIG><<<(unsigned)((p.B * p.T * p.H + 255) / 256), 256, 0, s>>>(p);
   return launch_check("gated_scan_backward");
 }
@@ -638,7 +987,7 @@ int check_sizes(const char* what, int64_t B, int64_t T, int64_t D, int64_t H) {
   if (D > 0 && (H < 1 || D % H != 0))
     return fail(MPB_ERR_SHAPE, "%s: %lld gates do not divide %lld channels", what, (long long)H, (long long)D);
   // tiles are counted in 32 bits (at 16 steps of one warp the least a tile covers)
-  if (B > 0x7fffffff || T > (int64_t)1 << 40 || D > 0x7fffffff ||
+  if (B > 0x7fffffff || T > 0x7ff00000 || D > 0x7fffffff ||
       (double)B * (double)(D + 32) * ((double)T / 128 + 1) > 2.0e9)
     return fail(MPB_ERR_SHAPE, "%s: (%lld, %lld, %lld) is too large", what, (long long)B, (long long)T, (long long)D);
   return MPB_OK;
@@ -724,10 +1073,10 @@ int mpb_gated_scan_step(int64_t B, int64_t D, int64_t H, const void* x, int x_dt
   });
 }
 
-int mpb_gated_scan_status(const void* scratch, int64_t T, mpb_stream_t stream) {
+int mpb_gated_scan_status(const void* scratch, mpb_stream_t stream) {
   uint32_t status = 0;
   cudaStream_t s = (cudaStream_t)stream;
-  if (!scratch || T <= kWarps * kSteps) return MPB_OK;  // one tile per chain: nothing waits
+  if (!scratch) return MPB_OK;
   if (int rc = cuda_check(cudaMemcpyAsync(&status, (const char*)scratch + 4, 4, cudaMemcpyDeviceToHost, s), "gated_scan_status"))
     return rc;
   if (int rc = cuda_check(cudaStreamSynchronize(s), "gated_scan_status")) return rc;
