@@ -27,19 +27,18 @@ struct Eight {
   MPB_D Eight() {}
 };
 
-// Each element's 16-bit half is compared with the threshold; what stays is
-// scaled in float and rounded once.
+// What stays is scaled in float and rounded once.
 template <class T>
 MPB_D void drop_eight(Eight<T>& x, const uint4& w, const Dropper& d) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float v = to_f(x.v[j]) * d.up;
-    x.v[j] = Cvt<T>::from(half_of(w, j) >= d.drop ? v : 0.0f);
+    x.v[j] = Cvt<T>::from(stays(d, w, j) ? v : 0.0f);
   }
 }
 
 template <class T>
-__global__ void __launch_bounds__(kThreads) k_dropout(const T* __restrict__ x, T* __restrict__ y, int64_t n,
+__global__ void __launch_bounds__(kThreads, 6) k_dropout(const T* __restrict__ x, T* __restrict__ y, int64_t n,
                                                       Dropper d) {
   const int64_t whole = n / 8, stride = (int64_t)gridDim.x * kThreads;
   const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
@@ -74,7 +73,7 @@ __global__ void __launch_bounds__(kThreads) k_dropout_any(const T* __restrict__ 
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int64_t i = b * 8 + j;
-      if (i < n) y[i] = half_of(w, j) >= d.drop ? Cvt<T>::from(to_f(x[i]) * d.up) : Cvt<T>::from(0.0f);
+      if (i < n) y[i] = stays(d, w, j) ? Cvt<T>::from(to_f(x[i]) * d.up) : Cvt<T>::from(0.0f);
     }
   }
 }
@@ -83,6 +82,7 @@ template <class T>
 int launch_dropout(const void* x, void* y, int64_t n, const Dropper& d, cudaStream_t s) {
   const int64_t want = ((n + 7) / 8 + kThreads - 1) / kThreads, cap = (int64_t)sm_count() * 64;
   const unsigned grid = (unsigned)(want < cap ? want : cap);
+  if (d.all) return cuda_check(cudaMemsetAsync(y, 0, (size_t)n * sizeof(T), s), "dropout");
   if (((uintptr_t)x | (uintptr_t)y) % 16 == 0) k_dropout<T><<<grid, kThreads, 0, s>>>((const T*)x, (T*)y, n, d);
   else k_dropout_any<T><<<grid, kThreads, 0, s>>>((const T*)x, (T*)y, n, d);
   return launch_check("dropout");

@@ -19,8 +19,9 @@ namespace mpb {
 
 struct Dropper {
   uint32_t k0, k1, c2, c3;  // key (seed) and upper counter words (offset)
-  uint32_t drop;            // dropped when the 16 bits are below this (0..65536)
+  uint32_t drop;            // dropped when the 16 bits, as the upper half of a word, are below this
   float up;                 // factor of what is kept
+  int all;                  // everything is dropped
 };
 
 // floor(p * 65536 + 1/2); what is kept is multiplied by 65536 / (65536 - drop).
@@ -30,8 +31,10 @@ inline Dropper make_dropper(double p, uint64_t seed, uint64_t offset) {
   d.k1 = (uint32_t)(seed >> 32);
   d.c2 = (uint32_t)offset;
   d.c3 = (uint32_t)(offset >> 32);
-  d.drop = (uint32_t)(p * 65536.0 + 0.5);
-  d.up = d.drop >= 65536u ? 0.0f : (float)(65536.0 / (65536.0 - (double)d.drop));
+  const uint32_t k = (uint32_t)(p * 65536.0 + 0.5);
+  d.all = k >= 65536u;
+  d.drop = d.all ? 0u : k << 16;
+  d.up = d.all ? 0.0f : (float)(65536.0 / (65536.0 - (double)k));
   return d;
 }
 
@@ -51,13 +54,15 @@ MPB_D uint4 philox(const Dropper& d, uint64_t block) {
   return make_uint4(c0, c1, c2, c3);
 }
 
-// 16-bit half number j (0..7) of the words.
-MPB_D uint32_t half_of(const uint4& w, int j) {
+// Whether element j (0..7) of a counter's words stays: its half against the
+// threshold. The upper half of a word needs no shift, as the lower bits do not
+// change whether the word reaches drop << 16.
+MPB_D bool stays(const Dropper& d, const uint4& w, int j) {
   const uint32_t v = j < 4 ? (j < 2 ? w.x : w.y) : (j < 6 ? w.z : w.w);
-  return (j & 1) ? v >> 16 : v & 0xffffu;
+  return ((j & 1) ? v : v << 16) >= d.drop;
 }
 
-// One element: its factor, 0 or d.up.
-MPB_D bool keeps(const Dropper& d, uint64_t i) { return half_of(philox(d, i >> 3), (int)(i & 7)) >= d.drop; }
+// Element i alone.
+MPB_D bool keeps(const Dropper& d, uint64_t i) { return stays(d, philox(d, i >> 3), (int)(i & 7)); }
 
 }  // namespace mpb

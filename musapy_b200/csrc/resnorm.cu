@@ -18,6 +18,13 @@
 // y). The backward pass takes y as it was stored and r_z, r_y as the forward
 // pass left them.
 //
+// A row lives in the registers of its threads (a warp or several, up to 512
+// threads with 32 elements each) between its reductions, so every input is
+// read once and every output written once. In the backward pass blocks take
+// rows in turn and add the weights' gradients up in shared memory, each thread
+// its own columns; a second kernel adds the blocks' sums in a fixed order.
+// Rows too long for that (above 16384 elements) are read again for each pass.
+//
 // Bound: memory.
 #include "common.cuh"
 #include "internal.h"
@@ -43,7 +50,10 @@ struct NormArgs {
   int dropping;
 };
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;     // a row longer than kInRegisters
+constexpr int kRowThreads = 512;  // of a row in registers, at most
+constexpr int kPerThread = 32;    // its elements per thread, at most
+constexpr int64_t kInRegisters = (int64_t)kRowThreads * kPerThread;
 
 MPB_D void act_of(int act, float g, float& v, float& slope) {
   if (act == MPB_ACT_LINEAR) {
@@ -70,6 +80,7 @@ MPB_D float gate_at(const NormArgs& p, int64_t r, int64_t c) {
 
 MPB_D float branch_factor(const NormArgs& p, int64_t r, int64_t c) {
   if (!p.dropping) return p.scale;
+  if (p.drop.all) return 0.0f;
   return keeps(p.drop, (uint64_t)(r * p.D + c)) ? p.scale * p.drop.up : 0.0f;
 }
 
@@ -87,9 +98,9 @@ MPB_D float stream_at(const NormArgs& p, int64_t r, int64_t c, float rz) {
   return y;
 }
 
-// One block per row.
+// Long rows, one block per row.
 template <class T>
-__global__ void __launch_bounds__(kThreads) k_norm_fwd(NormArgs p) {
+__global__ void __launch_bounds__(kThreads) k_norm_long(NormArgs p) {
   __shared__ float red[2][32];
   const int64_t r = blockIdx.x;
   float rz = 0.0f;
@@ -116,9 +127,9 @@ __global__ void __launch_bounds__(kThreads) k_norm_fwd(NormArgs p) {
   }
 }
 
-// One block per row: the row's gradients.
+// Long rows, one block per row: the row's gradients.
 template <class T>
-__global__ void __launch_bounds__(kThreads) k_norm_bwd(NormArgs p) {
+__global__ void __launch_bounds__(kThreads) k_norm_bwd_long(NormArgs p) {
   __shared__ float red[3][32];
   const int64_t r = blockIdx.x;
   const float rz = p.z ? p.rstd[r] : 0.0f, ry = p.rstd[(p.z ? p.R : 0) + r];
@@ -166,7 +177,7 @@ __global__ void __launch_bounds__(kThreads) k_norm_bwd(NormArgs p) {
 // One thread per column: the gradients of the weights and of a gate per channel. dx is read back
 // from where the row kernel left it.
 template <class T>
-__global__ void k_norm_bwd_cols(NormArgs p) {
+__global__ void k_norm_bwd_long_cols(NormArgs p) {
   const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (c >= p.D) return;
   float wpre = 0.0f, wpost = 0.0f, dgc = 0.0f;
@@ -190,7 +201,7 @@ __global__ void k_norm_bwd_cols(NormArgs p) {
 
 // dx in float for the column kernel.
 template <class T>
-__global__ void __launch_bounds__(kThreads) k_norm_bwd_dx(NormArgs p) {
+__global__ void __launch_bounds__(kThreads) k_norm_bwd_long_dx(NormArgs p) {
   __shared__ float red[32];
   const int64_t r = blockIdx.x;
   const float ry = p.rstd[(p.z ? p.R : 0) + r];
@@ -206,24 +217,519 @@ __global__ void __launch_bounds__(kThreads) k_norm_bwd_dx(NormArgs p) {
   }
 }
 
+// ------------------------------------------------------- rows in registers
+// W elements of T, one or two words of at most 16 bytes, worked on as pairs of
+// floats (W == 1: as single ones).
+template <class T, int W>
+struct Elems {
+  static constexpr int kBytes = (int)sizeof(T) * W, kWordBytes = kBytes > 16 ? 16 : kBytes, kWords = kBytes / kWordBytes;
+  static constexpr int kPer = W % 2 == 0 ? 2 : 1, kParts = W / kPer;
+  using F = Floats<kPer>;
+  using Wd = typename Word<kWordBytes>::type;
+  union {
+    Wd w[kWords];
+    T v[W];
+    typename Word<(int)sizeof(T) * kPer>::type part[kParts];
+  };
+  MPB_D Elems() {}
+  MPB_D void load(const T* q) {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) w[k] = __ldcs(reinterpret_cast<const Wd*>(q) + k);
+  }
+  MPB_D void store(T* q) const {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) __stcs(reinterpret_cast<Wd*>(q) + k, w[k]);
+  }
+  MPB_D F get(int i) const {
+    Pack<T, kPer> p;
+    p.w = part[i];
+    return unpack(p);
+  }
+  MPB_D void put(int i, F f) { part[i] = pack<T>(f).w; }
+};
+
+template <class T, int W>
+MPB_D void load_floats(const float* q, typename Elems<T, W>::F (&v)[Elems<T, W>::kParts]) {
+  if constexpr (W % 4 == 0) {
+#pragma unroll
+    for (int k = 0; k < W / 4; ++k) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(q) + k);
+      v[2 * k] = make_float2(f.x, f.y);
+      v[2 * k + 1] = make_float2(f.z, f.w);
+    }
+  } else if constexpr (W == 2) {
+    v[0] = make_float2(__ldg(q), __ldg(q + 1));
+  } else {
+    v[0] = __ldg(q);
+  }
+}
+
+// What dropout keeps of W elements from index i on (a multiple of W).
+template <int W>
+struct Kept {
+  uint4 w;
+  uint32_t first;
+  bool none;
+  MPB_D Kept(const Dropper& d, uint64_t i) : w(philox(d, i >> 3)), first((uint32_t)i & 7), none(d.all) {}
+  MPB_D bool operator()(const Dropper& d, int j) const {
+    if constexpr (W == 8) return !none && stays(d, w, j);
+    const uint32_t at = first + j, word = at < 4 ? (at < 2 ? w.x : w.y) : (at < 6 ? w.z : w.w);
+    return !none && ((at & 1) ? word : word << 16) >= d.drop;
+  }
+  // f where kept, g where dropped, of part i
+  MPB_D float pick(const Dropper& d, int i, float f, float g) const { return (*this)(d, i) ? f : g; }
+  MPB_D float2 pick(const Dropper& d, int i, float2 f, float2 g) const {
+    return make_float2((*this)(d, 2 * i) ? f.x : g.x, (*this)(d, 2 * i + 1) ? f.y : g.y);
+  }
+};
+
+// The value and the slope of a gate.
+template <class F>
+MPB_D void act_of_all(int act, F g, F one, F& v, F& slope) {
+  if (act == MPB_ACT_LINEAR) {
+    v = g;
+    slope = one;
+    return;
+  }
+  F s, om;
+  sigmoid2(g, s, om);
+  v = act == MPB_ACT_SIGMOID ? s : vmul(g, s);
+  slope = act == MPB_ACT_SIGMOID ? vmul(s, om) : vmul(s, vfma(g, om, one));
+}
+
+// Sum over a row's threads: a warp, or the whole block (blockDim.y == 1).
+MPB_D float row_sum(float v, float* red) { return blockDim.x == 32 ? warp_sum(v) : block_sum(v, red); }
+MPB_D float fold(float v) { return v; }
+MPB_D float fold(float2 v) { return v.x + v.y; }
+
+// The gate of part i of the pack at column c of row r: `full` has been loaded with the row's other operands.
+template <class T, int W>
+MPB_D typename Elems<T, W>::F gate_part(const NormArgs& p, const Elems<T, W>& full, int64_t r, int c, int i) {
+  using E = Elems<T, W>;
+  if (p.gate_kind == MPB_GATE_FULL) return full.get(i);
+  const T* q = (const T*)p.gate;
+  if (p.gate_kind == MPB_GATE_ROW) return vset<E::kPer>(to_f(q[r * p.g_sr]));
+  q += c + i * E::kPer;
+  if constexpr (E::kPer == 2) {
+    return make_float2(to_f(q[0]), to_f(q[1]));
+  } else {
+    return to_f(q[0]);
+  }
+}
+
+enum { kPlain = 0, kBranch = 1, kDropped = 2 };  // no branch, a branch, a branch with dropout
+
+// blockDim.x threads per row, blockDim.y rows per block (more than one only
+// for rows of a warp). A thread holds the packs threadIdx.x + k blockDim.x.
+template <class T, int W, int NV, int MODE>
+__global__ void __launch_bounds__(kRowThreads) k_norm_rows(NormArgs p) {
+  using E = Elems<T, W>;
+  using F = typename E::F;
+  constexpr int NP = E::kParts;
+  __shared__ float red[2][32];
+  const int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (r >= p.R) return;
+  const int D = (int)p.D, packs = D / W, tid = threadIdx.x, step = blockDim.x;
+  const F zero = vset<E::kPer>(0.0f), one = vset<E::kPer>(1.0f);
+  E x[NV], z[NV], g[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int q = tid + k * step;
+    if (q < packs) {
+      if (MODE != kPlain) z[k].load((const T*)p.z + r * p.z_sr + q * W);
+      x[k].load((const T*)p.x + r * p.x_sr + q * W);
+      if (MODE != kPlain && p.gate_kind == MPB_GATE_FULL) g[k].load((const T*)p.gate + r * p.g_sr + q * W);
+    }
+  }
+  F ss = zero, y[NV][NP];
+  float rz = 0.0f;
+  if (MODE != kPlain) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (tid + k * step < packs)
+#pragma unroll
+        for (int i = 0; i < NP; ++i) ss = vfma(z[k].get(i), z[k].get(i), ss);
+    rz = 1.0f / sqrtf(row_sum(fold(ss), red[0]) / (float)D + p.eps);
+    ss = zero;
+  }
+  const F factor = vset<E::kPer>(rz * (MODE == kDropped ? p.scale * p.drop.up : p.scale));
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int q = tid + k * step;
+    if (q < packs) {
+      if (MODE == kPlain) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) y[k][i] = x[k].get(i);
+      } else {
+        F w[NP];
+        load_floats<T, W>(p.w_post + q * W, w);
+        E out;
+        auto branch = [&](auto kept) {
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            F v = factor, slope;
+            if (p.gate_kind != MPB_GATE_NONE) {
+              act_of_all(p.act, gate_part<T, W>(p, g[k], r, q * W, i), one, v, slope);
+              v = vmul(v, factor);
+            }
+            y[k][i] = kept(i, vfma(vmul(z[k].get(i), w[i]), v, x[k].get(i)), x[k].get(i));
+            out.put(i, y[k][i]);
+          }
+        };
+        if constexpr (MODE == kDropped) {
+          const Kept<W> kept(p.drop, (uint64_t)(r * D + q * W));
+          branch([&](int i, F a, F b) { return kept.pick(p.drop, i, a, b); });
+        } else {
+          branch([](int, F a, F) { return a; });
+        }
+        out.store((T*)p.y + r * D + q * W);
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i) ss = vfma(y[k][i], y[k][i], ss);
+    }
+  }
+  const float ry = 1.0f / sqrtf(row_sum(fold(ss), red[1]) / (float)D + p.eps);
+  const F up = vset<E::kPer>(ry);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int q = tid + k * step;
+    if (q < packs) {
+      F w[NP];
+      load_floats<T, W>(p.w_pre + q * W, w);
+      E out;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) out.put(i, vmul(vmul(y[k][i], up), w[i]));
+      out.store((T*)p.u + r * D + q * W);
+    }
+  }
+  if (tid == 0) {
+    if (MODE != kPlain) p.rstd_out[r] = rz;
+    p.rstd_out[(MODE != kPlain ? p.R : 0) + r] = ry;
+  }
+}
+
+// A thread's column sums in shared memory: W floats of each of its packs, in
+// groups of four so that neighbouring threads touch neighbouring banks. Adds
+// v * by.
+template <class T, int W>
+MPB_D void add_columns(float* acc, int slots, int q, const typename Elems<T, W>::F (&v)[Elems<T, W>::kParts],
+                       typename Elems<T, W>::F by) {
+  if constexpr (W % 4 == 0) {
+#pragma unroll
+    for (int k = 0; k < W / 4; ++k) {
+      float4* a = reinterpret_cast<float4*>(acc) + k * slots + q;
+      const float4 f = *a;
+      const float2 lo = vfma(v[2 * k], by, make_float2(f.x, f.y)), hi = vfma(v[2 * k + 1], by, make_float2(f.z, f.w));
+      *a = make_float4(lo.x, lo.y, hi.x, hi.y);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < W; ++j) acc[j * slots + q] = fmaf(vget(v[0], j), vget(by, j), acc[j * slots + q]);
+  }
+}
+// Where column c of a row lies among `slots` packs of W.
+template <int W>
+MPB_D int column_at(int slots, int c) {
+  const int q = c / W, j = c % W;
+  return W % 4 == 0 ? ((j / 4) * slots + q) * 4 + j % 4 : j * slots + q;
+}
+
+// Rows in turn: blockIdx, blockIdx + grid, ... (times blockDim.y). p.part gets
+// the block's column sums: w_pre, w_post, gate per channel, each (grid, D).
+// Factors that a row's elements share are taken out of the products: with
+// s = m r_z the element's work is ez = dx z (0 where dropped),
+// dw_post += s ez v, dgate = s ez w slope, wn = dx v w,
+// dz = m r_z wn - z r_z^3 m mean(ez v w).
+template <class T, int W, int NV, int MODE>
+__global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
+  using E = Elems<T, W>;
+  using F = typename E::F;
+  constexpr int NP = E::kParts, PW = E::kPer;
+  extern __shared__ __align__(16) float columns[];
+  __shared__ float red[2][3][32];
+  const int D = (int)p.D, packs = D / W, tid = threadIdx.x, step = blockDim.x, slots = step * NV;
+  const int sums = MODE == kPlain ? 1 : p.gate_kind == MPB_GATE_CHANNEL ? 3 : 2;
+  const F zero = vset<PW>(0.0f), one = vset<PW>(1.0f);
+  float* acc = columns + (size_t)threadIdx.y * sums * slots * W;
+  for (int i = tid; i < sums * slots * W; i += step) acc[i] = 0.0f;
+  if (step == 32) __syncwarp();
+  else __syncthreads();
+  int side = 0;
+  for (int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; r < p.R;
+       r += (int64_t)gridDim.x * blockDim.y, side ^= 1) {
+    E dy[NV], du[NV], y[NV], z[NV], g[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int q = tid + k * step;
+      if (q < packs) {
+        if (p.du) {
+          du[k].load((const T*)p.du + r * p.du_sr + q * W);
+          y[k].load((const T*)p.yin + r * p.y_sr + q * W);
+        }
+        if (p.dy) dy[k].load((const T*)p.dy + r * p.dy_sr + q * W);
+        if (MODE != kPlain) {
+          z[k].load((const T*)p.z + r * p.z_sr + q * W);
+          if (p.gate_kind == MPB_GATE_FULL) g[k].load((const T*)p.gate + r * p.g_sr + q * W);
+        }
+      }
+    }
+    const float rz = MODE != kPlain ? p.rstd[r] : 0.0f, ry = p.rstd[(MODE != kPlain ? p.R : 0) + r];
+    float back = 0.0f;  // of y in dx: r_y^3 mean(y w du)
+    if (p.du) {
+      F dot = zero;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int q = tid + k * step;
+        if (q < packs) {
+          F w[NP], c[NP];
+          load_floats<T, W>(p.w_pre + q * W, w);
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            c[i] = vmul(du[k].get(i), y[k].get(i));
+            dot = vfma(c[i], w[i], dot);
+          }
+          add_columns<T, W>(acc, slots, q, c, vset<PW>(ry));
+        }
+      }
+      back = ry * ry * (ry * (row_sum(fold(dot), red[side][0]) / (float)D));
+    }
+    const float m = MODE == kDropped ? p.scale * p.drop.up : p.scale, s = m * rz;
+    F dotz = zero, dgr = zero, wn[NV][NP];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int q = tid + k * step;
+      if (q < packs) {
+        F dx[NP];
+        E out;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) dx[i] = p.dy ? dy[k].get(i) : zero;
+        if (p.du) {
+          F w[NP];
+          load_floats<T, W>(p.w_pre + q * W, w);
+#pragma unroll
+          for (int i = 0; i < NP; ++i)
+            dx[i] = vfma(vmul(du[k].get(i), w[i]), vset<PW>(ry), vfma(y[k].get(i), vset<PW>(-back), dx[i]));
+        }
+#pragma unroll
+        for (int i = 0; i < NP; ++i) out.put(i, dx[i]);
+        out.store((T*)p.dx + r * D + q * W);
+        if (MODE != kPlain) {
+          F w[NP], ezv[NP], dg[NP];
+          load_floats<T, W>(p.w_post + q * W, w);
+          auto branch = [&](auto kept) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+              F v = one, slope = zero;
+              if (p.gate_kind != MPB_GATE_NONE)
+                act_of_all(p.act, gate_part<T, W>(p, g[k], r, q * W, i), one, v, slope);
+              const F ez = vmul(dx[i], z[k].get(i)), dxv = kept(i, vmul(dx[i], v)), dgi = vmul(vmul(ez, w[i]), slope);
+              ezv[i] = vmul(dxv, z[k].get(i));
+              wn[k][i] = vmul(dxv, w[i]);
+              dg[i] = kept(i, vmul(dgi, vset<PW>(s)));
+              dotz = vfma(ezv[i], w[i], dotz);
+              dgr = vadd(dgr, dg[i]);
+            }
+          };
+          if constexpr (MODE == kDropped) {
+            const Kept<W> kept(p.drop, (uint64_t)(r * D + q * W));
+            branch([&](int i, F a) { return kept.pick(p.drop, i, a, zero); });
+          } else {
+            branch([](int, F a) { return a; });
+          }
+          add_columns<T, W>(acc + slots * W, slots, q, ezv, vset<PW>(s));
+          if (p.gate_kind == MPB_GATE_FULL) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) out.put(i, dg[i]);
+            out.store((T*)p.dgate + r * D + q * W);
+          } else if (p.gate_kind == MPB_GATE_CHANNEL) {
+            add_columns<T, W>(acc + 2 * slots * W, slots, q, dg, one);
+          }
+        }
+      }
+    }
+    if (MODE != kPlain) {
+      const float mz = rz * rz * (s * (row_sum(fold(dotz), red[side][1]) / (float)D));
+      if (p.gate_kind == MPB_GATE_ROW) {
+        const float sum = row_sum(fold(dgr), red[side][2]);
+        if (tid == 0) ((T*)p.dgate)[r] = Cvt<T>::from(sum);
+      }
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int q = tid + k * step;
+        if (q < packs) {
+          E out;
+#pragma unroll
+          for (int i = 0; i < NP; ++i)
+            out.put(i, vfma(z[k].get(i), vset<PW>(-mz), vmul(wn[k][i], vset<PW>(s))));
+          out.store((T*)p.dz + r * D + q * W);
+        }
+      }
+    }
+  }
+  // the block's sums over its rows of threads, in order
+  __syncthreads();
+  const int threads = blockDim.x * blockDim.y, me = threadIdx.y * blockDim.x + threadIdx.x;
+  for (int s = 0; s < sums; ++s)
+    for (int c = me; c < D; c += threads) {
+      const int at = s * slots * W + column_at<W>(slots, c);
+      float v = 0.0f;
+      for (int yy = 0; yy < (int)blockDim.y; ++yy) v += columns[(size_t)yy * sums * slots * W + at];
+      p.part[((size_t)s * gridDim.x + blockIdx.x) * D + c] = v;
+    }
+}
+
+// Adds the blocks' column sums: 32 columns per block, its 32 warps a part of the
+// blocks each, in a fixed order.
+template <class T>
+__global__ void __launch_bounds__(1024) k_norm_columns(NormArgs p, int blocks) {
+  __shared__ float part[32][33];
+  const int c = blockIdx.x * 32 + threadIdx.x, s = blockIdx.y;
+  float v = 0.0f;
+  if (c < p.D)
+    for (int b = threadIdx.y; b < blocks; b += 32) v += p.part[((size_t)s * blocks + b) * p.D + c];
+  part[threadIdx.y][threadIdx.x] = v;
+  __syncthreads();
+  v = warp_sum(part[threadIdx.x][threadIdx.y]);
+  const int mine = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x != 0 || mine >= p.D) return;
+  if (s == 0) p.dw_pre[mine] = v;
+  else if (s == 1) p.dw_post[mine] = v;
+  else ((T*)p.dgate)[mine] = Cvt<T>::from(v);
+}
+
+// ------------------------------------------------------------------- host
+// How a row is spread: W elements per pack, NV packs per thread.
+struct Spread {
+  int W, NV;
+  unsigned x, y;  // threads per row, rows per block
+};
+
+// W: 8 where every row of every operand starts on a 16-byte boundary and D is
+// a multiple of 8, else 2 (16-bit types on 4-byte boundaries) or 1. With fewer
+// rows than SMs a row takes as many threads as it has packs (a row's latency
+// counts); else a thread takes 32 elements forward and 16 backward or of
+// narrow packs (what its 128 registers hold), and 32 again where 512 threads
+// need them.
+Spread spread_of(int64_t R, int64_t D, int W, bool backward) {
+  Spread s;
+  s.W = W;
+  const int64_t packs = D / W;
+  const bool few = R < sm_count();
+  const int least = W == 1 ? 8 : W == 2 ? 8 : 1, usual = W == 8 ? (backward ? 2 : 4) : 16 / W;
+  s.NV = few ? least : packs <= 32 * least ? least : packs <= 64 && W == 8 ? 2 : usual;
+  while (s.NV * W < kPerThread && packs > (int64_t)s.NV * kRowThreads) s.NV *= 2;
+  const int64_t threads = (packs + s.NV - 1) / s.NV;
+  s.x = (unsigned)((threads + 31) / 32 * 32);
+  s.y = s.x == 32 && !few ? 4 : 1;
+  return s;
+}
+
+int sums_of(int mode, int gate_kind) { return mode == kPlain ? 1 : gate_kind == MPB_GATE_CHANNEL ? 3 : 2; }
+
+// Blocks of the backward kernel: what fits the SMs at up to 128 registers per
+// thread and by shared memory, or the rows if they are fewer.
+int64_t bwd_blocks(const Spread& s, int64_t R, int sums, size_t* smem) {
+  *smem = (size_t)s.x * s.NV * s.W * sizeof(float) * sums * s.y;
+  int64_t per_sm = kRowThreads / (s.x * s.y);
+  const int64_t by_smem = (int64_t)((220u << 10) / (*smem + 2048));
+  if (per_sm > by_smem) per_sm = by_smem;
+  if (per_sm < 1) per_sm = 1;
+  const int64_t most = per_sm * sm_count(), want = (R + s.y - 1) / s.y;
+  return want < most ? want : most;
+}
+
+template <auto kernel>
+int allow_smem(const char* what, size_t bytes) {
+  static size_t allowed[64] = {};
+  int dev = 0;
+  if (int rc = cuda_check(cudaGetDevice(&dev), what)) return rc;
+  if (bytes <= (40u << 10) || (dev >= 0 && dev < 64 && allowed[dev] >= bytes)) return MPB_OK;
+  if (int rc = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what))
+    return rc;
+  if (dev >= 0 && dev < 64) allowed[dev] = bytes;
+  return MPB_OK;
+}
+
+template <class T, int W, int NV, int MODE>
+int run_rows(const NormArgs& p, const Spread& sp, bool backward, cudaStream_t s) {
+  const dim3 block(sp.x, sp.y);
+  if (!backward) {
+    k_norm_rows<T, W, NV, MODE><<<(unsigned)((p.R + sp.y - 1) / sp.y), block, 0, s>>>(p);
+    return launch_check("gated_residual_norm");
+  }
+  const char* what = "gated_residual_norm_backward";
+  const int sums = sums_of(MODE, p.gate_kind);
+  size_t smem;
+  const int64_t blocks = bwd_blocks(sp, p.R, sums, &smem);
+  if (int rc = allow_smem<k_norm_bwd_rows<T, W, NV, MODE>>(what, smem)) return rc;
+  k_norm_bwd_rows<T, W, NV, MODE><<<(unsigned)blocks, block, smem, s>>>(p);
+  if (int rc = launch_check(what)) return rc;
+  k_norm_columns<T><<<dim3((unsigned)((p.D + 31) / 32), (unsigned)sums), dim3(32, 32), 0, s>>>(p, (int)blocks);
+  return launch_check(what);
+}
+
+template <class T, int MODE>
+int run_spread(const NormArgs& p, const Spread& sp, bool backward, cudaStream_t s) {
+  if (sp.W == 8)
+    return sp.NV == 1   ? run_rows<T, 8, 1, MODE>(p, sp, backward, s)
+           : sp.NV == 2 ? run_rows<T, 8, 2, MODE>(p, sp, backward, s)
+                        : run_rows<T, 8, 4, MODE>(p, sp, backward, s);
+  if constexpr (sizeof(T) == 2)
+    if (sp.W == 2) return sp.NV == 8 ? run_rows<T, 2, 8, MODE>(p, sp, backward, s) : run_rows<T, 2, 16, MODE>(p, sp, backward, s);
+  return sp.NV == 8    ? run_rows<T, 1, 8, MODE>(p, sp, backward, s)
+         : sp.NV == 16 ? run_rows<T, 1, 16, MODE>(p, sp, backward, s)
+                       : run_rows<T, 1, 32, MODE>(p, sp, backward, s);
+}
+
+// Elements per pack that every operand's rows allow.
+int width_of(const NormArgs& p, size_t size) {
+  const void* ptr[] = {p.x, p.z, p.gate_kind == MPB_GATE_FULL ? p.gate : nullptr, p.dy, p.du, p.yin, p.y, p.u, p.dx, p.dz,
+                       p.gate_kind == MPB_GATE_FULL ? p.dgate : nullptr};
+  const int64_t st[] = {p.x ? p.x_sr : 0, p.z ? p.z_sr : 0, p.gate_kind == MPB_GATE_FULL ? p.g_sr : 0, p.dy ? p.dy_sr : 0,
+                        p.du ? p.du_sr : 0, p.yin ? p.y_sr : 0, p.D};
+  const void* weights[] = {p.w_pre, p.w_post};
+  auto fits = [&](size_t bytes) {
+    for (const void* q : ptr)
+      if ((uintptr_t)q % bytes) return false;
+    for (int64_t v : st)
+      if (v * (int64_t)size % (int64_t)bytes) return false;
+    return true;
+  };
+  bool w16 = true;
+  for (const void* q : weights) w16 = w16 && (uintptr_t)q % 16 == 0;
+  if (p.D % 8 == 0 && w16 && fits(16)) return 8;
+  return size == 2 && p.D % 2 == 0 && fits(4) ? 2 : 1;
+}
+
+template <class T>
+int launch_rows(const NormArgs& p, bool backward, cudaStream_t s) {
+  const Spread sp = spread_of(p.R, p.D, width_of(p, sizeof(T)), backward);
+  return !p.z         ? run_spread<T, kPlain>(p, sp, backward, s)
+         : p.dropping ? run_spread<T, kDropped>(p, sp, backward, s)
+                      : run_spread<T, kBranch>(p, sp, backward, s);
+}
+
 template <class T>
 int launch_norm_fwd(const NormArgs& p, cudaStream_t s) {
-  k_norm_fwd<T><<<(unsigned)p.R, kThreads, 0, s>>>(p);
+  if (p.D <= kInRegisters) return launch_rows<T>(p, false, s);
+  k_norm_long<T><<<(unsigned)p.R, kThreads, 0, s>>>(p);
   return launch_check("gated_residual_norm");
 }
 
 template <class T>
 int launch_norm_bwd(const NormArgs& p, cudaStream_t s) {
+  const char* what = "gated_residual_norm_backward";
+  if (p.R > 0 && p.D <= kInRegisters) return launch_rows<T>(p, true, s);
   if (p.R > 0) {
-    k_norm_bwd<T><<<(unsigned)p.R, kThreads, 0, s>>>(p);
-    if (int rc = launch_check("gated_residual_norm_backward")) return rc;
+    k_norm_bwd_long<T><<<(unsigned)p.R, kThreads, 0, s>>>(p);
+    if (int rc = launch_check(what)) return rc;
     if (p.z) {
-      k_norm_bwd_dx<T><<<(unsigned)p.R, kThreads, 0, s>>>(p);
-      if (int rc = launch_check("gated_residual_norm_backward")) return rc;
+      k_norm_bwd_long_dx<T><<<(unsigned)p.R, kThreads, 0, s>>>(p);
+      if (int rc = launch_check(what)) return rc;
     }
   }
-  k_norm_bwd_cols<T><<<(unsigned)((p.D + 127) / 128), 128, 0, s>>>(p);
-  return launch_check("gated_residual_norm_backward");
+  k_norm_bwd_long_cols<T><<<(unsigned)((p.D + 127) / 128), 128, 0, s>>>(p);
+  return launch_check(what);
 }
 
 int check_norm(const char* what, const NormArgs& p, double dropout) {
@@ -256,7 +762,7 @@ int mpb_gated_residual_norm(int64_t R, int64_t D, int dtype, const void* x, int6
   p.scale = (float)scale, p.eps = (float)eps, p.y = y, p.u = u, p.rstd_out = rstd;
   if (int rc = check_norm("gated_residual_norm", p, dropout)) return rc;
   p.drop = make_dropper(dropout, seed, offset);
-  p.dropping = p.drop.drop != 0;
+  p.dropping = p.drop.drop != 0 || p.drop.all;
   if (dtype != MPB_F32 && dtype != MPB_F16 && dtype != MPB_BF16)
     return fail(MPB_ERR_DTYPE, "gated_residual_norm: dtype %d not supported (float16, bfloat16, float32)", dtype);
   if (R == 0 || D == 0) return MPB_OK;
@@ -267,7 +773,16 @@ int mpb_gated_residual_norm(int64_t R, int64_t D, int dtype, const void* x, int6
 }
 
 size_t mpb_gated_residual_norm_scratch_bytes(int64_t R, int64_t D, int dtype, int branch, int gate_kind) {
-  return branch ? (size_t)R * (size_t)D * sizeof(float) : 0;
+  if (R <= 0 || D <= 0) return 0;
+  if (D > kInRegisters) return branch ? (size_t)R * (size_t)D * sizeof(float) : 0;
+  const int sums = sums_of(branch ? kBranch : kPlain, gate_kind);
+  int64_t most = 0;  // blocks, for any width the addresses may allow
+  for (int W : {8, 2, 1}) {
+    size_t smem;
+    const int64_t n = bwd_blocks(spread_of(R, (D + W - 1) / W * W, W, true), R, sums, &smem);
+    most = n > most ? n : most;
+  }
+  return (size_t)most * sums * (size_t)D * sizeof(float);
 }
 
 int mpb_gated_residual_norm_backward(int64_t R, int64_t D, int dtype, const void* dy, int64_t dy_sr, const void* du,
@@ -285,7 +800,7 @@ int mpb_gated_residual_norm_backward(int64_t R, int64_t D, int dtype, const void
   p.dx = dx, p.dz = dz, p.dgate = dgate, p.dw_post = dw_post, p.dw_pre = dw_pre, p.part = (float*)scratch;
   if (int rc = check_norm(what, p, dropout)) return rc;
   p.drop = make_dropper(dropout, seed, offset);
-  p.dropping = p.drop.drop != 0;
+  p.dropping = p.drop.drop != 0 || p.drop.all;
   if (dtype != MPB_F32 && dtype != MPB_F16 && dtype != MPB_BF16)
     return fail(MPB_ERR_DTYPE, "%s: dtype %d not supported (float16, bfloat16, float32)", what, dtype);
   if (D == 0) return MPB_OK;
