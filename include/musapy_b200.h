@@ -233,7 +233,7 @@ int mpb_gated_scan_step(int64_t B, int64_t D, int64_t H, const void* x, int x_dt
                         int gate_dtype, int64_t g_sb, int mode, float* state, void* h, mpb_stream_t stream);
 
 /* Norms before and after a block with its gate, dropout and residual scale,
- * over R rows of D: n = z rms(z) w_post; y = x + scale * drop(act(gate) n);
+ * over R rows of D, less than 2^29 elements apart: n = z rms(z) w_post; y = x + scale * drop(act(gate) n);
  * u = y rms(y) w_pre, rms(v) = (mean v^2 + eps)^(-1/2). x, z, gate in
  * `dtype` with row strides x_sr, z_sr, g_sr; gate_kind says the gate's extent
  * (mpb_gate_kind), activation what it goes through (mpb_activation); the

@@ -24,6 +24,7 @@ _ACTIVATIONS = {"linear": 0, "sigmoid": 1, "silu": 2}
 _GATE_NONE, _GATE_FULL, _GATE_ROW, _GATE_CHANNEL = range(4)
 _ELEMENTS = (_dt.F16, _dt.BF16, _dt.F32)
 _U64 = (1 << 64) - 1
+_MOST_STRIDE = 1 << 29  # elements between rows, mpb_gated_residual_norm's limit
 
 
 # ---------------------------------------------------------------- checks
@@ -230,7 +231,10 @@ def _rows(x: Array):
             else:
                 break
         else:
-            return x, step if step is not None else shape[-1]
+            if step is None:
+                return x, 0  # one row
+            if abs(step) < _MOST_STRIDE:
+                return x, step
     return contiguous(x), shape[-1]
 
 

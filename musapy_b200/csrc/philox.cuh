@@ -33,7 +33,7 @@ inline Dropper make_dropper(double p, uint64_t seed, uint64_t offset) {
   d.c3 = (uint32_t)(offset >> 32);
   const uint32_t k = (uint32_t)(p * 65536.0 + 0.5);
   d.all = k >= 65536u;
-  d.drop = d.all ? 0u : k << 16;
+  d.drop = d.all ? 0xffffffffu : k << 16;
   d.up = d.all ? 0.0f : (float)(65536.0 / (65536.0 - (double)k));
   return d;
 }
@@ -62,7 +62,13 @@ MPB_D bool stays(const Dropper& d, const uint4& w, int j) {
   return ((j & 1) ? v : v << 16) >= d.drop;
 }
 
+// The words to compare: none reaches the threshold where everything is dropped.
+MPB_D uint4 drop_words(const Dropper& d, uint64_t block) {
+  const uint4 w = philox(d, block);
+  return d.all ? make_uint4(0, 0, 0, 0) : w;
+}
+
 // Element i alone.
-MPB_D bool keeps(const Dropper& d, uint64_t i) { return stays(d, philox(d, i >> 3), (int)(i & 7)); }
+MPB_D bool keeps(const Dropper& d, uint64_t i) { return stays(d, drop_words(d, i >> 3), (int)(i & 7)); }
 
 }  // namespace mpb

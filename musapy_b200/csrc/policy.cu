@@ -66,12 +66,21 @@ MPB_D void token_terms(const PolicyArgs& p, int64_t i, float logp, float& value,
   }
 }
 
+// Tokens in the mask, the same value in every thread: counted before, or here,
+// 16 bytes at a time where the mask is aligned.
 MPB_D float tokens_in_mask(const PolicyArgs& p, float* red) {
-  float n = 0.0f;
   if (!p.mask) return (float)p.N;
   if (p.count) return *p.count;
-  for (int64_t i = threadIdx.x; i < p.N; i += blockDim.x) n += p.mask[i] ? 1.0f : 0.0f;
-  return block_sum(n, red);
+  int n = 0;
+  const int64_t words = (uintptr_t)p.mask % 16 == 0 ? p.N / 16 : 0;
+  auto set = [](uint32_t v) { return __popc((v | ((v & 0x7f7f7f7fu) + 0x7f7f7f7fu)) & 0x80808080u); };  // bytes that are not 0
+#pragma unroll 4
+  for (int64_t w = threadIdx.x; w < words; w += blockDim.x) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.mask) + w);
+    n += set(v.x) + set(v.y) + set(v.z) + set(v.w);
+  }
+  for (int64_t i = words * 16 + threadIdx.x; i < p.N; i += blockDim.x) n += p.mask[i] ? 1 : 0;
+  return block_sum((float)n, red);
 }
 
 MPB_D float block_max(float v, float* red) {
@@ -105,12 +114,31 @@ MPB_D int64_t target_of(const PolicyArgs& p, int64_t i) {
   return p.targets64 ? ((const int64_t*)p.targets)[i] : ((const int32_t*)p.targets)[i];
 }
 
-// e^(z - base) of a pair.
-MPB_D float2 exp_from(float2 z, float2 minus_base) {
-  const float2 d = vmul(vadd(z, minus_base), vset<2>(-kMinusLog2e));
-  return make_float2(ex2f(d.x), ex2f(d.y));
-}
+// e^(z - base) of one value.
 MPB_D float exp_from(float z, float minus_base) { return ex2f((z + minus_base) * -kMinusLog2e); }
+
+// e^(z - base) of many. Near: 2^(z c + k) with c = log2 e and k = -base c, one
+// fused multiply-add each; k is rounded, which scales all of them alike, and
+// fix() is the factor that takes this out of them again. Far from zero, where
+// the rounding of k is no small number, the difference is taken first.
+constexpr float kNear = 65536.0f;  // k is off by at most 2^-8 below it
+template <bool NEAR>
+struct Exponent {
+  float base, k;
+  MPB_D explicit Exponent(float b) : base(b), k(b * kMinusLog2e) {}
+  MPB_D float fix() const { return NEAR ? ex2f(-fmaf(base, -kMinusLog2e, k)) : 1.0f; }
+  MPB_D float2 operator()(float2 z) const {
+    const float2 x = NEAR ? vfma(z, vset<2>(-kMinusLog2e), vset<2>(k))
+                          : vmul(vadd(z, vset<2>(-base)), vset<2>(-kMinusLog2e));
+    return make_float2(ex2f(x.x), ex2f(x.y));
+  }
+};
+// f with the form that goes with the base.
+template <class F>
+MPB_D void with_exponent(float base, F f) {
+  if (fabsf(base) <= kNear) f(Exponent<true>(base));
+  else f(Exponent<false>(base));
+}
 
 // 16 bytes of logits as pairs of floats.
 template <class T>
@@ -128,13 +156,38 @@ struct Sixteen {
     return unpack(p);
   }
   MPB_D void put(int i, float2 f) { pair[i] = pack<T>(f).w; }
-  MPB_D float top() const {
-    float2 m = get(0);
-#pragma unroll
-    for (int i = 1; i < kPairs; ++i) m = make_float2(fmaxf(m.x, get(i).x), fmaxf(m.y, get(i).y));
-    return fmaxf(m.x, m.y);
-  }
 };
+
+// The pairwise larger of 16 bytes of elements, and the largest of them as float.
+template <class T>
+MPB_D uint4 larger(uint4 a, uint4 b) {
+  auto two = [](uint32_t x, uint32_t y) -> uint32_t {
+    if constexpr (std::is_same<T, float>::value) {
+      return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&x), *reinterpret_cast<__half2*>(&y));
+      return *reinterpret_cast<const uint32_t*>(&m);
+    } else {
+      const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&x), *reinterpret_cast<__nv_bfloat162*>(&y));
+      return *reinterpret_cast<const uint32_t*>(&m);
+    }
+  };
+  return make_uint4(two(a.x, b.x), two(a.y, b.y), two(a.z, b.z), two(a.w, b.w));
+}
+template <class T>
+MPB_D float largest(uint4 a) {
+  const Sixteen<T> x(a);
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < Sixteen<T>::kPairs; ++i) m = fmaxf(m, fmaxf(x.get(i).x, x.get(i).y));
+  return m;
+}
+// 16 bytes of -inf: in the place of words that a thread does not have.
+template <class T>
+MPB_D uint4 no_words() {
+  const uint32_t w = std::is_same<T, float>::value ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  return make_uint4(w, w, w, w);
+}
 
 // The larger maximum, and the sum of exponentials taken from it. -inf with a
 // sum of zero is the empty set.
@@ -150,6 +203,7 @@ struct Fold {
 
 constexpr int kRowThreads = 256;
 constexpr int kGroups = 4;  // in which a block's copies arrive
+constexpr int kBatch = 4;   // words a thread folds at once: one maximum, one rescaling of its sum
 constexpr int kMostBlocks = 8;
 
 // Block `rank` of the row's cluster takes `per` 16-byte words of it. The
@@ -180,7 +234,8 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_policy_row(PolicyArgs p, int
   if (blocks > 1) cluster.barrier_arrive();  // every block of the cluster runs
   const uint4* src = reinterpret_cast<const uint4*>(z + head) + w0;
   const uint32_t dst = smem_u32(words);
-  const int each = (mine + threads - 1) / threads, quarter = (each + kGroups - 1) / kGroups;
+  const int each = (mine + threads - 1) / threads;
+  const int quarter = (each + kGroups * kBatch - 1) / (kGroups * kBatch) * kBatch;  // words per thread and group
 #pragma unroll
   for (int q = 0; q < kGroups; ++q) {
     for (int k = q * quarter; k < (q + 1) * quarter; ++k) {
@@ -206,25 +261,30 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_policy_row(PolicyArgs p, int
   const float zt = valid ? to_f(z[t]) : 0.0f;
   const float count = p.grad ? tokens_in_mask(p, red[0]) : 1.0f;
   auto fold_group = [&](int q) {
-    float top = -INFINITY;
-    for (int k = q * quarter; k < (q + 1) * quarter; ++k) {
-      const int w = tid + k * threads;
-      if (w < mine) top = fmaxf(top, Sixteen<T>(words[w]).top());
-    }
-    const float m = fmaxf(f.top, top), b = m == -INFINITY ? 0.0f : m;
-    f.sum *= exp_from(f.top, -b);
-    f.top = m;
-    const float2 from = vset<2>(-b);
-    float2 s = vset<2>(0.0f);
-    for (int k = q * quarter; k < (q + 1) * quarter; ++k) {
-      const int w = tid + k * threads;
-      if (w < mine) {
-        const Sixteen<T> x(words[w]);
+    for (int k = q * quarter; k < (q + 1) * quarter; k += kBatch) {
+      uint4 v[kBatch];
 #pragma unroll
-        for (int j = 0; j < Sixteen<T>::kPairs; ++j) s = vadd(s, exp_from(x.get(j), from));
+      for (int j = 0; j < kBatch; ++j) {
+        const int w = tid + (k + j) * threads;
+        v[j] = w < mine ? words[w] : no_words<T>();
       }
+      uint4 most = v[0];
+#pragma unroll
+      for (int j = 1; j < kBatch; ++j) most = larger<T>(most, v[j]);
+      const float m = fmaxf(f.top, largest<T>(most)), b = m == -INFINITY ? 0.0f : m;
+      f.sum *= exp_from(f.top, -b);
+      f.top = m;
+      with_exponent(b, [&](auto e) {
+        float2 s = vset<2>(0.0f);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const Sixteen<T> x(v[j]);
+#pragma unroll
+          for (int i = 0; i < Sixteen<T>::kPairs; ++i) s = vadd(s, e(x.get(i)));
+        }
+        f.sum = fmaf(s.x + s.y, e.fix(), f.sum);
+      });
     }
-    f.sum += s.x + s.y;
   };
   asm volatile("cp.async.wait_group 3;" ::: "memory");
   fold_group(0);
@@ -267,15 +327,17 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_policy_row(PolicyArgs p, int
   T* g = (T*)p.grad + i * p.V;
   slope *= p.grad_scale / count;
   const float down = -slope / sum;
-  const float2 from = vset<2>(-all_base), by = vset<2>(down);
   uint4* out = reinterpret_cast<uint4*>(g + head) + w0;
+  with_exponent(all_base, [&](auto e) {
+    const float2 by = vset<2>(down * e.fix());
 #pragma unroll 4
-  for (int w = tid; w < mine; w += threads) {
-    Sixteen<T> x(words[w]);
+    for (int w = tid; w < mine; w += threads) {
+      Sixteen<T> x(words[w]);
 #pragma unroll
-    for (int j = 0; j < Sixteen<T>::kPairs; ++j) x.put(j, vmul(exp_from(x.get(j), from), by));
-    st_stream16(out + w, x.w);
-  }
+      for (int j = 0; j < Sixteen<T>::kPairs; ++j) x.put(j, vmul(e(x.get(j)), by));
+      st_stream16(out + w, x.w);
+    }
+  });
   if (has_end) g[end_at] = Cvt<T>::from(fmaf(down, exp_from(end, -all_base), end_at == t ? slope : 0.0f));
   // the target's element again, by the thread that has written its word
   const int64_t tw = valid && t >= head && t < tail ? (t - head) / E - w0 : -1;
@@ -326,7 +388,13 @@ __global__ void __launch_bounds__(1024) k_policy_mean(PolicyArgs p) {
   __shared__ float red[2][32];
   const float count = tokens_in_mask(p, red[0]);
   float v = 0.0f;
-  for (int64_t i = threadIdx.x; i < p.N; i += 1024) v += p.each[i];
+#pragma unroll 4
+  for (int64_t w = threadIdx.x; w < p.N / 4; w += 1024) {
+    const float4 f = reinterpret_cast<const float4*>(p.each)[w];
+    v += (f.x + f.y) + (f.z + f.w);
+  }
+  const int64_t last = p.N / 4 * 4 + threadIdx.x;
+  if (last < p.N) v += p.each[last];
   v = block_sum(v, red[1]);
   if (threadIdx.x == 0) *p.loss = v / fmaxf(1.0f, count);
 }
@@ -338,9 +406,6 @@ __global__ void __launch_bounds__(1024) k_policy_count(PolicyArgs p, float* coun
 }
 
 // ------------------------------------------------------------------- host
-// Up to here every block counts the tokens in the mask itself while its copies
-// are under way (a byte each, from L2); beyond, a kernel before does.
-constexpr int64_t kCountedByAll = 8192;
 constexpr int kBlockBytes = 72 << 10;   // of a row, three blocks per SM
 constexpr int kMostBytes = 208 << 10;   // of a row, where eight blocks have to do
 
@@ -357,24 +422,33 @@ int allow_smem(int bytes) {
   return MPB_OK;
 }
 
+// Every block counts the tokens in the mask itself while its copies are under
+// way, as long as that is two loads for each of its threads; of more tokens the
+// number is taken by a kernel before.
+int count_before(PolicyArgs& p, int threads, cudaStream_t s) {
+  if (!p.mask || !p.grad || p.N <= 32 * threads) return MPB_OK;
+  float* count = p.each + p.N;
+  k_policy_count<<<1, 1024, 0, s>>>(p, count);
+  p.count = count;
+  return launch_check("policy_loss");
+}
+
 template <class T>
 int launch_policy(PolicyArgs& p, cudaStream_t s) {
   if (p.N > 0) {
-    if (p.mask && p.N > kCountedByAll) {
-      float* count = p.each + p.N;
-      k_policy_count<<<1, 1024, 0, s>>>(p, count);
-      if (int rc = launch_check("policy_loss")) return rc;
-      p.count = count;
-    }
-    const int64_t size = sizeof(T), words = p.V * size / 16 + 1;
+    const int64_t size = sizeof(T), words = p.V * size / 16 > 0 ? p.V * size / 16 : 1;
     int blocks = 1;
     while (blocks < kMostBlocks && (words + blocks - 1) / blocks * 16 > kBlockBytes) blocks *= 2;
     const int64_t per = (words + blocks - 1) / blocks;
     const bool same = !p.grad || (((uintptr_t)p.logits - (uintptr_t)p.grad) % 16 == 0 && (p.l_sr - p.V) * size % 16 == 0);
     if (same && per * 16 <= kMostBytes && p.N * blocks <= 0x7fffffffLL) {
       const int bytes = (int)per * 16;
-      int threads = (int)((per / 4 + 31) / 32 * 32);
-      threads = threads < 64 ? 64 : threads > kRowThreads ? kRowThreads : threads;
+      // 16 words per thread where rows are many (small blocks, many of them on
+      // an SM), 4 where a row's own latency counts
+      const int64_t share = p.N * blocks <= sm_count() * 3 ? 4 : 16;
+      int threads = (int)((per / share + 31) / 32 * 32);
+      threads = threads < 32 ? 32 : threads > kRowThreads ? kRowThreads : threads;
+      if (int rc = count_before(p, threads, s)) return rc;
       if (int rc = allow_smem<T>(bytes)) return rc;
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3((unsigned)(p.N * blocks));
@@ -390,6 +464,7 @@ int launch_policy(PolicyArgs& p, cudaStream_t s) {
       if (int rc = launch_check_pdl(cudaLaunchKernelEx(&cfg, k_policy_row<T>, p, (int)per, blocks), "policy_loss"))
         return rc;
     } else {
+      if (int rc = count_before(p, kThreads, s)) return rc;
       k_policy_passes<T><<<(unsigned)p.N, kThreads, 0, s>>>(p);
       if (int rc = launch_check("policy_loss")) return rc;
     }

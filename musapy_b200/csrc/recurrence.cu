@@ -66,7 +66,7 @@ struct ScanArgs {
   uint32_t groups;            // per sequence
   uint32_t heads_per, lanes_per, groups_per;  // shared gates: heads per group, lanes per head, groups per head
   uint32_t chains, chunks;    // B * groups, tiles per chain
-  FastDiv by_groups, by_groups_per, by_lanes_per, by_chains;
+  FastDiv by_groups, by_groups_per, by_lanes_per, by_chains, by_heads_per;
   int steps;                  // of a tile
   int walk;                   // a block takes whole chains
   // scratch
@@ -105,6 +105,8 @@ MPB_D float finite(float a) { return fminf(fmaxf(a, -3.0e38f), 3.0e38f); }
 // Where a lane works.
 struct Lane {
   int64_t b, ch, gate;  // sequence, first channel, its gate
+  int64_t head;         // the warp's first gate
+  int slot;             // the lane's gate among the warp's
   bool in;
 };
 
@@ -115,20 +117,24 @@ MPB_D Lane place(const ScanArgs& p, uint32_t chain, int lane) {
   Lane l;
   l.b = b;
   if (!SHARED) {
-    l.ch = l.gate = ((int64_t)group * 32 + lane) * V;
+    l.ch = l.gate = l.head = ((int64_t)group * 32 + lane) * V;
+    l.slot = 0;
     l.in = l.ch < p.D;
   } else if (p.groups_per > 1) {  // a head's channels in several groups
     uint32_t head, part;
     p.by_groups_per.divmod(group, head, part);
     const int64_t c = ((int64_t)part * 32 + lane) * V;
-    l.gate = head;
+    l.gate = l.head = head;
+    l.slot = 0;
     l.ch = head * p.P + c;
     l.in = c < p.P;
   } else {  // one or several heads in a group
     uint32_t head, at;
     p.by_lanes_per.divmod((uint32_t)lane, head, at);
     l.in = head < p.heads_per && (int64_t)group * p.heads_per + head < p.H;
-    l.gate = (int64_t)group * p.heads_per + head;
+    l.head = (int64_t)group * p.heads_per;
+    l.gate = l.head + head;
+    l.slot = l.in ? (int)head : 0;
     l.ch = l.gate * p.P + (int64_t)at * V;
   }
   if (!l.in) l.ch = l.gate = 0;
@@ -232,13 +238,22 @@ MPB_D void look_back(const ScanArgs& p, uint32_t chain, uint32_t chunk, int lane
       ok = ok && await(p.states + at(chunk - 1 - back) + v, w);
       carry[v] = __uint_as_float(w) + 0.0f;
     }
-  for (uint32_t k = chunk - back; k < chunk; ++k)
+  constexpr int kTogether = 8;  // maps fetched at once: their latencies overlap
+  for (uint32_t k0 = chunk - back; k0 < chunk; k0 += kTogether) {
+    uint64_t w[kTogether][V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      uint64_t w = 0;
-      ok = ok && await(p.maps + at(k) + v, w);
-      carry[v] = fmaf(__uint_as_float((uint32_t)w), carry[v], __uint_as_float((uint32_t)(w >> 32)));
-    }
+    for (int i = 0; i < kTogether; ++i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) w[i][v] = k0 + i < chunk ? ld_word(p.maps + at(k0 + i) + v) : 0;
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i)
+      if (k0 + i < chunk)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          if (!w[i][v]) ok = ok && await(p.maps + at(k0 + i) + v, w[i][v]);
+          carry[v] = fmaf(__uint_as_float((uint32_t)w[i][v]), carry[v], __uint_as_float((uint32_t)(w[i][v] >> 32)));
+        }
+  }
   if (!ok) {  // gave up: what follows is marked and NaN
     st_word(p.status, MPB_ERR_TIMEOUT);
 #pragma unroll
@@ -399,6 +414,29 @@ struct Column {
   }
 };
 
+// The gates of a warp's steps where channels share them: a word per step and
+// head of the warp, copied by one lane each and read by all of the head's.
+template <class G, int STEPS>
+struct HeadGates {
+  static constexpr int kElems = (int)sizeof(G);
+  static MPB_D uint32_t at(int e) { return ((threadIdx.x >> 5) * STEPS * 32 + e) * 4; }
+  // src: the gate of the warp's first head at its first step
+  static MPB_D void copy(uint32_t base, const char* src, int64_t st, int n, int per, int heads, FastDiv by_per) {
+    for (int e = threadIdx.x & 31; e < STEPS * per; e += 32) {
+      uint32_t i, j;
+      by_per.divmod((uint32_t)e, i, j);
+      if ((int)i < n && (int)j < heads) copy_word<kElems>(base + at(e), src + i * st + j * kElems);
+    }
+  }
+  static MPB_D Pack<G, 1> get(const char* base, int e, uint32_t half) {
+    Pack<G, 1> v;
+    const char* q = base + at(e);
+    if constexpr (kElems < 4) q += half & 2;
+    v.w = *reinterpret_cast<const typename Pack<G, 1>::W*>(q);
+    return v;
+  }
+};
+
 // What the tiles of a block are, in order. Walk: the chunks of chain blockIdx,
 // then of chain blockIdx + grid, ... Look-back: the tickets it took.
 template <bool WALK>
@@ -428,7 +466,9 @@ struct Order {
 template <bool WALK, int PER, int N>
 struct Place {
   const char* at[N];
-  int left;  // steps from the warp's first one to the end of the sequence; 0 on an idle lane
+  int left;   // steps from the warp's first one to the end of the sequence; 0 on an idle lane
+  int end;    // the same on every lane
+  int heads;  // gates of the warp, where channels share them
   template <class F>
   MPB_D void go(const ScanArgs& p, const Order<WALK>& o, int warp, const int64_t (&st)[N], F place_at) {
     if (!WALK || o.chunk == 0) {
@@ -437,6 +477,7 @@ struct Place {
 #pragma unroll
       for (int k = 0; k < N; ++k) at[k] += st[k] * p.steps;
       left -= p.steps;
+      end -= p.steps;
     }
   }
   MPB_D int steps() const { return left < PER ? left : PER; }
@@ -478,11 +519,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan(ScanArgs p) {
         const Lane l = place<V, SHARED>(p, o.chain, lane);
         const int64_t t0 = (int64_t)o.chunk * p.steps + warp * kFwd;
         f.at[0] = (const char*)((const X*)p.x + l.b * p.x_sb + t0 * p.x_st + l.ch);
-        f.at[1] = (const char*)((const G*)p.gate + l.b * p.g_sb + t0 * p.g_st + l.gate);
-        f.left = l.in ? (int)(p.T - t0) : 0;
+        f.at[1] = (const char*)((const G*)p.gate + l.b * p.g_sb + t0 * p.g_st + l.head);
+        f.end = (int)(p.T - t0);
+        f.left = l.in ? f.end : 0;
+        f.heads = SHARED ? (int)(p.H - l.head < p.heads_per ? p.H - l.head : p.heads_per) : 0;
       });
       Tile::CX::template copy<kFwd>(base + s * Tile::kBytes, from.at[0], in_st[0], from.left);
-      Tile::CG::template copy<kFwd>(base + s * Tile::kBytes + Tile::kG, from.at[1], in_st[1], from.left);
+      const uint32_t q = base + s * Tile::kBytes + Tile::kG;
+      if constexpr (SHARED) HeadGates<G, kFwd>::copy(q, from.at[1], in_st[1], from.end, (int)p.heads_per, from.heads, p.by_heads_per);
+      else Tile::CG::template copy<kFwd>(q, from.at[1], in_st[1], from.left);
       ahead.next(p);
     }
     copies_commit();
@@ -492,8 +537,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan(ScanArgs p) {
   int stage = 0;
   Floats<V> carry = vset<V>(0.0f);
   size_t state_at = 0;
+  int gate_slot = 0;
   uint32_t half_x = 0, half_g = 0;  // bit 1 of the addresses of single 16-bit elements at step 0
   for (int it = 0; cur.here(p, sh.tiles, it); ++it) {
+    if (SHARED) __syncwarp();  // the stage's gates have been read by every lane
     copy(it + NST - 1, stage == 0 ? NST - 1 : stage - 1);
     to.go(p, cur, warp, out_st, [&](const Order<WALK>& o, auto& f) {
       const Lane l = place<V, SHARED>(p, o.chain, lane);
@@ -501,6 +548,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan(ScanArgs p) {
       f.at[0] = (const char*)((const X*)p.h + (l.b * p.T + t0) * p.D + l.ch);
       f.left = l.in ? (int)(p.T - t0) : 0;
       state_at = (size_t)(l.b * p.D + l.ch);
+      gate_slot = l.slot;
       half_x = (uint32_t)(uintptr_t)((const X*)p.x + l.b * p.x_sb + l.ch);
       half_g = (uint32_t)(uintptr_t)((const G*)p.gate + l.b * p.g_sb + l.gate);
       if (o.chunk == 0 || !WALK)
@@ -519,6 +567,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan(ScanArgs p) {
                        : 0;
     }
     copies_wait<NST - 1>();
+    if (SHARED) __syncwarp();  // the gates that other lanes have copied
     const char* mine = ring + stage * Tile::kBytes;
     // Steps after the last are computed from whatever the ring holds: nothing
     // follows them in the chain, and they are not written.
@@ -527,7 +576,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan(ScanArgs p) {
     for (int i = 0; i < kFwd; ++i) {
       const Floats<V> x = unpack(Tile::CX::get(mine, i, half(half_x, in_st[0], i)));
       Floats<V> om;
-      gates_of<SIG, V>(Tile::CG::get(mine + Tile::kG, i, half(half_g, in_st[1], i)), a[i], om);
+      if constexpr (SHARED)
+        gates_of<SIG, V>(HeadGates<G, kFwd>::get(mine + Tile::kG, i * (int)p.heads_per + gate_slot, half(half_g, in_st[1], i)), a[i], om);
+      else
+        gates_of<SIG, V>(Tile::CG::get(mine + Tile::kG, i, half(half_g, in_st[1], i)), a[i], om);
       b[i] = SIG ? vmul(om, x) : x;
       ma = vmul(ma, a[i]);
       mb = vfma(a[i], mb, b[i]);
@@ -628,14 +680,17 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd(ScanArgs p) {
         f.at[0] = (const char*)((const X*)p.dh + l.b * p.dh_sb + t0 * p.dh_st + l.ch);
         f.at[1] = (const char*)((const X*)p.hsaved + l.b * p.h_sb + (t0 - 1) * p.h_st + l.ch);
         f.at[2] = (const char*)((const X*)p.x + l.b * p.x_sb + t0 * p.x_st + l.ch);
-        f.at[3] = (const char*)((const G*)p.gate + l.b * p.g_sb + t0 * p.g_st + l.gate);
-        f.left = l.in ? (int)(p.T - r0) : 0;
+        f.at[3] = (const char*)((const G*)p.gate + l.b * p.g_sb + t0 * p.g_st + l.head);
+        f.end = (int)(p.T - r0);
+        f.left = l.in ? f.end : 0;
+        f.heads = SHARED ? (int)(p.H - l.head < p.heads_per ? p.H - l.head : p.heads_per) : 0;
       });
       const uint32_t q = base + s * Tile::kBytes;
       Tile::CX::template copy<kBwd>(q, from.at[0], in_st[0], from.left);
       Tile::CX::template copy<kBwd>(q + Tile::kH, from.at[1], in_st[1], from.left - 1);  // h[-1] is h0
       if (SIG) Tile::CX::template copy<kBwd>(q + Tile::kX, from.at[2], in_st[2], from.left);
-      Tile::CG::template copy<kBwd>(q + Tile::kG, from.at[3], in_st[3], from.left);
+      if constexpr (SHARED) HeadGates<G, kBwd>::copy(q + Tile::kG, from.at[3], in_st[3], from.end, (int)p.heads_per, from.heads, p.by_heads_per);
+      else Tile::CG::template copy<kBwd>(q + Tile::kG, from.at[3], in_st[3], from.left);
       ahead.next(p);
     }
     copies_commit();
@@ -645,8 +700,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd(ScanArgs p) {
   int stage = 0;
   Floats<V> carry = vset<V>(0.0f);
   size_t state_at = 0;
+  int gate_slot = 0;
   uint32_t half0[4] = {};  // bit 1 of the addresses of single 16-bit elements at the sequence's last step
   for (int it = 0; cur.here(p, sh.tiles, it); ++it) {
+    if (SHARED) __syncwarp();  // the stage's gates have been read by every lane
     copy(it + NST - 1, stage == 0 ? NST - 1 : stage - 1);
     to.go(p, cur, warp, out_st, [&](const Order<WALK>& o, auto& f) {
       const Lane l = place<V, SHARED>(p, o.chain, lane);
@@ -655,6 +712,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd(ScanArgs p) {
       f.at[1] = (const char*)((const G*)p.dgate + (l.b * p.T + t0) * p.H + l.gate);
       f.left = l.in ? (int)(p.T - r0) : 0;
       state_at = (size_t)(l.b * p.D + l.ch);
+      gate_slot = l.slot;
       half0[0] = (uint32_t)(uintptr_t)((const X*)p.dh + l.b * p.dh_sb + (p.T - 1) * p.dh_st + l.ch);
       half0[1] = (uint32_t)(uintptr_t)((const X*)p.hsaved + l.b * p.h_sb + (p.T - 2) * p.h_st + l.ch);
       half0[2] = (uint32_t)(uintptr_t)((const X*)p.x + l.b * p.x_sb + (p.T - 1) * p.x_st + l.ch);
@@ -675,10 +733,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd(ScanArgs p) {
                        : 0;
     }
     copies_wait<NST - 1>();
+    if (SHARED) __syncwarp();  // the gates that other lanes have copied
     const char* mine = ring + stage * Tile::kBytes;
     Floats<V> ma = vset<V>(1.0f), mb = vset<V>(0.0f), in;
     auto gate_at = [&](int i, Floats<V>& a, Floats<V>& om) {
-      gates_of<SIG, V>(Tile::CG::get(mine + Tile::kG, i, half(3, i)), a, om);
+      if constexpr (SHARED) gates_of<SIG, V>(HeadGates<G, kBwd>::get(mine + Tile::kG, i * (int)p.heads_per + gate_slot, half(3, i)), a, om);
+      else gates_of<SIG, V>(Tile::CG::get(mine + Tile::kG, i, half(3, i)), a, om);
     };
 #pragma unroll
     for (int i = 0; i < kBwd; ++i) {
@@ -846,6 +906,7 @@ void lay_out(ScanArgs& p, int V, int per) {
   p.by_groups = FastDiv(p.groups);
   p.by_groups_per = FastDiv(p.groups_per);
   p.by_lanes_per = FastDiv(p.lanes_per);
+  p.by_heads_per = FastDiv(p.heads_per);
   p.by_chains = FastDiv(p.chains);
 }
 

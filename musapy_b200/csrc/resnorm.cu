@@ -26,6 +26,7 @@
 // Rows too long for that (above 16384 elements) are read again for each pass.
 //
 // Bound: memory.
+#include "async_copy.cuh"
 #include "common.cuh"
 #include "internal.h"
 #include "musapy_b200.h"
@@ -48,11 +49,13 @@ struct NormArgs {
   float scale, eps;
   Dropper drop;
   int dropping;
+  int ahead;  // backward: the next row is copied while one is worked on
 };
 
 constexpr int kThreads = 256;     // a row longer than kInRegisters
 constexpr int kRowThreads = 512;  // of a row in registers, at most
 constexpr int kPerThread = 32;    // its elements per thread, at most
+constexpr int64_t kMostStride = 1 << 29;  // between rows: its bytes are multiplied in 32 bits
 constexpr int64_t kInRegisters = (int64_t)kRowThreads * kPerThread;
 
 MPB_D void act_of(int act, float g, float& v, float& slope) {
@@ -80,7 +83,6 @@ MPB_D float gate_at(const NormArgs& p, int64_t r, int64_t c) {
 
 MPB_D float branch_factor(const NormArgs& p, int64_t r, int64_t c) {
   if (!p.dropping) return p.scale;
-  if (p.drop.all) return 0.0f;
   return keeps(p.drop, (uint64_t)(r * p.D + c)) ? p.scale * p.drop.up : 0.0f;
 }
 
@@ -236,6 +238,23 @@ struct Elems {
 #pragma unroll
     for (int k = 0; k < kWords; ++k) w[k] = __ldcs(reinterpret_cast<const Wd*>(q) + k);
   }
+  // cp.async of the words, to be read back with `fetch` by the same thread
+  MPB_D static void prefetch(uint32_t smem, uint32_t pitch, const T* q) {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      if constexpr (kWordBytes == 16) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem + k * pitch), "l"((const Wd*)q + k) : "memory");
+      } else if constexpr (kWordBytes >= 4) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem + k * pitch), "l"((const Wd*)q + k),
+                     "n"(kWordBytes)
+                     : "memory");
+      }
+    }
+  }
+  MPB_D void fetch(const char* smem, uint32_t pitch) {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) w[k] = *reinterpret_cast<const Wd*>(smem + k * pitch);
+  }
   MPB_D void store(T* q) const {
 #pragma unroll
     for (int k = 0; k < kWords; ++k) __stcs(reinterpret_cast<Wd*>(q) + k, w[k]);
@@ -269,12 +288,11 @@ template <int W>
 struct Kept {
   uint4 w;
   uint32_t first;
-  bool none;
-  MPB_D Kept(const Dropper& d, uint64_t i) : w(philox(d, i >> 3)), first((uint32_t)i & 7), none(d.all) {}
+  MPB_D Kept(const Dropper& d, uint64_t i) : w(drop_words(d, i >> 3)), first((uint32_t)i & 7) {}
   MPB_D bool operator()(const Dropper& d, int j) const {
-    if constexpr (W == 8) return !none && stays(d, w, j);
+    if constexpr (W == 8) return stays(d, w, j);
     const uint32_t at = first + j, word = at < 4 ? (at < 2 ? w.x : w.y) : (at < 6 ? w.z : w.w);
-    return !none && ((at & 1) ? word : word << 16) >= d.drop;
+    return ((at & 1) ? word : word << 16) >= d.drop;
   }
   // f where kept, g where dropped, of part i
   MPB_D float pick(const Dropper& d, int i, float f, float g) const { return (*this)(d, i) ? f : g; }
@@ -283,18 +301,11 @@ struct Kept {
   }
 };
 
-// The value and the slope of a gate.
-template <class F>
-MPB_D void act_of_all(int act, F g, F one, F& v, F& slope) {
-  if (act == MPB_ACT_LINEAR) {
-    v = g;
-    slope = one;
-    return;
-  }
-  F s, om;
-  sigmoid2(g, s, om);
-  v = act == MPB_ACT_SIGMOID ? s : vmul(g, s);
-  slope = act == MPB_ACT_SIGMOID ? vmul(s, om) : vmul(s, vfma(g, om, one));
+// Row r of an operand, `skip` elements on: the row's stride in bytes fits 32
+// bits (checked), so this is one wide multiply-add.
+template <class T>
+MPB_D const T* row_at(const void* base, int r, int64_t sr, int skip) {
+  return reinterpret_cast<const T*>((const char*)base + (int64_t)r * (int)(sr * (int)sizeof(T))) + skip;
 }
 
 // Sum over a row's threads: a warp, or the whole block (blockDim.y == 1).
@@ -302,18 +313,50 @@ MPB_D float row_sum(float v, float* red) { return blockDim.x == 32 ? warp_sum(v)
 MPB_D float fold(float v) { return v; }
 MPB_D float fold(float2 v) { return v.x + v.y; }
 
-// The gate of part i of the pack at column c of row r: `full` has been loaded with the row's other operands.
+// The values and slopes of the gate for the pack at column c of row r; `full`
+// has been loaded with the row's other operands. One switch for all elements.
 template <class T, int W>
-MPB_D typename Elems<T, W>::F gate_part(const NormArgs& p, const Elems<T, W>& full, int64_t r, int c, int i) {
+MPB_D void gate_pack(const NormArgs& p, const Elems<T, W>& full, int64_t r, int c,
+                     typename Elems<T, W>::F (&v)[Elems<T, W>::kParts],
+                     typename Elems<T, W>::F (&slope)[Elems<T, W>::kParts]) {
   using E = Elems<T, W>;
-  if (p.gate_kind == MPB_GATE_FULL) return full.get(i);
-  const T* q = (const T*)p.gate;
-  if (p.gate_kind == MPB_GATE_ROW) return vset<E::kPer>(to_f(q[r * p.g_sr]));
-  q += c + i * E::kPer;
-  if constexpr (E::kPer == 2) {
-    return make_float2(to_f(q[0]), to_f(q[1]));
+  using F = typename E::F;
+  constexpr int NP = E::kParts;
+  const F one = vset<E::kPer>(1.0f);
+  F g[NP];
+  if (p.gate_kind == MPB_GATE_FULL) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) g[i] = full.get(i);
+  } else if (p.gate_kind == MPB_GATE_NONE) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) v[i] = one, slope[i] = vset<E::kPer>(0.0f);
+    return;
   } else {
-    return to_f(q[0]);
+    const T* q = p.gate_kind == MPB_GATE_ROW ? (const T*)p.gate + r * p.g_sr : (const T*)p.gate + c;
+    const int st = p.gate_kind == MPB_GATE_ROW ? 0 : 1;
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+      for (int j = 0; j < E::kPer; ++j) vput(g[i], j, to_f(q[(i * E::kPer + j) * st]));
+  }
+  if (p.act == MPB_ACT_LINEAR) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) v[i] = g[i], slope[i] = one;
+  } else if (p.act == MPB_ACT_SIGMOID) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      F om;
+      sigmoid2(g[i], v[i], om);
+      slope[i] = vmul(v[i], om);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      F s, om;
+      sigmoid2(g[i], s, om);
+      v[i] = vmul(g[i], s);
+      slope[i] = vmul(s, vfma(g[i], om, one));
+    }
   }
 }
 
@@ -327,18 +370,22 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_rows(NormArgs p) {
   using F = typename E::F;
   constexpr int NP = E::kParts;
   __shared__ float red[2][32];
-  const int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (r >= p.R) return;
-  const int D = (int)p.D, packs = D / W, tid = threadIdx.x, step = blockDim.x;
-  const F zero = vset<E::kPer>(0.0f), one = vset<E::kPer>(1.0f);
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= p.R) return;
+  const int r = (int)row, D = (int)p.D, packs = D / W, tid = threadIdx.x, step = blockDim.x, skip = tid * W;
+  const F zero = vset<E::kPer>(0.0f);
+  const T *xr = row_at<T>(p.x, r, p.x_sr, skip), *zr = row_at<T>(p.z, r, p.z_sr, skip);
+  const T* gr = row_at<T>(p.gate, r, p.gate_kind == MPB_GATE_FULL ? p.g_sr : 0, skip);
+  T *yr = const_cast<T*>(row_at<T>(p.y, r, D, skip)), *ur = const_cast<T*>(row_at<T>(p.u, r, D, skip));
   E x[NV], z[NV], g[NV];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int q = tid + k * step;
     if (q < packs) {
-      if (MODE != kPlain) z[k].load((const T*)p.z + r * p.z_sr + q * W);
-      x[k].load((const T*)p.x + r * p.x_sr + q * W);
-      if (MODE != kPlain && p.gate_kind == MPB_GATE_FULL) g[k].load((const T*)p.gate + r * p.g_sr + q * W);
+      const int at = k * step * W;
+      if (MODE != kPlain) z[k].load(zr + at);
+      x[k].load(xr + at);
+      if (MODE != kPlain && p.gate_kind == MPB_GATE_FULL) g[k].load(gr + at);
     }
   }
   F ss = zero, y[NV][NP];
@@ -364,25 +411,22 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_rows(NormArgs p) {
         F w[NP];
         load_floats<T, W>(p.w_post + q * W, w);
         E out;
+        F v[NP], slope[NP];
+        gate_pack<T, W>(p, g[k], r, q * W, v, slope);
         auto branch = [&](auto kept) {
 #pragma unroll
           for (int i = 0; i < NP; ++i) {
-            F v = factor, slope;
-            if (p.gate_kind != MPB_GATE_NONE) {
-              act_of_all(p.act, gate_part<T, W>(p, g[k], r, q * W, i), one, v, slope);
-              v = vmul(v, factor);
-            }
-            y[k][i] = kept(i, vfma(vmul(z[k].get(i), w[i]), v, x[k].get(i)), x[k].get(i));
+            y[k][i] = kept(i, vfma(vmul(z[k].get(i), w[i]), vmul(v[i], factor), x[k].get(i)), x[k].get(i));
             out.put(i, y[k][i]);
           }
         };
         if constexpr (MODE == kDropped) {
-          const Kept<W> kept(p.drop, (uint64_t)(r * D + q * W));
+          const Kept<W> kept(p.drop, (uint64_t)((int64_t)r * D + q * W));
           branch([&](int i, F a, F b) { return kept.pick(p.drop, i, a, b); });
         } else {
           branch([](int, F a, F) { return a; });
         }
-        out.store((T*)p.y + r * D + q * W);
+        out.store(yr + k * step * W);
       }
 #pragma unroll
       for (int i = 0; i < NP; ++i) ss = vfma(y[k][i], y[k][i], ss);
@@ -399,7 +443,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_rows(NormArgs p) {
       E out;
 #pragma unroll
       for (int i = 0; i < NP; ++i) out.put(i, vmul(vmul(y[k][i], up), w[i]));
-      out.store((T*)p.u + r * D + q * W);
+      out.store(ur + k * step * W);
     }
   }
   if (tid == 0) {
@@ -447,32 +491,60 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
   constexpr int NP = E::kParts, PW = E::kPer;
   extern __shared__ __align__(16) float columns[];
   __shared__ float red[2][3][32];
-  const int D = (int)p.D, packs = D / W, tid = threadIdx.x, step = blockDim.x, slots = step * NV;
+  const int D = (int)p.D, packs = D / W, tid = threadIdx.x, step = blockDim.x, slots = step * NV, skip = tid * W;
   const int sums = MODE == kPlain ? 1 : p.gate_kind == MPB_GATE_CHANNEL ? 3 : 2;
   const F zero = vset<PW>(0.0f), one = vset<PW>(1.0f);
   float* acc = columns + (size_t)threadIdx.y * sums * slots * W;
   for (int i = tid; i < sums * slots * W; i += step) acc[i] = 0.0f;
   if (step == 32) __syncwarp();
   else __syncthreads();
-  int side = 0;
-  for (int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; r < p.R;
-       r += (int64_t)gridDim.x * blockDim.y, side ^= 1) {
-    E dy[NV], du[NV], y[NV], z[NV], g[NV];
+  // A row's words come through shared memory, copied while the row before is
+  // worked on; each thread copies and reads its own, so no barrier is needed.
+  // (Single 16-bit elements are too small for such copies and are loaded.)
+  const bool ahead = E::kWordBytes >= 4 && p.ahead;
+  const int all = blockDim.x * blockDim.y;
+  const uint32_t pitch = all * E::kWordBytes;
+  char* ring = reinterpret_cast<char*>(columns + (size_t)blockDim.y * sums * slots * W) +
+               (threadIdx.y * step + tid) * E::kWordBytes;
+  const int64_t stride = (int64_t)gridDim.x * blockDim.y;
+  const bool full_gate = MODE != kPlain && p.gate_kind == MPB_GATE_FULL;
+  // f(stream, pack, pointer) for every pack that the thread has of row r
+  auto streams = [&](int r, auto f) {
+    const T *dyr = row_at<T>(p.dy, r, p.dy_sr, skip), *dur = row_at<T>(p.du, r, p.du_sr, skip);
+    const T *yr = row_at<T>(p.yin, r, p.y_sr, skip), *zr = row_at<T>(p.z, r, p.z_sr, skip);
+    const T* gr = row_at<T>(p.gate, r, full_gate ? p.g_sr : 0, skip);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int q = tid + k * step;
-      if (q < packs) {
+    for (int k = 0; k < NV; ++k)
+      if (tid + k * step < packs) {
+        const int at = k * step * W;
         if (p.du) {
-          du[k].load((const T*)p.du + r * p.du_sr + q * W);
-          y[k].load((const T*)p.yin + r * p.y_sr + q * W);
+          f(0, k, dur + at);
+          f(1, k, yr + at);
         }
-        if (p.dy) dy[k].load((const T*)p.dy + r * p.dy_sr + q * W);
-        if (MODE != kPlain) {
-          z[k].load((const T*)p.z + r * p.z_sr + q * W);
-          if (p.gate_kind == MPB_GATE_FULL) g[k].load((const T*)p.gate + r * p.g_sr + q * W);
-        }
+        if (p.dy) f(2, k, dyr + at);
+        if (MODE != kPlain) f(3, k, zr + at);
+        if (full_gate) f(4, k, gr + at);
       }
+  };
+  auto slot = [&](int stream, int k) { return (uint32_t)(stream * NV + k) * E::kWords * pitch; };
+  auto copy_row = [&](int r) {
+    streams(r, [&](int stream, int k, const T* q) { E::prefetch(smem_u32(ring) + slot(stream, k), pitch, q); });
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const int64_t row0 = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (ahead && row0 < p.R) copy_row((int)row0);
+  int side = 0;
+  for (int64_t row = row0; row < p.R; row += stride, side ^= 1) {
+    const int r = (int)row;
+    E in[5][NV];
+    if (ahead) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      streams(r, [&](int stream, int k, const T*) { in[stream][k].fetch(ring + slot(stream, k), pitch); });
+      if (row + stride < p.R) copy_row((int)(row + stride));
+    } else {
+      streams(r, [&](int stream, int k, const T* q) { in[stream][k].load(q); });
     }
+    E(&du)[NV] = in[0], (&y)[NV] = in[1], (&dy)[NV] = in[2], (&z)[NV] = in[3], (&g)[NV] = in[4];
     const float rz = MODE != kPlain ? p.rstd[r] : 0.0f, ry = p.rstd[(MODE != kPlain ? p.R : 0) + r];
     float back = 0.0f;  // of y in dx: r_y^3 mean(y w du)
     if (p.du) {
@@ -512,17 +584,15 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
         }
 #pragma unroll
         for (int i = 0; i < NP; ++i) out.put(i, dx[i]);
-        out.store((T*)p.dx + r * D + q * W);
+        out.store(const_cast<T*>(row_at<T>(p.dx, r, D, skip)) + k * step * W);
         if (MODE != kPlain) {
-          F w[NP], ezv[NP], dg[NP];
+          F w[NP], ezv[NP], dg[NP], v[NP], slope[NP];
           load_floats<T, W>(p.w_post + q * W, w);
+          gate_pack<T, W>(p, g[k], r, q * W, v, slope);
           auto branch = [&](auto kept) {
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-              F v = one, slope = zero;
-              if (p.gate_kind != MPB_GATE_NONE)
-                act_of_all(p.act, gate_part<T, W>(p, g[k], r, q * W, i), one, v, slope);
-              const F ez = vmul(dx[i], z[k].get(i)), dxv = kept(i, vmul(dx[i], v)), dgi = vmul(vmul(ez, w[i]), slope);
+              const F ez = vmul(dx[i], z[k].get(i)), dxv = kept(i, vmul(dx[i], v[i])), dgi = vmul(vmul(ez, w[i]), slope[i]);
               ezv[i] = vmul(dxv, z[k].get(i));
               wn[k][i] = vmul(dxv, w[i]);
               dg[i] = kept(i, vmul(dgi, vset<PW>(s)));
@@ -531,7 +601,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
             }
           };
           if constexpr (MODE == kDropped) {
-            const Kept<W> kept(p.drop, (uint64_t)(r * D + q * W));
+            const Kept<W> kept(p.drop, (uint64_t)((int64_t)r * D + q * W));
             branch([&](int i, F a) { return kept.pick(p.drop, i, a, zero); });
           } else {
             branch([](int, F a) { return a; });
@@ -540,7 +610,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
           if (p.gate_kind == MPB_GATE_FULL) {
 #pragma unroll
             for (int i = 0; i < NP; ++i) out.put(i, dg[i]);
-            out.store((T*)p.dgate + r * D + q * W);
+            out.store(const_cast<T*>(row_at<T>(p.dgate, r, D, skip)) + k * step * W);
           } else if (p.gate_kind == MPB_GATE_CHANNEL) {
             add_columns<T, W>(acc + 2 * slots * W, slots, q, dg, one);
           }
@@ -561,7 +631,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
 #pragma unroll
           for (int i = 0; i < NP; ++i)
             out.put(i, vfma(z[k].get(i), vset<PW>(-mz), vmul(wn[k][i], vset<PW>(s))));
-          out.store((T*)p.dz + r * D + q * W);
+          out.store(const_cast<T*>(row_at<T>(p.dz, r, D, skip)) + k * step * W);
         }
       }
     }
@@ -607,16 +677,16 @@ struct Spread {
 // W: 8 where every row of every operand starts on a 16-byte boundary and D is
 // a multiple of 8, else 2 (16-bit types on 4-byte boundaries) or 1. With fewer
 // rows than SMs a row takes as many threads as it has packs (a row's latency
-// counts); else a thread takes 32 elements forward and 16 backward or of
-// narrow packs (what its 128 registers hold), and 32 again where 512 threads
-// need them.
-Spread spread_of(int64_t R, int64_t D, int W, bool backward) {
+// counts); else a thread takes 32 elements forward and 16 (of float 8) backward
+// or of narrow packs, what its 128 registers hold, and up to 32 again where 512
+// threads need them.
+Spread spread_of(int64_t R, int64_t D, int W, bool backward, int size) {
   Spread s;
   s.W = W;
   const int64_t packs = D / W;
   const bool few = R < sm_count();
-  const int least = W == 1 ? 8 : W == 2 ? 8 : 1, usual = W == 8 ? (backward ? 2 : 4) : 16 / W;
-  s.NV = few ? least : packs <= 32 * least ? least : packs <= 64 && W == 8 ? 2 : usual;
+  const int least = W == 1 ? 8 : W == 2 ? 8 : 1, usual = W == 8 ? (backward ? 4 / size : 4) : 16 / W;
+  s.NV = few ? least : packs <= 32 * least ? least : packs <= 64 && W == 8 ? (2 < usual ? 2 : usual) : usual;
   while (s.NV * W < kPerThread && packs > (int64_t)s.NV * kRowThreads) s.NV *= 2;
   const int64_t threads = (packs + s.NV - 1) / s.NV;
   s.x = (unsigned)((threads + 31) / 32 * 32);
@@ -628,10 +698,13 @@ int sums_of(int mode, int gate_kind) { return mode == kPlain ? 1 : gate_kind == 
 
 // Blocks of the backward kernel: what fits the SMs at up to 128 registers per
 // thread and by shared memory, or the rows if they are fewer.
-int64_t bwd_blocks(const Spread& s, int64_t R, int sums, size_t* smem) {
-  *smem = (size_t)s.x * s.NV * s.W * sizeof(float) * sums * s.y;
+int64_t bwd_blocks(const Spread& s, int64_t R, int sums, int size, size_t* smem, int* ahead) {
+  const size_t elements = (size_t)s.x * s.NV * s.W * s.y, room = 220u << 10;
+  *smem = elements * (sizeof(float) * sums + 5 * size);
+  *ahead = s.W * size >= 4 && *smem <= room;
+  if (!*ahead) *smem = elements * sizeof(float) * sums;
   int64_t per_sm = kRowThreads / (s.x * s.y);
-  const int64_t by_smem = (int64_t)((220u << 10) / (*smem + 2048));
+  const int64_t by_smem = (int64_t)((room + 4096) / (*smem + 2048));
   if (per_sm > by_smem) per_sm = by_smem;
   if (per_sm < 1) per_sm = 1;
   const int64_t most = per_sm * sm_count(), want = (R + s.y - 1) / s.y;
@@ -660,9 +733,10 @@ int run_rows(const NormArgs& p, const Spread& sp, bool backward, cudaStream_t s)
   const char* what = "gated_residual_norm_backward";
   const int sums = sums_of(MODE, p.gate_kind);
   size_t smem;
-  const int64_t blocks = bwd_blocks(sp, p.R, sums, &smem);
+  NormArgs q = p;
+  const int64_t blocks = bwd_blocks(sp, p.R, sums, (int)sizeof(T), &smem, &q.ahead);
   if (int rc = allow_smem<k_norm_bwd_rows<T, W, NV, MODE>>(what, smem)) return rc;
-  k_norm_bwd_rows<T, W, NV, MODE><<<(unsigned)blocks, block, smem, s>>>(p);
+  k_norm_bwd_rows<T, W, NV, MODE><<<(unsigned)blocks, block, smem, s>>>(q);
   if (int rc = launch_check(what)) return rc;
   k_norm_columns<T><<<dim3((unsigned)((p.D + 31) / 32), (unsigned)sums), dim3(32, 32), 0, s>>>(p, (int)blocks);
   return launch_check(what);
@@ -703,7 +777,7 @@ int width_of(const NormArgs& p, size_t size) {
 
 template <class T>
 int launch_rows(const NormArgs& p, bool backward, cudaStream_t s) {
-  const Spread sp = spread_of(p.R, p.D, width_of(p, sizeof(T)), backward);
+  const Spread sp = spread_of(p.R, p.D, width_of(p, sizeof(T)), backward, (int)sizeof(T));
   return !p.z         ? run_spread<T, kPlain>(p, sp, backward, s)
          : p.dropping ? run_spread<T, kDropped>(p, sp, backward, s)
                       : run_spread<T, kBranch>(p, sp, backward, s);
@@ -742,6 +816,9 @@ int check_norm(const char* what, const NormArgs& p, double dropout) {
   if (!(dropout >= 0.0 && dropout <= 1.0))
     return fail(MPB_ERR_INVALID, "%s: dropout %g outside [0, 1]", what, dropout);
   if (p.z && !p.w_post) return fail(MPB_ERR_INVALID, "%s: null w_post", what);
+  for (int64_t sr : {p.x_sr, p.z_sr, p.g_sr, p.dy_sr, p.du_sr, p.y_sr})
+    if (p.R > 1 && (sr <= -kMostStride || sr >= kMostStride))
+      return fail(MPB_ERR_SHAPE, "%s: row stride of %lld elements", what, (long long)sr);
   return MPB_OK;
 }
 
@@ -762,7 +839,7 @@ int mpb_gated_residual_norm(int64_t R, int64_t D, int dtype, const void* x, int6
   p.scale = (float)scale, p.eps = (float)eps, p.y = y, p.u = u, p.rstd_out = rstd;
   if (int rc = check_norm("gated_residual_norm", p, dropout)) return rc;
   p.drop = make_dropper(dropout, seed, offset);
-  p.dropping = p.drop.drop != 0 || p.drop.all;
+  p.dropping = p.drop.drop != 0;
   if (dtype != MPB_F32 && dtype != MPB_F16 && dtype != MPB_BF16)
     return fail(MPB_ERR_DTYPE, "gated_residual_norm: dtype %d not supported (float16, bfloat16, float32)", dtype);
   if (R == 0 || D == 0) return MPB_OK;
@@ -779,7 +856,9 @@ size_t mpb_gated_residual_norm_scratch_bytes(int64_t R, int64_t D, int dtype, in
   int64_t most = 0;  // blocks, for any width the addresses may allow
   for (int W : {8, 2, 1}) {
     size_t smem;
-    const int64_t n = bwd_blocks(spread_of(R, (D + W - 1) / W * W, W, true), R, sums, &smem);
+    int ahead;
+    const Spread sp = spread_of(R, (D + W - 1) / W * W, W, true, dtype == MPB_F32 ? 4 : 2);
+    const int64_t n = bwd_blocks(sp, R, sums, dtype == MPB_F32 ? 4 : 2, &smem, &ahead);
     most = n > most ? n : most;
   }
   return (size_t)most * sums * (size_t)D * sizeof(float);
@@ -800,7 +879,7 @@ int mpb_gated_residual_norm_backward(int64_t R, int64_t D, int dtype, const void
   p.dx = dx, p.dz = dz, p.dgate = dgate, p.dw_post = dw_post, p.dw_pre = dw_pre, p.part = (float*)scratch;
   if (int rc = check_norm(what, p, dropout)) return rc;
   p.drop = make_dropper(dropout, seed, offset);
-  p.dropping = p.drop.drop != 0 || p.drop.all;
+  p.dropping = p.drop.drop != 0;
   if (dtype != MPB_F32 && dtype != MPB_F16 && dtype != MPB_BF16)
     return fail(MPB_ERR_DTYPE, "%s: dtype %d not supported (float16, bfloat16, float32)", what, dtype);
   if (D == 0) return MPB_OK;
