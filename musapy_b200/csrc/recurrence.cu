@@ -69,6 +69,7 @@ struct ScanArgs {
   FastDiv by_groups, by_groups_per, by_lanes_per, by_chains, by_heads_per;
   int steps;                  // of a tile
   int walk;                   // a block takes whole chains
+  int wide;                   // every input's rows can be copied 16 bytes at a time
   // scratch
   uint32_t *ticket, *status;
   uint64_t* maps;    // (tiles, channels of a group): {A, B}
@@ -105,6 +106,7 @@ MPB_D float finite(float a) { return fminf(fmaxf(a, -3.0e38f), 3.0e38f); }
 // Where a lane works.
 struct Lane {
   int64_t b, ch, gate;  // sequence, first channel, its gate
+  int64_t ch0, end;     // the warp's first channel and the one after its last
   int64_t head;         // the warp's first gate
   int slot;             // the lane's gate among the warp's
   bool in;
@@ -119,6 +121,8 @@ MPB_D Lane place(const ScanArgs& p, uint32_t chain, int lane) {
   if (!SHARED) {
     l.ch = l.gate = l.head = ((int64_t)group * 32 + lane) * V;
     l.slot = 0;
+    l.ch0 = (int64_t)group * 32 * V;
+    l.end = p.D;
     l.in = l.ch < p.D;
   } else if (p.groups_per > 1) {  // a head's channels in several groups
     uint32_t head, part;
@@ -127,6 +131,8 @@ MPB_D Lane place(const ScanArgs& p, uint32_t chain, int lane) {
     l.gate = l.head = head;
     l.slot = 0;
     l.ch = head * p.P + c;
+    l.ch0 = head * p.P + (int64_t)part * 32 * V;
+    l.end = (head + 1) * p.P;
     l.in = c < p.P;
   } else {  // one or several heads in a group
     uint32_t head, at;
@@ -135,6 +141,8 @@ MPB_D Lane place(const ScanArgs& p, uint32_t chain, int lane) {
     l.head = (int64_t)group * p.heads_per;
     l.gate = l.head + head;
     l.slot = l.in ? (int)head : 0;
+    l.ch0 = l.head * p.P;
+    l.end = (l.head + p.heads_per < p.H ? l.head + p.heads_per : p.H) * p.P;
     l.ch = l.gate * p.P + (int64_t)at * V;
   }
   if (!l.in) l.ch = l.gate = 0;
@@ -404,6 +412,22 @@ struct Column {
       }
     }
   }
+  // 16 bytes at a time, a warp's rows of 32 words by as many lanes as a row
+  // takes: a quarter of the copies. src: the lane's part of the warp's first row;
+  // `mine`: it lies inside the row.
+  static constexpr int kLanes = kElems * 2;  // of 16 bytes, for a row of 32 lanes' elements
+  static constexpr int kRows = 32 / kLanes;  // rows per copy of the warp
+  template <int STEPS>
+  static MPB_D void copy_wide(uint32_t base, const char* src, int64_t st, int n, bool mine) {
+    const int lane = threadIdx.x & 31, row = lane / kLanes;
+    base += (row * kWarps * 32 + (threadIdx.x & ~31)) * kWord + lane % kLanes * 16;
+#pragma unroll
+    for (int j = 0; j < STEPS; j += kRows) {
+      if (mine && row + j < n)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + j * kWarps * 32 * kWord), "l"(src) : "memory");
+      src = ahead_by(src, st * kRows);
+    }
+  }
   // half: of a single 16-bit element, bit 1 of its address
   static MPB_D Pack<T, N> get(const char* base, int i, uint32_t half) {
     Pack<T, N> v;
@@ -469,6 +493,7 @@ struct Place {
   int left;   // steps from the warp's first one to the end of the sequence; 0 on an idle lane
   int end;    // the same on every lane
   int heads;  // gates of the warp, where channels share them
+  uint32_t wide;  // wide_lane
   template <class F>
   MPB_D void go(const ScanArgs& p, const Order<WALK>& o, int warp, const int64_t (&st)[N], F place_at) {
     if (!WALK || o.chunk == 0) {
@@ -482,6 +507,28 @@ struct Place {
   }
   MPB_D int steps() const { return left < PER ? left : PER; }
 };
+
+// Where a lane's copies of a column start, from the first row's start; st: bytes between steps.
+template <class C, class T>
+MPB_D const char* at_lane(const ScanArgs& p, const char* row, const Lane& l, int64_t st, int lane) {
+  return p.wide ? row + l.ch0 * (int)sizeof(T) + lane % C::kLanes * 16 + lane / C::kLanes * st : row + l.ch * (int)sizeof(T);
+}
+template <class C, int STEPS>
+MPB_D void copy_column(const ScanArgs& p, uint32_t base, const char* src, int64_t st, int left, int end, uint32_t wide) {
+  if (p.wide) C::template copy_wide<STEPS>(base, src, st, end, wide >> (C::kElems / 4) & 1);
+  else C::template copy<STEPS>(base, src, st, left);
+}
+// Bit n: the lane's 16 bytes of a row of 32 words of 4 n bytes lie inside the warp's channels.
+template <int V>
+MPB_D uint32_t wide_lane(const Lane& l, int lane) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int n = 1; n <= 2; ++n) {
+    const int per = 4 * V / n;  // channels in 16 bytes of such a row
+    if (per > 0 && l.ch0 + (lane % (8 * n)) * per < l.end) bits |= 1u << n;
+  }
+  return bits;
+}
 
 template <class X, class G, int V, bool SHARED>
 struct FwdTile {
@@ -503,11 +550,17 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan(ScanArgs p) {
   Order<WALK> cur, ahead;
   cur.first();
   ahead.first();
+  // The block's first tickets are taken one after the other, so that every
+  // running block has its first tile before any has its second: a tile's
+  // predecessors are then worked on at the same time, not behind others.
+  auto take = [&](int s) {
+    if (threadIdx.x == 0) sh.tiles[s] = atomicAdd(p.ticket, 1u);
+    __syncthreads();
+  };
   if (WALK) {
     if (p.status && blockIdx.x == 0 && threadIdx.x == 0) *p.status = MPB_OK;  // nothing waits
   } else {
-    if (threadIdx.x < NST) sh.tiles[threadIdx.x] = atomicAdd(p.ticket, 1u);
-    __syncthreads();
+    take(0);
   }
   const int64_t in_st[2] = {p.x_st * (int64_t)sizeof(X), p.g_st * (int64_t)sizeof(G)};
   const int64_t out_st[1] = {p.D * (int64_t)sizeof(X)};
@@ -518,29 +571,35 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan(ScanArgs p) {
       from.go(p, ahead, warp, in_st, [&](const Order<WALK>& o, auto& f) {
         const Lane l = place<V, SHARED>(p, o.chain, lane);
         const int64_t t0 = (int64_t)o.chunk * p.steps + warp * kFwd;
-        f.at[0] = (const char*)((const X*)p.x + l.b * p.x_sb + t0 * p.x_st + l.ch);
-        f.at[1] = (const char*)((const G*)p.gate + l.b * p.g_sb + t0 * p.g_st + l.head);
+        const char* x = (const char*)((const X*)p.x + l.b * p.x_sb + t0 * p.x_st);
+        const char* g = (const char*)((const G*)p.gate + l.b * p.g_sb + t0 * p.g_st);
+        f.at[0] = at_lane<typename Tile::CX, X>(p, x, l, in_st[0], lane);
+        f.at[1] = SHARED ? g + l.head * sizeof(G) : at_lane<typename Tile::CG, G>(p, g, l, in_st[1], lane);
+        f.wide = wide_lane<V>(l, lane);
         f.end = (int)(p.T - t0);
         f.left = l.in ? f.end : 0;
         f.heads = SHARED ? (int)(p.H - l.head < p.heads_per ? p.H - l.head : p.heads_per) : 0;
       });
-      Tile::CX::template copy<kFwd>(base + s * Tile::kBytes, from.at[0], in_st[0], from.left);
+      copy_column<typename Tile::CX, kFwd>(p, base + s * Tile::kBytes, from.at[0], in_st[0], from.left, from.end, from.wide);
       const uint32_t q = base + s * Tile::kBytes + Tile::kG;
       if constexpr (SHARED) HeadGates<G, kFwd>::copy(q, from.at[1], in_st[1], from.end, (int)p.heads_per, from.heads, p.by_heads_per);
-      else Tile::CG::template copy<kFwd>(q, from.at[1], in_st[1], from.left);
+      else copy_column<typename Tile::CG, kFwd>(p, q, from.at[1], in_st[1], from.left, from.end, from.wide);
       ahead.next(p);
     }
     copies_commit();
   };
 #pragma unroll
-  for (int s = 0; s < NST - 1; ++s) copy(s, s);
+  for (int s = 0; s < NST - 1; ++s) {
+    copy(s, s);
+    if (!WALK) take(s + 1);
+  }
   int stage = 0;
   Floats<V> carry = vset<V>(0.0f);
   size_t state_at = 0;
   int gate_slot = 0;
   uint32_t half_x = 0, half_g = 0;  // bit 1 of the addresses of single 16-bit elements at step 0
   for (int it = 0; cur.here(p, sh.tiles, it); ++it) {
-    if (SHARED) __syncwarp();  // the stage's gates have been read by every lane
+    __syncwarp();  // the stage that is filled next has been read by every lane
     copy(it + NST - 1, stage == 0 ? NST - 1 : stage - 1);
     to.go(p, cur, warp, out_st, [&](const Order<WALK>& o, auto& f) {
       const Lane l = place<V, SHARED>(p, o.chain, lane);
@@ -567,7 +626,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan(ScanArgs p) {
                        : 0;
     }
     copies_wait<NST - 1>();
-    if (SHARED) __syncwarp();  // the gates that other lanes have copied
+    __syncwarp();  // the words that other lanes have copied
     const char* mine = ring + stage * Tile::kBytes;
     // Steps after the last are computed from whatever the ring holds: nothing
     // follows them in the chain, and they are not written.
@@ -661,11 +720,17 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd(ScanArgs p) {
   Order<WALK> cur, ahead;
   cur.first();
   ahead.first();
+  // The block's first tickets are taken one after the other, so that every
+  // running block has its first tile before any has its second: a tile's
+  // predecessors are then worked on at the same time, not behind others.
+  auto take = [&](int s) {
+    if (threadIdx.x == 0) sh.tiles[s] = atomicAdd(p.ticket, 1u);
+    __syncthreads();
+  };
   if (WALK) {
     if (p.status && blockIdx.x == 0 && threadIdx.x == 0) *p.status = MPB_OK;  // nothing waits
   } else {
-    if (threadIdx.x < NST) sh.tiles[threadIdx.x] = atomicAdd(p.ticket, 1u);
-    __syncthreads();
+    take(0);
   }
   const int64_t in_st[4] = {-p.dh_st * (int64_t)sizeof(X), -p.h_st * (int64_t)sizeof(X), -p.x_st * (int64_t)sizeof(X),
                             -p.g_st * (int64_t)sizeof(G)};
@@ -677,33 +742,41 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd(ScanArgs p) {
       from.go(p, ahead, warp, in_st, [&](const Order<WALK>& o, auto& f) {
         const Lane l = place<V, SHARED>(p, o.chain, lane);
         const int64_t r0 = (int64_t)o.chunk * p.steps + warp * kBwd, t0 = p.T - 1 - r0;
-        f.at[0] = (const char*)((const X*)p.dh + l.b * p.dh_sb + t0 * p.dh_st + l.ch);
-        f.at[1] = (const char*)((const X*)p.hsaved + l.b * p.h_sb + (t0 - 1) * p.h_st + l.ch);
-        f.at[2] = (const char*)((const X*)p.x + l.b * p.x_sb + t0 * p.x_st + l.ch);
-        f.at[3] = (const char*)((const G*)p.gate + l.b * p.g_sb + t0 * p.g_st + l.head);
+        const char* g = (const char*)((const G*)p.gate + l.b * p.g_sb + t0 * p.g_st);
+        f.at[0] = at_lane<typename Tile::CX, X>(p, (const char*)((const X*)p.dh + l.b * p.dh_sb + t0 * p.dh_st), l, in_st[0], lane);
+        f.at[1] = at_lane<typename Tile::CX, X>(p, (const char*)((const X*)p.hsaved + l.b * p.h_sb + (t0 - 1) * p.h_st), l, in_st[1], lane);
+        f.at[2] = at_lane<typename Tile::CX, X>(p, (const char*)((const X*)p.x + l.b * p.x_sb + t0 * p.x_st), l, in_st[2], lane);
+        f.at[3] = SHARED ? g + l.head * sizeof(G) : at_lane<typename Tile::CG, G>(p, g, l, in_st[3], lane);
+        f.wide = wide_lane<V>(l, lane);
         f.end = (int)(p.T - r0);
         f.left = l.in ? f.end : 0;
         f.heads = SHARED ? (int)(p.H - l.head < p.heads_per ? p.H - l.head : p.heads_per) : 0;
       });
       const uint32_t q = base + s * Tile::kBytes;
-      Tile::CX::template copy<kBwd>(q, from.at[0], in_st[0], from.left);
-      Tile::CX::template copy<kBwd>(q + Tile::kH, from.at[1], in_st[1], from.left - 1);  // h[-1] is h0
-      if (SIG) Tile::CX::template copy<kBwd>(q + Tile::kX, from.at[2], in_st[2], from.left);
+      auto column = [&](uint32_t to, int k, int less) {
+        copy_column<typename Tile::CX, kBwd>(p, to, from.at[k], in_st[k], from.left - less, from.end - less, from.wide);
+      };
+      column(q, 0, 0);
+      column(q + Tile::kH, 1, 1);  // h[-1] is h0
+      if (SIG) column(q + Tile::kX, 2, 0);
       if constexpr (SHARED) HeadGates<G, kBwd>::copy(q + Tile::kG, from.at[3], in_st[3], from.end, (int)p.heads_per, from.heads, p.by_heads_per);
-      else Tile::CG::template copy<kBwd>(q + Tile::kG, from.at[3], in_st[3], from.left);
+      else copy_column<typename Tile::CG, kBwd>(p, q + Tile::kG, from.at[3], in_st[3], from.left, from.end, from.wide);
       ahead.next(p);
     }
     copies_commit();
   };
 #pragma unroll
-  for (int s = 0; s < NST - 1; ++s) copy(s, s);
+  for (int s = 0; s < NST - 1; ++s) {
+    copy(s, s);
+    if (!WALK) take(s + 1);
+  }
   int stage = 0;
   Floats<V> carry = vset<V>(0.0f);
   size_t state_at = 0;
   int gate_slot = 0;
   uint32_t half0[4] = {};  // bit 1 of the addresses of single 16-bit elements at the sequence's last step
   for (int it = 0; cur.here(p, sh.tiles, it); ++it) {
-    if (SHARED) __syncwarp();  // the stage's gates have been read by every lane
+    __syncwarp();  // the stage that is filled next has been read by every lane
     copy(it + NST - 1, stage == 0 ? NST - 1 : stage - 1);
     to.go(p, cur, warp, out_st, [&](const Order<WALK>& o, auto& f) {
       const Lane l = place<V, SHARED>(p, o.chain, lane);
@@ -733,7 +806,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd(ScanArgs p) {
                        : 0;
     }
     copies_wait<NST - 1>();
-    if (SHARED) __syncwarp();  // the gates that other lanes have copied
+    __syncwarp();  // the words that other lanes have copied
     const char* mine = ring + stage * Tile::kBytes;
     Floats<V> ma = vset<V>(1.0f), mb = vset<V>(0.0f), in;
     auto gate_at = [&](int i, Floats<V>& a, Floats<V>& om) {
@@ -883,6 +956,21 @@ bool pairs(const ScanArgs& p, int x_dt, int g_dt, bool backward) {
 // ((8, 4096, 2048) bf16) take 112 us walked and 143 us by look-back; 32 ((1, 65536,
 // 1000) f32) take 960 us walked and 696 us by look-back.
 constexpr uint32_t kWalkFrom = 148;
+
+// Copies of 16 bytes: every row of every input starts on such a boundary, and
+// so does every head. (Of 16-bit types with two channels per lane; with one the
+// words in shared memory are wider than the elements.)
+bool wide(const ScanArgs& p, int V, int x_dt, int g_dt, bool backward, bool sig) {
+  const int64_t xs = x_dt == MPB_F32 ? 4 : 2, gs = g_dt == MPB_F32 ? 4 : 2;
+  if (xs * V < 4) return false;
+  auto fits = [](const void* q, int64_t sb, int64_t st, int64_t size) {
+    return (uintptr_t)q % 16 == 0 && sb * size % 16 == 0 && st * size % 16 == 0;
+  };
+  if (p.D * xs % 16 != 0 || (p.H != p.D && p.P * xs % 16 != 0)) return false;
+  if ((!backward || sig) && !fits(p.x, p.x_sb, p.x_st, xs)) return false;
+  if (p.H == p.D && !fits(p.gate, p.g_sb, p.g_st, gs)) return false;
+  return !backward || (fits(p.dh, p.dh_sb, p.dh_st, xs) && fits(p.hsaved, p.h_sb, p.h_st, xs));
+}
 
 // The channel groups and tiles for V channels per lane and `per` steps per warp.
 void lay_out(ScanArgs& p, int V, int per) {
@@ -1091,6 +1179,7 @@ int mpb_gated_scan(int64_t B, int64_t T, int64_t D, int64_t H, const void* x, in
     if (!x || !gate || !h) return fail(MPB_ERR_INVALID, "%s: null pointer", what);
     if (int rc = check_scratch(what, scratch_need(p, false), scratch, scratch_bytes)) return rc;
     const int V = pairs(p, x_dtype, gate_dtype, false) ? 2 : 1;
+    p.wide = wide(p, V, x_dtype, gate_dtype, false, mode == MPB_SCAN_SIGMOID);
     return launch_fwd<decltype(xt), decltype(gt), decltype(sig)::value>(p, V, scratch, s);
   });
 }
@@ -1114,6 +1203,7 @@ int mpb_gated_scan_backward(int64_t B, int64_t T, int64_t D, int64_t H, const vo
     if (!dh || !x || !gate || !h || !dx || !dgate) return fail(MPB_ERR_INVALID, "%s: null pointer", what);
     if (int rc = check_scratch(what, scratch_need(p, true), scratch, scratch_bytes)) return rc;
     const int V = pairs(p, x_dtype, gate_dtype, true) ? 2 : 1;
+    p.wide = wide(p, V, x_dtype, gate_dtype, true, mode == MPB_SCAN_SIGMOID);
     return launch_bwd<decltype(xt), decltype(gt), decltype(sig)::value>(p, V, scratch, s);
   });
 }

@@ -26,7 +26,6 @@
 // Rows too long for that (above 16384 elements) are read again for each pass.
 //
 // Bound: memory.
-#include "async_copy.cuh"
 #include "common.cuh"
 #include "internal.h"
 #include "musapy_b200.h"
@@ -49,7 +48,6 @@ struct NormArgs {
   float scale, eps;
   Dropper drop;
   int dropping;
-  int ahead;  // backward: the next row is copied while one is worked on
 };
 
 constexpr int kThreads = 256;     // a row longer than kInRegisters
@@ -237,23 +235,6 @@ struct Elems {
   MPB_D void load(const T* q) {
 #pragma unroll
     for (int k = 0; k < kWords; ++k) w[k] = __ldcs(reinterpret_cast<const Wd*>(q) + k);
-  }
-  // cp.async of the words, to be read back with `fetch` by the same thread
-  MPB_D static void prefetch(uint32_t smem, uint32_t pitch, const T* q) {
-#pragma unroll
-    for (int k = 0; k < kWords; ++k) {
-      if constexpr (kWordBytes == 16) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem + k * pitch), "l"((const Wd*)q + k) : "memory");
-      } else if constexpr (kWordBytes >= 4) {
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem + k * pitch), "l"((const Wd*)q + k),
-                     "n"(kWordBytes)
-                     : "memory");
-      }
-    }
-  }
-  MPB_D void fetch(const char* smem, uint32_t pitch) {
-#pragma unroll
-    for (int k = 0; k < kWords; ++k) w[k] = *reinterpret_cast<const Wd*>(smem + k * pitch);
   }
   MPB_D void store(T* q) const {
 #pragma unroll
@@ -498,53 +479,28 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
   for (int i = tid; i < sums * slots * W; i += step) acc[i] = 0.0f;
   if (step == 32) __syncwarp();
   else __syncthreads();
-  // A row's words come through shared memory, copied while the row before is
-  // worked on; each thread copies and reads its own, so no barrier is needed.
-  // (Single 16-bit elements are too small for such copies and are loaded.)
-  const bool ahead = E::kWordBytes >= 4 && p.ahead;
-  const int all = blockDim.x * blockDim.y;
-  const uint32_t pitch = all * E::kWordBytes;
-  char* ring = reinterpret_cast<char*>(columns + (size_t)blockDim.y * sums * slots * W) +
-               (threadIdx.y * step + tid) * E::kWordBytes;
-  const int64_t stride = (int64_t)gridDim.x * blockDim.y;
-  const bool full_gate = MODE != kPlain && p.gate_kind == MPB_GATE_FULL;
-  // f(stream, pack, pointer) for every pack that the thread has of row r
-  auto streams = [&](int r, auto f) {
+  int side = 0;
+  for (int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; row < p.R;
+       row += (int64_t)gridDim.x * blockDim.y, side ^= 1) {
+    const int r = (int)row;
     const T *dyr = row_at<T>(p.dy, r, p.dy_sr, skip), *dur = row_at<T>(p.du, r, p.du_sr, skip);
     const T *yr = row_at<T>(p.yin, r, p.y_sr, skip), *zr = row_at<T>(p.z, r, p.z_sr, skip);
-    const T* gr = row_at<T>(p.gate, r, full_gate ? p.g_sr : 0, skip);
+    const T* gr = row_at<T>(p.gate, r, p.gate_kind == MPB_GATE_FULL ? p.g_sr : 0, skip);
+    E du[NV], y[NV], dy[NV], z[NV], g[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k)
       if (tid + k * step < packs) {
         const int at = k * step * W;
         if (p.du) {
-          f(0, k, dur + at);
-          f(1, k, yr + at);
+          du[k].load(dur + at);
+          y[k].load(yr + at);
         }
-        if (p.dy) f(2, k, dyr + at);
-        if (MODE != kPlain) f(3, k, zr + at);
-        if (full_gate) f(4, k, gr + at);
+        if (p.dy) dy[k].load(dyr + at);
+        if (MODE != kPlain) {
+          z[k].load(zr + at);
+          if (p.gate_kind == MPB_GATE_FULL) g[k].load(gr + at);
+        }
       }
-  };
-  auto slot = [&](int stream, int k) { return (uint32_t)(stream * NV + k) * E::kWords * pitch; };
-  auto copy_row = [&](int r) {
-    streams(r, [&](int stream, int k, const T* q) { E::prefetch(smem_u32(ring) + slot(stream, k), pitch, q); });
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  const int64_t row0 = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (ahead && row0 < p.R) copy_row((int)row0);
-  int side = 0;
-  for (int64_t row = row0; row < p.R; row += stride, side ^= 1) {
-    const int r = (int)row;
-    E in[5][NV];
-    if (ahead) {
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      streams(r, [&](int stream, int k, const T*) { in[stream][k].fetch(ring + slot(stream, k), pitch); });
-      if (row + stride < p.R) copy_row((int)(row + stride));
-    } else {
-      streams(r, [&](int stream, int k, const T* q) { in[stream][k].load(q); });
-    }
-    E(&du)[NV] = in[0], (&y)[NV] = in[1], (&dy)[NV] = in[2], (&z)[NV] = in[3], (&g)[NV] = in[4];
     const float rz = MODE != kPlain ? p.rstd[r] : 0.0f, ry = p.rstd[(MODE != kPlain ? p.R : 0) + r];
     float back = 0.0f;  // of y in dx: r_y^3 mean(y w du)
     if (p.du) {
@@ -698,13 +654,10 @@ int sums_of(int mode, int gate_kind) { return mode == kPlain ? 1 : gate_kind == 
 
 // Blocks of the backward kernel: what fits the SMs at up to 128 registers per
 // thread and by shared memory, or the rows if they are fewer.
-int64_t bwd_blocks(const Spread& s, int64_t R, int sums, int size, size_t* smem, int* ahead) {
-  const size_t elements = (size_t)s.x * s.NV * s.W * s.y, room = 220u << 10;
-  *smem = elements * (sizeof(float) * sums + 5 * size);
-  *ahead = s.W * size >= 4 && *smem <= room;
-  if (!*ahead) *smem = elements * sizeof(float) * sums;
+int64_t bwd_blocks(const Spread& s, int64_t R, int sums, size_t* smem) {
+  *smem = (size_t)s.x * s.NV * s.W * s.y * sizeof(float) * sums;
   int64_t per_sm = kRowThreads / (s.x * s.y);
-  const int64_t by_smem = (int64_t)((room + 4096) / (*smem + 2048));
+  const int64_t by_smem = (int64_t)((224u << 10) / (*smem + 2048));
   if (per_sm > by_smem) per_sm = by_smem;
   if (per_sm < 1) per_sm = 1;
   const int64_t most = per_sm * sm_count(), want = (R + s.y - 1) / s.y;
@@ -733,10 +686,9 @@ int run_rows(const NormArgs& p, const Spread& sp, bool backward, cudaStream_t s)
   const char* what = "gated_residual_norm_backward";
   const int sums = sums_of(MODE, p.gate_kind);
   size_t smem;
-  NormArgs q = p;
-  const int64_t blocks = bwd_blocks(sp, p.R, sums, (int)sizeof(T), &smem, &q.ahead);
+  const int64_t blocks = bwd_blocks(sp, p.R, sums, &smem);
   if (int rc = allow_smem<k_norm_bwd_rows<T, W, NV, MODE>>(what, smem)) return rc;
-  k_norm_bwd_rows<T, W, NV, MODE><<<(unsigned)blocks, block, smem, s>>>(q);
+  k_norm_bwd_rows<T, W, NV, MODE><<<(unsigned)blocks, block, smem, s>>>(p);
   if (int rc = launch_check(what)) return rc;
   k_norm_columns<T><<<dim3((unsigned)((p.D + 31) / 32), (unsigned)sums), dim3(32, 32), 0, s>>>(p, (int)blocks);
   return launch_check(what);
@@ -856,9 +808,8 @@ size_t mpb_gated_residual_norm_scratch_bytes(int64_t R, int64_t D, int dtype, in
   int64_t most = 0;  // blocks, for any width the addresses may allow
   for (int W : {8, 2, 1}) {
     size_t smem;
-    int ahead;
     const Spread sp = spread_of(R, (D + W - 1) / W * W, W, true, dtype == MPB_F32 ? 4 : 2);
-    const int64_t n = bwd_blocks(sp, R, sums, dtype == MPB_F32 ? 4 : 2, &smem, &ahead);
+    const int64_t n = bwd_blocks(sp, R, sums, &smem);
     most = n > most ? n : most;
   }
   return (size_t)most * sums * (size_t)D * sizeof(float);
