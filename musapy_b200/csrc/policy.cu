@@ -17,7 +17,8 @@
 // barrier guards them), folds maximum and sum of exponentials as the copies
 // arrive, joins them over the cluster, and turns the row into its gradient
 // from shared memory. Blocks of up to 72 KB leave room for three per SM, so one
-// row's copies run under another's stores. Rows that are too long for eight
+// row's copies run under another's stores. Rows of at most 4 KB are a warp's,
+// held in registers. Rows that are too long for eight
 // blocks, or whose gradient is aligned otherwise than the logits, take three
 // passes over global memory.
 //
@@ -93,18 +94,18 @@ MPB_D float block_max(float v, float* red) {
 
 // A masked token: zeros.
 template <class T>
-MPB_D void write_masked(const PolicyArgs& p, int64_t i, int64_t from, int64_t to) {
+MPB_D void write_masked(const PolicyArgs& p, int64_t i, int64_t from, int64_t to, int tid, int threads) {
   T* g = (T*)p.grad + i * p.V;
   if (p.grad) {
     // whole 16-byte words where the row has them
     constexpr int E = 16 / sizeof(T);
     const int64_t head = (int64_t)((16 - ((uintptr_t)(g + from) & 15)) & 15) / (int64_t)sizeof(T);
     const int64_t body = from + (head < to - from ? head : to - from), words = (to - body) / E;
-    for (int64_t j = from + threadIdx.x; j < body; j += blockDim.x) g[j] = Cvt<T>::from(0.0f);
-    for (int64_t w = threadIdx.x; w < words; w += blockDim.x) st_stream16(g + body + w * E, make_uint4(0, 0, 0, 0));
-    for (int64_t j = body + words * E + threadIdx.x; j < to; j += blockDim.x) g[j] = Cvt<T>::from(0.0f);
+    for (int64_t j = from + tid; j < body; j += threads) g[j] = Cvt<T>::from(0.0f);
+    for (int64_t w = tid; w < words; w += threads) st_stream16(g + body + w * E, make_uint4(0, 0, 0, 0));
+    for (int64_t j = body + words * E + tid; j < to; j += threads) g[j] = Cvt<T>::from(0.0f);
   }
-  if (from == 0 && threadIdx.x == 0) {
+  if (from == 0 && tid == 0) {
     p.each[i] = p.logp[i] = p.kl[i] = 0.0f;
     p.clipped[i] = 0;
   }
@@ -228,7 +229,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_policy_row(PolicyArgs p, int
   const int mine = (int)(all_words - w0 < per ? (all_words > w0 ? all_words - w0 : 0) : per);
   if (p.mask && !p.mask[i]) {  // the whole cluster leaves here
     const int64_t from = rank == 0 ? 0 : head + w0 * E, to = rank == blocks - 1 ? p.V : head + (w0 + per) * E;
-    write_masked<T>(p, i, from < p.V ? from : p.V, to < p.V ? to : p.V);
+    write_masked<T>(p, i, from < p.V ? from : p.V, to < p.V ? to : p.V, threadIdx.x, blockDim.x);
     return;
   }
   if (blocks > 1) cluster.barrier_arrive();  // every block of the cluster runs
@@ -345,6 +346,86 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_policy_row(PolicyArgs p, int
     g[t] = Cvt<T>::from(fmaf(down, exp_from(zt, -all_base), slope));
 }
 
+// A warp per token, its logits in registers: rows of at most kLaneWords 16-byte
+// words per lane.
+constexpr int kLaneWords = 8;
+constexpr int kWarpRows = 8;  // warps, tokens, per block
+
+template <class T>
+__global__ void __launch_bounds__(kWarpRows * 32) k_policy_warp(PolicyArgs p) {
+  __shared__ float red[32];
+  constexpr int E = 16 / (int)sizeof(T);
+  const int lane = threadIdx.x & 31;
+  const int64_t i = (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5);
+  const float count = p.grad ? tokens_in_mask(p, red) : 1.0f;
+  if (i >= p.N) return;
+  if (p.mask && !p.mask[i]) {
+    write_masked<T>(p, i, 0, p.V, lane, 32);
+    return;
+  }
+  const T* z = (const T*)p.logits + i * p.l_sr;
+  int head = (int)((16 - ((uintptr_t)z & 15)) & 15) / (int)sizeof(T);
+  if (head > p.V) head = (int)p.V;
+  const int words = ((int)p.V - head) / E, tail = head + words * E;
+  const uint4* src = reinterpret_cast<const uint4*>(z + head);
+  uint4 v[kLaneWords];
+#pragma unroll
+  for (int k = 0; k < kLaneWords; ++k) v[k] = lane + k * 32 < words ? ld_stream16(src + lane + k * 32) : no_words<T>();
+  const int end_at = lane < head ? lane : tail + (lane - head);
+  const bool has_end = lane < head + ((int)p.V - tail);
+  const float end = has_end ? to_f(z[end_at]) : -INFINITY;
+  const int64_t t = target_of(p, i);
+  const bool valid = t >= 0 && t < p.V;
+  const float zt = valid ? to_f(z[t]) : 0.0f;
+  uint4 most = v[0];
+#pragma unroll
+  for (int k = 1; k < kLaneWords; ++k) most = larger<T>(most, v[k]);
+  const float top = warp_max(fmaxf(largest<T>(most), end)), base = top == -INFINITY ? 0.0f : top;
+  float sum = has_end ? exp_from(end, -base) : 0.0f;
+  with_exponent(base, [&](auto e) {
+    float2 s = vset<2>(0.0f);
+#pragma unroll
+    for (int k = 0; k < kLaneWords; ++k) {
+      const Sixteen<T> x(v[k]);
+      if (k * 32 < words)
+#pragma unroll
+        for (int j = 0; j < Sixteen<T>::kPairs; ++j) s = vadd(s, e(x.get(j)));
+    }
+    sum = fmaf(s.x + s.y, e.fix(), sum);
+  });
+  sum = warp_sum(sum);
+  const float logp = valid ? zt - base - logf(sum) : NAN;
+  float value, kl, slope;
+  bool clipped;
+  token_terms(p, i, logp, value, kl, clipped, slope);
+  if (lane == 0) {
+    p.each[i] = value;
+    p.logp[i] = logp;
+    p.kl[i] = kl;
+    p.clipped[i] = clipped;
+  }
+  if (!p.grad) return;
+  T* g = (T*)p.grad + i * p.V;
+  slope *= p.grad_scale / count;
+  const float down = -slope / sum;
+  uint4* out = reinterpret_cast<uint4*>(g + head);
+  with_exponent(base, [&](auto e) {
+    const float2 by = vset<2>(down * e.fix());
+#pragma unroll
+    for (int k = 0; k < kLaneWords; ++k)
+      if (lane + k * 32 < words) {
+        Sixteen<T> x(v[k]);
+#pragma unroll
+        for (int j = 0; j < Sixteen<T>::kPairs; ++j) x.put(j, vmul(e(x.get(j)), by));
+        st_stream16(out + lane + k * 32, x.w);
+      }
+  });
+  if (has_end) g[end_at] = Cvt<T>::from(fmaf(down, exp_from(end, -base), end_at == t ? slope : 0.0f));
+  // the target's element again, by the lane that has written its word
+  if (valid && t >= head && t < tail && (t - head) / E % 32 == lane)
+    g[t] = Cvt<T>::from(fmaf(down, exp_from(zt, -base), slope));
+}
+
 // One block per token, three passes over its logits: maximum, sum, gradient.
 template <class T>
 __global__ void __launch_bounds__(kThreads) k_policy_passes(PolicyArgs p) {
@@ -353,7 +434,7 @@ __global__ void __launch_bounds__(kThreads) k_policy_passes(PolicyArgs p) {
   const T* z = (const T*)p.logits + i * p.l_sr;
   T* g = p.grad ? (T*)p.grad + i * p.V : nullptr;
   if (p.mask && !p.mask[i]) {
-    write_masked<T>(p, i, 0, p.V);
+    write_masked<T>(p, i, 0, p.V, threadIdx.x, blockDim.x);
     return;
   }
   const float count = tokens_in_mask(p, red[0]);
@@ -441,7 +522,11 @@ int launch_policy(PolicyArgs& p, cudaStream_t s) {
     while (blocks < kMostBlocks && (words + blocks - 1) / blocks * 16 > kBlockBytes) blocks *= 2;
     const int64_t per = (words + blocks - 1) / blocks;
     const bool same = !p.grad || (((uintptr_t)p.logits - (uintptr_t)p.grad) % 16 == 0 && (p.l_sr - p.V) * size % 16 == 0);
-    if (same && per * 16 <= kMostBytes && p.N * blocks <= 0x7fffffffLL) {
+    if (same && words <= kLaneWords * 32) {
+      if (int rc = count_before(p, kWarpRows * 32, s)) return rc;
+      k_policy_warp<T><<<(unsigned)((p.N + kWarpRows - 1) / kWarpRows), kWarpRows * 32, 0, s>>>(p);
+      if (int rc = launch_check("policy_loss")) return rc;
+    } else if (same && per * 16 <= kMostBytes && p.N * blocks <= 0x7fffffffLL) {
       const int bytes = (int)per * 16;
       // 16 words per thread where rows are many (small blocks, many of them on
       // an SM), 4 where a row's own latency counts

@@ -238,21 +238,25 @@ MPB_D void look_back(const ScanArgs& p, uint32_t chain, uint32_t chunk, int lane
       break;
     }
   }
-  // the other channels' words of those tiles are there or about to be
-  if (chunk > back && ok)
+  // The other channels' words of those tiles are there or about to be. The
+  // state and the first maps are fetched together: one round trip.
+  constexpr int kTogether = 8;
+  uint32_t state[V] = {};
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      uint32_t w = 0;
-      ok = ok && await(p.states + at(chunk - 1 - back) + v, w);
-      carry[v] = __uint_as_float(w) + 0.0f;
-    }
-  constexpr int kTogether = 8;  // maps fetched at once: their latencies overlap
-  for (uint32_t k0 = chunk - back; k0 < chunk; k0 += kTogether) {
+  for (int v = 0; v < V; ++v)
+    if (chunk > back && ok) state[v] = ld_word(p.states + at(chunk - 1 - back) + v);
+  for (uint32_t k0 = chunk - back, first = 1; first || k0 < chunk; k0 += kTogether, first = 0) {
     uint64_t w[kTogether][V];
 #pragma unroll
     for (int i = 0; i < kTogether; ++i)
 #pragma unroll
       for (int v = 0; v < V; ++v) w[i][v] = k0 + i < chunk ? ld_word(p.maps + at(k0 + i) + v) : 0;
+    if (first && chunk > back && ok)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (!state[v]) ok = await(p.states + at(chunk - 1 - back) + v, state[v]) && ok;
+        carry[v] = __uint_as_float(state[v]) + 0.0f;
+      }
 #pragma unroll
     for (int i = 0; i < kTogether; ++i)
       if (k0 + i < chunk)
@@ -952,10 +956,10 @@ bool pairs(const ScanArgs& p, int x_dt, int g_dt, bool backward) {
   return ok;
 }
 
-// From this many chains on a block walks a chain: a block per SM. 256 chains
-// ((8, 4096, 2048) bf16) take 112 us walked and 143 us by look-back; 32 ((1, 65536,
-// 1000) f32) take 960 us walked and 696 us by look-back.
-constexpr uint32_t kWalkFrom = 148;
+// From this many chains on a block walks a chain. T = 4096, bf16, forward: 64
+// chains take 53 us walked and 44 us by look-back, 96 chains 54 and 58 us, 128
+// chains 55 and 70 us, 256 chains 83 and 107 us.
+constexpr uint32_t kWalkFrom = 80;
 
 // Copies of 16 bytes: every row of every input starts on such a boundary, and
 // so does every head. (Of 16-bit types with two channels per lane; with one the
