@@ -16,7 +16,7 @@ import torch
 from . import dtypes as _dt
 from . import errors
 from ._lib import LIB, NATIVE, check
-from .array import Array
+from .array import _LAYOUTS, Array, contiguous_strides
 from .ops import _CHECK_SCAN_STATUS, _alias, _check_out, _launch, _out, _same_device, _stream, contiguous, full
 
 _MODES = {"linear": 0, "sigmoid": 1}
@@ -52,7 +52,7 @@ def _of(name: str, what: str, x, shape: tuple, d: _dt.Dtype) -> Array:
 def _floats(name: str, what: str, x, shape: tuple) -> Array:
     """A C-contiguous float32 array of `shape`."""
     _of(name, what, x, shape, _dt.float32)
-    return x if x._is_c_contiguous() else contiguous(x)
+    return x if _dense(x) else contiguous(x)
 
 
 def _choice(name: str, what: str, value, table: dict) -> int:
@@ -84,6 +84,30 @@ def _scratch(nbytes: int, dev: int):
 
 def _sptr(scratch):
     return scratch.data_ptr() if scratch is not None else None
+
+
+def _dense(x: Array) -> bool:
+    """x is C-contiguous (by the cached strides of its shape where they are known)."""
+    lay = _LAYOUTS.get(x._shape)
+    return (lay is not None and lay[0] == x._strides) or x._is_c_contiguous()
+
+
+def _carve(dev: int, *parts):
+    """Several small results in one allocation: an Array for each (shape, dtype). To the alias checks each is an
+    allocation of its own (they do not overlap)."""
+    total, at = 0, []
+    for shape, d in parts:
+        at.append(total)
+        total += (_prod(shape) * d.itemsize + 15) & ~15
+    first = _out((max(total, 16),), _dt.uint8, dev)
+    made = []
+    for (shape, d), start in zip(parts, at):
+        a = Array.__new__(Array)
+        a._buf, a._shape, a._strides, a._offset = first._buf, shape, contiguous_strides(shape), start // d.itemsize
+        a._dtype, a._dev, a._name, a._dev_src, a._dt_src = d, dev, None, first._dev_src, first._dt_src
+        a._ptr = a._sid = first._ptr + start
+        made.append(a)
+    return made
 
 
 # ------------------------------------------------------------ gated scan
@@ -195,7 +219,7 @@ def gated_scan_step(state, x, gate, mode="linear", out=None):
     m = _choice(name, "mode", mode, _MODES)
     x, gate, B, _, D, H = _scan_inputs(name, x, gate, False)
     _of(name, "state", state, (B, D), _dt.float32)
-    if not state._is_c_contiguous():
+    if not _dense(state):
         raise errors.ShapeError(f"{name}: state must be C-contiguous (it is updated in place)")
     dev = _same_device(name, x, gate, state)
     if _alias(state, x, gate):
@@ -217,7 +241,7 @@ def _rows(x: Array):
     """(array, row stride): x with unit inner stride and its leading dims as rows one stride apart; a copy of x when
     its layout is another."""
     shape, st = x._shape, x._strides
-    if x._is_c_contiguous():
+    if _dense(x):
         return x, shape[-1]
     if st[-1] == 1 or shape[-1] == 1:
         step, extent = None, None
@@ -262,7 +286,7 @@ def _gate(name: str, gate, x: Array):
         g, sr = _rows(gate)
         return g, _GATE_ROW, sr
     if gate._shape == x._shape[-1:]:
-        return (gate if gate._is_c_contiguous() else contiguous(gate)), _GATE_CHANNEL, 0
+        return (gate if _dense(gate) else contiguous(gate)), _GATE_CHANNEL, 0
     raise errors.ShapeError(f"{name}: gate shape {list(gate.shape)} is neither that of x {list(x.shape)}, a value per "
                             f"row {list(x.shape[:-1]) + [1]} nor per channel {list(x.shape[-1:])}")
 
@@ -367,9 +391,10 @@ def _norm_backward(name, dy, du, y, z, w_post, w_pre, rstd, gate, activation, sc
         return (_out(y._shape, y._dtype, dev), _out(y._shape, y._dtype, dev) if branch else None,
                 zeros(g._shape, y._dtype) if g is not None else None, zeros((D,), _dt.float32) if branch else None,
                 zeros((D,), _dt.float32))
-    dx, dpre = _out(y._shape, y._dtype, dev), _out((D,), _dt.float32, dev)
+    dx = _out(y._shape, y._dtype, dev)
     dz = _out(y._shape, y._dtype, dev) if branch else None
     dpost = _out((D,), _dt.float32, dev) if branch else None
+    dpre = _out((D,), _dt.float32, dev)
     dgate = _out(g._shape, y._dtype, dev) if g is not None else None
     nbytes = NATIVE.gated_residual_norm_scratch_bytes(R, D, y._dtype.code, int(branch), kind)
     scratch = _scratch(nbytes, dev)
@@ -394,7 +419,7 @@ def dropout(x, p, seed, offset=0, out=None):
         _check_out(out, x._shape, x._dtype, dev, name)
         if _alias(out, x):
             raise errors.MemoryError("out= aliases an input buffer (AliasDetected)")
-    src = x if x._is_c_contiguous() else contiguous(x)
+    src = x if _dense(x) else contiguous(x)
     y = out if out is not None else _out(x._shape, x._dtype, dev)
     check(NATIVE.dropout(src.size, src._ptr, src._dtype.code, p, seed, offset, y._ptr, _launch(name, dev, src, y)), name)
     return y
@@ -431,7 +456,7 @@ def policy_loss(logits, targets, old_logp, advantages, ref_logp=None, mask=None,
         raise errors.ShapeError(f"{name}: targets shape {list(targets.shape)} != expected {list(lead)}")
     if targets._dtype.code not in (_dt.I32, _dt.I64):
         raise errors.DtypeError(f"{name}: targets dtype {targets.dtype} not supported (int32, int64)")
-    targets = targets if targets._is_c_contiguous() else contiguous(targets)
+    targets = targets if _dense(targets) else contiguous(targets)
     old, adv = _floats(name, "old_logp", old_logp, lead), _floats(name, "advantages", advantages, lead)
     ins = [z, targets, old, adv]
     if ref_logp is not None:
@@ -441,7 +466,7 @@ def policy_loss(logits, targets, old_logp, advantages, ref_logp=None, mask=None,
         raise errors.MusapyError(f"{name}: kl_coef {kl_coef!r} without ref_logp")
     if mask is not None:
         _of(name, "mask", mask, lead, _dt.bool_)
-        mask = mask if mask._is_c_contiguous() else contiguous(mask)
+        mask = mask if _dense(mask) else contiguous(mask)
         ins.append(mask)
     if clip_high is None:
         clip_high = clip_low
@@ -451,13 +476,12 @@ def policy_loss(logits, targets, old_logp, advantages, ref_logp=None, mask=None,
     if N and V == 0:
         raise errors.ShapeError(f"{name}: empty vocabulary")
     dev = _same_device(name, *ins)
-    loss, logp, kl = _out((), _dt.float32, dev), _out(lead, _dt.float32, dev), _out(lead, _dt.float32, dev)
-    clipped = _out(lead, _dt.bool_, dev)
-    dlogits = _out(z._shape, z._dtype, dev) if grad else None
     nbytes = NATIVE.policy_loss_scratch_bytes(N, V, z._dtype.code)
-    scratch = _scratch(nbytes, dev)
+    loss, logp, kl, clipped, scratch = _carve(dev, ((), _dt.float32), (lead, _dt.float32), (lead, _dt.float32),
+                                              (lead, _dt.bool_), ((nbytes,), _dt.uint8))
+    dlogits = _out(z._shape, z._dtype, dev) if grad else None
     check(NATIVE.policy_loss(N, V, z._ptr, z._dtype.code, zr, targets._ptr, targets._dtype.code, old._ptr, adv._ptr,
                              _ptr(ref_logp), _ptr(mask), float(clip_low), float(clip_high), float(kl_coef),
                              float(grad_scale), loss._ptr, logp._ptr, kl._ptr, clipped._ptr, _ptr(dlogits),
-                             _sptr(scratch), nbytes, _launch(name, dev, *ins, loss, logp, kl, clipped, dlogits)), name)
+                             scratch._ptr, nbytes, _launch(name, dev, *ins, loss, dlogits)), name)
     return PolicyLoss(loss, logp, kl, clipped, dlogits)

@@ -16,8 +16,8 @@
 // its shared memory, in 16-byte words that each thread takes for itself (so no
 // barrier guards them), folds maximum and sum of exponentials as the copies
 // arrive, joins them over the cluster, and turns the row into its gradient
-// from shared memory. Blocks of up to 72 KB leave room for three per SM, so one
-// row's copies run under another's stores. Rows of at most 4 KB are a warp's,
+// from shared memory. Blocks of 64 KB leave room for three per SM, so one row's
+// copies run under another's stores. Rows of at most 4 KB are a warp's,
 // held in registers. Rows that are too long for eight
 // blocks, or whose gradient is aligned otherwise than the logits, take three
 // passes over global memory.
@@ -51,16 +51,23 @@ struct PolicyArgs {
   const float* count;  // tokens in the mask, where a kernel before has counted them
 };
 
+// What a token brings besides its logits, loaded before they are waited for.
+struct Token {
+  float adv, old, ref;
+  MPB_D Token(const PolicyArgs& p, int64_t i) : adv(p.adv[i]), old(p.old_logp[i]), ref(p.ref_logp ? p.ref_logp[i] : 0.0f) {}
+};
+
 // What a token's logp makes of the loss: its value, kl, clipped and d loss / d logp (without the mean's divisor).
-MPB_D void token_terms(const PolicyArgs& p, int64_t i, float logp, float& value, float& kl, bool& clipped, float& slope) {
-  const float a = p.adv[i], rho = __expf(logp - p.old_logp[i]);
+MPB_D void token_terms(const PolicyArgs& p, const Token& token, float logp, float& value, float& kl, bool& clipped,
+                       float& slope) {
+  const float a = token.adv, rho = __expf(logp - token.old);
   clipped = (a > 0.0f && rho > 1.0f + p.hi) || (a < 0.0f && rho < 1.0f - p.lo);
   const float bound = a > 0.0f ? 1.0f + p.hi : 1.0f - p.lo;
   value = -(clipped ? bound : rho) * a;
   slope = clipped ? 0.0f : -rho * a;
   kl = 0.0f;
   if (p.ref_logp) {
-    const float q = p.ref_logp[i] - logp, em = expm1f(q);
+    const float q = token.ref - logp, em = expm1f(q);
     kl = em - q;
     value = fmaf(p.beta, kl, value);
     slope = fmaf(-p.beta, em, slope);
@@ -207,6 +214,10 @@ constexpr int kGroups = 4;  // in which a block's copies arrive
 constexpr int kBatch = 4;   // words a thread folds at once: one maximum, one rescaling of its sum
 constexpr int kMostBlocks = 8;
 
+MPB_D void copy_word16(uint32_t dst, const uint4* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // Block `rank` of the row's cluster takes `per` 16-byte words of it. The
 // elements before the first aligned word and after the last, fewer than a word
 // each, go to the first threads of rank 0.
@@ -227,22 +238,29 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_policy_row(PolicyArgs p, int
   const int64_t all_words = (p.V - head) / E, tail = head + all_words * E;
   const int64_t w0 = (int64_t)rank * per;
   const int mine = (int)(all_words - w0 < per ? (all_words > w0 ? all_words - w0 : 0) : per);
+  const int64_t t = target_of(p, i);
+  const Token token(p, i);
   if (p.mask && !p.mask[i]) {  // the whole cluster leaves here
     const int64_t from = rank == 0 ? 0 : head + w0 * E, to = rank == blocks - 1 ? p.V : head + (w0 + per) * E;
     write_masked<T>(p, i, from < p.V ? from : p.V, to < p.V ? to : p.V, threadIdx.x, blockDim.x);
     return;
   }
-  if (blocks > 1) cluster.barrier_arrive();  // every block of the cluster runs
+  // every block of the cluster runs (nothing is made visible by this)
+  if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const uint4* src = reinterpret_cast<const uint4*>(z + head) + w0;
   const uint32_t dst = smem_u32(words);
   const int each = (mine + threads - 1) / threads;
   const int quarter = (each + kGroups * kBatch - 1) / (kGroups * kBatch) * kBatch;  // words per thread and group
+  // the usual block: sixteen words for every thread, no bounds to check
+  const bool full = mine == kGroups * kBatch * threads;
 #pragma unroll
   for (int q = 0; q < kGroups; ++q) {
-    for (int k = q * quarter; k < (q + 1) * quarter; ++k) {
-      const int w = tid + k * threads;
-      if (w < mine)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + w * 16), "l"(src + w) : "memory");
+    if (full) {
+#pragma unroll
+      for (int k = q * kBatch; k < (q + 1) * kBatch; ++k) copy_word16(dst + (tid + k * threads) * 16, src + tid + k * threads);
+    } else {
+      for (int k = q * quarter; k < (q + 1) * quarter; ++k)
+        if (tid + k * threads < mine) copy_word16(dst + (tid + k * threads) * 16, src + tid + k * threads);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
@@ -257,34 +275,42 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_policy_row(PolicyArgs p, int
     f.top = end == -INFINITY ? -INFINITY : fmaxf(end, -INFINITY);
     f.sum = exp_from(end, -(end == -INFINITY ? 0.0f : end));
   }
-  const int64_t t = target_of(p, i);
   const bool valid = t >= 0 && t < p.V;
   const float zt = valid ? to_f(z[t]) : 0.0f;
   const float count = p.grad ? tokens_in_mask(p, red[0]) : 1.0f;
+  auto fold_batch = [&](const uint4 (&v)[kBatch]) {
+    uint4 most = v[0];
+#pragma unroll
+    for (int j = 1; j < kBatch; ++j) most = larger<T>(most, v[j]);
+    const float m = fmaxf(f.top, largest<T>(most)), b = m == -INFINITY ? 0.0f : m;
+    f.sum *= exp_from(f.top, -b);
+    f.top = m;
+    with_exponent(b, [&](auto e) {
+      float2 s = vset<2>(0.0f);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const Sixteen<T> x(v[j]);
+#pragma unroll
+        for (int i = 0; i < Sixteen<T>::kPairs; ++i) s = vadd(s, e(x.get(i)));
+      }
+      f.sum = fmaf(s.x + s.y, e.fix(), f.sum);
+    });
+  };
   auto fold_group = [&](int q) {
+    uint4 v[kBatch];
+    if (full) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) v[j] = words[tid + (q * kBatch + j) * threads];
+      fold_batch(v);
+      return;
+    }
     for (int k = q * quarter; k < (q + 1) * quarter; k += kBatch) {
-      uint4 v[kBatch];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         const int w = tid + (k + j) * threads;
         v[j] = w < mine ? words[w] : no_words<T>();
       }
-      uint4 most = v[0];
-#pragma unroll
-      for (int j = 1; j < kBatch; ++j) most = larger<T>(most, v[j]);
-      const float m = fmaxf(f.top, largest<T>(most)), b = m == -INFINITY ? 0.0f : m;
-      f.sum *= exp_from(f.top, -b);
-      f.top = m;
-      with_exponent(b, [&](auto e) {
-        float2 s = vset<2>(0.0f);
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const Sixteen<T> x(v[j]);
-#pragma unroll
-          for (int i = 0; i < Sixteen<T>::kPairs; ++i) s = vadd(s, e(x.get(i)));
-        }
-        f.sum = fmaf(s.x + s.y, e.fix(), f.sum);
-      });
+      fold_batch(v);
     }
   };
   asm volatile("cp.async.wait_group 3;" ::: "memory");
@@ -305,7 +331,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_policy_row(PolicyArgs p, int
   float sum = block_sum(f.sum * exp_from(f.top, -base), red[1]);
   float all_top = top;
   if (blocks > 1) {
-    cluster.barrier_wait();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (tid < blocks) *cluster.map_shared_rank(&folds[rank], tid) = make_float2(top, sum);
     cluster.sync();
     Fold c{folds[0].x, folds[0].y};
@@ -317,7 +343,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_policy_row(PolicyArgs p, int
   const float logp = valid ? zt - all_base - logf(sum) : NAN;
   float value, kl, slope;
   bool clipped;
-  token_terms(p, i, logp, value, kl, clipped, slope);
+  token_terms(p, token, logp, value, kl, clipped, slope);
   if (rank == 0 && tid == 0) {
     p.each[i] = value;
     p.logp[i] = logp;
@@ -331,12 +357,17 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_policy_row(PolicyArgs p, int
   uint4* out = reinterpret_cast<uint4*>(g + head) + w0;
   with_exponent(all_base, [&](auto e) {
     const float2 by = vset<2>(down * e.fix());
-#pragma unroll 4
-    for (int w = tid; w < mine; w += threads) {
+    auto word = [&](int w) {
       Sixteen<T> x(words[w]);
 #pragma unroll
       for (int j = 0; j < Sixteen<T>::kPairs; ++j) x.put(j, vmul(e(x.get(j)), by));
       st_stream16(out + w, x.w);
+    };
+    if (full) {
+#pragma unroll
+      for (int k = 0; k < kGroups * kBatch; ++k) word(tid + k * threads);
+    } else {
+      for (int w = tid; w < mine; w += threads) word(w);
     }
   });
   if (has_end) g[end_at] = Cvt<T>::from(fmaf(down, exp_from(end, -all_base), end_at == t ? slope : 0.0f));
@@ -359,6 +390,7 @@ __global__ void __launch_bounds__(kWarpRows * 32) k_policy_warp(PolicyArgs p) {
   const int64_t i = (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5);
   const float count = p.grad ? tokens_in_mask(p, red) : 1.0f;
   if (i >= p.N) return;
+  const Token token(p, i);
   if (p.mask && !p.mask[i]) {
     write_masked<T>(p, i, 0, p.V, lane, 32);
     return;
@@ -397,7 +429,7 @@ __global__ void __launch_bounds__(kWarpRows * 32) k_policy_warp(PolicyArgs p) {
   const float logp = valid ? zt - base - logf(sum) : NAN;
   float value, kl, slope;
   bool clipped;
-  token_terms(p, i, logp, value, kl, clipped, slope);
+  token_terms(p, token, logp, value, kl, clipped, slope);
   if (lane == 0) {
     p.each[i] = value;
     p.logp[i] = logp;
@@ -447,10 +479,11 @@ __global__ void __launch_bounds__(kThreads) k_policy_passes(PolicyArgs p) {
   sum = block_sum(sum, red[2]);
   const int64_t t = target_of(p, i);
   const bool valid = t >= 0 && t < p.V;
+  const Token token(p, i);
   const float logp = valid ? to_f(z[t]) - base - logf(sum) : NAN;
   float value, kl, slope;
   bool clipped;
-  token_terms(p, i, logp, value, kl, clipped, slope);
+  token_terms(p, token, logp, value, kl, clipped, slope);
   if (threadIdx.x == 0) {
     p.each[i] = value;
     p.logp[i] = logp;
@@ -487,7 +520,7 @@ __global__ void __launch_bounds__(1024) k_policy_count(PolicyArgs p, float* coun
 }
 
 // ------------------------------------------------------------------- host
-constexpr int kBlockBytes = 72 << 10;   // of a row, three blocks per SM
+constexpr int64_t kPart = kRowThreads * kGroups * kBatch;
 constexpr int kMostBytes = 208 << 10;   // of a row, where eight blocks have to do
 
 template <class T>
@@ -518,9 +551,10 @@ template <class T>
 int launch_policy(PolicyArgs& p, cudaStream_t s) {
   if (p.N > 0) {
     const int64_t size = sizeof(T), words = p.V * size / 16 > 0 ? p.V * size / 16 : 1;
-    int blocks = 1;
-    while (blocks < kMostBlocks && (words + blocks - 1) / blocks * 16 > kBlockBytes) blocks *= 2;
-    const int64_t per = (words + blocks - 1) / blocks;
+    // parts of sixteen words for each of 256 threads (64 KB, three blocks per SM); longer rows share by eight
+    int64_t blocks64 = (words + kPart - 1) / kPart;
+    const int blocks = blocks64 < kMostBlocks ? (int)blocks64 : kMostBlocks;
+    const int64_t per = blocks64 <= kMostBlocks ? (words < kPart ? words : kPart) : (words + blocks - 1) / blocks;
     const bool same = !p.grad || (((uintptr_t)p.logits - (uintptr_t)p.grad) % 16 == 0 && (p.l_sr - p.V) * size % 16 == 0);
     if (same && words <= kLaneWords * 32) {
       if (int rc = count_before(p, kWarpRows * 32, s)) return rc;
@@ -528,10 +562,7 @@ int launch_policy(PolicyArgs& p, cudaStream_t s) {
       if (int rc = launch_check("policy_loss")) return rc;
     } else if (same && per * 16 <= kMostBytes && p.N * blocks <= 0x7fffffffLL) {
       const int bytes = (int)per * 16;
-      // 16 words per thread where rows are many (small blocks, many of them on
-      // an SM), 4 where a row's own latency counts
-      const int64_t share = p.N * blocks <= sm_count() * 3 ? 4 : 16;
-      int threads = (int)((per / share + 31) / 32 * 32);
+      int threads = (int)((per / (kGroups * kBatch) + 31) / 32 * 32);
       threads = threads < 32 ? 32 : threads > kRowThreads ? kRowThreads : threads;
       if (int rc = count_before(p, threads, s)) return rc;
       if (int rc = allow_smem<T>(bytes)) return rc;
