@@ -461,11 +461,12 @@ MPB_D int column_at(int slots, int c) {
 
 // Rows in turn: blockIdx, blockIdx + grid, ... (times blockDim.y). p.part gets
 // the block's column sums: w_pre, w_post, gate per channel, each (grid, D).
+// ALL: both gradients are given and every thread has all of its packs.
 // Factors that a row's elements share are taken out of the products: with
 // s = m r_z the element's work is ez = dx z (0 where dropped),
 // dw_post += s ez v, dgate = s ez w slope, wn = dx v w,
 // dz = m r_z wn - z r_z^3 m mean(ez v w).
-template <class T, int W, int NV, int MODE>
+template <class T, int W, int NV, int MODE, bool ALL>
 __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
   using E = Elems<T, W>;
   using F = typename E::F;
@@ -489,13 +490,13 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
     E du[NV], y[NV], dy[NV], z[NV], g[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-      if (tid + k * step < packs) {
+      if (ALL || tid + k * step < packs) {
         const int at = k * step * W;
-        if (p.du) {
+        if (ALL || p.du) {
           du[k].load(dur + at);
           y[k].load(yr + at);
         }
-        if (p.dy) dy[k].load(dyr + at);
+        if (ALL || p.dy) dy[k].load(dyr + at);
         if (MODE != kPlain) {
           z[k].load(zr + at);
           if (p.gate_kind == MPB_GATE_FULL) g[k].load(gr + at);
@@ -503,12 +504,12 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
       }
     const float rz = MODE != kPlain ? p.rstd[r] : 0.0f, ry = p.rstd[(MODE != kPlain ? p.R : 0) + r];
     float back = 0.0f;  // of y in dx: r_y^3 mean(y w du)
-    if (p.du) {
+    if (ALL || p.du) {
       F dot = zero;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int q = tid + k * step;
-        if (q < packs) {
+        if (ALL || q < packs) {
           F w[NP], c[NP];
           load_floats<T, W>(p.w_pre + q * W, w);
 #pragma unroll
@@ -526,12 +527,12 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int q = tid + k * step;
-      if (q < packs) {
+      if (ALL || q < packs) {
         F dx[NP];
         E out;
 #pragma unroll
-        for (int i = 0; i < NP; ++i) dx[i] = p.dy ? dy[k].get(i) : zero;
-        if (p.du) {
+        for (int i = 0; i < NP; ++i) dx[i] = ALL || p.dy ? dy[k].get(i) : zero;
+        if (ALL || p.du) {
           F w[NP];
           load_floats<T, W>(p.w_pre + q * W, w);
 #pragma unroll
@@ -582,7 +583,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int q = tid + k * step;
-        if (q < packs) {
+        if (ALL || q < packs) {
           E out;
 #pragma unroll
           for (int i = 0; i < NP; ++i)
@@ -687,8 +688,14 @@ int run_rows(const NormArgs& p, const Spread& sp, bool backward, cudaStream_t s)
   const int sums = sums_of(MODE, p.gate_kind);
   size_t smem;
   const int64_t blocks = bwd_blocks(sp, p.R, sums, &smem);
-  if (int rc = allow_smem<k_norm_bwd_rows<T, W, NV, MODE>>(what, smem)) return rc;
-  k_norm_bwd_rows<T, W, NV, MODE><<<(unsigned)blocks, block, smem, s>>>(p);
+  auto run = [&](auto all) {
+    constexpr auto kernel = k_norm_bwd_rows<T, W, NV, MODE, decltype(all)::value>;
+    if (int rc = allow_smem<kernel>(what, smem)) return rc;
+    kernel<<<(unsigned)blocks, block, smem, s>>>(p);
+    return (int)MPB_OK;
+  };
+  const bool all = W == 8 && p.du && p.dy && p.D == (int64_t)W * NV * sp.x;
+  if (int rc = all ? run(std::integral_constant<bool, W == 8>()) : run(std::false_type())) return rc;
   if (int rc = launch_check(what)) return rc;
   k_norm_columns<T><<<dim3((unsigned)((p.D + 31) / 32), (unsigned)sums), dim3(32, 32), 0, s>>>(p, (int)blocks);
   return launch_check(what);
