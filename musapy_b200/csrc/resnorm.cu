@@ -653,11 +653,12 @@ Spread spread_of(int64_t R, int64_t D, int W, bool backward, int size) {
 
 int sums_of(int mode, int gate_kind) { return mode == kPlain ? 1 : gate_kind == MPB_GATE_CHANNEL ? 3 : 2; }
 
-// Blocks of the backward kernel: what fits the SMs at up to 128 registers per
-// thread and by shared memory, or the rows if they are fewer.
+// Blocks of the backward kernel: what fits the SMs at 128 registers per thread
+// (half of that with one pack) and by shared memory, or the rows if they are
+// fewer.
 int64_t bwd_blocks(const Spread& s, int64_t R, int sums, size_t* smem) {
   *smem = (size_t)s.x * s.NV * s.W * s.y * sizeof(float) * sums;
-  int64_t per_sm = kRowThreads / (s.x * s.y);
+  int64_t per_sm = (s.NV == 1 ? 2 : 1) * kRowThreads / (s.x * s.y);
   const int64_t by_smem = (int64_t)((224u << 10) / (*smem + 2048));
   if (per_sm > by_smem) per_sm = by_smem;
   if (per_sm < 1) per_sm = 1;
