@@ -196,12 +196,11 @@ MPB_D bool await(const W* p, W& w) {
 }
 
 // Warp 0 of a tile: the state that enters it, per lane and channel (carry
-// holds the one before the chain). (a, b) is the tile's own map, published
-// when the tile before has no state yet; early: that tile's words as seen
-// before this tile's data came.
+// holds the one before the chain). early: the words of the tile before as seen
+// some time ago.
 template <int V>
-MPB_D void look_back(const ScanArgs& p, uint32_t chain, uint32_t chunk, int lane, const float (&a)[V],
-                     const float (&b)[V], uint32_t (&early)[V], float (&carry)[V]) {
+MPB_D void look_back(const ScanArgs& p, uint32_t chain, uint32_t chunk, int lane, uint32_t (&early)[V],
+                     float (&carry)[V]) {
   constexpr int C = 32 * V;
   if (chunk == 0) return;
   auto at = [&](uint32_t k) { return (size_t)(k * p.chains + chain) * C + lane * V; };
@@ -216,8 +215,6 @@ MPB_D void look_back(const ScanArgs& p, uint32_t chain, uint32_t chunk, int lane
     for (int v = 0; v < V; ++v) carry[v] = __uint_as_float(early[v]) + 0.0f;
     return;
   }
-#pragma unroll
-  for (int v = 0; v < V; ++v) st_word(p.maps + at(chunk) + v, map_word(a[v], b[v]));
   // lane i looks at the first channel of the tile i + 1 before this one;
   // before the chain's first tile stands the initial state
   uint32_t back;
@@ -275,8 +272,9 @@ MPB_D void look_back(const ScanArgs& p, uint32_t chain, uint32_t chunk, int lane
 
 template <int V>
 struct Shared {
-  __align__(8) float a[2][kWarps][32 * V];  // the warps' maps, of this tile and of the one before
-  __align__(8) float b[2][kWarps][32 * V];
+  // the warps' maps, of three tiles in turn
+  __align__(8) float a[3][kWarps][32 * V];
+  __align__(8) float b[3][kWarps][32 * V];
   __align__(8) float carry[32 * V];
   uint32_t tiles[4];
 };
@@ -288,52 +286,26 @@ MPB_D Floats<V> through(const Shared<V>& sh, int side, int w, int lane, Floats<V
               *reinterpret_cast<const Floats<V>*>(&sh.b[side][w][lane * V]));
 }
 
-// Joins the maps of the block's warps (a, b: this warp's). carry: the state
-// that enters the tile (look-back: before the chain) and, on return, the one
-// that leaves it (walk). Returns in `in` the state that enters the warp's steps.
-template <int V, bool WALK>
-MPB_D void join(const ScanArgs& p, Shared<V>& sh, int side, uint32_t chain, uint32_t chunk, int warp, int lane,
-                Floats<V> a, Floats<V> b, uint32_t (&early)[V], Floats<V>& carry, Floats<V>& in) {
-  constexpr int C = 32 * V;
+template <int V>
+MPB_D void put_map(Shared<V>& sh, int side, int warp, int lane, Floats<V> a, Floats<V> b) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    sh.a[side][warp][lane * V + v] = finite(vget(a, v));
+    sh.b[side][warp][lane * V + v] = vget(b, v);
+  }
+}
+
+// A walk's tile: joins the maps of the block's warps (a, b: this warp's). carry:
+// the state that enters the tile and, on return, the one that leaves it (of
+// a single warp the caller's steps end there). Returns in `in` the state that
+// enters the warp's steps.
+template <int V>
+MPB_D void join(Shared<V>& sh, int side, int warp, int lane, Floats<V> a, Floats<V> b, Floats<V>& carry, Floats<V>& in) {
   const int warps = blockDim.x >> 5;
-  if (warps > 1 || !WALK) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      sh.a[side][warp][lane * V + v] = finite(vget(a, v));
-      sh.b[side][warp][lane * V + v] = vget(b, v);
-    }
-    __syncthreads();
-  }
-  if (!WALK) {
-    if (warp == 0) {
-      float ta[V], tb[V], c[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        c[v] = vget(carry, v);
-        ta[v] = finite(vget(a, v)), tb[v] = vget(b, v);
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) {
-          const float aw = sh.a[side][w][lane * V + v];
-          tb[v] = fmaf(aw, tb[v], sh.b[side][w][lane * V + v]);
-          ta[v] = finite(ta[v] * aw);
-        }
-      }
-      look_back<V>(p, chain, chunk, lane, ta, tb, early, c);
-      if (chunk + 1 < p.chunks) {
-        const size_t at = (size_t)(chunk * p.chains + chain) * C + lane * V;
-#pragma unroll
-        for (int v = 0; v < V; ++v) st_word(p.states + at + v, state_word(fmaf(ta[v], c[v], tb[v])));
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) sh.carry[lane * V + v] = c[v];
-    }
-    __syncthreads();
-    in = *reinterpret_cast<const Floats<V>*>(&sh.carry[lane * V]);
-    for (int w = 0; w < warp; ++w) in = through<V>(sh, side, w, lane, in);
-    return;
-  }
   in = carry;
-  if (warps == 1) return;  // the warp's own steps end the tile: the caller carries on from them
+  if (warps == 1) return;
+  put_map<V>(sh, side, warp, lane, a, b);
+  __syncthreads();
   if (warps == kWarps) {
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
@@ -465,52 +437,132 @@ struct HeadGates {
   }
 };
 
-// What the tiles of a block are, in order. Walk: the chunks of chain blockIdx,
-// then of chain blockIdx + grid, ... Look-back: the tickets it took.
-template <bool WALK>
+// The tiles of a walk, in order: the chunks of chain blockIdx, then of chain
+// blockIdx + grid, ...
 struct Order {
   uint32_t chain, chunk;
-  MPB_D void first() {
-    chain = blockIdx.x;
-    chunk = 0;
-  }
-  // The tile number `it` of the block (walk: the one it stands at); false when there is none.
-  MPB_D bool here(const ScanArgs& p, const uint32_t* tiles, int it) {
-    if (WALK) return chain < p.chains;
-    const uint32_t t = tiles[it & 3];
-    p.by_chains.divmod(t, chunk, chain);
-    return t < p.chains * p.chunks;
-  }
+  MPB_D Order() : chain(blockIdx.x), chunk(0) {}
+  MPB_D bool here(const ScanArgs& p) const { return chain < p.chains; }
   MPB_D void next(const ScanArgs& p) {
-    if (WALK && ++chunk == p.chunks) {
+    if (++chunk == p.chunks) {
       chunk = 0;
       chain += gridDim.x;
     }
   }
 };
 
-// Where a thread's words of a tile lie: placed anew for every tile of a
-// look-back, but along a chain only moved on.
-template <bool WALK, int PER, int N>
+// Where a thread's words of a tile lie.
+template <int PER, int N>
 struct Place {
   const char* at[N];
-  int left;   // steps from the warp's first one to the end of the sequence; 0 on an idle lane
-  int end;    // the same on every lane
-  int heads;  // gates of the warp, where channels share them
+  int left;       // steps from the warp's first one to the end of the sequence; 0 on an idle lane
+  int end;        // the same on every lane
+  int heads;      // gates of the warp, where channels share them
   uint32_t wide;  // wide_lane
-  template <class F>
-  MPB_D void go(const ScanArgs& p, const Order<WALK>& o, int warp, const int64_t (&st)[N], F place_at) {
-    if (!WALK || o.chunk == 0) {
-      place_at(o, *this);
-    } else {
+  // Along a chain: the next chunk.
+  MPB_D void move(const ScanArgs& p, const int64_t (&st)[N]) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) at[k] += st[k] * p.steps;
-      left -= p.steps;
-      end -= p.steps;
-    }
+    for (int k = 0; k < N; ++k) at[k] += st[k] * p.steps;
+    left -= p.steps;
+    end -= p.steps;
   }
   MPB_D int steps() const { return left < PER ? left : PER; }
 };
+
+// The tiles of a look-back, taken by ticket. Work on a tile is in two parts: its
+// map is published one tile before its state is asked for, so that the wait
+// for one tile's state runs under the folding of the next tile's map, and
+// the tiles of a chain find each other's maps ready.
+//   front(o, stage, side)  folds tile o's maps into sh side
+//   first(o, c)            the state before the chain, warp 0 (of the first 32 chunks:
+//                          as far as a look-back reaches)
+//   rest(o, stage, in)     runs the warp's steps from the state `in`
+//   copy(it, stage)        copies the block's tile number `it`, and commits
+template <int V, class Front, class First, class Rest, class Copy>
+MPB_D void look_back_tiles(const ScanArgs& p, Shared<V>& sh, int warp, int lane, Front front, First first, Rest rest,
+                           Copy copy) {
+  constexpr int C = 32 * V;
+  const uint32_t total = p.chains * p.chunks;
+  struct At {
+    uint32_t chain, chunk;
+  };
+  auto tile = [&](int it, At& o) {  // false when there is none
+    const uint32_t t = sh.tiles[it & 3];
+    p.by_chains.divmod(t, o.chunk, o.chain);
+    return t < total;
+  };
+  // The first tickets are taken one after the other, so that every running
+  // block has its first tile before any has its second: a tile's predecessors
+  // are then worked on at the same time, not behind others.
+  for (int s = 0; s < 3; ++s) {
+    if (threadIdx.x == 0) sh.tiles[s] = atomicAdd(p.ticket, 1u);
+    __syncthreads();
+    At o;
+    copy(tile(s, o), o.chain, o.chunk, s);
+  }
+  At cur, nxt;
+  float ta[V], tb[V];  // the tile's map, warp 0
+  auto publish = [&](const At& o, int side) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      ta[v] = sh.a[side][0][lane * V + v], tb[v] = sh.b[side][0][lane * V + v];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) {
+        const float aw = sh.a[side][w][lane * V + v];
+        tb[v] = fmaf(aw, tb[v], sh.b[side][w][lane * V + v]);
+        ta[v] = finite(ta[v] * aw);
+      }
+      if (o.chunk + 1 < p.chunks)
+        st_word(p.maps + (size_t)(o.chunk * p.chains + o.chain) * C + lane * V + v, map_word(ta[v], tb[v]));
+    }
+  };
+  bool have = tile(0, cur);
+  copies_wait<2>();
+  __syncwarp();  // the words that other lanes have copied
+  if (have) front(cur.chain, cur.chunk, 0, 0);
+  __syncthreads();
+  if (have && warp == 0) publish(cur, 0);
+  int stage = 0;
+  for (int it = 0; have; ++it) {
+    const int after = stage == 2 ? 0 : stage + 1;
+    const bool more = tile(it + 1, nxt);
+    if (threadIdx.x == 0) sh.tiles[(it + 3) & 3] = atomicAdd(p.ticket, 1u);
+    uint32_t early[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      early[v] = warp == 0 && cur.chunk > 0
+                     ? ld_word(p.states + (size_t)((cur.chunk - 1) * p.chains + cur.chain) * C + lane * V + v)
+                     : 0;
+    copies_wait<1>();
+    __syncwarp();
+    if (more) front(nxt.chain, nxt.chunk, after, after);
+    __syncthreads();
+    if (warp == 0) {
+      float a[V], b[V], c[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) a[v] = ta[v], b[v] = tb[v];
+      if (more) publish(nxt, after);
+      first(cur.chain, cur.chunk, c);
+      look_back<V>(p, cur.chain, cur.chunk, lane, early, c);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (cur.chunk + 1 < p.chunks)
+          st_word(p.states + (size_t)(cur.chunk * p.chains + cur.chain) * C + lane * V + v, state_word(fmaf(a[v], c[v], b[v])));
+        sh.carry[lane * V + v] = c[v];
+      }
+    }
+    __syncthreads();
+    Floats<V> in = *reinterpret_cast<const Floats<V>*>(&sh.carry[lane * V]);
+    for (int w = 0; w < warp; ++w) in = through<V>(sh, stage, w, lane, in);
+    rest(cur.chain, cur.chunk, stage, in);
+    __syncwarp();  // the stage has been read by every lane
+    At far;
+    copy(tile(it + 3, far), far.chain, far.chunk, stage);
+    cur = nxt;
+    have = more;
+    stage = after;
+  }
+}
 
 // Where a lane's copies of a column start, from the first row's start; st: bytes between steps.
 template <class C, class T>
@@ -538,141 +590,192 @@ template <class X, class G, int V, bool SHARED>
 struct FwdTile {
   using CX = Column<X, V>;
   using CG = Column<G, SHARED ? 1 : V>;
+  using HG = HeadGates<G, kFwd>;
   static constexpr uint32_t kG = CX::bytes(kFwd), kBytes = kG + CG::bytes(kFwd);
-  static constexpr int kStages = kRing / kBytes < 3 ? kRing / kBytes : 3;
+  static constexpr int kStages = kRing / kBytes < 3 ? kRing / kBytes : 3;  // of a walk
   static_assert(kStages >= 2, "a tile is copied while another is computed");
 };
 
-template <class X, class G, bool SIG, int V, bool SHARED, bool WALK>
-__global__ void __launch_bounds__(kWarps * 32, 2) k_gscan(ScanArgs p) {
+// What the forward kernels share: copies, and the decay and input of a step.
+template <class X, class G, bool SIG, int V, bool SHARED>
+struct Forward {
   using Tile = FwdTile<X, G, V, SHARED>;
-  constexpr int NST = Tile::kStages;
-  extern __shared__ __align__(16) char ring[];
-  __shared__ Shared<V> sh;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t base = smem_u32(ring);
-  Order<WALK> cur, ahead;
-  cur.first();
-  ahead.first();
-  // The block's first tickets are taken one after the other, so that every
-  // running block has its first tile before any has its second: a tile's
-  // predecessors are then worked on at the same time, not behind others.
-  auto take = [&](int s) {
-    if (threadIdx.x == 0) sh.tiles[s] = atomicAdd(p.ticket, 1u);
-    __syncthreads();
-  };
-  if (WALK) {
-    if (p.status && blockIdx.x == 0 && threadIdx.x == 0) *p.status = MPB_OK;  // nothing waits
-  } else {
-    take(0);
+  const ScanArgs& p;
+  const int64_t in_st[2], out_st;
+  const int lane, warp;
+  int gate_slot;
+  uint32_t half_x, half_g;  // bit 1 of the addresses of single 16-bit elements at step 0
+  size_t state_at;
+  MPB_D explicit Forward(const ScanArgs& args)
+      : p(args), in_st{args.x_st * (int64_t)sizeof(X), args.g_st * (int64_t)sizeof(G)}, out_st(args.D * (int64_t)sizeof(X)),
+        lane(threadIdx.x & 31), warp(threadIdx.x >> 5) {}
+  MPB_D void inputs(uint32_t chain, uint32_t chunk, Place<kFwd, 2>& f) const {
+    const Lane l = place<V, SHARED>(p, chain, lane);
+    const int64_t t0 = (int64_t)chunk * p.steps + warp * kFwd;
+    const char* x = (const char*)((const X*)p.x + l.b * p.x_sb + t0 * p.x_st);
+    const char* g = (const char*)((const G*)p.gate + l.b * p.g_sb + t0 * p.g_st);
+    f.at[0] = at_lane<typename Tile::CX, X>(p, x, l, in_st[0], lane);
+    f.at[1] = SHARED ? g + l.head * sizeof(G) : at_lane<typename Tile::CG, G>(p, g, l, in_st[1], lane);
+    f.wide = wide_lane<V>(l, lane);
+    f.end = (int)(p.T - t0);
+    f.left = l.in ? f.end : 0;
+    f.heads = SHARED ? (int)(p.H - l.head < p.heads_per ? p.H - l.head : p.heads_per) : 0;
   }
-  const int64_t in_st[2] = {p.x_st * (int64_t)sizeof(X), p.g_st * (int64_t)sizeof(G)};
-  const int64_t out_st[1] = {p.D * (int64_t)sizeof(X)};
-  Place<WALK, kFwd, 2> from;
-  Place<WALK, kFwd, 1> to;
-  auto copy = [&](int it, int s) {  // the block's tile number `it` into stage s
-    if (ahead.here(p, sh.tiles, it)) {
-      from.go(p, ahead, warp, in_st, [&](const Order<WALK>& o, auto& f) {
-        const Lane l = place<V, SHARED>(p, o.chain, lane);
-        const int64_t t0 = (int64_t)o.chunk * p.steps + warp * kFwd;
-        const char* x = (const char*)((const X*)p.x + l.b * p.x_sb + t0 * p.x_st);
-        const char* g = (const char*)((const G*)p.gate + l.b * p.g_sb + t0 * p.g_st);
-        f.at[0] = at_lane<typename Tile::CX, X>(p, x, l, in_st[0], lane);
-        f.at[1] = SHARED ? g + l.head * sizeof(G) : at_lane<typename Tile::CG, G>(p, g, l, in_st[1], lane);
-        f.wide = wide_lane<V>(l, lane);
-        f.end = (int)(p.T - t0);
-        f.left = l.in ? f.end : 0;
-        f.heads = SHARED ? (int)(p.H - l.head < p.heads_per ? p.H - l.head : p.heads_per) : 0;
-      });
-      copy_column<typename Tile::CX, kFwd>(p, base + s * Tile::kBytes, from.at[0], in_st[0], from.left, from.end, from.wide);
-      const uint32_t q = base + s * Tile::kBytes + Tile::kG;
-      if constexpr (SHARED) HeadGates<G, kFwd>::copy(q, from.at[1], in_st[1], from.end, (int)p.heads_per, from.heads, p.by_heads_per);
-      else copy_column<typename Tile::CG, kFwd>(p, q, from.at[1], in_st[1], from.left, from.end, from.wide);
-      ahead.next(p);
-    }
-    copies_commit();
-  };
-#pragma unroll
-  for (int s = 0; s < NST - 1; ++s) {
-    copy(s, s);
-    if (!WALK) take(s + 1);
+  MPB_D void copy(uint32_t base, const Place<kFwd, 2>& f) const {
+    copy_column<typename Tile::CX, kFwd>(p, base, f.at[0], in_st[0], f.left, f.end, f.wide);
+    if constexpr (SHARED) Tile::HG::copy(base + Tile::kG, f.at[1], in_st[1], f.end, (int)p.heads_per, f.heads, p.by_heads_per);
+    else copy_column<typename Tile::CG, kFwd>(p, base + Tile::kG, f.at[1], in_st[1], f.left, f.end, f.wide);
   }
-  int stage = 0;
-  Floats<V> carry = vset<V>(0.0f);
-  size_t state_at = 0;
-  int gate_slot = 0;
-  uint32_t half_x = 0, half_g = 0;  // bit 1 of the addresses of single 16-bit elements at step 0
-  for (int it = 0; cur.here(p, sh.tiles, it); ++it) {
-    __syncwarp();  // the stage that is filled next has been read by every lane
-    copy(it + NST - 1, stage == 0 ? NST - 1 : stage - 1);
-    to.go(p, cur, warp, out_st, [&](const Order<WALK>& o, auto& f) {
-      const Lane l = place<V, SHARED>(p, o.chain, lane);
-      const int64_t t0 = (int64_t)o.chunk * p.steps + warp * kFwd;
-      f.at[0] = (const char*)((const X*)p.h + (l.b * p.T + t0) * p.D + l.ch);
-      f.left = l.in ? (int)(p.T - t0) : 0;
-      state_at = (size_t)(l.b * p.D + l.ch);
-      gate_slot = l.slot;
-      half_x = (uint32_t)(uintptr_t)((const X*)p.x + l.b * p.x_sb + l.ch);
-      half_g = (uint32_t)(uintptr_t)((const G*)p.gate + l.b * p.g_sb + l.gate);
-      if (o.chunk == 0 || !WALK)
-#pragma unroll
-        for (int v = 0; v < V; ++v) vput(carry, v, o.chunk == 0 && l.in && p.h0 ? p.h0[state_at + v] : 0.0f);
-    });
-    const uint32_t t0 = cur.chunk * p.steps + warp * kFwd;
-    auto half = [&](uint32_t at0, int64_t st, int i) { return at0 + (t0 + i) * (uint32_t)st; };
-    uint32_t early[V];
-    if (!WALK) {
-      if (threadIdx.x == 0) sh.tiles[(it + NST) & 3] = atomicAdd(p.ticket, 1u);
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        early[v] = warp == 0 && cur.chunk > 0
-                       ? ld_word(p.states + (size_t)((cur.chunk - 1) * p.chains + cur.chain) * 32 * V + lane * V + v)
-                       : 0;
-    }
-    copies_wait<NST - 1>();
-    __syncwarp();  // the words that other lanes have copied
-    const char* mine = ring + stage * Tile::kBytes;
-    // Steps after the last are computed from whatever the ring holds: nothing
-    // follows them in the chain, and they are not written.
-    Floats<V> a[kFwd], b[kFwd], ma = vset<V>(1.0f), mb = vset<V>(0.0f), in;
-#pragma unroll
-    for (int i = 0; i < kFwd; ++i) {
-      const Floats<V> x = unpack(Tile::CX::get(mine, i, half(half_x, in_st[0], i)));
-      Floats<V> om;
-      if constexpr (SHARED)
-        gates_of<SIG, V>(HeadGates<G, kFwd>::get(mine + Tile::kG, i * (int)p.heads_per + gate_slot, half(half_g, in_st[1], i)), a[i], om);
-      else
-        gates_of<SIG, V>(Tile::CG::get(mine + Tile::kG, i, half(half_g, in_st[1], i)), a[i], om);
-      b[i] = SIG ? vmul(om, x) : x;
-      ma = vmul(ma, a[i]);
-      mb = vfma(a[i], mb, b[i]);
-    }
-    join<V, WALK>(p, sh, it & 1, cur.chain, cur.chunk, warp, lane, ma, mb, early, carry, in);
+  MPB_D void output(uint32_t chain, uint32_t chunk, Place<kFwd, 1>& f) {
+    const Lane l = place<V, SHARED>(p, chain, lane);
+    const int64_t t0 = (int64_t)chunk * p.steps + warp * kFwd;
+    f.at[0] = (const char*)((const X*)p.h + (l.b * p.T + t0) * p.D + l.ch);
+    f.left = l.in ? (int)(p.T - t0) : 0;
+    state_at = (size_t)(l.b * p.D + l.ch);
+    sub_words(l);
+  }
+  MPB_D void sub_words(const Lane& l) {
+    gate_slot = l.slot;
+    half_x = (uint32_t)(uintptr_t)((const X*)p.x + l.b * p.x_sb + l.ch);
+    half_g = (uint32_t)(uintptr_t)((const G*)p.gate + l.b * p.g_sb + l.gate);
+  }
+  // t0: the warp's first step in the tile
+  MPB_D void step(const char* mine, int i, uint32_t t0, Floats<V>& a, Floats<V>& b) const {
+    const Floats<V> x = unpack(Tile::CX::get(mine, i, half_x + (t0 + i) * (uint32_t)in_st[0]));
+    const uint32_t half = half_g + (t0 + i) * (uint32_t)in_st[1];
+    Floats<V> om;
+    if constexpr (SHARED) gates_of<SIG, V>(Tile::HG::get(mine + Tile::kG, i * (int)p.heads_per + gate_slot, half), a, om);
+    else gates_of<SIG, V>(Tile::CG::get(mine + Tile::kG, i, half), a, om);
+    b = SIG ? vmul(om, x) : x;
+  }
+  // Runs f(i) over the warp's steps of a tile; f returns the state to write.
+  template <class F>
+  MPB_D void write(const Place<kFwd, 1>& to, Floats<V>& in, F f) const {
     const int n = to.steps();
     char* h = const_cast<char*>(to.at[0]);
     if (__all_sync(0xffffffffu, n == kFwd)) {
 #pragma unroll
       for (int i = 0; i < kFwd; ++i) {
-        in = vfma(a[i], in, b[i]);
+        f(i);
         put_global(h, pack<X>(in));
-        h = ahead_by(h, out_st[0]);
+        h = ahead_by(h, out_st);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kFwd; ++i)
         if (i < n) {
-          in = vfma(a[i], in, b[i]);
+          f(i);
           put_global(h, pack<X>(in));
-          h = ahead_by(h, out_st[0]);
+          h = ahead_by(h, out_st);
         }
     }
     if (p.state && n > 0 && n == to.left)
 #pragma unroll
       for (int v = 0; v < V; ++v) p.state[state_at + v] = vget(in, v);
-    if (WALK && blockDim.x == 32) carry = in;
+  }
+};
+
+template <class X, class G, bool SIG, int V, bool SHARED>
+__global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_walk(ScanArgs p) {
+  using Tile = FwdTile<X, G, V, SHARED>;
+  constexpr int NST = Tile::kStages;
+  extern __shared__ __align__(16) char ring[];
+  __shared__ Shared<V> sh;
+  Forward<X, G, SIG, V, SHARED> fw(p);
+  const uint32_t base = smem_u32(ring);
+  if (p.status && blockIdx.x == 0 && threadIdx.x == 0) *p.status = MPB_OK;  // nothing waits
+  Order cur, ahead;
+  Place<kFwd, 2> from;
+  Place<kFwd, 1> to;
+  const int64_t out_st[1] = {fw.out_st};
+  auto copy = [&](int s) {  // the walk's next tile into stage s
+    if (ahead.here(p)) {
+      if (ahead.chunk == 0) fw.inputs(ahead.chain, 0, from);
+      else from.move(p, fw.in_st);
+      fw.copy(base + s * Tile::kBytes, from);
+      ahead.next(p);
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < NST - 1; ++s) copy(s);
+  int stage = 0;
+  Floats<V> carry = vset<V>(0.0f);
+  for (int it = 0; cur.here(p); ++it) {
+    __syncwarp();  // the stage that is filled next has been read by every lane
+    copy(stage == 0 ? NST - 1 : stage - 1);
+    if (cur.chunk == 0) {
+      fw.output(cur.chain, 0, to);
+#pragma unroll
+      for (int v = 0; v < V; ++v) vput(carry, v, to.left > 0 && p.h0 ? p.h0[fw.state_at + v] : 0.0f);
+    } else {
+      to.move(p, out_st);
+    }
+    copies_wait<NST - 1>();
+    __syncwarp();  // the words that other lanes have copied
+    const char* mine = ring + stage * Tile::kBytes;
+    const uint32_t t0 = cur.chunk * p.steps + fw.warp * kFwd;
+    // Steps after the last are computed from whatever the ring holds: nothing
+    // follows them in the chain, and they are not written.
+    Floats<V> a[kFwd], b[kFwd], ma = vset<V>(1.0f), mb = vset<V>(0.0f), in;
+#pragma unroll
+    for (int i = 0; i < kFwd; ++i) {
+      fw.step(mine, i, t0, a[i], b[i]);
+      ma = vmul(ma, a[i]);
+      mb = vfma(a[i], mb, b[i]);
+    }
+    join<V>(sh, it & 1, fw.warp, fw.lane, ma, mb, carry, in);
+    fw.write(to, in, [&](int i) { in = vfma(a[i], in, b[i]); });
+    if (blockDim.x == 32) carry = in;
     cur.next(p);
     stage = stage + 1 == NST ? 0 : stage + 1;
   }
+}
+
+template <class X, class G, bool SIG, int V, bool SHARED>
+__global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_far(ScanArgs p) {
+  using Tile = FwdTile<X, G, V, SHARED>;
+  extern __shared__ __align__(16) char ring[];
+  __shared__ Shared<V> sh;
+  Forward<X, G, SIG, V, SHARED> fw(p);
+  const uint32_t base = smem_u32(ring);
+  auto t0_of = [&](uint32_t chunk) { return chunk * p.steps + fw.warp * kFwd; };
+  look_back_tiles<V>(
+      p, sh, fw.warp, fw.lane,
+      [&](uint32_t chain, uint32_t chunk, int stage, int side) {
+        fw.sub_words(place<V, SHARED>(p, chain, fw.lane));
+        Floats<V> ma = vset<V>(1.0f), mb = vset<V>(0.0f);
+#pragma unroll
+        for (int i = 0; i < kFwd; ++i) {
+          Floats<V> a, b;
+          fw.step(ring + stage * Tile::kBytes, i, t0_of(chunk), a, b);
+          ma = vmul(ma, a);
+          mb = vfma(a, mb, b);
+        }
+        put_map<V>(sh, side, fw.warp, fw.lane, ma, mb);
+      },
+      [&](uint32_t chain, uint32_t chunk, float (&c)[V]) {
+        const Lane l = place<V, SHARED>(p, chain, fw.lane);
+#pragma unroll
+        for (int v = 0; v < V; ++v) c[v] = chunk < 32 && l.in && p.h0 ? p.h0[l.b * p.D + l.ch + v] : 0.0f;
+      },
+      [&](uint32_t chain, uint32_t chunk, int stage, Floats<V> in) {
+        Place<kFwd, 1> to;
+        fw.output(chain, chunk, to);
+        fw.write(to, in, [&](int i) {
+          Floats<V> a, b;
+          fw.step(ring + stage * Tile::kBytes, i, t0_of(chunk), a, b);
+          in = vfma(a, in, b);
+        });
+      },
+      [&](bool is, uint32_t chain, uint32_t chunk, int stage) {
+        if (is) {
+          Place<kFwd, 2> from;
+          fw.inputs(chain, chunk, from);
+          fw.copy(base + stage * Tile::kBytes, from);
+        }
+        copies_commit();
+      });
 }
 
 // Sums over the `lanes` (a power of two) neighbours of a lane of kBwd values
@@ -705,134 +808,97 @@ template <class X, class G, bool SIG, int V, bool SHARED>
 struct BwdTile {
   using CX = Column<X, V>;
   using CG = Column<G, SHARED ? 1 : V>;
+  using HG = HeadGates<G, kBwd>;
   static constexpr uint32_t kH = CX::bytes(kBwd), kX = 2 * kH, kG = SIG ? 3 * kH : kX, kBytes = kG + CG::bytes(kBwd);
-  static constexpr int kStages = kRing / kBytes < 3 ? kRing / kBytes : 3;
+  static constexpr int kStages = kRing / kBytes < 3 ? kRing / kBytes : 3;  // of a walk
   static_assert(kStages >= 2, "a tile is copied while another is computed");
 };
 
-// As k_gscan, from the last step to the first. The gate is taken from shared
+// As Forward, from the last step to the first. The gate is taken from shared
 // memory twice rather than kept (backward moves twice the bytes per element,
 // so the second exponential fits beside them).
-template <class X, class G, bool SIG, int V, bool SHARED, bool WALK>
-__global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd(ScanArgs p) {
+template <class X, class G, bool SIG, int V, bool SHARED>
+struct Backward {
   using Tile = BwdTile<X, G, SIG, V, SHARED>;
-  constexpr int NST = Tile::kStages;
-  extern __shared__ __align__(16) char ring[];
-  __shared__ Shared<V> sh;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t base = smem_u32(ring);
-  Order<WALK> cur, ahead;
-  cur.first();
-  ahead.first();
-  // The block's first tickets are taken one after the other, so that every
-  // running block has its first tile before any has its second: a tile's
-  // predecessors are then worked on at the same time, not behind others.
-  auto take = [&](int s) {
-    if (threadIdx.x == 0) sh.tiles[s] = atomicAdd(p.ticket, 1u);
-    __syncthreads();
-  };
-  if (WALK) {
-    if (p.status && blockIdx.x == 0 && threadIdx.x == 0) *p.status = MPB_OK;  // nothing waits
-  } else {
-    take(0);
+  const ScanArgs& p;
+  const int64_t in_st[4], out_st[2];
+  const int lane, warp;
+  int gate_slot;
+  uint32_t half0[4];  // bit 1 of the addresses of single 16-bit elements at the sequence's last step
+  size_t state_at;
+  MPB_D explicit Backward(const ScanArgs& args)
+      : p(args), in_st{-args.dh_st * (int64_t)sizeof(X), -args.h_st * (int64_t)sizeof(X), -args.x_st * (int64_t)sizeof(X),
+                       -args.g_st * (int64_t)sizeof(G)},
+        out_st{-args.D * (int64_t)sizeof(X), -args.H * (int64_t)sizeof(G)}, lane(threadIdx.x & 31), warp(threadIdx.x >> 5) {}
+  MPB_D void inputs(uint32_t chain, uint32_t chunk, Place<kBwd, 4>& f) const {
+    const Lane l = place<V, SHARED>(p, chain, lane);
+    const int64_t r0 = (int64_t)chunk * p.steps + warp * kBwd, t0 = p.T - 1 - r0;
+    auto row = [&](const void* q, int64_t sb, int64_t st, int64_t t) { return (const char*)((const X*)q + l.b * sb + t * st); };
+    const char* g = (const char*)((const G*)p.gate + l.b * p.g_sb + t0 * p.g_st);
+    f.at[0] = at_lane<typename Tile::CX, X>(p, row(p.dh, p.dh_sb, p.dh_st, t0), l, in_st[0], lane);
+    f.at[1] = at_lane<typename Tile::CX, X>(p, row(p.hsaved, p.h_sb, p.h_st, t0 - 1), l, in_st[1], lane);
+    f.at[2] = at_lane<typename Tile::CX, X>(p, row(p.x, p.x_sb, p.x_st, t0), l, in_st[2], lane);
+    f.at[3] = SHARED ? g + l.head * sizeof(G) : at_lane<typename Tile::CG, G>(p, g, l, in_st[3], lane);
+    f.wide = wide_lane<V>(l, lane);
+    f.end = (int)(p.T - r0);
+    f.left = l.in ? f.end : 0;
+    f.heads = SHARED ? (int)(p.H - l.head < p.heads_per ? p.H - l.head : p.heads_per) : 0;
   }
-  const int64_t in_st[4] = {-p.dh_st * (int64_t)sizeof(X), -p.h_st * (int64_t)sizeof(X), -p.x_st * (int64_t)sizeof(X),
-                            -p.g_st * (int64_t)sizeof(G)};
-  const int64_t out_st[2] = {-p.D * (int64_t)sizeof(X), -p.H * (int64_t)sizeof(G)};
-  Place<WALK, kBwd, 4> from;
-  Place<WALK, kBwd, 2> to;
-  auto copy = [&](int it, int s) {  // the block's tile number `it` into stage s
-    if (ahead.here(p, sh.tiles, it)) {
-      from.go(p, ahead, warp, in_st, [&](const Order<WALK>& o, auto& f) {
-        const Lane l = place<V, SHARED>(p, o.chain, lane);
-        const int64_t r0 = (int64_t)o.chunk * p.steps + warp * kBwd, t0 = p.T - 1 - r0;
-        const char* g = (const char*)((const G*)p.gate + l.b * p.g_sb + t0 * p.g_st);
-        f.at[0] = at_lane<typename Tile::CX, X>(p, (const char*)((const X*)p.dh + l.b * p.dh_sb + t0 * p.dh_st), l, in_st[0], lane);
-        f.at[1] = at_lane<typename Tile::CX, X>(p, (const char*)((const X*)p.hsaved + l.b * p.h_sb + (t0 - 1) * p.h_st), l, in_st[1], lane);
-        f.at[2] = at_lane<typename Tile::CX, X>(p, (const char*)((const X*)p.x + l.b * p.x_sb + t0 * p.x_st), l, in_st[2], lane);
-        f.at[3] = SHARED ? g + l.head * sizeof(G) : at_lane<typename Tile::CG, G>(p, g, l, in_st[3], lane);
-        f.wide = wide_lane<V>(l, lane);
-        f.end = (int)(p.T - r0);
-        f.left = l.in ? f.end : 0;
-        f.heads = SHARED ? (int)(p.H - l.head < p.heads_per ? p.H - l.head : p.heads_per) : 0;
-      });
-      const uint32_t q = base + s * Tile::kBytes;
-      auto column = [&](uint32_t to, int k, int less) {
-        copy_column<typename Tile::CX, kBwd>(p, to, from.at[k], in_st[k], from.left - less, from.end - less, from.wide);
-      };
-      column(q, 0, 0);
-      column(q + Tile::kH, 1, 1);  // h[-1] is h0
-      if (SIG) column(q + Tile::kX, 2, 0);
-      if constexpr (SHARED) HeadGates<G, kBwd>::copy(q + Tile::kG, from.at[3], in_st[3], from.end, (int)p.heads_per, from.heads, p.by_heads_per);
-      else copy_column<typename Tile::CG, kBwd>(p, q + Tile::kG, from.at[3], in_st[3], from.left, from.end, from.wide);
-      ahead.next(p);
-    }
-    copies_commit();
-  };
-#pragma unroll
-  for (int s = 0; s < NST - 1; ++s) {
-    copy(s, s);
-    if (!WALK) take(s + 1);
-  }
-  int stage = 0;
-  Floats<V> carry = vset<V>(0.0f);
-  size_t state_at = 0;
-  int gate_slot = 0;
-  uint32_t half0[4] = {};  // bit 1 of the addresses of single 16-bit elements at the sequence's last step
-  for (int it = 0; cur.here(p, sh.tiles, it); ++it) {
-    __syncwarp();  // the stage that is filled next has been read by every lane
-    copy(it + NST - 1, stage == 0 ? NST - 1 : stage - 1);
-    to.go(p, cur, warp, out_st, [&](const Order<WALK>& o, auto& f) {
-      const Lane l = place<V, SHARED>(p, o.chain, lane);
-      const int64_t r0 = (int64_t)o.chunk * p.steps + warp * kBwd, t0 = p.T - 1 - r0;
-      f.at[0] = (const char*)((const X*)p.dx + (l.b * p.T + t0) * p.D + l.ch);
-      f.at[1] = (const char*)((const G*)p.dgate + (l.b * p.T + t0) * p.H + l.gate);
-      f.left = l.in ? (int)(p.T - r0) : 0;
-      state_at = (size_t)(l.b * p.D + l.ch);
-      gate_slot = l.slot;
-      half0[0] = (uint32_t)(uintptr_t)((const X*)p.dh + l.b * p.dh_sb + (p.T - 1) * p.dh_st + l.ch);
-      half0[1] = (uint32_t)(uintptr_t)((const X*)p.hsaved + l.b * p.h_sb + (p.T - 2) * p.h_st + l.ch);
-      half0[2] = (uint32_t)(uintptr_t)((const X*)p.x + l.b * p.x_sb + (p.T - 1) * p.x_st + l.ch);
-      half0[3] = (uint32_t)(uintptr_t)((const G*)p.gate + l.b * p.g_sb + (p.T - 1) * p.g_st + l.gate);
-      if (o.chunk == 0 || !WALK)
-#pragma unroll
-        for (int v = 0; v < V; ++v) vput(carry, v, o.chunk == 0 && l.in && p.dstate ? p.dstate[state_at + v] : 0.0f);
-    });
-    const uint32_t r0 = cur.chunk * p.steps + warp * kBwd;  // steps counted from the end
-    auto half = [&](int k, int i) { return half0[k] + (r0 + i) * (uint32_t)in_st[k]; };
-    uint32_t early[V];
-    if (!WALK) {
-      if (threadIdx.x == 0) sh.tiles[(it + NST) & 3] = atomicAdd(p.ticket, 1u);
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        early[v] = warp == 0 && cur.chunk > 0
-                       ? ld_word(p.states + (size_t)((cur.chunk - 1) * p.chains + cur.chain) * 32 * V + lane * V + v)
-                       : 0;
-    }
-    copies_wait<NST - 1>();
-    __syncwarp();  // the words that other lanes have copied
-    const char* mine = ring + stage * Tile::kBytes;
-    Floats<V> ma = vset<V>(1.0f), mb = vset<V>(0.0f), in;
-    auto gate_at = [&](int i, Floats<V>& a, Floats<V>& om) {
-      if constexpr (SHARED) gates_of<SIG, V>(HeadGates<G, kBwd>::get(mine + Tile::kG, i * (int)p.heads_per + gate_slot, half(3, i)), a, om);
-      else gates_of<SIG, V>(Tile::CG::get(mine + Tile::kG, i, half(3, i)), a, om);
+  MPB_D void copy(uint32_t q, const Place<kBwd, 4>& f) const {
+    auto column = [&](uint32_t to, int k, int less) {
+      copy_column<typename Tile::CX, kBwd>(p, to, f.at[k], in_st[k], f.left - less, f.end - less, f.wide);
     };
+    column(q, 0, 0);
+    column(q + Tile::kH, 1, 1);  // h[-1] is h0
+    if (SIG) column(q + Tile::kX, 2, 0);
+    if constexpr (SHARED) Tile::HG::copy(q + Tile::kG, f.at[3], in_st[3], f.end, (int)p.heads_per, f.heads, p.by_heads_per);
+    else copy_column<typename Tile::CG, kBwd>(p, q + Tile::kG, f.at[3], in_st[3], f.left, f.end, f.wide);
+  }
+  MPB_D void sub_words(const Lane& l) {
+    gate_slot = l.slot;
+    auto bit = [&](const void* q, int64_t sb, int64_t st, int64_t t) {
+      return (uint32_t)(uintptr_t)((const X*)q + l.b * sb + t * st + l.ch);
+    };
+    half0[0] = bit(p.dh, p.dh_sb, p.dh_st, p.T - 1);
+    half0[1] = bit(p.hsaved, p.h_sb, p.h_st, p.T - 2);
+    half0[2] = bit(p.x, p.x_sb, p.x_st, p.T - 1);
+    half0[3] = (uint32_t)(uintptr_t)((const G*)p.gate + l.b * p.g_sb + (p.T - 1) * p.g_st + l.gate);
+  }
+  MPB_D void output(uint32_t chain, uint32_t chunk, Place<kBwd, 2>& f) {
+    const Lane l = place<V, SHARED>(p, chain, lane);
+    const int64_t r0 = (int64_t)chunk * p.steps + warp * kBwd, t0 = p.T - 1 - r0;
+    f.at[0] = (const char*)((const X*)p.dx + (l.b * p.T + t0) * p.D + l.ch);
+    f.at[1] = (const char*)((const G*)p.dgate + (l.b * p.T + t0) * p.H + l.gate);
+    f.left = l.in ? (int)(p.T - r0) : 0;
+    state_at = (size_t)(l.b * p.D + l.ch);
+    sub_words(l);
+  }
+  // r0: the warp's first step in the tile, counted from the end
+  MPB_D uint32_t half(int k, uint32_t r0, int i) const { return half0[k] + (r0 + i) * (uint32_t)in_st[k]; }
+  MPB_D void gate_at(const char* mine, int i, uint32_t r0, Floats<V>& a, Floats<V>& om) const {
+    if constexpr (SHARED) gates_of<SIG, V>(Tile::HG::get(mine + Tile::kG, i * (int)p.heads_per + gate_slot, half(3, r0, i)), a, om);
+    else gates_of<SIG, V>(Tile::CG::get(mine + Tile::kG, i, half(3, r0, i)), a, om);
+  }
+  MPB_D void fold(const char* mine, uint32_t r0, Floats<V>& ma, Floats<V>& mb) const {
+    ma = vset<V>(1.0f), mb = vset<V>(0.0f);
 #pragma unroll
     for (int i = 0; i < kBwd; ++i) {
       Floats<V> a, om;
-      gate_at(i, a, om);
+      gate_at(mine, i, r0, a, om);
       ma = vmul(ma, a);
-      mb = vmul(a, vadd(mb, unpack(Tile::CX::get(mine, i, half(0, i)))));
+      mb = vmul(a, vadd(mb, unpack(Tile::CX::get(mine, i, half(0, r0, i)))));
     }
-    join<V, WALK>(p, sh, it & 1, cur.chain, cur.chunk, warp, lane, ma, mb, early, carry, in);
+  }
+  // The warp's steps from the state `in` (u of the step after).
+  MPB_D void write(const char* mine, uint32_t chain, uint32_t r0, const Place<kBwd, 2>& to, Floats<V>& in) const {
     const int n = to.steps();
     char *dx = const_cast<char*>(to.at[0]), *dg = const_cast<char*>(to.at[1]);
     float sum[kBwd];
     auto step = [&](int i, Floats<V> low) {  // low: h[t - 1]
       Floats<V> a, om;
-      gate_at(i, a, om);
-      const Floats<V> s = vadd(unpack(Tile::CX::get(mine, i, half(0, i))), in);
-      if constexpr (SIG) low = vfma(unpack(Tile::CX::get(mine + Tile::kX, i, half(2, i))), vset<V>(-1.0f), low);
+      gate_at(mine, i, r0, a, om);
+      const Floats<V> s = vadd(unpack(Tile::CX::get(mine, i, half(0, r0, i))), in);
+      if constexpr (SIG) low = vfma(unpack(Tile::CX::get(mine + Tile::kX, i, half(2, r0, i))), vset<V>(-1.0f), low);
       put_global(dx, pack<X>(SIG ? vmul(om, s) : s));
       dx = ahead_by(dx, out_st[0]);
       in = vmul(a, s);
@@ -844,15 +910,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd(ScanArgs p) {
         dg = ahead_by(dg, out_st[1]);
       }
     };
+    auto before = [&](int i) { return unpack(Tile::CX::get(mine + Tile::kH, i, half(1, r0, i))); };
     if (__all_sync(0xffffffffu, to.left > kBwd)) {
 #pragma unroll
-      for (int i = 0; i < kBwd; ++i) step(i, unpack(Tile::CX::get(mine + Tile::kH, i, half(1, i))));
+      for (int i = 0; i < kBwd; ++i) step(i, before(i));
     } else {
 #pragma unroll
       for (int i = 0; i < kBwd; ++i) {
         sum[i] = 0.0f;
         if (i < n) {
-          Floats<V> low = unpack(Tile::CX::get(mine + Tile::kH, i, half(1, i)));
+          Floats<V> low = before(i);
           if (to.left - 1 == i)  // the first step of the sequence
 #pragma unroll
             for (int v = 0; v < V; ++v) vput(low, v, p.h0 ? p.h0[state_at + v] : 0.0f);
@@ -863,37 +930,119 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd(ScanArgs p) {
     if (p.dh0 && n > 0 && n == to.left)
 #pragma unroll
       for (int v = 0; v < V; ++v) p.dh0[state_at + v] = vget(in, v);
-    if (SHARED) {
-      // a head's lanes: a power of two of them, or the whole warp (idle lanes add zeros)
-      const int lanes = p.heads_per > 1 ? (int)p.lanes_per : 32;
-      int first, left;
-      sum_over_lanes(sum, lane, lanes, first, left);
-      // of the lanes that hold the same sums the one with the upper bits clear writes
-      const int at = p.heads_per > 1 ? lane & (lanes - 1) : lane;
-      const uint32_t b = p.by_groups.div(cur.chain), group = cur.chain - b * p.groups;
-      const int64_t head = p.groups_per > 1 ? (int64_t)p.by_groups_per.div(group)
-                                            : (int64_t)group * p.heads_per + (p.heads_per > 1 ? lane / lanes : 0);
-      if (at < kBwd && head < p.H) {
-        const int64_t bt = (int64_t)b * p.T;
+    if constexpr (SHARED) head_sums(sum, chain, r0);
+  }
+  MPB_D void head_sums(float (&sum)[kBwd], uint32_t chain, uint32_t r0) const {
+    // a head's lanes: a power of two of them, or the whole warp (idle lanes add zeros)
+    const int lanes = p.heads_per > 1 ? (int)p.lanes_per : 32;
+    int first, left;
+    sum_over_lanes(sum, lane, lanes, first, left);
+    // of the lanes that hold the same sums the one with the upper bits clear writes
+    const int at = p.heads_per > 1 ? lane & (lanes - 1) : lane;
+    const uint32_t b = p.by_groups.div(chain), group = chain - b * p.groups;
+    const int64_t head = p.groups_per > 1 ? (int64_t)p.by_groups_per.div(group)
+                                          : (int64_t)group * p.heads_per + (p.heads_per > 1 ? lane / lanes : 0);
+    if (at >= kBwd || head >= p.H) return;
+    const int64_t bt = (int64_t)b * p.T;
 #pragma unroll
-        for (int i = 0; i < kBwd; ++i) {
-          const int64_t t = p.T - 1 - (int64_t)r0 - (first + i);
-          if (i < left && t >= 0) {
-            if (p.groups_per > 1) {
-              p.part[((bt + t) * p.H + head) * p.groups_per + (group - (uint32_t)head * p.groups_per)] = sum[i];
-            } else {
-              float a, om;
-              gate_of<SIG>(to_f(((const G*)p.gate)[(int64_t)b * p.g_sb + t * p.g_st + head]), a, om);
-              ((G*)p.dgate)[(bt + t) * p.H + head] = Cvt<G>::from(SIG ? sum[i] * (a * om) : sum[i]);
-            }
-          }
+    for (int i = 0; i < kBwd; ++i) {
+      const int64_t t = p.T - 1 - (int64_t)r0 - (first + i);
+      if (i < left && t >= 0) {
+        if (p.groups_per > 1) {
+          p.part[((bt + t) * p.H + head) * p.groups_per + (group - (uint32_t)head * p.groups_per)] = sum[i];
+        } else {
+          float a, om;
+          gate_of<SIG>(to_f(((const G*)p.gate)[(int64_t)b * p.g_sb + t * p.g_st + head]), a, om);
+          ((G*)p.dgate)[(bt + t) * p.H + head] = Cvt<G>::from(SIG ? sum[i] * (a * om) : sum[i]);
         }
       }
     }
-    if (WALK && blockDim.x == 32) carry = in;
+  }
+};
+
+template <class X, class G, bool SIG, int V, bool SHARED>
+__global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd_walk(ScanArgs p) {
+  using Tile = BwdTile<X, G, SIG, V, SHARED>;
+  constexpr int NST = Tile::kStages;
+  extern __shared__ __align__(16) char ring[];
+  __shared__ Shared<V> sh;
+  Backward<X, G, SIG, V, SHARED> bw(p);
+  const uint32_t base = smem_u32(ring);
+  if (p.status && blockIdx.x == 0 && threadIdx.x == 0) *p.status = MPB_OK;  // nothing waits
+  Order cur, ahead;
+  Place<kBwd, 4> from;
+  Place<kBwd, 2> to;
+  auto copy = [&](int s) {  // the walk's next tile into stage s
+    if (ahead.here(p)) {
+      if (ahead.chunk == 0) bw.inputs(ahead.chain, 0, from);
+      else from.move(p, bw.in_st);
+      bw.copy(base + s * Tile::kBytes, from);
+      ahead.next(p);
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < NST - 1; ++s) copy(s);
+  int stage = 0;
+  Floats<V> carry = vset<V>(0.0f);
+  for (int it = 0; cur.here(p); ++it) {
+    __syncwarp();  // the stage that is filled next has been read by every lane
+    copy(stage == 0 ? NST - 1 : stage - 1);
+    if (cur.chunk == 0) {
+      bw.output(cur.chain, 0, to);
+#pragma unroll
+      for (int v = 0; v < V; ++v) vput(carry, v, to.left > 0 && p.dstate ? p.dstate[bw.state_at + v] : 0.0f);
+    } else {
+      to.move(p, bw.out_st);
+    }
+    copies_wait<NST - 1>();
+    __syncwarp();  // the words that other lanes have copied
+    const char* mine = ring + stage * Tile::kBytes;
+    const uint32_t r0 = cur.chunk * p.steps + bw.warp * kBwd;
+    Floats<V> ma, mb, in;
+    bw.fold(mine, r0, ma, mb);
+    join<V>(sh, it & 1, bw.warp, bw.lane, ma, mb, carry, in);
+    bw.write(mine, cur.chain, r0, to, in);
+    if (blockDim.x == 32) carry = in;
     cur.next(p);
     stage = stage + 1 == NST ? 0 : stage + 1;
   }
+}
+
+template <class X, class G, bool SIG, int V, bool SHARED>
+__global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd_far(ScanArgs p) {
+  using Tile = BwdTile<X, G, SIG, V, SHARED>;
+  extern __shared__ __align__(16) char ring[];
+  __shared__ Shared<V> sh;
+  Backward<X, G, SIG, V, SHARED> bw(p);
+  const uint32_t base = smem_u32(ring);
+  auto r0_of = [&](uint32_t chunk) { return chunk * p.steps + bw.warp * kBwd; };
+  look_back_tiles<V>(
+      p, sh, bw.warp, bw.lane,
+      [&](uint32_t chain, uint32_t chunk, int stage, int side) {
+        bw.sub_words(place<V, SHARED>(p, chain, bw.lane));
+        Floats<V> ma, mb;
+        bw.fold(ring + stage * Tile::kBytes, r0_of(chunk), ma, mb);
+        put_map<V>(sh, side, bw.warp, bw.lane, ma, mb);
+      },
+      [&](uint32_t chain, uint32_t chunk, float (&c)[V]) {
+        const Lane l = place<V, SHARED>(p, chain, bw.lane);
+#pragma unroll
+        for (int v = 0; v < V; ++v) c[v] = chunk < 32 && l.in && p.dstate ? p.dstate[l.b * p.D + l.ch + v] : 0.0f;
+      },
+      [&](uint32_t chain, uint32_t chunk, int stage, Floats<V> in) {
+        Place<kBwd, 2> to;
+        bw.output(chain, chunk, to);
+        bw.write(ring + stage * Tile::kBytes, chain, r0_of(chunk), to, in);
+      },
+      [&](bool is, uint32_t chain, uint32_t chunk, int stage) {
+        if (is) {
+          Place<kBwd, 4> from;
+          bw.inputs(chain, chunk, from);
+          bw.copy(base + stage * Tile::kBytes, from);
+        }
+        copies_commit();
+      });
 }
 
 // Heads of more channels than a block holds: the sum of their groups' sums, in order.
@@ -1062,17 +1211,16 @@ int launch_tiles(const char* what, const ScanArgs& p, int per, int smem, cudaStr
 template <class X, class G, bool SIG, int V, bool SHARED>
 int launch_fwd_v(const ScanArgs& p, cudaStream_t s) {
   using Tile = FwdTile<X, G, V, SHARED>;
-  constexpr int smem = Tile::kStages * Tile::kBytes;
-  return p.walk ? launch_tiles<k_gscan<X, G, SIG, V, SHARED, true>>("gated_scan", p, kFwd, smem, s)
-                : launch_tiles<k_gscan<X, G, SIG, V, SHARED, false>>("gated_scan", p, kFwd, smem, s);
+  return p.walk ? launch_tiles<k_gscan_walk<X, G, SIG, V, SHARED>>("gated_scan", p, kFwd, Tile::kStages * Tile::kBytes, s)
+                : launch_tiles<k_gscan_far<X, G, SIG, V, SHARED>>("gated_scan", p, kFwd, 3 * Tile::kBytes, s);
 }
 
 template <class X, class G, bool SIG, int V, bool SHARED>
 int launch_bwd_v(const ScanArgs& p, cudaStream_t s) {
   using Tile = BwdTile<X, G, SIG, V, SHARED>;
-  constexpr int smem = Tile::kStages * Tile::kBytes;
-  return p.walk ? launch_tiles<k_gscan_bwd<X, G, SIG, V, SHARED, true>>("gated_scan_backward", p, kBwd, smem, s)
-                : launch_tiles<k_gscan_bwd<X, G, SIG, V, SHARED, false>>("gated_scan_backward", p, kBwd, smem, s);
+  const char* what = "gated_scan_backward";
+  return p.walk ? launch_tiles<k_gscan_bwd_walk<X, G, SIG, V, SHARED>>(what, p, kBwd, Tile::kStages * Tile::kBytes, s)
+                : launch_tiles<k_gscan_bwd_far<X, G, SIG, V, SHARED>>(what, p, kBwd, 3 * Tile::kBytes, s);
 }
 
 template <class X, class G, bool SIG>

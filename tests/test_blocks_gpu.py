@@ -110,6 +110,22 @@ def test_scan_without_batch_and_out(ms):
     assert torch.equal(h.torch(), full.torch()[0]) and torch.equal(last.torch(), flast.torch()[0])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,T,D", [(1, 1000, 70), (1, 300, 33), (2, 4000, 64), (1, 6000, 1), (120, 500, 64)])
+def test_scan_carries_the_first_state_undiminished(ms, B, T, D, dtype):
+    """Gates of one and no input: every state is the first one, whichever pieces a long sequence was joined from and
+    however early they met; backward every gradient is that of the last state."""
+    A = ms.from_torch
+    one, zero = torch.ones(B, T, D, dtype=TORCH[dtype], device="cuda"), torch.zeros(B, T, D, dtype=TORCH[dtype], device="cuda")
+    h0 = rand(B, D, seed=1)
+    want = h0.to(TORCH[dtype])[:, None].expand(B, T, D)
+    for _ in range(20):
+        h, last = ms.gated_scan(A(zero), A(one), A(h0), return_state=True)
+        assert torch.equal(h.torch(), want) and torch.equal(last.torch(), h0)
+        dx, _, dh0 = ms.gated_scan_backward(A(zero), A(zero), A(one), h, A(h0), A(h0))
+        assert torch.equal(dx.torch(), want) and torch.equal(dh0.torch(), h0)
+
+
 @pytest.mark.parametrize("T", [5, 700, 20000])
 def test_scan_restarts_where_the_gate_is_zero(ms, T):
     """Sequences packed along time: a zero gate drops what came before it, in every layout of the pieces."""
