@@ -269,6 +269,7 @@ template <int W>
 struct Kept {
   uint4 w;
   uint32_t first;
+  MPB_D Kept() {}
   MPB_D Kept(const Dropper& d, uint64_t i) : w(drop_words(d, i >> 3)), first((uint32_t)i & 7) {}
   MPB_D bool operator()(const Dropper& d, int j) const {
     if constexpr (W == 8) return stays(d, w, j);
@@ -293,6 +294,25 @@ MPB_D const T* row_at(const void* base, int r, int64_t sr, int skip) {
 MPB_D float row_sum(float v, float* red) { return blockDim.x == 32 ? warp_sum(v) : block_sum(v, red); }
 MPB_D float fold(float v) { return v; }
 MPB_D float fold(float2 v) { return v.x + v.y; }
+
+// What dropout keeps of a row. EARLY: drawn while the row's loads are under way,
+// where that is a counter per pack; else drawn at each pack. (16384 x 4096 bf16:
+// backward 232 us early, 243 us late; forward, where the words cost a resident
+// block, 144 and 130 us.)
+template <int W, int NV, bool EARLY>
+struct KeptRow {
+  static constexpr bool kEarly = EARLY && W == 8;
+  Kept<W> all[kEarly ? NV : 1];
+  MPB_D KeptRow(const NormArgs& p, int r, int skip, int step) {
+    if constexpr (kEarly)
+#pragma unroll
+      for (int k = 0; k < NV; ++k) all[k] = Kept<W>(p.drop, (uint64_t)((int64_t)r * p.D + skip + k * step * W));
+  }
+  MPB_D Kept<W> at(const NormArgs& p, int r, int k, int c) const {
+    if constexpr (kEarly) return all[k];
+    else return Kept<W>(p.drop, (uint64_t)((int64_t)r * p.D + c));
+  }
+};
 
 // The values and slopes of the gate for the pack at column c of row r; `full`
 // has been loaded with the row's other operands. One switch for all elements.
@@ -369,6 +389,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_rows(NormArgs p) {
       if (MODE != kPlain && p.gate_kind == MPB_GATE_FULL) g[k].load(gr + at);
     }
   }
+  const KeptRow<W, NV, false> kept_row(p, r, skip, step);
   F ss = zero, y[NV][NP];
   float rz = 0.0f;
   if (MODE != kPlain) {
@@ -402,7 +423,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_rows(NormArgs p) {
           }
         };
         if constexpr (MODE == kDropped) {
-          const Kept<W> kept(p.drop, (uint64_t)((int64_t)r * D + q * W));
+          const Kept<W> kept = kept_row.at(p, r, k, q * W);
           branch([&](int i, F a, F b) { return kept.pick(p.drop, i, a, b); });
         } else {
           branch([](int, F a, F) { return a; });
@@ -503,6 +524,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
         }
       }
     const float rz = MODE != kPlain ? p.rstd[r] : 0.0f, ry = p.rstd[(MODE != kPlain ? p.R : 0) + r];
+    const KeptRow<W, NV, MODE == kDropped> kept_row(p, r, skip, step);
     float back = 0.0f;  // of y in dx: r_y^3 mean(y w du)
     if (ALL || p.du) {
       F dot = zero;
@@ -558,7 +580,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
             }
           };
           if constexpr (MODE == kDropped) {
-            const Kept<W> kept(p.drop, (uint64_t)((int64_t)r * D + q * W));
+            const Kept<W> kept = kept_row.at(p, r, k, q * W);
             branch([&](int i, F a) { return kept.pick(p.drop, i, a, zero); });
           } else {
             branch([](int, F a) { return a; });
