@@ -204,7 +204,7 @@ int mpb_cumsum_status(const void* scratch, mpb_stream_t stream);
  * zero. mode MPB_SCAN_LINEAR: h[t] = g h[t-1] + x[t]; MPB_SCAN_SIGMOID:
  * h[t] = s h[t-1] + (1 - s) x[t], s = sigmoid(g). Writes h (B, T, D) in x's
  * type and, when state is not NULL, h[T-1] (h0 when T == 0) in float; state
- * may be h0 itself. Scratch: mpb_gated_scan_scratch_bytes(..., backward = 0). */
+ * may not overlap h0. Scratch: mpb_gated_scan_scratch_bytes(..., backward = 0). */
 size_t mpb_gated_scan_scratch_bytes(int64_t B, int64_t T, int64_t D, int64_t H, int x_dtype, int gate_dtype,
                                     int backward);
 int mpb_gated_scan(int64_t B, int64_t T, int64_t D, int64_t H, const void* x, int x_dtype, int64_t x_sb, int64_t x_st,

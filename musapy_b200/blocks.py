@@ -16,8 +16,9 @@ import torch
 from . import dtypes as _dt
 from . import errors
 from ._lib import LIB, NATIVE, check
-from .array import _LAYOUTS, Array, contiguous_strides
-from .ops import _CHECK_SCAN_STATUS, _alias, _check_out, _launch, _out, _same_device, _stream, contiguous, full
+from . import streams as _streams
+from .array import _LAYOUTS, _TORCH_DEVICES, Array, contiguous_strides
+from .ops import _CHECK_SCAN_STATUS, _alias, _check_out, _out, _same_device, _stream, contiguous, full
 
 _MODES = {"linear": 0, "sigmoid": 1}
 _ACTIVATIONS = {"linear": 0, "sigmoid": 1, "silu": 2}
@@ -63,13 +64,13 @@ def _choice(name: str, what: str, value, table: dict) -> int:
 
 
 def _probability(name: str, p) -> float:
-    if not isinstance(p, numbers.Real) or not 0.0 <= p <= 1.0:
+    if (type(p) is not float and not isinstance(p, numbers.Real)) or not 0.0 <= p <= 1.0:
         raise errors.MusapyError(f"{name}: dropout probability {p!r} outside [0, 1]")
     return float(p)
 
 
 def _counter(name: str, what: str, v) -> int:
-    if not isinstance(v, numbers.Integral):
+    if type(v) is not int and not isinstance(v, numbers.Integral):
         raise TypeError(f"{name}: {what} must be an integer, got {type(v).__name__}")
     return int(v) & _U64
 
@@ -86,23 +87,40 @@ def _sptr(scratch):
     return scratch.data_ptr() if scratch is not None else None
 
 
+_empty, _U8, _new_array = torch.empty, torch.uint8, Array.__new__
+
+
+def _new(s, shape: tuple, d: _dt.Dtype, dev: int) -> Array:
+    """A result on the stream `s`: what ``ops._out`` makes, with the stream looked up once per operator."""
+    lay, tdev = _LAYOUTS.get(shape), _TORCH_DEVICES.get(dev)
+    if lay is None or tdev is None:
+        return _out(shape, d, dev)
+    buf = _empty(max(16, (lay[1] * d.itemsize + 15) & ~15), dtype=_U8, device=tdev)
+    buf._mpb_owner = s
+    a = _new_array(Array)
+    a._buf, a._shape, a._strides, a._offset, a._dtype, a._dev, a._name = buf, shape, lay[0], 0, d, dev, None
+    a._dev_src = a._dt_src = "input_array"
+    a._ptr = a._sid = buf.data_ptr()
+    return a
+
+
 def _dense(x: Array) -> bool:
     """x is C-contiguous (by the cached strides of its shape where they are known)."""
     lay = _LAYOUTS.get(x._shape)
     return (lay is not None and lay[0] == x._strides) or x._is_c_contiguous()
 
 
-def _carve(dev: int, *parts):
+def _carve(s, dev: int, *parts):
     """Several small results in one allocation: an Array for each (shape, dtype). To the alias checks each is an
     allocation of its own (they do not overlap)."""
     total, at = 0, []
     for shape, d in parts:
         at.append(total)
         total += (_prod(shape) * d.itemsize + 15) & ~15
-    first = _out((max(total, 16),), _dt.uint8, dev)
+    first = _new(s, (max(total, 16),), _dt.uint8, dev)
     made = []
     for (shape, d), start in zip(parts, at):
-        a = Array.__new__(Array)
+        a = _new_array(Array)
         a._buf, a._shape, a._strides, a._offset = first._buf, shape, contiguous_strides(shape), start // d.itemsize
         a._dtype, a._dev, a._name, a._dev_src, a._dt_src = d, dev, None, first._dev_src, first._dt_src
         a._ptr = a._sid = first._ptr + start
@@ -167,8 +185,9 @@ def gated_scan(x, gate, h0=None, mode="linear", return_state=False, out=None):
         _check_out(out, x._shape, x._dtype, dev, name)
         if _alias(out, *ins):
             raise errors.MemoryError("out= aliases an input buffer (AliasDetected)")
-    h = out if out is not None else _out(x._shape, x._dtype, dev)
-    state = _out(sshape, _dt.float32, dev) if return_state else None
+    s = _streams.current_stream(dev)
+    h = out if out is not None else _new(s, x._shape, x._dtype, dev)
+    state = _new(s, sshape, _dt.float32, dev) if return_state else None
     if B * D:
         nbytes = NATIVE.gated_scan_scratch_bytes(B, T, D, H, x._dtype.code, gate._dtype.code, 0)
         scratch = _scratch(nbytes, dev)
@@ -176,7 +195,7 @@ def gated_scan(x, gate, h0=None, mode="linear", return_state=False, out=None):
         gb, gt = _btd(gate)
         check(NATIVE.gated_scan(B, T, D, H, x._ptr, x._dtype.code, xb, xt, gate._ptr, gate._dtype.code, gb, gt,
                                 _ptr(h0), m, h._ptr, _ptr(state), _sptr(scratch), nbytes,
-                                _launch(name, dev, *ins, h, state)), name)
+                                _streams.launch_on(s, name, *ins, h, state)), name)
         _scan_status(name, scratch, dev)
     return (h, state) if return_state else h
 
@@ -199,15 +218,16 @@ def gated_scan_backward(dh, x, gate, h, h0=None, dstate=None, mode="linear"):
         dstate = _floats(name, "dstate", dstate, sshape)
         ins.append(dstate)
     dev = _same_device(name, *ins)
-    dx, dgate = _out(x._shape, x._dtype, dev), _out(gate._shape, gate._dtype, dev)
-    dh0 = _out(sshape, _dt.float32, dev)
+    s = _streams.current_stream(dev)
+    dx, dgate = _new(s, x._shape, x._dtype, dev), _new(s, gate._shape, gate._dtype, dev)
+    dh0 = _new(s, sshape, _dt.float32, dev)
     if B * D:
         nbytes = NATIVE.gated_scan_scratch_bytes(B, T, D, H, x._dtype.code, gate._dtype.code, 1)
         scratch = _scratch(nbytes, dev)
         check(NATIVE.gated_scan_backward(B, T, D, H, dh._ptr, *_btd(dh), x._ptr, x._dtype.code, *_btd(x), gate._ptr,
                                          gate._dtype.code, *_btd(gate), h._ptr, *_btd(h), _ptr(h0), _ptr(dstate), m,
                                          dx._ptr, dgate._ptr, dh0._ptr, _sptr(scratch), nbytes,
-                                         _launch(name, dev, *ins, dx, dgate, dh0)), name)
+                                         _streams.launch_on(s, name, *ins, dx, dgate, dh0)), name)
         _scan_status(name, scratch, dev)
     return dx, dgate, dh0
 
@@ -228,11 +248,12 @@ def gated_scan_step(state, x, gate, mode="linear", out=None):
         _check_out(out, x._shape, x._dtype, dev, name)
         if _alias(out, x, gate, state):
             raise errors.MemoryError("out= aliases an input buffer (AliasDetected)")
-    h = out if out is not None else _out(x._shape, x._dtype, dev)
+    s = _streams.current_stream(dev)
+    h = out if out is not None else _new(s, x._shape, x._dtype, dev)
     if B * D:
         check(NATIVE.gated_scan_step(B, D, H, x._ptr, x._dtype.code, x._strides[0], gate._ptr, gate._dtype.code,
                                      gate._strides[0], m, state._ptr, h._ptr,
-                                     _launch(name, dev, x, gate, state, h)), name)
+                                     _streams.launch_on(s, name, x, gate, state, h)), name)
     return h
 
 
@@ -306,13 +327,14 @@ def rms_norm(x, weight, eps=1e-6):
     D = x._shape[-1]
     w = _vector(name, "weight", weight, D)
     dev = _same_device(name, x, w)
+    s = _streams.current_stream(dev)
     lead = x._shape[:-1]
-    u, rstd = _out(x._shape, x._dtype, dev), _out(lead, _dt.float32, dev)
+    u, rstd = _new(s, x._shape, x._dtype, dev), _new(s, lead, _dt.float32, dev)
     R = _prod(lead)
     if R * D:
         check(NATIVE.gated_residual_norm(R, D, x._dtype.code, x._ptr, xr, None, 0, None, 0, 0, 0, None, w._ptr, 1.0,
                                          float(eps), 0.0, 0, 0, None, u._ptr, rstd._ptr,
-                                         _launch(name, dev, x, w, u, rstd)), name)
+                                         _streams.launch_on(s, name, x, w, u, rstd)), name)
     return u, rstd
 
 
@@ -342,13 +364,14 @@ def gated_residual_norm(x, z, w_post, w_pre, gate=None, activation="linear", sca
     g, kind, gr = _gate(name, gate, x)
     ins = [x, z, post, pre] if g is None else [x, z, post, pre, g]
     dev = _same_device(name, *ins)
-    y, u = _out(x._shape, x._dtype, dev), _out(x._shape, x._dtype, dev)
-    rstd = _out((2,) + lead, _dt.float32, dev)
+    s = _streams.current_stream(dev)
+    y, u = _new(s, x._shape, x._dtype, dev), _new(s, x._shape, x._dtype, dev)
+    rstd = _new(s, (2,) + lead, _dt.float32, dev)
     R = _prod(lead)
     if R * D:
         check(NATIVE.gated_residual_norm(R, D, x._dtype.code, x._ptr, xr, z._ptr, zr, _ptr(g), gr, kind, act, post._ptr,
                                          pre._ptr, float(scale), float(eps), p, seed, offset, y._ptr, u._ptr, rstd._ptr,
-                                         _launch(name, dev, *ins, y, u, rstd)), name)
+                                         _streams.launch_on(s, name, *ins, y, u, rstd)), name)
     return y, u, rstd
 
 
@@ -386,22 +409,23 @@ def _norm_backward(name, dy, du, y, z, w_post, w_pre, rstd, gate, activation, sc
     g, kind, gr = _gate(name, gate, y)
     ins += [pre, rstd] if g is None else [pre, rstd, g]
     dev = _same_device(name, *ins)
+    s = _streams.current_stream(dev)
     if R * D == 0:  # nothing to read: the sums over rows or channels are zero
         zeros = lambda shape, d: full(shape, 0.0, d, dev)
-        return (_out(y._shape, y._dtype, dev), _out(y._shape, y._dtype, dev) if branch else None,
+        return (_new(s, y._shape, y._dtype, dev), _new(s, y._shape, y._dtype, dev) if branch else None,
                 zeros(g._shape, y._dtype) if g is not None else None, zeros((D,), _dt.float32) if branch else None,
                 zeros((D,), _dt.float32))
-    dx = _out(y._shape, y._dtype, dev)
-    dz = _out(y._shape, y._dtype, dev) if branch else None
-    dpost = _out((D,), _dt.float32, dev) if branch else None
-    dpre = _out((D,), _dt.float32, dev)
-    dgate = _out(g._shape, y._dtype, dev) if g is not None else None
+    dx = _new(s, y._shape, y._dtype, dev)
+    dz = _new(s, y._shape, y._dtype, dev) if branch else None
+    dpost = _new(s, (D,), _dt.float32, dev) if branch else None
+    dpre = _new(s, (D,), _dt.float32, dev)
+    dgate = _new(s, g._shape, y._dtype, dev) if g is not None else None
     nbytes = NATIVE.gated_residual_norm_scratch_bytes(R, D, y._dtype.code, int(branch), kind)
     scratch = _scratch(nbytes, dev)
     check(NATIVE.gated_residual_norm_backward(
         R, D, y._dtype.code, _ptr(dy), dyr, _ptr(du), dur, y._ptr, yr, _ptr(z), zr, _ptr(g), gr, kind, act, _ptr(post),
         pre._ptr, rstd._ptr, float(scale), p, seed, offset, dx._ptr, _ptr(dz), _ptr(dgate), _ptr(dpost), dpre._ptr, _sptr(scratch), nbytes,
-        _launch(name, dev, *ins, dx, dz, dgate, dpost, dpre)), name)
+        _streams.launch_on(s, name, *ins, dx, dz, dgate, dpost, dpre)), name)
     return dx, dz, dgate, dpost, dpre
 
 
@@ -420,8 +444,9 @@ def dropout(x, p, seed, offset=0, out=None):
         if _alias(out, x):
             raise errors.MemoryError("out= aliases an input buffer (AliasDetected)")
     src = x if _dense(x) else contiguous(x)
-    y = out if out is not None else _out(x._shape, x._dtype, dev)
-    check(NATIVE.dropout(src.size, src._ptr, src._dtype.code, p, seed, offset, y._ptr, _launch(name, dev, src, y)), name)
+    s = _streams.current_stream(dev)
+    y = out if out is not None else _new(s, x._shape, x._dtype, dev)
+    check(NATIVE.dropout(src.size, src._ptr, src._dtype.code, p, seed, offset, y._ptr, _streams.launch_on(s, name, src, y)), name)
     return y
 
 
@@ -476,12 +501,13 @@ def policy_loss(logits, targets, old_logp, advantages, ref_logp=None, mask=None,
     if N and V == 0:
         raise errors.ShapeError(f"{name}: empty vocabulary")
     dev = _same_device(name, *ins)
+    s = _streams.current_stream(dev)
     nbytes = NATIVE.policy_loss_scratch_bytes(N, V, z._dtype.code)
-    loss, logp, kl, clipped, scratch = _carve(dev, ((), _dt.float32), (lead, _dt.float32), (lead, _dt.float32),
+    loss, logp, kl, clipped, scratch = _carve(s, dev, ((), _dt.float32), (lead, _dt.float32), (lead, _dt.float32),
                                               (lead, _dt.bool_), ((nbytes,), _dt.uint8))
-    dlogits = _out(z._shape, z._dtype, dev) if grad else None
+    dlogits = _new(s, z._shape, z._dtype, dev) if grad else None
     check(NATIVE.policy_loss(N, V, z._ptr, z._dtype.code, zr, targets._ptr, targets._dtype.code, old._ptr, adv._ptr,
                              _ptr(ref_logp), _ptr(mask), float(clip_low), float(clip_high), float(kl_coef),
                              float(grad_scale), loss._ptr, logp._ptr, kl._ptr, clipped._ptr, _ptr(dlogits),
-                             scratch._ptr, nbytes, _launch(name, dev, *ins, loss, dlogits)), name)
+                             scratch._ptr, nbytes, _streams.launch_on(s, name, *ins, loss, dlogits)), name)
     return PolicyLoss(loss, logp, kl, clipped, dlogits)

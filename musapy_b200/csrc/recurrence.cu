@@ -20,9 +20,10 @@
 // (backward 8) steps. A warp folds its steps to the map c -> A c + B that they
 // apply to the state; the block joins the maps of its warps, and each warp
 // then runs its steps once more from the state that enters them and writes.
-// Each thread copies the words it will use itself into shared memory some
-// tiles ahead (cp.async), so the copies of the next tiles are in flight while
-// a tile is computed, and no barrier guards them.
+// A warp copies its own steps' rows into shared memory some tiles ahead
+// (cp.async, 16 bytes per lane where the layout allows), so the copies of the
+// next tiles are in flight while a tile is computed, and no block barrier
+// guards them.
 //
 // Along time either a block walks a chain (the tiles of 32 V channels of a
 // sequence) and carries the state, or, where there are too few chains to
@@ -37,7 +38,14 @@
 // wait is bounded. The backward pass is the same walk with time reversed, over
 // the map u -> a (u + dh).
 //
-// Bound: memory.
+// Bound: memory by the bytes; what is reached is set by the latency of a tile
+// (its barrier, the maps' join, in a look-back two round trips to L2) at 16
+// warps per SM, which is what the registers and the copies under way leave.
+// Measured, (8, 4096, 2048) bf16 sigmoid: walked forward 83 us (4.9 TB/s),
+// backward 161 us (5.0 TB/s); f32 linear 155 us (5.2 TB/s) and 232 us (5.8 TB/s).
+// By look-back (1, 65536, 1000) f32: 241 us (3.3 TB/s) and 449 us. One 4-byte
+// copy per lane instead of 16 bytes: forward 112 us. Values in registers
+// from plain loads, no copies ahead: 266 us.
 #include "async_copy.cuh"
 #include "common.cuh"
 #include "internal.h"

@@ -178,7 +178,11 @@ def launch(op: str, dev: int, *arrays) -> int:
     Each buffer remembers the Stream that last used it (`_mpb_stream`); the
     Stream objects are unique per CUDA stream, so the common case - the same
     stream again - is one identity test."""
-    s = current_stream(dev)
+    return launch_on(current_stream(dev), op, *arrays)
+
+
+def launch_on(s: Stream, op: str, *arrays) -> int:
+    """`launch` on the stream `s`."""
     if s._poison is not None:
         raise errors.StreamError(s._poison)
     capturing = None
