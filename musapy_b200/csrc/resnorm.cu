@@ -313,10 +313,10 @@ template <int W, int NV, bool EARLY>
 struct KeptRow {
   static constexpr bool kEarly = EARLY && W == 8;
   Kept<W> all[kEarly ? NV : 1];
-  MPB_D KeptRow(const NormArgs& p, int r, int skip, int step) {
+  MPB_D KeptRow(const NormArgs& p, int r, int skip) {
     if constexpr (kEarly)
 #pragma unroll
-      for (int k = 0; k < NV; ++k) all[k] = Kept<W>(p.drop, (uint64_t)((int64_t)r * p.D + skip + k * step * W));
+      for (int k = 0; k < NV; ++k) all[k] = Kept<W>(p.drop, (uint64_t)((int64_t)r * p.D + skip + k * 32 * W));
   }
   MPB_D Kept<W> at(const NormArgs& p, int r, int k, int c) const {
     if constexpr (kEarly) return all[k];
@@ -374,7 +374,8 @@ MPB_D void gate_pack(const NormArgs& p, const Elems<T, W>& full, int64_t r, int 
 enum { kPlain = 0, kBranch = 1, kDropped = 2 };  // no branch, a branch, a branch with dropout
 
 // blockDim.x threads per row, blockDim.y rows per block (more than one only
-// for rows of a warp). A thread holds the packs threadIdx.x + k blockDim.x.
+// for rows of a warp). A warp holds 32 NV packs one after the other, a lane every
+// 32nd of them: the distances within a thread are constants.
 template <class T, int W, int NV, int MODE>
 __global__ void __launch_bounds__(kRowThreads) k_norm_rows(NormArgs p) {
   using E = Elems<T, W>;
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_rows(NormArgs p) {
   __shared__ float red[2][32];
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= p.R) return;
-  const int r = (int)row, D = (int)p.D, packs = D / W, tid = threadIdx.x, step = blockDim.x, skip = tid * W;
+  const int r = (int)row, D = (int)p.D, packs = D / W, tid = threadIdx.x, step = blockDim.x, q0 = (tid >> 5) * 32 * NV + (tid & 31), skip = q0 * W;
   const F zero = vset<E::kPer>(0.0f);
   const T *xr = row_at<T>(p.x, r, p.x_sr, skip), *zr = row_at<T>(p.z, r, p.z_sr, skip);
   const T* gr = row_at<T>(p.gate, r, p.gate_kind == MPB_GATE_FULL ? p.g_sr : 0, skip);
@@ -391,21 +392,21 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_rows(NormArgs p) {
   E x[NV], z[NV], g[NV];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int q = tid + k * step;
+    const int q = q0 + k * 32;
     if (q < packs) {
-      const int at = k * step * W;
+      const int at = k * 32 * W;
       if (MODE != kPlain) z[k].load(zr + at);
       x[k].load(xr + at);
       if (MODE != kPlain && p.gate_kind == MPB_GATE_FULL) g[k].load(gr + at);
     }
   }
-  const KeptRow<W, NV, false> kept_row(p, r, skip, step);
+  const KeptRow<W, NV, false> kept_row(p, r, skip);
   F ss = zero, y[NV][NP];
   float rz = 0.0f;
   if (MODE != kPlain) {
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-      if (tid + k * step < packs)
+      if (q0 + k * 32 < packs)
 #pragma unroll
         for (int i = 0; i < NP; ++i) ss = vfma(z[k].get(i), z[k].get(i), ss);
     rz = 1.0f / sqrtf(row_sum(fold(ss), red[0]) / (float)D + p.eps);
@@ -414,7 +415,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_rows(NormArgs p) {
   const F factor = vset<E::kPer>(rz * (MODE == kDropped ? p.scale * p.drop.up : p.scale));
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int q = tid + k * step;
+    const int q = q0 + k * 32;
     if (q < packs) {
       if (MODE == kPlain) {
 #pragma unroll
@@ -438,7 +439,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_rows(NormArgs p) {
         } else {
           branch([](int, F a, F) { return a; });
         }
-        out.store(yr + k * step * W);
+        out.store(yr + k * 32 * W);
       }
 #pragma unroll
       for (int i = 0; i < NP; ++i) ss = vfma(y[k][i], y[k][i], ss);
@@ -448,14 +449,14 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_rows(NormArgs p) {
   const F up = vset<E::kPer>(ry);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int q = tid + k * step;
+    const int q = q0 + k * 32;
     if (q < packs) {
       F w[NP];
       load_floats<T, W>(p.w_pre + q * W, w);
       E out;
 #pragma unroll
       for (int i = 0; i < NP; ++i) out.put(i, vmul(vmul(y[k][i], up), w[i]));
-      out.store(ur + k * step * W);
+      out.store(ur + k * 32 * W);
     }
   }
   if (tid == 0) {
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
   constexpr int NP = E::kParts, PW = E::kPer;
   extern __shared__ __align__(16) float columns[];
   __shared__ float red[2][3][32];
-  const int D = (int)p.D, packs = D / W, tid = threadIdx.x, step = blockDim.x, slots = step * NV, skip = tid * W;
+  const int D = (int)p.D, packs = D / W, tid = threadIdx.x, step = blockDim.x, slots = step * NV, q0 = (tid >> 5) * 32 * NV + (tid & 31), skip = q0 * W;
   const int sums = MODE == kPlain ? 1 : p.gate_kind == MPB_GATE_CHANNEL ? 3 : 2;
   const F zero = vset<PW>(0.0f), one = vset<PW>(1.0f);
   float* acc = columns + (size_t)threadIdx.y * sums * slots * W;
@@ -521,8 +522,8 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
     E du[NV], y[NV], dy[NV], z[NV], g[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-      if (ALL || tid + k * step < packs) {
-        const int at = k * step * W;
+      if (ALL || q0 + k * 32 < packs) {
+        const int at = k * 32 * W;
         if (ALL || p.du) {
           du[k].load(dur + at);
           y[k].load(yr + at);
@@ -534,13 +535,13 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
         }
       }
     const float rz = MODE != kPlain ? p.rstd[r] : 0.0f, ry = p.rstd[(MODE != kPlain ? p.R : 0) + r];
-    const KeptRow<W, NV, MODE == kDropped> kept_row(p, r, skip, step);
+    const KeptRow<W, NV, MODE == kDropped> kept_row(p, r, skip);
     float back = 0.0f;  // of y in dx: r_y^3 mean(y w du)
     if (ALL || p.du) {
       F dot = zero;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int q = tid + k * step;
+        const int q = q0 + k * 32;
         if (ALL || q < packs) {
           F w[NP], c[NP];
           load_floats<T, W>(p.w_pre + q * W, w);
@@ -558,7 +559,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
     F dotz = zero, dgr = zero, wn[NV][NP];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int q = tid + k * step;
+      const int q = q0 + k * 32;
       if (ALL || q < packs) {
         F dx[NP];
         E out;
@@ -573,7 +574,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
         }
 #pragma unroll
         for (int i = 0; i < NP; ++i) out.put(i, dx[i]);
-        out.store(const_cast<T*>(row_at<T>(p.dx, r, D, skip)) + k * step * W);
+        out.store(const_cast<T*>(row_at<T>(p.dx, r, D, skip)) + k * 32 * W);
         if (MODE != kPlain) {
           F w[NP], ezv[NP], dg[NP], v[NP], slope[NP];
           load_floats<T, W>(p.w_post + q * W, w);
@@ -599,7 +600,7 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
           if (p.gate_kind == MPB_GATE_FULL) {
 #pragma unroll
             for (int i = 0; i < NP; ++i) out.put(i, dg[i]);
-            out.store(const_cast<T*>(row_at<T>(p.dgate, r, D, skip)) + k * step * W);
+            out.store(const_cast<T*>(row_at<T>(p.dgate, r, D, skip)) + k * 32 * W);
           } else if (p.gate_kind == MPB_GATE_CHANNEL) {
             add_columns<T, W>(acc + 2 * slots * W, slots, q, dg, one);
           }
@@ -614,13 +615,13 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
       }
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int q = tid + k * step;
+        const int q = q0 + k * 32;
         if (ALL || q < packs) {
           E out;
 #pragma unroll
           for (int i = 0; i < NP; ++i)
             out.put(i, vfma(z[k].get(i), vset<PW>(-mz), vmul(wn[k][i], vset<PW>(s))));
-          out.store(const_cast<T*>(row_at<T>(p.dz, r, D, skip)) + k * step * W);
+          out.store(const_cast<T*>(row_at<T>(p.dz, r, D, skip)) + k * 32 * W);
         }
       }
     }
