@@ -17,7 +17,7 @@
 // float whatever the element type.
 //
 // One pass over the data, in tiles of 32 lanes x V channels by S warps x 16
-// (backward 8) steps. A warp folds its steps to the map c -> A c + B that they
+// (backward 8 or 16) steps. A warp folds its steps to the map c -> A c + B that they
 // apply to the state; the block joins the maps of its warps, and each warp
 // then runs its steps once more from the state that enters them and writes.
 // A warp copies its own steps' rows into shared memory some tiles ahead
@@ -58,7 +58,13 @@ namespace {
 
 constexpr int kWarps = 8;       // warps of a full tile
 constexpr int kFwd = 16;        // steps per warp and tile, forward
-constexpr int kBwd = 8;         // backward: four inputs instead of two
+// Steps per warp and tile, backward. The more, the fewer joins; 16 where two tiles
+// of that many fit a block's share of shared memory: three inputs of one word
+// per step. (Linear, a gate per head, (4, 4095, 32 x 64) bf16: 80 us with 16 steps,
+// 103 us with 8; sigmoid, four inputs, (8, 4096, 2048) bf16: 172 and 161 us.)
+constexpr int bwd_steps(bool sig, int gate_bytes, int V, bool shared) {
+  return !sig && (shared || gate_bytes * V <= 4) ? 16 : 8;
+}
 constexpr int kRing = 96 << 10; // shared memory of a block for tiles under way, two blocks per SM
 
 struct ScanArgs {
@@ -786,16 +792,17 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_far(ScanArgs p) {
       });
 }
 
-// Sums over the `lanes` (a power of two) neighbours of a lane of kBwd values
+// Sums over the `lanes` (a power of two) neighbours of a lane of N values
 // each: every round gives half of the values to the partner and takes its
-// half of the others', so 9 shuffles do for 8 values over 32 lanes. On
+// half of the others', so 16 shuffles do for 16 values over 32 lanes. On
 // return val[0..left) of a lane are the sums of the steps first..first + left,
-// the same in the lanes that differ in bits from log2(kBwd) on.
-MPB_D void sum_over_lanes(float (&val)[kBwd], int lane, int lanes, int& first, int& left) {
+// the same in the lanes that differ in bits from log2(N) on.
+template <int N>
+MPB_D void sum_over_lanes(float (&val)[N], int lane, int lanes, int& first, int& left) {
   first = 0;
-  left = kBwd;
+  left = N;
 #pragma unroll
-  for (int half = kBwd / 2, bit = 1; half > 0; half >>= 1, bit <<= 1) {
+  for (int half = N / 2, bit = 1; half > 0; half >>= 1, bit <<= 1) {
     if (bit < lanes) {
       const bool up = lane & bit;
 #pragma unroll
@@ -808,12 +815,13 @@ MPB_D void sum_over_lanes(float (&val)[kBwd], int lane, int lanes, int& first, i
     }
   }
 #pragma unroll
-  for (int bit = kBwd; bit < 32; bit <<= 1)
+  for (int bit = N; bit < 32; bit <<= 1)
     if (bit < lanes) val[0] += __shfl_xor_sync(0xffffffffu, val[0], bit);
 }
 
 template <class X, class G, bool SIG, int V, bool SHARED>
 struct BwdTile {
+  static constexpr int kBwd = bwd_steps(SIG, (int)sizeof(G), V, SHARED);
   using CX = Column<X, V>;
   using CG = Column<G, SHARED ? 1 : V>;
   using HG = HeadGates<G, kBwd>;
@@ -828,6 +836,7 @@ struct BwdTile {
 template <class X, class G, bool SIG, int V, bool SHARED>
 struct Backward {
   using Tile = BwdTile<X, G, SIG, V, SHARED>;
+  static constexpr int kBwd = Tile::kBwd;
   const ScanArgs& p;
   const int64_t in_st[4], out_st[2];
   const int lane, warp;
@@ -971,7 +980,7 @@ struct Backward {
 template <class X, class G, bool SIG, int V, bool SHARED>
 __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd_walk(ScanArgs p) {
   using Tile = BwdTile<X, G, SIG, V, SHARED>;
-  constexpr int NST = Tile::kStages;
+  constexpr int NST = Tile::kStages, kBwd = Tile::kBwd;
   extern __shared__ __align__(16) char ring[];
   __shared__ Shared<V> sh;
   Backward<X, G, SIG, V, SHARED> bw(p);
@@ -1020,6 +1029,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd_walk(ScanArgs p) {
 template <class X, class G, bool SIG, int V, bool SHARED>
 __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd_far(ScanArgs p) {
   using Tile = BwdTile<X, G, SIG, V, SHARED>;
+  constexpr int kBwd = Tile::kBwd;
   extern __shared__ __align__(16) char ring[];
   __shared__ Shared<V> sh;
   Backward<X, G, SIG, V, SHARED> bw(p);
@@ -1181,19 +1191,21 @@ size_t scratch_of(ScanArgs& p, int V, bool backward, void* base, size_t* cleared
   return at > 16 ? at : 0;
 }
 
-// Enough for either V: the choice needs addresses and strides.
+// Enough for either V and number of steps: the choice needs addresses, strides and the mode.
 size_t scratch_need(ScanArgs p, bool backward) {
   size_t most = 0, cleared;
-  for (int V = 1; V <= 2; ++V) {
-    lay_out(p, V, backward ? kBwd : kFwd);
-    const size_t n = scratch_of(p, V, backward, nullptr, &cleared);
-    most = n > most ? n : most;
-  }
+  for (int V = 1; V <= 2; ++V)
+    for (int per : {8, 16}) {
+      if (!backward && per != kFwd) continue;
+      lay_out(p, V, per);
+      const size_t n = scratch_of(p, V, backward, nullptr, &cleared);
+      most = n > most ? n : most;
+    }
   return most;
 }
 
-int prepare(const char* what, ScanArgs& p, int V, bool backward, void* scratch, cudaStream_t s) {
-  lay_out(p, V, backward ? kBwd : kFwd);
+int prepare(const char* what, ScanArgs& p, int V, int per, bool backward, void* scratch, cudaStream_t s) {
+  lay_out(p, V, per);
   size_t cleared;
   if (scratch_need(p, backward)) p.status = (uint32_t*)((char*)scratch + 4);
   scratch_of(p, V, backward, scratch, &cleared);
@@ -1227,13 +1239,13 @@ template <class X, class G, bool SIG, int V, bool SHARED>
 int launch_bwd_v(const ScanArgs& p, cudaStream_t s) {
   using Tile = BwdTile<X, G, SIG, V, SHARED>;
   const char* what = "gated_scan_backward";
-  return p.walk ? launch_tiles<k_gscan_bwd_walk<X, G, SIG, V, SHARED>>(what, p, kBwd, Tile::kStages * Tile::kBytes, s)
-                : launch_tiles<k_gscan_bwd_far<X, G, SIG, V, SHARED>>(what, p, kBwd, 3 * Tile::kBytes, s);
+  return p.walk ? launch_tiles<k_gscan_bwd_walk<X, G, SIG, V, SHARED>>(what, p, Tile::kBwd, Tile::kStages * Tile::kBytes, s)
+                : launch_tiles<k_gscan_bwd_far<X, G, SIG, V, SHARED>>(what, p, Tile::kBwd, 3 * Tile::kBytes, s);
 }
 
 template <class X, class G, bool SIG>
 int launch_fwd(ScanArgs& p, int V, void* scratch, cudaStream_t s) {
-  if (int rc = prepare("gated_scan", p, V, false, scratch, s)) return rc;
+  if (int rc = prepare("gated_scan", p, V, kFwd, false, scratch, s)) return rc;
   constexpr int W = sizeof(X) == 2 ? 2 : 1;
   if (p.H != p.D) return V == 2 ? launch_fwd_v<X, G, SIG, W, true>(p, s) : launch_fwd_v<X, G, SIG, 1, true>(p, s);
   return V == 2 ? launch_fwd_v<X, G, SIG, W, false>(p, s) : launch_fwd_v<X, G, SIG, 1, false>(p, s);
@@ -1241,7 +1253,7 @@ int launch_fwd(ScanArgs& p, int V, void* scratch, cudaStream_t s) {
 
 template <class X, class G, bool SIG>
 int launch_bwd(ScanArgs& p, int V, void* scratch, cudaStream_t s) {
-  if (int rc = prepare("gated_scan_backward", p, V, true, scratch, s)) return rc;
+  if (int rc = prepare("gated_scan_backward", p, V, bwd_steps(SIG, (int)sizeof(G), V, p.H != p.D), true, scratch, s)) return rc;
   constexpr int W = sizeof(X) == 2 ? 2 : 1;
   if (p.H == p.D) return V == 2 ? launch_bwd_v<X, G, SIG, W, false>(p, s) : launch_bwd_v<X, G, SIG, 1, false>(p, s);
   if (int rc = V == 2 ? launch_bwd_v<X, G, SIG, W, true>(p, s) : launch_bwd_v<X, G, SIG, 1, true>(p, s)) return rc;
