@@ -42,10 +42,13 @@
 // (its barrier, the maps' join, in a look-back two round trips to L2) at 16
 // warps per SM, which is what the registers and the copies under way leave.
 // Measured, (8, 4096, 2048) bf16 sigmoid: walked forward 83 us (4.9 TB/s),
-// backward 161 us (5.0 TB/s); f32 linear 155 us (5.2 TB/s) and 232 us (5.8 TB/s).
-// By look-back (1, 65536, 1000) f32: 241 us (3.3 TB/s) and 449 us. One 4-byte
-// copy per lane instead of 16 bytes: forward 112 us. Values in registers
-// from plain loads, no copies ahead: 266 us.
+// backward 161 us (5.0 TB/s); f32 linear 153 us (5.3 TB/s) and 226 us (5.9 TB/s);
+// 32 gates for heads of 64, bf16 linear, 68 us (4.0 TB/s) and 113 us (3.6 TB/s).
+// By look-back (1, 65536, 1000) f32: 241 us (3.3 TB/s) and 412 us. One 4-byte
+// copy per lane instead of 16 bytes: forward 112 us. Values in registers from
+// plain loads, no copies ahead: 266 us. 16 warps of 8 (backward 4) steps instead
+// of 8 of 16 (8): 109 and 223 us, the join and the places of a tile being done by
+// twice the threads.
 #include "async_copy.cuh"
 #include "common.cuh"
 #include "internal.h"

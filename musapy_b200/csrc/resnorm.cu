@@ -26,16 +26,16 @@
 // Rows too long for that (above 16384 elements) are read again for each pass.
 //
 // Bound: memory. Measured, 16384 x 4096 with a full gate, f32: forward 204 us
-// (6.6 TB/s), backward 437 us (4.9 TB/s); bf16: forward 111 us (6.0 TB/s), with
-// dropout 130 us, backward 209 us (5.1 TB/s) and 232 us. The backward pass runs
+// (6.6 TB/s), backward 438 us (4.9 TB/s); bf16: forward 113 us (6.0 TB/s), with
+// dropout 130 us, backward 222 us (4.8 TB/s) and 227 us. The backward pass runs
 // about 60 instructions per element at 16 warps per SM (the registers of 16
 // elements' five inputs and sums): their issue, half of it stalled on the
 // row's loads and the two reductions, is what is left above the bytes.
 // Copying the next row ahead into shared memory took 243 us instead of 237 us
 // (bf16, no dropout) and 576 instead of 435 us (f32: fewer resident blocks); one
 // pack per thread and 512 threads per row 240 instead of 209 us. Rows that no
-// 16-byte access may use go element by element (odd width, f32: forward 320 us,
-// backward 783 us; bf16 two at a time or one: 305 and 756 us).
+// 16-byte access may use go element by element (16383 x 4095, f32: forward 239 us,
+// backward 692 us; bf16: 209 and 636 us).
 #include "common.cuh"
 #include "internal.h"
 #include "musapy_b200.h"
