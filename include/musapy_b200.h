@@ -196,13 +196,15 @@ int mpb_cumsum_status(const void* scratch, mpb_stream_t stream);
 /* The operators below are new: musapy has no counterpart. Element types are
  * MPB_F32, MPB_F16 and MPB_BF16, arithmetic is in float, outputs are
  * C-contiguous, the innermost stride of every input is 1 and the other
- * strides are given in elements. */
+ * strides are given in elements. Scratch is 16-byte aligned; what a call
+ * leaves in it is of no use to the next. */
 
 /* Gated linear recurrence over time. x is (B, T, D) with strides x_sb, x_st
  * over sequences and steps; gate is (B, T, H), H a divisor of D (channel d
  * has gate d / (D / H)), of x's type or MPB_F32; h0 (B, D) floats or NULL for
  * zero. mode MPB_SCAN_LINEAR: h[t] = g h[t-1] + x[t]; MPB_SCAN_SIGMOID:
- * h[t] = s h[t-1] + (1 - s) x[t], s = sigmoid(g). Writes h (B, T, D) in x's
+ * h[t] = s h[t-1] + (1 - s) x[t], s = sigmoid(g). Linear gates may exceed one
+ * as long as no product of 128 successive ones leaves the float range. Writes h (B, T, D) in x's
  * type and, when state is not NULL, h[T-1] (h0 when T == 0) in float; state
  * may not overlap h0. Scratch: mpb_gated_scan_scratch_bytes(..., backward = 0). */
 size_t mpb_gated_scan_scratch_bytes(int64_t B, int64_t T, int64_t D, int64_t H, int x_dtype, int gate_dtype,

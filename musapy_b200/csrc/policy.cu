@@ -207,7 +207,6 @@ MPB_D uint4 no_words() {
 // sum of zero is the empty set.
 struct Fold {
   float top, sum;
-  MPB_D float base() const { return top == -INFINITY ? 0.0f : top; }
   MPB_D void join(float t, float s) {
     const float m = fmaxf(top, t), b = m == -INFINITY ? 0.0f : m;
     sum = sum * exp_from(top, -b) + s * exp_from(t, -b);
@@ -622,6 +621,7 @@ int mpb_policy_loss(int64_t N, int64_t V, const void* logits, int dtype, int64_t
   const size_t need = mpb_policy_loss_scratch_bytes(N, V, dtype);
   if (need > scratch_bytes || (need && !scratch))
     return fail(MPB_ERR_SCRATCH, "policy_loss: %zu bytes of scratch, %zu needed", scratch_bytes, need);
+  if (need && (uintptr_t)scratch % 16 != 0) return fail(MPB_ERR_INVALID, "policy_loss: scratch not 16-byte aligned");
   PolicyArgs p = {};
   p.N = N, p.V = V, p.logits = logits, p.l_sr = l_sr, p.targets = targets, p.targets64 = targets_dtype == MPB_I64;
   p.old_logp = old_logp, p.adv = advantages, p.ref_logp = ref_logp, p.mask = (const uint8_t*)mask;

@@ -1320,6 +1320,7 @@ int check_sizes(const char* what, int64_t B, int64_t T, int64_t D, int64_t H) {
 int check_scratch(const char* what, size_t need, const void* scratch, size_t bytes) {
   if (need > bytes || (need && !scratch))
     return fail(MPB_ERR_SCRATCH, "%s: %zu bytes of scratch, %zu needed", what, bytes, need);
+  if (need && (uintptr_t)scratch % 16 != 0) return fail(MPB_ERR_INVALID, "%s: scratch not 16-byte aligned", what);
   return MPB_OK;
 }
 

@@ -384,7 +384,8 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_rows(NormArgs p) {
   __shared__ float red[2][32];
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= p.R) return;
-  const int r = (int)row, D = (int)p.D, packs = D / W, tid = threadIdx.x, step = blockDim.x, q0 = (tid >> 5) * 32 * NV + (tid & 31), skip = q0 * W;
+  const int r = (int)row, D = (int)p.D, packs = D / W, tid = threadIdx.x;
+  const int q0 = (tid >> 5) * 32 * NV + (tid & 31), skip = q0 * W;
   const F zero = vset<E::kPer>(0.0f);
   const T *xr = row_at<T>(p.x, r, p.x_sr, skip), *zr = row_at<T>(p.z, r, p.z_sr, skip);
   const T* gr = row_at<T>(p.gate, r, p.gate_kind == MPB_GATE_FULL ? p.g_sr : 0, skip);
@@ -505,7 +506,8 @@ __global__ void __launch_bounds__(kRowThreads) k_norm_bwd_rows(NormArgs p) {
   constexpr int NP = E::kParts, PW = E::kPer;
   extern __shared__ __align__(16) float columns[];
   __shared__ float red[2][3][32];
-  const int D = (int)p.D, packs = D / W, tid = threadIdx.x, step = blockDim.x, slots = step * NV, q0 = (tid >> 5) * 32 * NV + (tid & 31), skip = q0 * W;
+  const int D = (int)p.D, packs = D / W, tid = threadIdx.x, step = blockDim.x, slots = step * NV;
+  const int q0 = (tid >> 5) * 32 * NV + (tid & 31), skip = q0 * W;
   const int sums = MODE == kPlain ? 1 : p.gate_kind == MPB_GATE_CHANNEL ? 3 : 2;
   const F zero = vset<PW>(0.0f), one = vset<PW>(1.0f);
   float* acc = columns + (size_t)threadIdx.y * sums * slots * W;

@@ -233,6 +233,10 @@ def test_c_entry_points_return_status():
     assert pol(z=0) == MPB_ERR_INVALID and pol(loss=0) == MPB_ERR_INVALID
     if need:
         assert pol(nb=need - 1) == MPB_ERR_SCRATCH and pol(sc=0) == MPB_ERR_SCRATCH
+        assert pol(sc=24) == MPB_ERR_INVALID and "aligned" in last_error()
+    long_need = N.gated_scan_scratch_bytes(1, 1000, 4, 4, f32, f32, 0)
+    assert long_need > 0
+    assert scan(B=1, T=1000, sc=16, nb=long_need - 1) == MPB_ERR_SCRATCH and scan(B=1, T=1000, sc=24, nb=long_need) == MPB_ERR_INVALID
 
 
 def test_native_bindings_check_their_arguments():
