@@ -217,7 +217,7 @@ int mpb_gated_scan(int64_t B, int64_t T, int64_t D, int64_t H, const void* x, in
  * and dstate (B, D) or NULL, that of the last state in float. h is the
  * forward pass's output as it stored it, h0 what it started from. Writes dx
  * (B, T, D), dgate (B, T, H, summed over a gate's channels in a fixed order,
- * in the gate's type) and dh0 (B, D) in float when not NULL. */
+ * in the gate's type; zeros when D == 0) and dh0 (B, D) in float when not NULL. */
 int mpb_gated_scan_backward(int64_t B, int64_t T, int64_t D, int64_t H, const void* dh, int64_t dh_sb, int64_t dh_st,
                             const void* x, int x_dtype, int64_t x_sb, int64_t x_st, const void* gate, int gate_dtype,
                             int64_t g_sb, int64_t g_st, const void* h, int64_t h_sb, int64_t h_st, const float* h0,

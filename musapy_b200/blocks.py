@@ -222,7 +222,7 @@ def gated_scan_backward(dh, x, gate, h, h0=None, dstate=None, mode="linear"):
     s = _streams.current_stream(dev)
     dx, dgate = _new(s, x._shape, x._dtype, dev), _new(s, gate._shape, gate._dtype, dev)
     dh0 = _new(s, sshape, _dt.float32, dev)
-    if B * D:
+    if B * D or dgate.size:  # without channels the gates' gradients are zeros
         nbytes = NATIVE.gated_scan_scratch_bytes(B, T, D, H, x._dtype.code, gate._dtype.code, 1)
         scratch = _scratch(nbytes, dev)
         check(NATIVE.gated_scan_backward(B, T, D, H, dh._ptr, *_btd(dh), x._ptr, x._dtype.code, *_btd(x), gate._ptr,

@@ -1311,7 +1311,7 @@ int check_sizes(const char* what, int64_t B, int64_t T, int64_t D, int64_t H) {
   if (D > 0 && (H < 1 || D % H != 0))
     return fail(MPB_ERR_SHAPE, "%s: %lld gates do not divide %lld channels", what, (long long)H, (long long)D);
   // tiles are counted in 32 bits (at 16 steps of one warp the least a tile covers)
-  if (B > 0x7fffffff || T > 0x7ff00000 || D > 0x7fffffff ||
+  if (B > 0x7fffffff || T > 0x7ff00000 || D > 0x7fffffff || H > 0x7fffffff ||
       (double)B * (double)(D + 32) * ((double)T / 128 + 1) > 2.0e9)
     return fail(MPB_ERR_SHAPE, "%s: (%lld, %lld, %lld) is too large", what, (long long)B, (long long)T, (long long)D);
   return MPB_OK;
@@ -1374,7 +1374,12 @@ int mpb_gated_scan_backward(int64_t B, int64_t T, int64_t D, int64_t H, const vo
   p.h0 = h0, p.dstate = dstate, p.dx = dx, p.dgate = dgate, p.dh0 = dh0;
   cudaStream_t s = (cudaStream_t)stream;
   return by_types(what, x_dtype, gate_dtype, mode, [&](auto xt, auto gt, auto sig) {
-    if (B * D == 0) return (int)MPB_OK;
+    if (B * D == 0) {  // gates of no channels: sums of nothing
+      const int64_t n = B * T * H;
+      if (n == 0) return (int)MPB_OK;
+      if (!dgate) return fail(MPB_ERR_INVALID, "%s: null pointer", what);
+      return cuda_check(cudaMemsetAsync(dgate, 0, (size_t)n * sizeof(gt), s), what);
+    }
     if (T == 0) return pass_state(what, dstate, dh0, B * D, s);
     if (!dh || !x || !gate || !h || !dx || !dgate) return fail(MPB_ERR_INVALID, "%s: null pointer", what);
     if (int rc = check_scratch(what, scratch_need(p, true), scratch, scratch_bytes)) return rc;
