@@ -241,8 +241,8 @@ int mpb_gated_scan_step(int64_t B, int64_t D, int64_t H, const void* x, int x_dt
  * (mpb_gate_kind), activation what it goes through (mpb_activation); the
  * weights are D floats. dropout > 0 drops elements of the branch as
  * mpb_dropout does, by their index in (R, D). Writes y and u (R, D) and
- * rstd (2, R): the two rms factors. z == NULL: the plain norm u = x rms(x)
- * w_pre, no y, rstd (1, R). */
+ * rstd (2, R): the two rms factors, NaN when D == 0. z == NULL: the plain norm
+ * u = x rms(x) w_pre, no y, rstd (1, R). */
 int mpb_gated_residual_norm(int64_t R, int64_t D, int dtype, const void* x, int64_t x_sr, const void* z, int64_t z_sr,
                             const void* gate, int64_t g_sr, int gate_kind, int activation, const float* w_post,
                             const float* w_pre, double scale, double eps, double dropout, uint64_t seed,

@@ -8,6 +8,7 @@ copied first; every other stride is read in place. Results are new arrays.
 """
 from __future__ import annotations
 
+import math
 import numbers
 from typing import NamedTuple, Optional
 
@@ -336,6 +337,8 @@ def rms_norm(x, weight, eps=1e-6):
         check(NATIVE.gated_residual_norm(R, D, x._dtype.code, x._ptr, xr, None, 0, None, 0, 0, 0, None, w._ptr, 1.0,
                                          float(eps), 0.0, 0, 0, None, u._ptr, rstd._ptr,
                                          _streams.launch_on(s, name, x, w, u, rstd)), name)
+    elif R:  # the mean of no squares
+        rstd = full(lead, math.nan, _dt.float32, dev)
     return u, rstd
 
 
@@ -373,6 +376,8 @@ def gated_residual_norm(x, z, w_post, w_pre, gate=None, activation="linear", sca
         check(NATIVE.gated_residual_norm(R, D, x._dtype.code, x._ptr, xr, z._ptr, zr, _ptr(g), gr, kind, act, post._ptr,
                                          pre._ptr, float(scale), float(eps), p, seed, offset, y._ptr, u._ptr, rstd._ptr,
                                          _streams.launch_on(s, name, *ins, y, u, rstd)), name)
+    elif R:  # the means of no squares
+        rstd = full((2,) + lead, math.nan, _dt.float32, dev)
     return y, u, rstd
 
 

@@ -837,9 +837,13 @@ int mpb_gated_residual_norm(int64_t R, int64_t D, int dtype, const void* x, int6
   p.dropping = p.drop.drop != 0;
   if (dtype != MPB_F32 && dtype != MPB_F16 && dtype != MPB_BF16)
     return fail(MPB_ERR_DTYPE, "gated_residual_norm: dtype %d not supported (float16, bfloat16, float32)", dtype);
-  if (R == 0 || D == 0) return MPB_OK;
-  if (!x || !w_pre || !u || !rstd || (z && !y)) return fail(MPB_ERR_INVALID, "gated_residual_norm: null pointer");
+  if (R == 0) return MPB_OK;
   cudaStream_t s = (cudaStream_t)stream;
+  if (D == 0) {  // the factors of a mean of nothing: NaN, which all bits set are
+    if (!rstd) return fail(MPB_ERR_INVALID, "gated_residual_norm: null pointer");
+    return cuda_check(cudaMemsetAsync(rstd, 0xff, (size_t)R * (z ? 2 : 1) * sizeof(float), s), "gated_residual_norm");
+  }
+  if (!x || !w_pre || !u || !rstd || (z && !y)) return fail(MPB_ERR_INVALID, "gated_residual_norm: null pointer");
   return dtype == MPB_F32 ? launch_norm_fwd<float>(p, s)
                           : dtype == MPB_F16 ? launch_norm_fwd<__half>(p, s) : launch_norm_fwd<__nv_bfloat16>(p, s);
 }
@@ -876,14 +880,18 @@ int mpb_gated_residual_norm_backward(int64_t R, int64_t D, int dtype, const void
   p.dropping = p.drop.drop != 0;
   if (dtype != MPB_F32 && dtype != MPB_F16 && dtype != MPB_BF16)
     return fail(MPB_ERR_DTYPE, "%s: dtype %d not supported (float16, bfloat16, float32)", what, dtype);
-  if (D == 0) return MPB_OK;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (D == 0) {  // a gate per row has the sum over no channels as its gradient
+    if (gate_kind != MPB_GATE_ROW || R == 0) return MPB_OK;
+    if (!dgate) return fail(MPB_ERR_INVALID, "%s: null pointer", what);
+    return cuda_check(cudaMemsetAsync(dgate, 0, (size_t)R * (dtype == MPB_F32 ? 4 : 2), s), what);
+  }
   if (!dw_pre || (z && !dw_post) || (gate_kind != MPB_GATE_NONE && !dgate) || !w_pre)
     return fail(MPB_ERR_INVALID, "%s: null pointer", what);
   if (R > 0 && (!y || !rstd || !dx || (z && !dz))) return fail(MPB_ERR_INVALID, "%s: null pointer", what);
   const size_t need = mpb_gated_residual_norm_scratch_bytes(R, D, dtype, z != nullptr, gate_kind);
   if (need > scratch_bytes || (need && !scratch))
     return fail(MPB_ERR_SCRATCH, "%s: %zu bytes of scratch, %zu needed", what, scratch_bytes, need);
-  cudaStream_t s = (cudaStream_t)stream;
   return dtype == MPB_F32 ? launch_norm_bwd<float>(p, s)
                           : dtype == MPB_F16 ? launch_norm_bwd<__half>(p, s) : launch_norm_bwd<__nv_bfloat16>(p, s);
 }

@@ -38,3 +38,34 @@ def test_gates_of_no_channels_at_the_c_entry(ms):
     assert call(dgate.data_ptr()) == MPB_OK
     assert not bool(dgate.any())
     assert call(0) == MPB_ERR_INVALID
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_norm_factors_of_rows_without_channels(ms, dtype):
+    """The mean of no squares is NaN, as ms.mean's is, not what the memory held."""
+    A = ms.from_torch
+    e, w = rand(40, 0, seed=1, dtype=dtype), rand(0, seed=1)
+    used_memory()
+    _, rstd = ms.rms_norm(A(e), A(w))
+    assert rstd.shape == (40,) and bool(rstd.torch().isnan().all())
+    used_memory()
+    _, _, rstd = ms.gated_residual_norm(A(e), A(e), A(w), A(w))
+    assert rstd.shape == (2, 40) and bool(rstd.torch().isnan().all())
+
+
+def test_rows_without_channels_at_the_c_entry(ms):
+    from musapy_b200._lib import MPB_OK, NATIVE
+
+    s = torch.cuda.current_stream().cuda_stream
+    rstd = torch.ones(2 * 7, device="cuda")
+    assert NATIVE.gated_residual_norm(7, 0, 10, 16, 0, 16, 0, 0, 0, 0, 0, 16, 16, 1.0, 1e-6, 0.0, 0, 0, 16, 16,
+                                      rstd.data_ptr(), s) == MPB_OK
+    assert bool(rstd.isnan().all())
+    rstd = torch.ones(2 * 7, device="cuda")  # the plain norm has one factor per row
+    assert NATIVE.gated_residual_norm(7, 0, 10, 16, 0, 0, 0, 0, 0, 0, 0, 0, 16, 1.0, 1e-6, 0.0, 0, 0, 0, 16,
+                                      rstd.data_ptr(), s) == MPB_OK
+    assert bool(rstd[:7].isnan().all()) and bool((rstd[7:] == 1).all())
+    dgate = torch.ones(7, device="cuda")  # a gate per row: a sum over no channels
+    assert NATIVE.gated_residual_norm_backward(7, 0, 10, 16, 0, 16, 0, 16, 0, 16, 0, 16, 1, 2, 0, 16, 16, 16, 1.0, 0.0, 0, 0,
+                                               16, 16, dgate.data_ptr(), 16, 16, 0, 0, s) == MPB_OK
+    assert not bool(dgate.any())
