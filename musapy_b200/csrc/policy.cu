@@ -64,19 +64,25 @@ struct Token {
 };
 
 // What a token's logp makes of the loss: its value, kl, clipped and d loss / d logp (without the mean's divisor).
+// rho and e^q may be beyond float where they count for nothing: an advantage of
+// zero makes rho A zero for every finite exponent, a coefficient of zero leaves
+// the KL term out.
 MPB_D void token_terms(const PolicyArgs& p, const Token& token, float logp, float& value, float& kl, bool& clipped,
                        float& slope) {
-  const float a = token.adv, rho = __expf(logp - token.old);
+  const float a = token.adv, x = logp - token.old, rho = __expf(x);
   clipped = (a > 0.0f && rho > 1.0f + p.hi) || (a < 0.0f && rho < 1.0f - p.lo);
   const float bound = a > 0.0f ? 1.0f + p.hi : 1.0f - p.lo;
-  value = -(clipped ? bound : rho) * a;
-  slope = clipped ? 0.0f : -rho * a;
+  const float gain = a == 0.0f && fabsf(x) < INFINITY ? 0.0f : rho * a;
+  value = clipped ? -bound * a : -gain;
+  slope = clipped ? 0.0f : -gain;
   kl = 0.0f;
   if (p.ref_logp) {
     const float q = token.ref - logp, em = expm1f(q);
     kl = em - q;
-    value = fmaf(p.beta, kl, value);
-    slope = fmaf(-p.beta, em, slope);
+    if (p.beta != 0.0f) {
+      value = fmaf(p.beta, kl, value);
+      slope = fmaf(-p.beta, em, slope);
+    }
   }
 }
 

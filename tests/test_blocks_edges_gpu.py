@@ -1,9 +1,13 @@
 """The block operators at the edges of their ranges on the GPU, against their formulas in 64 bits: results without
-elements to sum."""
+elements to sum and factors of zero beside exponentials that overflow. Tolerances are the bounds that blocks_plain
+derives."""
+import math
+
 import pytest
 import torch
 
-from .test_blocks_gpu import rand
+from . import blocks_plain as P
+from .test_blocks_gpu import make_policy, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +73,34 @@ def test_rows_without_channels_at_the_c_entry(ms):
     assert NATIVE.gated_residual_norm_backward(7, 0, 10, 16, 0, 16, 0, 16, 0, 16, 0, 16, 1, 2, 0, 16, 16, 16, 1.0, 0.0, 0, 0,
                                                16, 16, dgate.data_ptr(), 16, 16, 0, 0, s) == MPB_OK
     assert not bool(dgate.any())
+
+
+# ------------------------------------------- zero times an exponential
+@pytest.mark.parametrize("layout", ["aligned", "apart"])
+@pytest.mark.parametrize("V", [40, 5000])
+def test_policy_zero_factors_beside_large_exponentials(ms, V, layout):
+    """A token of advantage zero whose ratio is beyond float, and a KL term of coefficient zero whose estimate is:
+    both add nothing to the loss and its gradient."""
+    A = ms.from_torch
+    c = make_policy(24, V, "f32", 0.0)
+    if layout == "apart":  # logits and gradient start at different places of a 16-byte word
+        w = torch.zeros(24, V + 3, device="cuda")
+        w[:, 3:] = c["z"]
+        c["z"] = w[:, 3:]
+    c["adv"][::3] = 0.0
+    c["old"][::3] -= 150.0
+    args = lambda beta, ref: P.policy(c["z"].double(), c["t"], c["old"].double(), c["adv"].double(), ref.double(), c["mask"],
+                                      0.2, 0.3, beta, 1.0)
+    for beta in (0.0, 0.1):
+        ref = c["ref"].clone()
+        if beta == 0.0:
+            ref[1::3] += 150.0
+        r = ms.policy_loss(A(c["z"]), A(c["t"]), A(c["old"]), A(c["adv"]), A(ref), clip_low=0.2, clip_high=0.3, kl_coef=beta)
+        want, err = args(beta, ref)
+        for k in ("logp", "loss", "dlogits"):
+            P.close(getattr(r, k).torch(), want[k], err[k], f"beta {beta} {k}")
+    # what the formula itself makes NaN stays NaN: an infinite ratio, a target outside
+    c["old"][0], c["t"][3] = -math.inf, V
+    r = ms.policy_loss(A(c["z"]), A(c["t"]), A(c["old"]), A(c["adv"]), clip_low=0.2, clip_high=0.3)
+    rows = r.dlogits.torch().isnan().all(1)
+    assert bool(rows[0]) and bool(rows[3]) and int(rows.sum()) == 2 and bool(r.loss.torch().isnan())
