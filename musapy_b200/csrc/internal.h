@@ -2,6 +2,7 @@
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <atomic>
 #include "mpb_types.h"
 
 namespace mpb {
@@ -21,6 +22,23 @@ int launch_check_pdl(cudaError_t e, const char* what);
 void set_preserve_last_error(bool on);
 // Multiprocessor count of the current device (cached per device).
 int sm_count();
+
+// Lets `kernel` be launched with BYTES of dynamic shared memory, the most that
+// any of its calls asks for. The limit is the kernel's and every host thread's:
+// set to the size of a call, it could be lowered by one thread between another's
+// call and its launch.
+template <auto kernel, int BYTES>
+int allow_smem(const char* what) {
+  static_assert(BYTES <= 227 << 10, "a block's share of an SM's shared memory");
+  if (BYTES <= 40 << 10) return 0;  // allowed anyway
+  static std::atomic<bool> set[64];  // per device
+  int dev = 0;
+  if (int rc = cuda_check(cudaGetDevice(&dev), what)) return rc;
+  if (dev >= 0 && dev < 64 && set[dev].load(std::memory_order_acquire)) return 0;
+  if (int rc = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES), what)) return rc;
+  if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_release);
+  return 0;
+}
 
 struct EwReq {
   int op;

@@ -534,19 +534,6 @@ __global__ void __launch_bounds__(1024) k_policy_count(PolicyArgs p, float* coun
 constexpr int64_t kPart = kRowThreads * kGroups * kBatch;
 constexpr int kMostBytes = 208 << 10;   // of a row, where eight blocks have to do
 
-template <class T>
-int allow_smem(int bytes) {
-  static int allowed[64] = {};
-  int dev = 0;
-  if (int rc = cuda_check(cudaGetDevice(&dev), "policy_loss")) return rc;
-  if (bytes <= (40 << 10) || (dev >= 0 && dev < 64 && allowed[dev] >= bytes)) return MPB_OK;
-  if (int rc = cuda_check(cudaFuncSetAttribute(k_policy_row<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
-                          "policy_loss"))
-    return rc;
-  if (dev >= 0 && dev < 64) allowed[dev] = bytes;
-  return MPB_OK;
-}
-
 // Every block counts the tokens in the mask itself while its copies are under
 // way, as long as that is two loads for each of its threads; of more tokens the
 // number is taken by a kernel before.
@@ -576,7 +563,7 @@ int launch_policy(PolicyArgs& p, cudaStream_t s) {
       int threads = (int)((per / (kGroups * kBatch) + 31) / 32 * 32);
       threads = threads < 32 ? 32 : threads > kRowThreads ? kRowThreads : threads;
       if (int rc = count_before(p, threads, s)) return rc;
-      if (int rc = allow_smem<T>(bytes)) return rc;
+      if (int rc = allow_smem<k_policy_row<T>, kMostBytes>("policy_loss")) return rc;
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3((unsigned)(p.N * blocks));
       cfg.blockDim = dim3((unsigned)threads);

@@ -1216,34 +1216,29 @@ int prepare(const char* what, ScanArgs& p, int V, int per, bool backward, void* 
   return MPB_OK;
 }
 
-// The block's shared memory for tiles under way needs the opt-in above 48 KB, once per kernel and device.
-template <auto kernel>
-int launch_tiles(const char* what, const ScanArgs& p, int per, int smem, cudaStream_t s) {
-  static bool set[64] = {};
-  int dev = 0;
-  if (int rc = cuda_check(cudaGetDevice(&dev), what)) return rc;
-  if (dev < 0 || dev >= 64 || !set[dev]) {
-    if (int rc = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what)) return rc;
-    if (dev >= 0 && dev < 64) set[dev] = true;
-  }
+// SMEM: the block's tiles under way.
+template <auto kernel, int SMEM>
+int launch_tiles(const char* what, const ScanArgs& p, int per, cudaStream_t s) {
+  if (int rc = allow_smem<kernel, SMEM>(what)) return rc;
   const uint32_t most = (uint32_t)sm_count() * 2, tiles = p.walk ? p.chains : p.chains * p.chunks;
-  kernel<<<tiles < most ? tiles : most, (unsigned)(p.steps / per) * 32, smem, s>>>(p);
+  kernel<<<tiles < most ? tiles : most, (unsigned)(p.steps / per) * 32, SMEM, s>>>(p);
   return launch_check(what);
 }
 
 template <class X, class G, bool SIG, int V, bool SHARED>
 int launch_fwd_v(const ScanArgs& p, cudaStream_t s) {
   using Tile = FwdTile<X, G, V, SHARED>;
-  return p.walk ? launch_tiles<k_gscan_walk<X, G, SIG, V, SHARED>>("gated_scan", p, kFwd, Tile::kStages * Tile::kBytes, s)
-                : launch_tiles<k_gscan_far<X, G, SIG, V, SHARED>>("gated_scan", p, kFwd, 3 * Tile::kBytes, s);
+  const char* what = "gated_scan";
+  return p.walk ? launch_tiles<k_gscan_walk<X, G, SIG, V, SHARED>, Tile::kStages * Tile::kBytes>(what, p, kFwd, s)
+                : launch_tiles<k_gscan_far<X, G, SIG, V, SHARED>, 3 * Tile::kBytes>(what, p, kFwd, s);
 }
 
 template <class X, class G, bool SIG, int V, bool SHARED>
 int launch_bwd_v(const ScanArgs& p, cudaStream_t s) {
   using Tile = BwdTile<X, G, SIG, V, SHARED>;
   const char* what = "gated_scan_backward";
-  return p.walk ? launch_tiles<k_gscan_bwd_walk<X, G, SIG, V, SHARED>>(what, p, Tile::kBwd, Tile::kStages * Tile::kBytes, s)
-                : launch_tiles<k_gscan_bwd_far<X, G, SIG, V, SHARED>>(what, p, Tile::kBwd, 3 * Tile::kBytes, s);
+  return p.walk ? launch_tiles<k_gscan_bwd_walk<X, G, SIG, V, SHARED>, Tile::kStages * Tile::kBytes>(what, p, Tile::kBwd, s)
+                : launch_tiles<k_gscan_bwd_far<X, G, SIG, V, SHARED>, 3 * Tile::kBytes>(what, p, Tile::kBwd, s);
 }
 
 template <class X, class G, bool SIG>

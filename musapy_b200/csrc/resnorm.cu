@@ -701,18 +701,6 @@ int64_t bwd_blocks(const Spread& s, int64_t R, int sums, size_t* smem) {
   return want < most ? want : most;
 }
 
-template <auto kernel>
-int allow_smem(const char* what, size_t bytes) {
-  static size_t allowed[64] = {};
-  int dev = 0;
-  if (int rc = cuda_check(cudaGetDevice(&dev), what)) return rc;
-  if (bytes <= (40u << 10) || (dev >= 0 && dev < 64 && allowed[dev] >= bytes)) return MPB_OK;
-  if (int rc = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what))
-    return rc;
-  if (dev >= 0 && dev < 64) allowed[dev] = bytes;
-  return MPB_OK;
-}
-
 template <class T, int W, int NV, int MODE>
 int run_rows(const NormArgs& p, const Spread& sp, bool backward, cudaStream_t s) {
   const dim3 block(sp.x, sp.y);
@@ -726,7 +714,8 @@ int run_rows(const NormArgs& p, const Spread& sp, bool backward, cudaStream_t s)
   const int64_t blocks = bwd_blocks(sp, p.R, sums, &smem);
   auto run = [&](auto all) {
     constexpr auto kernel = k_norm_bwd_rows<T, W, NV, MODE, decltype(all)::value>;
-    if (int rc = allow_smem<kernel>(what, smem)) return rc;
+    constexpr int most = kRowThreads * NV * W * (int)sizeof(float) * (MODE == kPlain ? 1 : 3);
+    if (int rc = allow_smem<kernel, most>(what)) return rc;
     kernel<<<(unsigned)blocks, block, smem, s>>>(p);
     return (int)MPB_OK;
   };
