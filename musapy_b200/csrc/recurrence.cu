@@ -38,6 +38,12 @@
 // wait is bounded. The backward pass is the same walk with time reversed, over
 // the map u -> a (u + dh).
 //
+// A product of decays (16 steps of a warp, or a look-back's tile) may leave the
+// range of float where the states do not. Above it, with linear gates beyond one,
+// the tile's warps run one after the other instead, each from the state that the
+// one before it ends with. Below it the product counts as zero: what is lost is
+// below 2^-126 of the state before.
+//
 // Bound: memory by the bytes; what is reached is set by the latency of a tile
 // (its barrier, the maps' join, in a look-back two round trips to L2) at 16
 // warps per SM, which is what the registers and the copies under way leave.
@@ -116,9 +122,14 @@ MPB_D void gates_of(const P& g, Floats<V>& a, Floats<V>& om) {
   }
 }
 
-// The product of a warp's decays, kept finite: gates above one may overflow it
-// where no state does, and an infinity would turn a state of zero into NaN.
-MPB_D float finite(float a) { return fminf(fmaxf(a, -3.0e38f), 3.0e38f); }
+// Whether a map's values are numbers on every channel of the lane (zero times an
+// infinity or a NaN is NaN). Linear gates above one may take a product of decays
+// out of the range of float where no state leaves it: such a map stands for nothing.
+template <int V>
+MPB_D bool numbers(Floats<V> a, Floats<V> b) {
+  const Floats<V> zero = vfma(a, vset<V>(0.0f), vmul(b, vset<V>(0.0f)));
+  return vget(zero, 0) + vget(zero, V - 1) == 0.0f;
+}
 
 // Where a lane works.
 struct Lane {
@@ -294,6 +305,7 @@ struct Shared {
   __align__(8) float b[3][kWarps][32 * V];
   __align__(8) float carry[32 * V];
   uint32_t tiles[4];
+  int turns;  // of a look-back's tile: its warps run in turn
 };
 
 // The state after warp w's steps.
@@ -307,22 +319,42 @@ template <int V>
 MPB_D void put_map(Shared<V>& sh, int side, int warp, int lane, Floats<V> a, Floats<V> b) {
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    sh.a[side][warp][lane * V + v] = finite(vget(a, v));
+    sh.a[side][warp][lane * V + v] = vget(a, v);
     sh.b[side][warp][lane * V + v] = vget(b, v);
   }
+}
+
+// Warps in turn, where a warp's map is not made of numbers: each waits for the
+// state that the one before it ends with. To start: the state that enters the
+// warp's steps, for the first warp the tile's. To end: the state after the steps.
+template <int V>
+MPB_D void start_turn(const Shared<V>& sh, int warp, int lane, Floats<V>& in) {
+  for (int w = 0; w < warp; ++w) __syncthreads();
+  if (warp) in = *reinterpret_cast<const Floats<V>*>(&sh.carry[lane * V]);
+}
+template <int V>
+MPB_D void end_turn(Shared<V>& sh, int warp, int lane, Floats<V> in) {
+  *reinterpret_cast<Floats<V>*>(&sh.carry[lane * V]) = in;
+  for (int w = warp; w < (int)(blockDim.x >> 5); ++w) __syncthreads();
 }
 
 // A walk's tile: joins the maps of the block's warps (a, b: this warp's). carry:
 // the state that enters the tile and, on return, the one that leaves it (of
 // a single warp the caller's steps end there). Returns in `in` the state that
-// enters the warp's steps.
-template <int V>
-MPB_D void join(Shared<V>& sh, int side, int warp, int lane, Floats<V> a, Floats<V> b, Floats<V>& carry, Floats<V>& in) {
+// enters the warp's steps. With TURNS, true and nothing joined (in = carry) where a
+// map is not sound: the warps run in turn.
+template <int V, bool TURNS>
+MPB_D bool join(Shared<V>& sh, int side, int warp, int lane, bool sound, Floats<V> a, Floats<V> b, Floats<V>& carry,
+                Floats<V>& in) {
   const int warps = blockDim.x >> 5;
   in = carry;
-  if (warps == 1) return;
+  if (warps == 1) return false;
   put_map<V>(sh, side, warp, lane, a, b);
-  __syncthreads();
+  if constexpr (TURNS) {
+    if (__syncthreads_or(!sound)) return true;
+  } else {
+    __syncthreads();
+  }
   if (warps == kWarps) {
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
@@ -335,6 +367,7 @@ MPB_D void join(Shared<V>& sh, int side, int warp, int lane, Floats<V> a, Floats
       carry = through<V>(sh, side, w, lane, carry);
     }
   }
+  return false;
 }
 
 // cp.async of the word that holds the element(s): 4 bytes for one 32-bit or
@@ -493,9 +526,11 @@ struct Place {
 //   front(o, stage, side)  folds tile o's maps into sh side
 //   first(o, c)            the state before the chain, warp 0 (of the first 32 chunks:
 //                          as far as a look-back reaches)
-//   rest(o, stage, in)     runs the warp's steps from the state `in`
+//   rest(o, stage, in, in_turn)  runs the warp's steps from the state `in` to the one after them
 //   copy(it, stage)        copies the block's tile number `it`, and commits
-template <int V, class Front, class First, class Rest, class Copy>
+// With TURNS, a tile whose map is not made of numbers publishes none: the tiles
+// after it wait for its state, which its last warp publishes.
+template <int V, bool TURNS, class Front, class First, class Rest, class Copy>
 MPB_D void look_back_tiles(const ScanArgs& p, Shared<V>& sh, int warp, int lane, Front front, First first, Rest rest,
                            Copy copy) {
   constexpr int C = 32 * V;
@@ -519,7 +554,9 @@ MPB_D void look_back_tiles(const ScanArgs& p, Shared<V>& sh, int warp, int lane,
   }
   At cur, nxt;
   float ta[V], tb[V];  // the tile's map, warp 0
+  bool sound = true;   // on every lane
   auto publish = [&](const At& o, int side) {
+    bool mine = true;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       ta[v] = sh.a[side][0][lane * V + v], tb[v] = sh.b[side][0][lane * V + v];
@@ -527,11 +564,15 @@ MPB_D void look_back_tiles(const ScanArgs& p, Shared<V>& sh, int warp, int lane,
       for (int w = 1; w < kWarps; ++w) {
         const float aw = sh.a[side][w][lane * V + v];
         tb[v] = fmaf(aw, tb[v], sh.b[side][w][lane * V + v]);
-        ta[v] = finite(ta[v] * aw);
+        ta[v] *= aw;
       }
-      if (o.chunk + 1 < p.chunks)
-        st_word(p.maps + (size_t)(o.chunk * p.chains + o.chain) * C + lane * V + v, map_word(ta[v], tb[v]));
+      mine = mine && numbers<1>(ta[v], tb[v]);
     }
+    if (TURNS) sound = __all_sync(0xffffffffu, mine);
+    if (o.chunk + 1 < p.chunks && sound)
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        st_word(p.maps + (size_t)(o.chunk * p.chains + o.chain) * C + lane * V + v, map_word(ta[v], tb[v]));
   };
   bool have = tile(0, cur);
   copies_wait<2>();
@@ -555,6 +596,7 @@ MPB_D void look_back_tiles(const ScanArgs& p, Shared<V>& sh, int warp, int lane,
     if (more) front(nxt.chain, nxt.chunk, after, after);
     __syncthreads();
     if (warp == 0) {
+      const bool whole = sound;
       float a[V], b[V], c[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) a[v] = ta[v], b[v] = tb[v];
@@ -563,15 +605,28 @@ MPB_D void look_back_tiles(const ScanArgs& p, Shared<V>& sh, int warp, int lane,
       look_back<V>(p, cur.chain, cur.chunk, lane, early, c);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        if (cur.chunk + 1 < p.chunks)
+        if (cur.chunk + 1 < p.chunks && whole)
           st_word(p.states + (size_t)(cur.chunk * p.chains + cur.chain) * C + lane * V + v, state_word(fmaf(a[v], c[v], b[v])));
         sh.carry[lane * V + v] = c[v];
       }
+      if (TURNS && lane == 0) sh.turns = !whole;
     }
     __syncthreads();
-    Floats<V> in = *reinterpret_cast<const Floats<V>*>(&sh.carry[lane * V]);
-    for (int w = 0; w < warp; ++w) in = through<V>(sh, stage, w, lane, in);
-    rest(cur.chain, cur.chunk, stage, in);
+    const bool turns = TURNS && sh.turns;
+    Floats<V> in = vset<V>(0.0f);
+    if (!turns || warp == 0) in = *reinterpret_cast<const Floats<V>*>(&sh.carry[lane * V]);
+    if (!turns) {
+      for (int w = 0; w < warp; ++w) in = through<V>(sh, stage, w, lane, in);
+      rest(cur.chain, cur.chunk, stage, in, std::false_type());
+    } else if constexpr (TURNS) {
+      start_turn<V>(sh, warp, lane, in);
+      rest(cur.chain, cur.chunk, stage, in, std::true_type());
+      if (warp == kWarps - 1 && cur.chunk + 1 < p.chunks)
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          st_word(p.states + (size_t)(cur.chunk * p.chains + cur.chain) * C + lane * V + v, state_word(vget(in, v)));
+      end_turn<V>(sh, warp, lane, in);
+    }
     __syncwarp();  // the stage has been read by every lane
     At far;
     copy(tile(it + 3, far), far.chain, far.chunk, stage);
@@ -686,6 +741,23 @@ struct Forward {
           h = ahead_by(h, out_st);
         }
     }
+    ended(to, n, in);
+  }
+  // The same for a warp in turn, in short code.
+  MPB_D void write_in_turn(const char* mine, uint32_t t0, const Place<kFwd, 1>& to, Floats<V>& in) const {
+    const int n = to.steps();
+    char* h = const_cast<char*>(to.at[0]);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      Floats<V> a, b;
+      step(mine, i, t0, a, b);
+      in = vfma(a, in, b);
+      put_global(h, pack<X>(in));
+      h = ahead_by(h, out_st);
+    }
+    ended(to, n, in);
+  }
+  MPB_D void ended(const Place<kFwd, 1>& to, int n, Floats<V> in) const {
     if (p.state && n > 0 && n == to.left)
 #pragma unroll
       for (int v = 0; v < V; ++v) p.state[state_at + v] = vget(in, v);
@@ -741,8 +813,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_walk(ScanArgs p) {
       ma = vmul(ma, a[i]);
       mb = vfma(a[i], mb, b[i]);
     }
-    join<V>(sh, it & 1, fw.warp, fw.lane, ma, mb, carry, in);
-    fw.write(to, in, [&](int i) { in = vfma(a[i], in, b[i]); });
+    const bool sound = SIG || to.left < kFwd || numbers<V>(ma, mb);
+    const bool turns = join<V, !SIG>(sh, it & 1, fw.warp, fw.lane, sound, ma, mb, carry, in);
+    if (turns) {
+      start_turn<V>(sh, fw.warp, fw.lane, in);
+      fw.write_in_turn(mine, t0, to, in);
+      end_turn<V>(sh, fw.warp, fw.lane, in);
+      carry = *reinterpret_cast<const Floats<V>*>(&sh.carry[fw.lane * V]);
+    } else {
+      fw.write(to, in, [&](int i) { in = vfma(a[i], in, b[i]); });
+    }
     if (blockDim.x == 32) carry = in;
     cur.next(p);
     stage = stage + 1 == NST ? 0 : stage + 1;
@@ -757,10 +837,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_far(ScanArgs p) {
   Forward<X, G, SIG, V, SHARED> fw(p);
   const uint32_t base = smem_u32(ring);
   auto t0_of = [&](uint32_t chunk) { return chunk * p.steps + fw.warp * kFwd; };
-  look_back_tiles<V>(
+  look_back_tiles<V, !SIG>(
       p, sh, fw.warp, fw.lane,
       [&](uint32_t chain, uint32_t chunk, int stage, int side) {
-        fw.sub_words(place<V, SHARED>(p, chain, fw.lane));
+        const Lane l = place<V, SHARED>(p, chain, fw.lane);
+        fw.sub_words(l);
         Floats<V> ma = vset<V>(1.0f), mb = vset<V>(0.0f);
 #pragma unroll
         for (int i = 0; i < kFwd; ++i) {
@@ -769,6 +850,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_far(ScanArgs p) {
           ma = vmul(ma, a);
           mb = vfma(a, mb, b);
         }
+        // steps after the last and idle lanes were computed from whatever the ring held
+        if (!SIG && !(l.in && p.T - t0_of(chunk) >= kFwd)) ma = vset<V>(1.0f), mb = vset<V>(0.0f);
         put_map<V>(sh, side, fw.warp, fw.lane, ma, mb);
       },
       [&](uint32_t chain, uint32_t chunk, float (&c)[V]) {
@@ -776,14 +859,18 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_far(ScanArgs p) {
 #pragma unroll
         for (int v = 0; v < V; ++v) c[v] = chunk < 32 && l.in && p.h0 ? p.h0[l.b * p.D + l.ch + v] : 0.0f;
       },
-      [&](uint32_t chain, uint32_t chunk, int stage, Floats<V> in) {
+      [&](uint32_t chain, uint32_t chunk, int stage, Floats<V>& in, auto in_turn) {
         Place<kFwd, 1> to;
         fw.output(chain, chunk, to);
-        fw.write(to, in, [&](int i) {
-          Floats<V> a, b;
-          fw.step(ring + stage * Tile::kBytes, i, t0_of(chunk), a, b);
-          in = vfma(a, in, b);
-        });
+        if constexpr (decltype(in_turn)::value) {
+          fw.write_in_turn(ring + stage * Tile::kBytes, t0_of(chunk), to, in);
+        } else {
+          fw.write(to, in, [&](int i) {
+            Floats<V> a, b;
+            fw.step(ring + stage * Tile::kBytes, i, t0_of(chunk), a, b);
+            in = vfma(a, in, b);
+          });
+        }
       },
       [&](bool is, uint32_t chain, uint32_t chunk, int stage) {
         if (is) {
@@ -909,74 +996,109 @@ struct Backward {
       mb = vmul(a, vadd(mb, unpack(Tile::CX::get(mine, i, half(0, r0, i)))));
     }
   }
+  // Step i from `in`, u of the step after, with low = h[t - 1]: writes dx and the gradient of a gate of the lane's
+  // own, leaves u in `in` and returns da.
+  MPB_D Floats<V> step(const char* mine, int i, uint32_t r0, Floats<V> low, char*& dx, char*& dg, Floats<V>& in) const {
+    Floats<V> a, om;
+    gate_at(mine, i, r0, a, om);
+    const Floats<V> s = vadd(unpack(Tile::CX::get(mine, i, half(0, r0, i))), in);
+    if constexpr (SIG) low = vfma(unpack(Tile::CX::get(mine + Tile::kX, i, half(2, r0, i))), vset<V>(-1.0f), low);
+    put_global(dx, pack<X>(SIG ? vmul(om, s) : s));
+    dx = ahead_by(dx, out_st[0]);
+    in = vmul(a, s);
+    const Floats<V> da = vmul(s, low);
+    if constexpr (!SHARED) {
+      put_global(dg, pack<G>(SIG ? vmul(da, vmul(a, om)) : da));
+      dg = ahead_by(dg, out_st[1]);
+    }
+    return da;
+  }
+  static MPB_D float over_channels(Floats<V> da) { return V == 2 ? vget(da, 0) + vget(da, 1) : vget(da, 0); }
+  MPB_D Floats<V> before(const char* mine, int i, uint32_t r0) const {
+    return unpack(Tile::CX::get(mine + Tile::kH, i, half(1, r0, i)));
+  }
+  // h0 before the first step of the sequence, which is the last of `to`
+  MPB_D Floats<V> before_any(const char* mine, int i, uint32_t r0, const Place<kBwd, 2>& to) const {
+    Floats<V> low = before(mine, i, r0);
+    if (to.left - 1 == i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) vput(low, v, p.h0 ? p.h0[state_at + v] : 0.0f);
+    return low;
+  }
+  MPB_D void ended(const Place<kBwd, 2>& to, int n, Floats<V> in) const {
+    if (p.dh0 && n > 0 && n == to.left)
+#pragma unroll
+      for (int v = 0; v < V; ++v) p.dh0[state_at + v] = vget(in, v);
+  }
   // The warp's steps from the state `in` (u of the step after).
   MPB_D void write(const char* mine, uint32_t chain, uint32_t r0, const Place<kBwd, 2>& to, Floats<V>& in) const {
     const int n = to.steps();
     char *dx = const_cast<char*>(to.at[0]), *dg = const_cast<char*>(to.at[1]);
     float sum[kBwd];
-    auto step = [&](int i, Floats<V> low) {  // low: h[t - 1]
-      Floats<V> a, om;
-      gate_at(mine, i, r0, a, om);
-      const Floats<V> s = vadd(unpack(Tile::CX::get(mine, i, half(0, r0, i))), in);
-      if constexpr (SIG) low = vfma(unpack(Tile::CX::get(mine + Tile::kX, i, half(2, r0, i))), vset<V>(-1.0f), low);
-      put_global(dx, pack<X>(SIG ? vmul(om, s) : s));
-      dx = ahead_by(dx, out_st[0]);
-      in = vmul(a, s);
-      const Floats<V> da = vmul(s, low);
-      if constexpr (SHARED) {
-        sum[i] = V == 2 ? vget(da, 0) + vget(da, 1) : vget(da, 0);
-      } else {
-        put_global(dg, pack<G>(SIG ? vmul(da, vmul(a, om)) : da));
-        dg = ahead_by(dg, out_st[1]);
-      }
-    };
-    auto before = [&](int i) { return unpack(Tile::CX::get(mine + Tile::kH, i, half(1, r0, i))); };
     if (__all_sync(0xffffffffu, to.left > kBwd)) {
 #pragma unroll
-      for (int i = 0; i < kBwd; ++i) step(i, before(i));
+      for (int i = 0; i < kBwd; ++i) sum[i] = over_channels(step(mine, i, r0, before(mine, i, r0), dx, dg, in));
     } else {
 #pragma unroll
       for (int i = 0; i < kBwd; ++i) {
         sum[i] = 0.0f;
-        if (i < n) {
-          Floats<V> low = before(i);
-          if (to.left - 1 == i)  // the first step of the sequence
-#pragma unroll
-            for (int v = 0; v < V; ++v) vput(low, v, p.h0 ? p.h0[state_at + v] : 0.0f);
-          step(i, low);
-        }
+        if (i < n) sum[i] = over_channels(step(mine, i, r0, before_any(mine, i, r0, to), dx, dg, in));
       }
     }
-    if (p.dh0 && n > 0 && n == to.left)
-#pragma unroll
-      for (int v = 0; v < V; ++v) p.dh0[state_at + v] = vget(in, v);
+    ended(to, n, in);
     if constexpr (SHARED) head_sums(sum, chain, r0);
   }
-  MPB_D void head_sums(float (&sum)[kBwd], uint32_t chain, uint32_t r0) const {
-    // a head's lanes: a power of two of them, or the whole warp (idle lanes add zeros)
-    const int lanes = p.heads_per > 1 ? (int)p.lanes_per : 32;
-    int first, left;
-    sum_over_lanes(sum, lane, lanes, first, left);
-    // of the lanes that hold the same sums the one with the upper bits clear writes
-    const int at = p.heads_per > 1 ? lane & (lanes - 1) : lane;
-    const uint32_t b = p.by_groups.div(chain), group = chain - b * p.groups;
-    const int64_t head = p.groups_per > 1 ? (int64_t)p.by_groups_per.div(group)
-                                          : (int64_t)group * p.heads_per + (p.heads_per > 1 ? lane / lanes : 0);
-    if (at >= kBwd || head >= p.H) return;
-    const int64_t bt = (int64_t)b * p.T;
-#pragma unroll
+  // The same for a warp in turn, in short code.
+  MPB_D void write_in_turn(const char* mine, uint32_t chain, uint32_t r0, const Place<kBwd, 2>& to, Floats<V>& in) const {
+    const int n = to.steps();
+    char *dx = const_cast<char*>(to.at[0]), *dg = const_cast<char*>(to.at[1]);
+    const Heads q(p, chain, lane);
+#pragma unroll 1
     for (int i = 0; i < kBwd; ++i) {
-      const int64_t t = p.T - 1 - (int64_t)r0 - (first + i);
-      if (i < left && t >= 0) {
-        if (p.groups_per > 1) {
-          p.part[((bt + t) * p.H + head) * p.groups_per + (group - (uint32_t)head * p.groups_per)] = sum[i];
-        } else {
-          float a, om;
-          gate_of<SIG>(to_f(((const G*)p.gate)[(int64_t)b * p.g_sb + t * p.g_st + head]), a, om);
-          ((G*)p.dgate)[(bt + t) * p.H + head] = Cvt<G>::from(SIG ? sum[i] * (a * om) : sum[i]);
-        }
+      float sum = 0.0f;
+      if (i < n) sum = over_channels(step(mine, i, r0, before_any(mine, i, r0, to), dx, dg, in));
+      if constexpr (SHARED) {
+        for (int bit = 1; bit < q.lanes; bit <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, bit);
+        if (q.at == 0) put_head(q, p.T - 1 - (int64_t)r0 - i, sum);
       }
     }
+    ended(to, n, in);
+  }
+  // A head's lanes: a power of two of them, or the whole warp (idle lanes add zeros).
+  struct Heads {
+    int lanes, at;
+    int64_t b, head;
+    uint32_t group;
+    MPB_D Heads(const ScanArgs& p, uint32_t chain, int lane) {
+      lanes = p.heads_per > 1 ? (int)p.lanes_per : 32;
+      at = p.heads_per > 1 ? lane & (lanes - 1) : lane;
+      b = p.by_groups.div(chain);
+      group = chain - (uint32_t)b * p.groups;
+      head = p.groups_per > 1 ? (int64_t)p.by_groups_per.div(group)
+                              : (int64_t)group * p.heads_per + (p.heads_per > 1 ? lane / lanes : 0);
+    }
+  };
+  // The sum over a head's channels (of the group) at step t.
+  MPB_D void put_head(const Heads& q, int64_t t, float sum) const {
+    if (t < 0 || q.head >= p.H) return;
+    const int64_t bt = q.b * p.T;
+    if (p.groups_per > 1) {
+      p.part[((bt + t) * p.H + q.head) * p.groups_per + (q.group - (uint32_t)q.head * p.groups_per)] = sum;
+    } else {
+      float a, om;
+      gate_of<SIG>(to_f(((const G*)p.gate)[q.b * p.g_sb + t * p.g_st + q.head]), a, om);
+      ((G*)p.dgate)[(bt + t) * p.H + q.head] = Cvt<G>::from(SIG ? sum * (a * om) : sum);
+    }
+  }
+  MPB_D void head_sums(float (&sum)[kBwd], uint32_t chain, uint32_t r0) const {
+    const Heads q(p, chain, lane);
+    int first, left;
+    sum_over_lanes(sum, lane, q.lanes, first, left);
+    // of the lanes that hold the same sums the one with the upper bits clear writes
+    if (q.at >= kBwd) return;
+#pragma unroll
+    for (int i = 0; i < kBwd; ++i)
+      if (i < left) put_head(q, p.T - 1 - (int64_t)r0 - (first + i), sum[i]);
   }
 };
 
@@ -1021,8 +1143,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd_walk(ScanArgs p) {
     const uint32_t r0 = cur.chunk * p.steps + bw.warp * kBwd;
     Floats<V> ma, mb, in;
     bw.fold(mine, r0, ma, mb);
-    join<V>(sh, it & 1, bw.warp, bw.lane, ma, mb, carry, in);
-    bw.write(mine, cur.chain, r0, to, in);
+    const bool sound = SIG || to.left < kBwd || numbers<V>(ma, mb);
+    const bool turns = join<V, !SIG>(sh, it & 1, bw.warp, bw.lane, sound, ma, mb, carry, in);
+    if (turns) {
+      start_turn<V>(sh, bw.warp, bw.lane, in);
+      bw.write_in_turn(mine, cur.chain, r0, to, in);
+      end_turn<V>(sh, bw.warp, bw.lane, in);
+      carry = *reinterpret_cast<const Floats<V>*>(&sh.carry[bw.lane * V]);
+    } else {
+      bw.write(mine, cur.chain, r0, to, in);
+    }
     if (blockDim.x == 32) carry = in;
     cur.next(p);
     stage = stage + 1 == NST ? 0 : stage + 1;
@@ -1038,12 +1168,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd_far(ScanArgs p) {
   Backward<X, G, SIG, V, SHARED> bw(p);
   const uint32_t base = smem_u32(ring);
   auto r0_of = [&](uint32_t chunk) { return chunk * p.steps + bw.warp * kBwd; };
-  look_back_tiles<V>(
+  look_back_tiles<V, !SIG>(
       p, sh, bw.warp, bw.lane,
       [&](uint32_t chain, uint32_t chunk, int stage, int side) {
-        bw.sub_words(place<V, SHARED>(p, chain, bw.lane));
+        const Lane l = place<V, SHARED>(p, chain, bw.lane);
+        bw.sub_words(l);
         Floats<V> ma, mb;
         bw.fold(ring + stage * Tile::kBytes, r0_of(chunk), ma, mb);
+        if (!SIG && !(l.in && p.T - r0_of(chunk) >= kBwd)) ma = vset<V>(1.0f), mb = vset<V>(0.0f);
         put_map<V>(sh, side, bw.warp, bw.lane, ma, mb);
       },
       [&](uint32_t chain, uint32_t chunk, float (&c)[V]) {
@@ -1051,10 +1183,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_gscan_bwd_far(ScanArgs p) {
 #pragma unroll
         for (int v = 0; v < V; ++v) c[v] = chunk < 32 && l.in && p.dstate ? p.dstate[l.b * p.D + l.ch + v] : 0.0f;
       },
-      [&](uint32_t chain, uint32_t chunk, int stage, Floats<V> in) {
+      [&](uint32_t chain, uint32_t chunk, int stage, Floats<V>& in, auto in_turn) {
         Place<kBwd, 2> to;
         bw.output(chain, chunk, to);
-        bw.write(ring + stage * Tile::kBytes, chain, r0_of(chunk), to, in);
+        if constexpr (decltype(in_turn)::value) bw.write_in_turn(ring + stage * Tile::kBytes, chain, r0_of(chunk), to, in);
+        else bw.write(ring + stage * Tile::kBytes, chain, r0_of(chunk), to, in);
       },
       [&](bool is, uint32_t chain, uint32_t chunk, int stage) {
         if (is) {

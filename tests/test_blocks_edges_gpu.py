@@ -1,13 +1,13 @@
 """The block operators at the edges of their ranges on the GPU, against their formulas in 64 bits: results without
-elements to sum and factors of zero beside exponentials that overflow. Tolerances are the bounds that blocks_plain
-derives."""
+elements to sum, factors of zero beside exponentials that overflow, and products of gates that leave the float range.
+Tolerances are the bounds that blocks_plain derives."""
 import math
 
 import pytest
 import torch
 
 from . import blocks_plain as P
-from .test_blocks_gpu import make_policy, rand
+from .test_blocks_gpu import TORCH, gates, make_policy, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -104,3 +104,73 @@ def test_policy_zero_factors_beside_large_exponentials(ms, V, layout):
     r = ms.policy_loss(A(c["z"]), A(c["t"]), A(c["old"]), A(c["adv"]), clip_low=0.2, clip_high=0.3)
     rows = r.dlogits.torch().isnan().all(1)
     assert bool(rows[0]) and bool(rows[3]) and int(rows.sum()) == 2 and bool(r.loss.torch().isnan())
+
+
+# ------------------------------------- products of gates beyond float
+def _swings(B, T, H, up, run, seed, sign):
+    """Gates near `up` for `run` steps, then near 0.55 until that is undone, in turn; each channel starts
+    elsewhere. Nothing shrinks below 2^-126 of itself in 128 steps, so nothing may count as zero."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    period = run + int(run * math.log2(up) / -math.log2(0.55))
+    t = torch.arange(T, device="cuda")[None, :, None] + torch.randint(0, period, (B, 1, H), device="cuda", generator=g)
+    gate = torch.where(t % period < run, up, 0.55) * (torch.rand(B, T, H, device="cuda", generator=g) * 0.1 + 0.95)
+    return gate * (torch.where(t % 3 == 0, -1.0, 1.0) if sign else 1.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,T,D,H", [(1, 700, 40, 40), (1, 1500, 64, 64), (2, 700, 96, 6), (3, 700, 1500, 1500),
+                                     (170, 300, 60, 60), (3, 401, 2048, 32)])
+@pytest.mark.parametrize("up,run,sign", [(2.5, 110, True), (1024.0, 16, False), (2.0 ** 20, 9, True)])
+def test_scan_with_gates_beyond_one(ms, B, T, D, H, up, run, sign, dtype):
+    """States that grow and shrink again by up to 2^180 within float, while the products of the gates alone do not stay
+    in it: in few chains and in many."""
+    gate = _swings(B, T, H, up, run, 1, sign).to(TORCH[dtype])
+    gate[:, 0] = 0.0
+    gate[:, T // 2] = 0.0
+    tiny = 2.0 ** -100
+    x = (rand(B, T, D, seed=2) * tiny).to(TORCH[dtype])
+    A = ms.from_torch
+    for h0 in (None, rand(B, D, seed=3) * tiny):
+        if h0 is not None:
+            gate[:, 0] = up
+        opt = None if h0 is None else h0.double()
+        h, last = ms.gated_scan(A(x), A(gate), None if h0 is None else A(h0), return_state=True)
+        wh, wl, eh, el = P.scan(x.double(), gate.double(), opt, "linear")
+        P.close(h.torch(), wh, eh, "h")
+        P.close(last.torch(), wl, el, "state")
+        dh, ds = (rand(B, T, D, seed=4) * tiny).to(x.dtype), rand(B, D, seed=5) * tiny
+        got = ms.gated_scan_backward(A(dh), A(x), A(gate), h, None if h0 is None else A(h0), A(ds))
+        want, err = P.scan_backward(dh.double(), x.double(), gate.double(), h.torch().double(), opt, ds.double(), "linear")
+        # a gate's gradient sums products that may each be rounded below the normal range, to half of 2^-149
+        for g, w, e, n in zip(got, want, (err[0], err[1] + D // H * 2.0 ** -150, err[2]), ("dx", "dgate", "dh0")):
+            P.close(g.torch(), w, e, n)
+
+
+@pytest.mark.parametrize("B,T,D", [(1, 900, 70), (4, 900, 900)])
+def test_scan_with_gates_beyond_one_is_repeatable(ms, B, T, D):
+    gate, x = _swings(B, T, D, 1024.0, 16, 1, True), rand(B, T, D, seed=2) * 2.0 ** -100
+    A = ms.from_torch
+    runs = []
+    for _ in range(6):
+        used_memory()
+        h = ms.gated_scan(A(x), A(gate))
+        runs.append((h.torch(),) + tuple(v.torch() for v in ms.gated_scan_backward(A(x), A(x), A(gate), h)))
+    for other in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
+@pytest.mark.parametrize("B,T,D", [(2, 300, 36), (4, 300, 900)])
+def test_scan_keeps_what_is_not_finite_in_its_channel(ms, B, T, D):
+    """Linear: an infinite or NaN gate or input makes its channel what the formula makes it from that step on, up to
+    where the gate is zero again (zero times an infinity stays NaN); the other channels keep their values."""
+    x, g, h0 = rand(B, T, D, seed=1), gates(B, T, D, "linear", "f32", 2), rand(B, D, seed=3)
+    A = ms.from_torch
+    clean = ms.gated_scan(A(x), A(g), A(h0)).torch()
+    x[0, 40, 3], g[0, 90, 9], g[1, 100, 20], x[1, 7, 30] = math.inf, math.nan, math.inf, math.nan
+    h = ms.gated_scan(A(x), A(g), A(h0)).torch()
+    want, _, _, _ = P.scan(x.double(), g.double(), h0.double(), "linear")
+    assert torch.equal(h.isnan(), want.isnan()) and torch.equal(h.isinf(), want.isinf())
+    same = torch.ones(B, T, D, dtype=torch.bool, device="cuda")
+    for b, t, d in ((0, 40, 3), (0, 90, 9), (1, 100, 20), (1, 7, 30)):
+        same[b, t:, d] = False
+    torch.testing.assert_close(h[same], clean[same], rtol=1e-5, atol=1e-5)
