@@ -100,25 +100,25 @@ struct ScanArgs {
   float* part;       // (B, T, H, groups_per)
 };
 
-// The decay a and what the input is weighted with, om, of a gate.
-template <bool SIG, class F>
+// The decay a and what the input is weighted with, om, of a gate of type G.
+template <bool SIG, class G, class F>
 MPB_D void gate_of(F g, F& a, F& om) {
   if constexpr (SIG) {
-    sigmoid2(g, a, om);
+    sigmoid2<sizeof(G) == 4>(g, a, om);
   } else {
     a = om = g;
   }
 }
 // Of a gate's pack; one that the lane's channels share is evaluated once.
-template <bool SIG, int V, class P>
-MPB_D void gates_of(const P& g, Floats<V>& a, Floats<V>& om) {
-  if constexpr (sizeof(P::v) == sizeof(g.v[0]) && V == 2) {
+template <bool SIG, int V, class G, int N>
+MPB_D void gates_of(const Pack<G, N>& g, Floats<V>& a, Floats<V>& om) {
+  if constexpr (N == 1 && V == 2) {
     float sa, so;
-    gate_of<SIG>(to_f(g.v[0]), sa, so);
+    gate_of<SIG, G>(to_f(g.v[0]), sa, so);
     a = vset<V>(sa);
     om = vset<V>(so);
   } else {
-    gate_of<SIG>(unpack(g), a, om);
+    gate_of<SIG, G>(unpack(g), a, om);
   }
 }
 
@@ -1086,7 +1086,7 @@ struct Backward {
       p.part[((bt + t) * p.H + q.head) * p.groups_per + (q.group - (uint32_t)q.head * p.groups_per)] = sum;
     } else {
       float a, om;
-      gate_of<SIG>(to_f(((const G*)p.gate)[q.b * p.g_sb + t * p.g_st + q.head]), a, om);
+      gate_of<SIG, G>(to_f(((const G*)p.gate)[q.b * p.g_sb + t * p.g_st + q.head]), a, om);
       ((G*)p.dgate)[(bt + t) * p.H + q.head] = Cvt<G>::from(SIG ? sum * (a * om) : sum);
     }
   }
@@ -1208,7 +1208,7 @@ __global__ void __launch_bounds__(256) k_gscan_heads(ScanArgs p) {
   float s = 0.0f;
   for (uint32_t k = 0; k < p.groups_per; ++k) s += p.part[i * p.groups_per + k];
   float a, om;
-  gate_of<SIG>(to_f(((const G*)p.gate)[b * p.g_sb + t * p.g_st + head]), a, om);
+  gate_of<SIG, G>(to_f(((const G*)p.gate)[b * p.g_sb + t * p.g_st + head]), a, om);
   ((G*)p.dgate)[i] = Cvt<G>::from(SIG ? s * (a * om) : s);
 }
 

@@ -66,6 +66,7 @@ constexpr int kPerThread = 32;    // its elements per thread, at most
 constexpr int64_t kMostStride = 1 << 29;  // between rows: its bytes are multiplied in 32 bits
 constexpr int64_t kInRegisters = (int64_t)kRowThreads * kPerThread;
 
+template <class T>
 MPB_D void act_of(int act, float g, float& v, float& slope) {
   if (act == MPB_ACT_LINEAR) {
     v = g;
@@ -73,7 +74,7 @@ MPB_D void act_of(int act, float g, float& v, float& slope) {
     return;
   }
   float s, om;
-  sigmoid2(g, s, om);
+  sigmoid2<sizeof(T) == 4>(g, s, om);
   if (act == MPB_ACT_SIGMOID) {
     v = s;
     slope = s * om;
@@ -101,7 +102,7 @@ MPB_D float stream_at(const NormArgs& p, int64_t r, int64_t c, float rz) {
     const float m = branch_factor(p, r, c);
     if (m != 0.0f) {
       float v = 1.0f, slope;
-      if (p.gate_kind != MPB_GATE_NONE) act_of(p.act, gate_at<T>(p, r, c), v, slope);
+      if (p.gate_kind != MPB_GATE_NONE) act_of<T>(p.act, gate_at<T>(p, r, c), v, slope);
       y += m * v * (to_f(((const T*)p.z)[r * p.z_sr + c]) * rz * p.w_post[c]);
     }
   }
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(kThreads) k_norm_bwd_long(NormArgs p) {
     if (!p.z) continue;
     const float m = branch_factor(p, r, c);
     float v = 1.0f, slope = 0.0f;
-    if (p.gate_kind != MPB_GATE_NONE) act_of(p.act, gate_at<T>(p, r, c), v, slope);
+    if (p.gate_kind != MPB_GATE_NONE) act_of<T>(p.act, gate_at<T>(p, r, c), v, slope);
     const float zh = to_f(z[c]) * rz;
     const float d = m == 0.0f ? 0.0f : dx * m;
     if (m != 0.0f) dotz = fmaf(d * v * p.w_post[c], zh, dotz);
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(kThreads) k_norm_bwd_long(NormArgs p) {
   for (int64_t c = threadIdx.x; c < p.D; c += kThreads) {
     const float m = branch_factor(p, r, c);
     float v = 1.0f, slope;
-    if (p.gate_kind != MPB_GATE_NONE) act_of(p.act, gate_at<T>(p, r, c), v, slope);
+    if (p.gate_kind != MPB_GATE_NONE) act_of<T>(p.act, gate_at<T>(p, r, c), v, slope);
     const float dn = m == 0.0f ? 0.0f : dx_at(c) * m * v;
     ((T*)p.dz)[r * p.D + c] = Cvt<T>::from(rz * (dn * p.w_post[c] - to_f(z[c]) * rz * mz));
   }
@@ -198,7 +199,7 @@ __global__ void k_norm_bwd_long_cols(NormArgs p) {
     const float m = branch_factor(p, r, c);
     if (m == 0.0f) continue;
     float v = 1.0f, slope = 0.0f;
-    if (p.gate_kind != MPB_GATE_NONE) act_of(p.act, gate_at<T>(p, r, c), v, slope);
+    if (p.gate_kind != MPB_GATE_NONE) act_of<T>(p.act, gate_at<T>(p, r, c), v, slope);
     const float zh = to_f(((const T*)p.z)[r * p.z_sr + c]) * p.rstd[r];
     const float d = p.part[r * p.D + c] * m;
     wpost += d * v * zh;
@@ -357,14 +358,14 @@ MPB_D void gate_pack(const NormArgs& p, const Elems<T, W>& full, int64_t r, int 
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       F om;
-      sigmoid2(g[i], v[i], om);
+      sigmoid2<sizeof(T) == 4>(g[i], v[i], om);
       slope[i] = vmul(v[i], om);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       F s, om;
-      sigmoid2(g[i], s, om);
+      sigmoid2<sizeof(T) == 4>(g[i], s, om);
       v[i] = vmul(g[i], s);
       slope[i] = vmul(s, vfma(g[i], om, one));
     }

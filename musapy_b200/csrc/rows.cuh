@@ -95,19 +95,38 @@ MPB_D float min_nan(float a, float b) {
 constexpr float kMinusLog2e = -1.44269504088896340736f;
 
 // s = sigmoid(g) = 1 / (1 + e) and 1 - s = e s with e = 2^(-g log2 e): neither is
-// a difference of nearly equal numbers, so both keep their relative precision
-// (a few units in the last place). e is held at 2^126, and its 2^-126 is taken
-// off s again: a gate of -inf gives an exact 0, and a sigmoid that is not
-// below 2^-102 does not notice. NaN stays NaN.
+// a difference of nearly equal numbers, so both keep their relative precision:
+// a few units in the last place, and what the rounding of -g log2 e to float
+// makes of e, up to |g| units of 2^-24. FINE takes that out again: x being the rounded
+// argument, e = 2^x (1 + t) with t = -g - x ln 2, which is exact enough in two fused
+// multiply-adds. It is for gates in 32 bits; the results of 16-bit gates are
+// rounded to far more than the 2^-17 that |g| units come to at most.
+// e is held at 2^126, and its 2^-126 is taken off s again: a gate of -inf gives an
+// exact 0, and a sigmoid that is not below 2^-102 does not notice. NaN stays NaN.
 constexpr float kLeastSigmoid = 1.1754943508222875e-38f;  // 2^-126
+constexpr float kMinusLn2 = -0.69314718055994530942f;
+constexpr float kMinusLn2Rest = (float)(-0.69314718055994530942 - (double)kMinusLn2);
+template <bool FINE>
 MPB_D void sigmoid2(float g, float& s, float& one_minus) {
-  const float e = ex2f(min_nan(g * kMinusLog2e, 126.0f)), r = rcpf(1.0f + e);
+  const float x = g * kMinusLog2e;
+  float e = ex2f(min_nan(x, 126.0f));
+  if (FINE) {
+    const float t = fmaf(x, kMinusLn2Rest, fmaf(x, kMinusLn2, -g));
+    e = fmaf(e, fabsf(x) > 126.0f ? 0.0f : t, e);
+  }
+  const float r = rcpf(1.0f + e);
   s = r - kLeastSigmoid;
   one_minus = e * r;
 }
+template <bool FINE>
 MPB_D void sigmoid2(float2 g, float2& s, float2& one_minus) {
   const float2 x = vmul(g, vset<2>(kMinusLog2e));
-  const float2 e = make_float2(ex2f(min_nan(x.x, 126.0f)), ex2f(min_nan(x.y, 126.0f)));
+  float2 e = make_float2(ex2f(min_nan(x.x, 126.0f)), ex2f(min_nan(x.y, 126.0f)));
+  if (FINE) {
+    float2 t = vfma(x, vset<2>(kMinusLn2Rest), vfma(x, vset<2>(kMinusLn2), make_float2(-g.x, -g.y)));
+    t = make_float2(fabsf(x.x) > 126.0f ? 0.0f : t.x, fabsf(x.y) > 126.0f ? 0.0f : t.y);
+    e = vfma(e, t, e);
+  }
   const float2 d = vadd(e, vset<2>(1.0f)), r = make_float2(rcpf(d.x), rcpf(d.y));
   s = vadd(r, vset<2>(-kLeastSigmoid));
   one_minus = vmul(e, r);

@@ -1,13 +1,13 @@
 """The block operators at the edges of their ranges on the GPU, against their formulas in 64 bits: results without
-elements to sum, factors of zero beside exponentials that overflow, and products of gates that leave the float range.
-Tolerances are the bounds that blocks_plain derives."""
+elements to sum, factors of zero beside exponentials that overflow, products of gates that leave the float range, and
+saturated gates. Tolerances are the bounds that blocks_plain derives."""
 import math
 
 import pytest
 import torch
 
 from . import blocks_plain as P
-from .test_blocks_gpu import TORCH, gates, make_policy, rand
+from .test_blocks_gpu import TORCH, check_scan, gates, make_policy, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -174,3 +174,23 @@ def test_scan_keeps_what_is_not_finite_in_its_channel(ms, B, T, D):
     for b, t, d in ((0, 40, 3), (0, 90, 9), (1, 100, 20), (1, 7, 30)):
         same[b, t:, d] = False
     torch.testing.assert_close(h[same], clean[same], rtol=1e-5, atol=1e-5)
+
+
+# ------------------------------------------------------ saturated gates
+@pytest.mark.parametrize("B,T,D,H", [(2, 1, 64, 64), (3, 40, 33, 33), (1, 300, 70, 70), (4, 200, 900, 900), (2, 60, 96, 6)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scan_saturated_float_gates(ms, B, T, D, H, dtype, sign):
+    """Gates of 16 to 64 in 32 bits: one minus the sigmoid, or the sigmoid, is as small as 2^-92 and keeps its
+    relative precision, and so do the gradients that it enters."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    gate = (torch.rand(B, T, H, device="cuda", generator=g) * 48 + 16) * sign
+    check_scan(ms, rand(B, T, D, seed=2, dtype=dtype), gate, torch.zeros(B, D, device="cuda") if sign > 0 else rand(B, D, seed=3),
+               "sigmoid")
+    x = rand(B, D, seed=4, dtype=dtype) if sign > 0 else torch.zeros(B, D, dtype=TORCH[dtype], device="cuda")
+    s0 = torch.zeros(B, D, device="cuda") if sign > 0 else rand(B, D, seed=5)
+    want, wl, e, el = P.scan(x[:, None].double(), gate[:, :1].double(), s0.double(), "sigmoid")
+    state = ms.from_torch(s0.clone())
+    h = ms.gated_scan_step(state, ms.from_torch(x), ms.from_torch(gate[:, 0].contiguous()), mode="sigmoid")
+    P.close(h.torch(), want[:, 0], e[:, 0], "step")
+    P.close(state.torch(), wl, el, "state")
