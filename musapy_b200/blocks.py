@@ -111,22 +111,21 @@ def _dense(x: Array) -> bool:
     return (lay is not None and lay[0] == x._strides) or x._is_c_contiguous()
 
 
-def _carve(s, dev: int, *parts):
-    """Several small results in one allocation: an Array for each (shape, dtype). To the alias checks each is an
-    allocation of its own (they do not overlap)."""
-    total, at = 0, []
-    for shape, d in parts:
-        at.append(total)
-        total += (_prod(shape) * d.itemsize + 15) & ~15
-    first = _new(s, (max(total, 16),), _dt.uint8, dev)
-    made = []
-    for (shape, d), start in zip(parts, at):
+def _carve(s, dev: int, shape: tuple, nbytes: int, *kinds):
+    """Several small results of one shape and nbytes of scratch in one allocation: an Array for each dtype, and the
+    scratch's address. To the alias checks each is an allocation of its own (they do not overlap)."""
+    lay = _LAYOUTS.get(shape)
+    strides, n = lay[:2] if lay is not None else (contiguous_strides(shape), _prod(shape))
+    first = _new(s, (sum((n * d.itemsize + 15) & ~15 for d in kinds) + max(nbytes, 16),), _dt.uint8, dev)
+    made, at = [], 0
+    for d in kinds:
         a = _new_array(Array)
-        a._buf, a._shape, a._strides, a._offset = first._buf, shape, contiguous_strides(shape), start // d.itemsize
+        a._buf, a._shape, a._strides, a._offset = first._buf, shape, strides, at // d.itemsize
         a._dtype, a._dev, a._name, a._dev_src, a._dt_src = d, dev, None, first._dev_src, first._dt_src
-        a._ptr = a._sid = first._ptr + start
+        a._ptr = a._sid = first._ptr + at
         made.append(a)
-    return made
+        at += (n * d.itemsize + 15) & ~15
+    return made, first._ptr + at
 
 
 # ------------------------------------------------------------ gated scan
@@ -509,11 +508,11 @@ def policy_loss(logits, targets, old_logp, advantages, ref_logp=None, mask=None,
     dev = _same_device(name, *ins)
     s = _streams.current_stream(dev)
     nbytes = NATIVE.policy_loss_scratch_bytes(N, V, z._dtype.code)
-    loss, logp, kl, clipped, scratch = _carve(s, dev, ((), _dt.float32), (lead, _dt.float32), (lead, _dt.float32),
-                                              (lead, _dt.bool_), ((nbytes,), _dt.uint8))
+    loss = _new(s, (), _dt.float32, dev)  # alone: programs keep it for longer than the tokens' results
+    (logp, kl, clipped), scratch = _carve(s, dev, lead, nbytes, _dt.float32, _dt.float32, _dt.bool_)
     dlogits = _new(s, z._shape, z._dtype, dev) if grad else None
     check(NATIVE.policy_loss(N, V, z._ptr, z._dtype.code, zr, targets._ptr, targets._dtype.code, old._ptr, adv._ptr,
                              _ptr(ref_logp), _ptr(mask), float(clip_low), float(clip_high), float(kl_coef),
                              float(grad_scale), loss._ptr, logp._ptr, kl._ptr, clipped._ptr, _ptr(dlogits),
-                             scratch._ptr, nbytes, _streams.launch_on(s, name, *ins, loss, dlogits)), name)
+                             scratch, nbytes, _streams.launch_on(s, name, *ins, loss, logp, dlogits)), name)
     return PolicyLoss(loss, logp, kl, clipped, dlogits)

@@ -1,6 +1,6 @@
 """The block operators at the edges of their ranges on the GPU, against their formulas in 64 bits: results without
-elements to sum, factors of zero beside exponentials that overflow, products of gates that leave the float range, and
-saturated gates. Tolerances are the bounds that blocks_plain derives."""
+elements to sum, factors of zero beside exponentials that overflow, products of gates that leave the float range,
+saturated gates, and what a result keeps alive. Tolerances are the bounds that blocks_plain derives."""
 import math
 
 import pytest
@@ -194,3 +194,12 @@ def test_scan_saturated_float_gates(ms, B, T, D, H, dtype, sign):
     h = ms.gated_scan_step(state, ms.from_torch(x), ms.from_torch(gate[:, 0].contiguous()), mode="sigmoid")
     P.close(h.torch(), want[:, 0], e[:, 0], "step")
     P.close(state.torch(), wl, el, "state")
+
+
+# --------------------------------------------------------------- memory
+def test_a_kept_loss_keeps_only_itself(ms):
+    """A program that collects the losses of its steps holds 16 bytes for each, not the tokens' results."""
+    A = ms.from_torch
+    c = make_policy(5000, 40, "f32", 0.0)
+    r = ms.policy_loss(A(c["z"]), A(c["t"]), A(c["old"]), A(c["adv"]))
+    assert r.loss.torch().untyped_storage().nbytes() <= 16
