@@ -69,7 +69,7 @@ struct Token {
 // the KL term out.
 MPB_D void token_terms(const PolicyArgs& p, const Token& token, float logp, float& value, float& kl, bool& clipped,
                        float& slope) {
-  const float a = token.adv, x = logp - token.old, rho = __expf(x);
+  const float a = token.adv, x = logp - token.old, rho = expf(x);
   clipped = (a > 0.0f && rho > 1.0f + p.hi) || (a < 0.0f && rho < 1.0f - p.lo);
   const float bound = a > 0.0f ? 1.0f + p.hi : 1.0f - p.lo;
   const float gain = a == 0.0f && fabsf(x) < INFINITY ? 0.0f : rho * a;

@@ -106,6 +106,27 @@ def test_policy_zero_factors_beside_large_exponentials(ms, V, layout):
     assert bool(rows[0]) and bool(rows[3]) and int(rows.sum()) == 2 and bool(r.loss.torch().isnan())
 
 
+def test_policy_ratio_keeps_its_precision(ms):
+    """One word in the vocabulary: logp is exactly 0, and with advantage -1 the loss is e^-old alone, to the error of a
+    float exponential (an ulp, here allowed two) whatever its size; so is the per-token slope in the gradient of two
+    even words."""
+    A = ms.from_torch
+    for old in (-80.0, -40.5, -20.25, -3.0, 0.0, 7.5, 30.0):
+        z, t = torch.zeros(1, 1, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")
+        o, a = torch.full((1,), old, device="cuda"), torch.full((1,), -1.0, device="cuda")
+        loss = float(ms.policy_loss(A(z), A(t), A(o), A(a), clip_low=1.0).loss.torch())
+        want = math.exp(-old)
+        assert abs(loss - want) <= 2 * 2.0 ** -23 * want, (old, loss, want)
+        # two even words: logp = -ln 2 in float, so e^(logp - old) is taken of the same float here
+        z = torch.zeros(1, 2, device="cuda")
+        r = ms.policy_loss(A(z), A(t), A(o), A(a), clip_low=1.0)
+        x = float(r.logp.torch()) - old
+        x = float(torch.tensor(x, dtype=torch.float32))
+        want = math.exp(x) / 2
+        g = r.dlogits.torch()[0].double()
+        assert float((g - torch.tensor([want, -want], device="cuda")).abs().max()) <= 4 * 2.0 ** -23 * want, (old, g, want)
+
+
 # ------------------------------------- products of gates beyond float
 def _swings(B, T, H, up, run, seed, sign):
     """Gates near `up` for `run` steps, then near 0.55 until that is undone, in turn; each channel starts
