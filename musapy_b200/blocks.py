@@ -475,9 +475,9 @@ def policy_loss(logits, targets, old_logp, advantages, ref_logp=None, mask=None,
     logits are (..., V); targets (int32 or int64), old_logp, advantages, ref_logp (float32) and mask (bool, None for
     all tokens) have the leading shape. With rho = exp(logp - old_logp) a token adds
     ``-min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(q) - q - 1)``, q = ref_logp - logp (no KL
-    term without ref_logp, nor with kl_coef 0, where kl is still returned); the loss is the mean over the mask, 0 when it is empty. clip_high defaults to clip_low.
-    Tokens outside the mask have zero gradient, logp and kl whatever they hold; a target outside [0, V) makes its
-    token's values NaN."""
+    term without ref_logp, nor with kl_coef 0, where kl is still returned); the loss is the mean over the mask, 0 when
+    it is empty. clip_high defaults to clip_low. Tokens outside the mask have zero gradient, logp and kl whatever they
+    hold; a target outside [0, V) makes its token's values NaN."""
     name = "policy_loss"
     z, zr = _rows(_norm_input(name, "logits", logits))
     V, lead = z._shape[-1], z._shape[:-1]

@@ -24,11 +24,12 @@
 //
 // Bound: memory (logits read, gradient written); next to it the two exponentials
 // per element, 119 us each for 4096 x 131072 at 16 per clock and SM. Measured,
-// loss and gradient: 4096 x 131072 bf16 421 us (5.1 TB/s), 2048 x 131072 f32 369 us
-// (5.8 TB/s), 8192 x 32000 bf16 196 us (5.4 TB/s), 65536 x 1000 bf16 68 us. Three
-// passes over global memory took 1314 us for the first; blocks of 32 KB, six
-// per SM, 463 us; one maximum and one rescaling per 16-byte word instead of
-// four, and bounds checked per word, 571 us.
+// loss and gradient: 4096 x 131072 bf16 423 us (5.1 TB/s), 2048 x 131072 f32 370 us
+// (5.8 TB/s), 8192 x 32000 bf16 195 us (5.4 TB/s), 65536 x 1000 bf16 67 us (3.9 TB/s);
+// the loss alone, half the bytes, 250 us (4.3 TB/s), 221, 119 and 45 us. Three passes
+// over global memory took 1314 us for the first; blocks of 32 KB, six per SM,
+// 463 us; one maximum and one rescaling per 16-byte word instead of four, and
+// bounds checked per word, 571 us.
 #include <cooperative_groups.h>
 #include "async_copy.cuh"
 #include "common.cuh"

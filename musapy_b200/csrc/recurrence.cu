@@ -46,15 +46,19 @@
 //
 // Bound: memory by the bytes; what is reached is set by the latency of a tile
 // (its barrier, the maps' join, in a look-back two round trips to L2) at 16
-// warps per SM, which is what the registers and the copies under way leave.
-// Measured, (8, 4096, 2048) bf16 sigmoid: walked forward 83 us (4.9 TB/s),
-// backward 161 us (5.0 TB/s); f32 linear 153 us (5.3 TB/s) and 226 us (5.9 TB/s);
-// 32 gates for heads of 64, bf16 linear, 68 us (4.0 TB/s) and 113 us (3.6 TB/s).
-// By look-back (1, 65536, 1000) f32: 241 us (3.3 TB/s) and 412 us. One 4-byte
-// copy per lane instead of 16 bytes: forward 112 us. Values in registers from
-// plain loads, no copies ahead: 266 us. 16 warps of 8 (backward 4) steps instead
-// of 8 of 16 (8): 109 and 223 us, the join and the places of a tile being done by
-// twice the threads.
+// warps per SM (8 where kRing says so), which is what the registers and the copies
+// under way leave. Measured, (8, 4096, 2048) bf16 sigmoid, 256 chains: walked
+// forward 78 us (5.1 TB/s), backward 150 us (5.4 TB/s); f32 linear 153 us (5.3 TB/s)
+// and 205 us (6.5 TB/s); 32 gates for heads of 64, bf16 linear, 66 us (4.1 TB/s) and
+// 104 us (3.9 TB/s). With 96 to 128 chains an SM has one block: 0.45 to 0.64 of the
+// copy rate for the first, 0.33 to 0.54 for the last. By look-back (1, 65536, 1000)
+// f32 linear: 239 us (3.3 TB/s) and 418 us; (1, 4096, 2048) bf16 sigmoid 27 and 41 us.
+// Forms tried against earlier ones of 83 us forward and 161 us backward: one 4-byte
+// copy per lane instead of 16 bytes 112 us forward; values in registers from plain
+// loads, no copies ahead, 266 us; 16 warps of 8 (backward 4) steps instead of 8 of
+// 16 (8) 109 and 223 us, the join and the places of a tile being done by twice the
+// threads. Warps in turn through the unrolled steps instead of a short loop of their
+// own cost heads backward 115 us.
 #include "async_copy.cuh"
 #include "common.cuh"
 #include "internal.h"
@@ -69,12 +73,18 @@ constexpr int kWarps = 8;       // warps of a full tile
 constexpr int kFwd = 16;        // steps per warp and tile, forward
 // Steps per warp and tile, backward. The more, the fewer joins; 16 where two tiles
 // of that many fit a block's share of shared memory: three inputs of one word
-// per step. (Linear, a gate per head, (4, 4095, 32 x 64) bf16: 80 us with 16 steps,
-// 103 us with 8; sigmoid, four inputs, (8, 4096, 2048) bf16: 172 and 161 us.)
+// per step. (Linear, a gate per head of 64, bf16, T = 4096: 74 us with 16 steps and
+// 98 us with 8 at 128 chains, 104 and 129 us at 256, but 43 us with either by
+// look-back at 32; f32 with a gate per channel 55 and 64 us at 128 chains, 100 and 97
+// at 256. Sigmoid, four inputs, (8, 4096, 2048) bf16, in an earlier form: 172 us with
+// 16 and 161 with 8.)
 constexpr int bwd_steps(bool sig, int gate_bytes, int V, bool shared) {
   return !sig && (shared || gate_bytes * V <= 4) ? 16 : 8;
 }
-constexpr int kRing = 96 << 10; // shared memory of a block for tiles under way, two blocks per SM
+// Shared memory of a walk's block for tiles under way, two blocks per SM. A look-back
+// always has three tiles under way; where a tile takes 48 KB (16-bit inputs with a
+// 32-bit gate per channel; linear, backward, 16 steps) that leaves one block per SM.
+constexpr int kRing = 96 << 10;
 
 struct ScanArgs {
   int64_t B, T, D, H, P;  // P = D / H channels per gate
@@ -1259,9 +1269,17 @@ bool pairs(const ScanArgs& p, int x_dt, int g_dt, bool backward) {
   return ok;
 }
 
-// From this many chains on a block walks a chain. T = 4096, bf16, forward: 64
-// chains take 53 us walked and 44 us by look-back, 96 chains 54 and 58 us, 128
-// chains 55 and 70 us, 256 chains 83 and 107 us.
+// From this many chains on a block walks a chain; one number for all types, modes and
+// directions. T = 4096, walked / by look-back in us, forward then backward:
+//   chains   bf16 sigmoid          bf16 linear, per head   f32 linear
+//     32      51 / 27    96 / 41    39 / 26    72 / 43      33 / 22   49 / 33
+//     64      51 / 43    96 / 70    39 / 38    72 / 64      33 / 37   49 / 55
+//     96      51 / 56    97 / 90    39 / 51    73 / 85      35 / 47   51 / 70
+//    128      51 / 67    97 / 111   39 / 60    74 / 107     35 / 57   54 / 84
+//    160      78 / 78   150 / 129   62 / 69   101 / 129     58 / 65   85 / 97
+//    256      78 / 110  150 / 184   66 / 93   104 / 201     75 / 91  100 / 148
+// So it loses 12 % for f32 at 64 chains, 8 % for sigmoid backward at 96, and 16 %
+// for that at 160, where some SMs walk two chains and some one.
 constexpr uint32_t kWalkFrom = 80;
 
 // Copies of 16 bytes: every row of every input starts on such a boundary, and

@@ -20,22 +20,32 @@
 //
 // A row lives in the registers of its threads (a warp or several, up to 512
 // threads with 32 elements each) between its reductions, so every input is
-// read once and every output written once. In the backward pass blocks take
+// read once and every output written once. At 32 elements per thread, rows above 8192
+// elements, the backward pass does not fit 128 registers and spills 130 to 230
+// bytes per thread in 16-bit types, 300 to 400 in float, and 700 to 940 where
+// bounds are checked or the packs are single elements (forward 80 at most). In the backward pass blocks take
 // rows in turn and add the weights' gradients up in shared memory, each thread
 // its own columns; a second kernel adds the blocks' sums in a fixed order.
-// Rows too long for that (above 16384 elements) are read again for each pass.
+// Rows too long for that (above 16384 elements) are read again for each pass, and
+// their column sums are taken by one thread per column over all rows.
 //
-// Bound: memory. Measured, 16384 x 4096 with a full gate, f32: forward 204 us
-// (6.6 TB/s), backward 438 us (4.9 TB/s); bf16: forward 113 us (6.0 TB/s), with
-// dropout 130 us, backward 222 us (4.8 TB/s) and 227 us. The backward pass runs
+// Bound: memory. Measured, 16384 x 4096 with a full gate, f32: forward 203 us
+// (6.6 TB/s), backward 432 us (5.0 TB/s); bf16: forward 111 us (6.0 TB/s), with
+// dropout 130 us, backward 221 us (4.9 TB/s) and 226 us; the plain norm 46 us (5.9
+// TB/s) and 123 us (3.3 TB/s), f32 84 and 155 us. 4096 x 16384 bf16: 174 and 281 us.
+// 2048 x 32768 bf16 (re-read): 1044 and 5065 us. The backward pass runs
 // about 60 instructions per element at 16 warps per SM (the registers of 16
 // elements' five inputs and sums): their issue, half of it stalled on the
 // row's loads and the two reductions, is what is left above the bytes.
-// Copying the next row ahead into shared memory took 243 us instead of 237 us
-// (bf16, no dropout) and 576 instead of 435 us (f32: fewer resident blocks); one
-// pack per thread and 512 threads per row 240 instead of 209 us. Rows that no
-// 16-byte access may use go element by element (16383 x 4095, f32: forward 239 us,
-// backward 692 us; bf16: 209 and 636 us).
+// Tried against earlier forms: copying the next row ahead into shared memory, 243 us
+// against 237 (bf16, no dropout) and 576 against 435 us (f32: fewer resident blocks);
+// one pack per thread and 512 threads per row, 240 us against 209. That 209 us was
+// a warp's packs 32 apart over the whole row; one warp's packs after the other, as
+// now, costs 221 us there and saves odd widths a sixth or more. Rows that no 16-byte
+// access may use go element by element (16383 x 4095, f32: forward 238 us, backward
+// 690 us; bf16: 208 and 630 us) or, 16-bit types of even width, by pairs (16384 x
+// 4094 bf16: 142 and 302 us), and with dropout they draw a counter for each element
+// or pair (bf16: 436 and 803 us; pairs 242 and 434 us).
 #include "common.cuh"
 #include "internal.h"
 #include "musapy_b200.h"
@@ -307,9 +317,9 @@ MPB_D float fold(float v) { return v; }
 MPB_D float fold(float2 v) { return v.x + v.y; }
 
 // What dropout keeps of a row. EARLY: drawn while the row's loads are under way,
-// where that is a counter per pack; else drawn at each pack. (16384 x 4096 bf16:
-// backward 232 us early, 243 us late; forward, where the words cost a resident
-// block, 144 and 130 us.)
+// where that is a counter per pack; else drawn at each pack. (16384 x 4096 bf16, the
+// backward form then: 232 us early, 243 us late; forward, where the words cost a
+// resident block, 144 and 130 us.)
 template <int W, int NV, bool EARLY>
 struct KeptRow {
   static constexpr bool kEarly = EARLY && W == 8;
