@@ -204,7 +204,7 @@ int mpb_cumsum_status(const void* scratch, mpb_stream_t stream);
  * has gate d / (D / H)), of x's type or MPB_F32; h0 (B, D) floats or NULL for
  * zero. mode MPB_SCAN_LINEAR: h[t] = g h[t-1] + x[t]; MPB_SCAN_SIGMOID:
  * h[t] = s h[t-1] + (1 - s) x[t], s = sigmoid(g). Linear gates may exceed one;
- * what shrinks below 2^-126 of itself within 128 steps may count as zero. Writes h (B, T, D) in x's
+ * what shrinks below 2^-126 of itself within 128 steps may be lost. Writes h (B, T, D) in x's
  * type and, when state is not NULL, h[T-1] (h0 when T == 0) in float; state
  * may not overlap h0. Scratch: mpb_gated_scan_scratch_bytes(..., backward = 0). */
 size_t mpb_gated_scan_scratch_bytes(int64_t B, int64_t T, int64_t D, int64_t H, int x_dtype, int gate_dtype,

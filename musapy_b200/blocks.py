@@ -170,8 +170,8 @@ def gated_scan(x, gate, h0=None, mode="linear", return_state=False, out=None):
     ``mode="linear"``: a = gate, b = x; ``mode="sigmoid"``: a = sigmoid(gate), b = (1 - a) x. x is (B, T, D) or
     (T, D); gate has x's shape, or one value for the D / H channels of each of H heads: (B, T, H). It has x's dtype or
     float32. h0, (B, D) float32 ((D,) for a 2-D x), is the state before the first step (zero when None). The state
-    runs in float32. Linear gates may exceed one; what shrinks below 2^-126 of itself within 128 steps may count as
-    zero. Returns h in x's dtype; with ``return_state`` also the last state in float32 (h0 or zeros when T is 0). A
+    runs in float32. Linear gates may exceed one; what shrinks below 2^-126 of itself within 128 steps may be
+    lost. Returns h in x's dtype; with ``return_state`` also the last state in float32 (h0 or zeros when T is 0). A
     zero gate drops a finite state: sequences packed along time restart where it is zero."""
     name = "gated_scan"
     m = _choice(name, "mode", mode, _MODES)

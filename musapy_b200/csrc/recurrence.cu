@@ -41,8 +41,10 @@
 // A product of decays (16 steps of a warp, or a look-back's tile) may leave the
 // range of float where the states do not. Above it, with linear gates beyond one,
 // the tile's warps run one after the other instead, each from the state that the
-// one before it ends with. Below it the product counts as zero: what is lost is
-// below 2^-126 of the state before.
+// one before it ends with (where that is every tile, (8, 4096, 2048) f32 forward
+// takes 332 us instead of 149, a gate per head of 64 in bf16 197 instead of 66, and
+// (1, 65536, 1000) f32 by look-back 3.5 ms instead of 239 us). Below it the product
+// is zero or a few bits: what is lost is below 2^-126 of the state before.
 //
 // Bound: memory by the bytes; what is reached is set by the latency of a tile
 // (its barrier, the maps' join, in a look-back two round trips to L2) at 16

@@ -180,6 +180,28 @@ def test_scan_with_gates_beyond_one_is_repeatable(ms, B, T, D):
         assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
 
 
+def test_scan_long_look_back_without_maps(ms):
+    """Every tile of a long sequence waits for the state of the one before it, and no wait gives up."""
+    T = 12000
+    gate, x = _swings(1, T, 5, 2.0 ** 20, 9, 1, False), rand(1, T, 5, seed=2) * 2.0 ** -100
+    A = ms.from_torch
+    from musapy_b200 import ops
+
+    ops.set_scan_status_check(True)
+    try:
+        h = ms.gated_scan(A(x), A(gate))
+        got = ms.gated_scan_backward(A(x), A(x), A(gate), h)
+        nan = ms.gated_scan(A(torch.full((1, 400000, 2), math.nan, device="cuda")), A(torch.ones(1, 400000, 2, device="cuda")))
+    finally:
+        ops.set_scan_status_check(False)
+    wh, _, eh, _ = P.scan(x.double(), gate.double(), None, "linear")
+    P.close(h.torch(), wh, eh)
+    want, err = P.scan_backward(x.double(), x.double(), gate.double(), h.torch().double(), None, None, "linear")
+    for g, w, e in zip(got, want, err):
+        P.close(g.torch(), w, e)
+    assert bool(nan.torch().isnan().all())
+
+
 @pytest.mark.parametrize("B,T,D", [(2, 300, 36), (4, 300, 900)])
 def test_scan_keeps_what_is_not_finite_in_its_channel(ms, B, T, D):
     """Linear: an infinite or NaN gate or input makes its channel what the formula makes it from that step on, up to
