@@ -114,18 +114,25 @@ def _dense(x: Array) -> bool:
 def _carve(s, dev: int, shape: tuple, nbytes: int, *kinds):
     """Several small results of one shape and nbytes of scratch in one allocation: an Array for each dtype, and the
     scratch's address. To the alias checks each is an allocation of its own (they do not overlap)."""
-    lay = _LAYOUTS.get(shape)
-    strides, n = lay[:2] if lay is not None else (contiguous_strides(shape), _prod(shape))
-    first = _new(s, (sum((n * d.itemsize + 15) & ~15 for d in kinds) + max(nbytes, 16),), _dt.uint8, dev)
-    made, at = [], 0
+    lay, tdev = _LAYOUTS.get(shape), _TORCH_DEVICES.get(dev)
+    strides, n = lay if lay is not None else (contiguous_strides(shape), _prod(shape))
+    total = max(nbytes, 16)
+    for d in kinds:
+        total += (n * d.itemsize + 15) & ~15
+    if tdev is not None:
+        buf = _empty(total, dtype=_U8, device=tdev)
+        buf._mpb_owner = s
+    else:
+        buf = _new(s, (total,), _dt.uint8, dev)._buf
+    base, made, at = buf.data_ptr(), [], 0
     for d in kinds:
         a = _new_array(Array)
-        a._buf, a._shape, a._strides, a._offset = first._buf, shape, strides, at // d.itemsize
-        a._dtype, a._dev, a._name, a._dev_src, a._dt_src = d, dev, None, first._dev_src, first._dt_src
-        a._ptr = a._sid = first._ptr + at
+        a._buf, a._shape, a._strides, a._offset, a._dtype, a._dev, a._name = buf, shape, strides, at // d.itemsize, d, dev, None
+        a._dev_src = a._dt_src = "input_array"
+        a._ptr = a._sid = base + at
         made.append(a)
         at += (n * d.itemsize + 15) & ~15
-    return made, first._ptr + at
+    return made, base + at
 
 
 # ------------------------------------------------------------ gated scan
