@@ -1,6 +1,6 @@
 """A small recurrent policy, sampled and trained with the block operators.
 
-Two blocks, each: input norm -> projection to a value, a forget gate and an output gate -> gated scan over time ->
+Token embedding, then two blocks, each: input norm -> projection to a value, a forget gate and an output gate -> gated scan over time ->
 projection back -> norm, gate, dropout and residual add, fused with the next block's input norm. Tokens are sampled one
 at a time from the running states (gated_scan_step), then the policy is trained on what it sampled (gated_scan,
 gated_residual_norm and their backward passes) with the clipped policy loss and its KL term. The matrix products and
@@ -55,7 +55,7 @@ def sample(p, start, generator):
     states = [ms.zeros((BATCH, DIM), "f32", "cuda:0") for _ in range(BLOCKS)]
     token, tokens, logps = start, [], []
     for _ in range(TIME):
-        x = arr(p["embed"][token])
+        x = ms.embedding(arr(p["embed"]), arr(token))
         u, _ = ms.rms_norm(x, arr(p["pre0"]))
         for i in range(BLOCKS):
             v, g, o = split(u.torch() @ p[f"in{i}"])
@@ -70,7 +70,7 @@ def sample(p, start, generator):
 
 def logits_of(p, fed, dropout=0.0, seed=0):
     """Logits (BATCH, TIME, VOCAB) of whole sequences, and what the backward pass needs."""
-    x = arr(p["embed"][fed])
+    x = ms.embedding(arr(p["embed"]), arr(fed))
     u, rstd0 = ms.rms_norm(x, arr(p["pre0"]))
     kept = [(x, rstd0)]
     for i in range(BLOCKS):
@@ -101,7 +101,7 @@ def gradients(p, fed, dlogits, u, kept, dropout, seed):
     x, rstd0 = kept[0]
     dx, dpre = ms.rms_norm_backward(arr(du), x, arr(p["pre0"]), rstd0, dy=dy)
     grads["pre0"] = dpre.torch()
-    grads["embed"] = torch.zeros_like(p["embed"]).index_add_(0, fed.reshape(-1), flat(dx.torch()))
+    grads["embed"] = ms.embedding_backward(dx, arr(fed), rows=VOCAB).torch()
     return grads
 
 

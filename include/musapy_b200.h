@@ -284,6 +284,73 @@ int mpb_policy_loss(int64_t N, int64_t V, const void* logits, int dtype, int64_t
                     float* logp, float* kl, void* clipped, void* dlogits, void* scratch, size_t scratch_bytes,
                     mpb_stream_t stream);
 
+/* ------------------------------------- recurrent language model operators */
+
+/* New too, with the conventions of the operators above. */
+
+/* Linear attention with a decay for each head. q and k are (B, T, Hq, DK) and v
+ * is (B, T, H, DV), Hq a divisor of H (head h has q and k of head h / (H / Hq)), in
+ * `dtype` with strides over sequences, steps and heads; log_decay is (B, T, H)
+ * floats with strides g_sb, g_st, g_sh (0 repeats it). From state0 (B, H, DK, DV)
+ * floats, NULL for zero:
+ *   S = e^log_decay S + k v',   o = scale S' q.
+ * Writes o (B, T, H, DV) and, when state is not NULL, the last S (state0 when T == 0); state may
+ * not overlap state0. A log-decay below -104 is a decay of zero: what came before has no part from there on.
+ * Channels per head: 1 to 256. Values are finite: one that is not may reach every result of its chunk of 64 steps
+ * and the later ones. */
+size_t mpb_linear_attention_scratch_bytes(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK, int64_t DV, int dtype,
+                                          int backward, int decay_by_head);
+int mpb_linear_attention(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK, int64_t DV, int dtype, const void* q,
+                         int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh,
+                         const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh, const float* log_decay, int64_t g_sb,
+                         int64_t g_st, int64_t g_sh, const float* state0, double scale, void* o, float* state, void* scratch,
+                         size_t scratch_bytes, mpb_stream_t stream);
+
+/* Gradients of mpb_linear_attention from dout (B, T, H, DV) and dstate (B, H, DK, DV) floats or NULL, that of the
+ * last state. Writes dq and dk (B, T, Hq, DK, summed over the heads that share one), dv (B, T, H, DV), dlog_decay
+ * (B, T, H) floats, or with decay_by_head (H) floats, summed over sequences and steps in a fixed order, and
+ * dstate0 (B, H, DK, DV) floats, which may not overlap dstate. */
+int mpb_linear_attention_backward(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK, int64_t DV, int dtype, const void* dout,
+                                  int64_t do_sb, int64_t do_st, int64_t do_sh, const void* q, int64_t q_sb, int64_t q_st,
+                                  int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v,
+                                  int64_t v_sb, int64_t v_st, int64_t v_sh, const float* log_decay, int64_t g_sb, int64_t g_st,
+                                  int64_t g_sh, const float* state0, const float* dstate, double scale, void* dq, void* dk,
+                                  void* dv, float* dlog_decay, int decay_by_head, float* dstate0, void* scratch,
+                                  size_t scratch_bytes, mpb_stream_t stream);
+
+/* One step of B running sequences: q and k (B, Hq, DK), v (B, H, DV), log_decay (B, H); updates state (B, H, DK, DV)
+ * floats, 16-byte aligned, in place and writes o (B, H, DV). */
+int mpb_linear_attention_step(int64_t B, int64_t H, int64_t Hq, int64_t DK, int64_t DV, int dtype, const void* q, int64_t q_sb,
+                              int64_t q_sh, const void* k, int64_t k_sb, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_sh,
+                              const float* log_decay, int64_t g_sb, int64_t g_sh, double scale, float* state, void* o,
+                              mpb_stream_t stream);
+
+/* Distillation from a teacher's top logits: N tokens of V logits (row stride l_sr) in `dtype`; ids (N, K) MPB_I32 or
+ * MPB_I64 places in the vocabulary and teacher (N, K) the teacher's logits there (MPB_F32, MPB_F16 or MPB_BF16),
+ * C-contiguous, K at most 1024. Per token kl = sum p (log p - log q), p the softmax of the K over the temperature
+ * (0.001 to 1000), q that of the V; loss = temperature^2 times the mean over the mask (N bytes or NULL). Writes kl
+ * (N floats), the loss and, when dlogits is not NULL, the gradient of grad_scale * loss (N, V) in `dtype`. Entries of
+ * -inf are left out whatever their id; a token without entries gives zeros, a place outside [0, V) or a NaN
+ * entry NaN, tokens outside the mask zeros whatever they hold. */
+size_t mpb_distill_loss_scratch_bytes(int64_t N);
+int mpb_distill_loss(int64_t N, int64_t V, int64_t K, const void* logits, int dtype, int64_t l_sr, const void* ids,
+                     int ids_dtype, const void* teacher, int teacher_dtype, const void* mask, double temperature,
+                     double grad_scale, float* loss, float* kl, void* dlogits, void* scratch, size_t scratch_bytes,
+                     mpb_stream_t stream);
+
+/* Rows of a table (V, D) in `dtype`, row stride t_sr, for N tokens (MPB_I32 or MPB_I64), times a scale, to out (N, D);
+ * a token outside [0, V) gives a row of NaN. */
+int mpb_embedding(int64_t N, int64_t V, int64_t D, const void* table, int dtype, int64_t t_sr, const void* tokens,
+                  int tokens_dtype, double scale, void* out, mpb_stream_t stream);
+
+/* The table's gradient from dout (N, D) in `dtype`, row stride d_sr: scale times the sum, in their order, of the rows
+ * whose token names a row, in float. Writes dtable (V, D) floats whole, or with `into` adds to it where tokens name a
+ * row. Tokens outside [0, V) have no part. */
+size_t mpb_embedding_backward_scratch_bytes(int64_t N, int64_t V, int64_t D, int into);
+int mpb_embedding_backward(int64_t N, int64_t V, int64_t D, const void* dout, int dtype, int64_t d_sr, const void* tokens,
+                           int tokens_dtype, double scale, int into, float* dtable, void* scratch, size_t scratch_bytes,
+                           mpb_stream_t stream);
+
 /* ---------------------------------------------------------------- creation */
 
 /* Fills `out` (n contiguous elements of `dtype`) with start + i*step, each

@@ -8,7 +8,9 @@ cumsum, ``Array.astype`` and the dunders, plus the array creation and view
 helpers those ops need. The operators of a recurrent block (blocks.py) come
 beside them: gated_scan, gated_scan_backward, gated_scan_step, rms_norm,
 rms_norm_backward, gated_residual_norm, gated_residual_norm_backward, dropout
-and policy_loss. Every op runs on the CUDA kernels of
+and policy_loss; and those of a recurrent language model (sequence.py):
+linear_attention, linear_attention_backward, linear_attention_step,
+distill_loss, embedding and embedding_backward. Every op runs on the CUDA kernels of
 ``_lib/libmusapy_b200.so``; there is no CPU execution path.
 """
 from . import dtypes as _dtype_mod
@@ -45,6 +47,15 @@ from .blocks import (
     policy_loss,
     rms_norm,
     rms_norm_backward,
+)
+from .sequence import (
+    DistillLoss,
+    distill_loss,
+    embedding,
+    embedding_backward,
+    linear_attention,
+    linear_attention_backward,
+    linear_attention_step,
 )
 from .dtypes import (
     Dtype,

@@ -22,8 +22,10 @@
 //   reduce(op, shape, strides, a, in_dtype, axes_mask, out, out_dtype,
 //          compute_dtype, nan_first_rule, scratch, scratch_bytes, stream)
 //   gated_scan, gated_scan_backward, gated_scan_step, gated_residual_norm,
-//   gated_residual_norm_backward, dropout, policy_loss: the arguments of the
-//   mpb_* function of that name, in its order; *_scratch_bytes -> bytes
+//   gated_residual_norm_backward, dropout, policy_loss, linear_attention,
+//   linear_attention_backward, linear_attention_step, distill_loss, embedding,
+//   embedding_backward: the arguments of the mpb_* function of that name, in
+//   its order; *_scratch_bytes -> bytes
 // Pointers and streams are ints (0 or None for none); a_strides / b_strides
 // may be None where the C-ABI accepts a null array.
 #define PY_SSIZE_T_CLEAN
@@ -374,6 +376,102 @@ PyObject* py_policy_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
                                          (size_t)v.bytes, (mpb_stream_t)v.stream));
 }
 
+PyObject* py_linear_attention_scratch_bytes(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 9, "linear_attention_scratch_bytes");
+  struct { int64_t B, T, H, Hq, DK, DV; int dt, back, by; } v{a.l(), a.l(), a.l(), a.l(), a.l(), a.l(), a.i(), a.i(), a.i()};
+  if (!a) return nullptr;
+  return PyLong_FromSize_t(mpb_linear_attention_scratch_bytes(v.B, v.T, v.H, v.Hq, v.DK, v.DV, v.dt, v.back, v.by));
+}
+
+PyObject* py_linear_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 30, "linear_attention");
+  struct {
+    int64_t B, T, H, Hq, DK, DV; int dt;
+    void* q; int64_t qb, qt, qh; void* k; int64_t kb, kt, kh; void* v; int64_t vb, vt, vh;
+    float* g; int64_t gb, gt, gh; float* s0; double scale; void* o; float* s; void* scratch; int64_t bytes; void* stream;
+  } v{a.l(), a.l(), a.l(), a.l(), a.l(), a.l(), a.i(), a.p(), a.l(), a.l(), a.l(), a.p(), a.l(), a.l(), a.l(), a.p(),
+      a.l(), a.l(), a.l(), a.p<float>(), a.l(), a.l(), a.l(), a.p<float>(), a.d(), a.p(), a.p<float>(), a.p(), a.l(), a.p()};
+  if (!a) return nullptr;
+  return PyLong_FromLong(mpb_linear_attention(v.B, v.T, v.H, v.Hq, v.DK, v.DV, v.dt, v.q, v.qb, v.qt, v.qh, v.k, v.kb, v.kt,
+                                              v.kh, v.v, v.vb, v.vt, v.vh, v.g, v.gb, v.gt, v.gh, v.s0, v.scale, v.o, v.s,
+                                              v.scratch, (size_t)v.bytes, (mpb_stream_t)v.stream));
+}
+
+PyObject* py_linear_attention_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 39, "linear_attention_backward");
+  struct {
+    int64_t B, T, H, Hq, DK, DV; int dt;
+    void* d; int64_t db, dst, dh; void* q; int64_t qb, qt, qh; void* k; int64_t kb, kt, kh; void* v; int64_t vb, vt, vh;
+    float* g; int64_t gb, gt, gh; float *s0, *ds; double scale; void *dq, *dk, *dv; float* dg; int by; float* ds0;
+    void* scratch; int64_t bytes; void* stream;
+  } v{a.l(), a.l(), a.l(), a.l(), a.l(), a.l(), a.i(), a.p(), a.l(), a.l(), a.l(), a.p(), a.l(), a.l(), a.l(), a.p(),
+      a.l(), a.l(), a.l(), a.p(), a.l(), a.l(), a.l(), a.p<float>(), a.l(), a.l(), a.l(), a.p<float>(), a.p<float>(), a.d(),
+      a.p(), a.p(), a.p(), a.p<float>(), a.i(), a.p<float>(), a.p(), a.l(), a.p()};
+  if (!a) return nullptr;
+  return PyLong_FromLong(mpb_linear_attention_backward(
+      v.B, v.T, v.H, v.Hq, v.DK, v.DV, v.dt, v.d, v.db, v.dst, v.dh, v.q, v.qb, v.qt, v.qh, v.k, v.kb, v.kt, v.kh, v.v, v.vb,
+      v.vt, v.vh, v.g, v.gb, v.gt, v.gh, v.s0, v.ds, v.scale, v.dq, v.dk, v.dv, v.dg, v.by, v.ds0, v.scratch, (size_t)v.bytes,
+      (mpb_stream_t)v.stream));
+}
+
+PyObject* py_linear_attention_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 22, "linear_attention_step");
+  struct {
+    int64_t B, H, Hq, DK, DV; int dt; void* q; int64_t qb, qh; void* k; int64_t kb, kh; void* v; int64_t vb, vh;
+    float* g; int64_t gb, gh; double scale; float* state; void *o, *stream;
+  } v{a.l(), a.l(), a.l(), a.l(), a.l(), a.i(), a.p(), a.l(), a.l(), a.p(), a.l(), a.l(), a.p(), a.l(), a.l(),
+      a.p<float>(), a.l(), a.l(), a.d(), a.p<float>(), a.p(), a.p()};
+  if (!a) return nullptr;
+  return PyLong_FromLong(mpb_linear_attention_step(v.B, v.H, v.Hq, v.DK, v.DV, v.dt, v.q, v.qb, v.qh, v.k, v.kb, v.kh, v.v,
+                                                   v.vb, v.vh, v.g, v.gb, v.gh, v.scale, v.state, v.o,
+                                                   (mpb_stream_t)v.stream));
+}
+
+PyObject* py_distill_loss_scratch_bytes(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 1, "distill_loss_scratch_bytes");
+  const int64_t N = a.l();
+  if (!a) return nullptr;
+  return PyLong_FromSize_t(mpb_distill_loss_scratch_bytes(N));
+}
+
+PyObject* py_distill_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 19, "distill_loss");
+  struct {
+    int64_t N, V, K; void* z; int dt; int64_t sr; void* ids; int idt; void* t; int tdt; void* mask; double tau, gs;
+    float *loss, *kl; void *grad, *scratch; int64_t bytes; void* stream;
+  } v{a.l(), a.l(), a.l(), a.p(), a.i(), a.l(), a.p(), a.i(), a.p(), a.i(), a.p(), a.d(), a.d(), a.p<float>(),
+      a.p<float>(), a.p(), a.p(), a.l(), a.p()};
+  if (!a) return nullptr;
+  return PyLong_FromLong(mpb_distill_loss(v.N, v.V, v.K, v.z, v.dt, v.sr, v.ids, v.idt, v.t, v.tdt, v.mask, v.tau, v.gs,
+                                          v.loss, v.kl, v.grad, v.scratch, (size_t)v.bytes, (mpb_stream_t)v.stream));
+}
+
+PyObject* py_embedding(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 11, "embedding");
+  struct { int64_t N, V, D; void* t; int dt; int64_t sr; void* ids; int idt; double scale; void *out, *stream; } v{
+      a.l(), a.l(), a.l(), a.p(), a.i(), a.l(), a.p(), a.i(), a.d(), a.p(), a.p()};
+  if (!a) return nullptr;
+  return PyLong_FromLong(mpb_embedding(v.N, v.V, v.D, v.t, v.dt, v.sr, v.ids, v.idt, v.scale, v.out, (mpb_stream_t)v.stream));
+}
+
+PyObject* py_embedding_backward_scratch_bytes(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 4, "embedding_backward_scratch_bytes");
+  struct { int64_t N, V, D; int into; } v{a.l(), a.l(), a.l(), a.i()};
+  if (!a) return nullptr;
+  return PyLong_FromSize_t(mpb_embedding_backward_scratch_bytes(v.N, v.V, v.D, v.into));
+}
+
+PyObject* py_embedding_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 14, "embedding_backward");
+  struct {
+    int64_t N, V, D; void* d; int dt; int64_t sr; void* ids; int idt; double scale; int into; float* table;
+    void* scratch; int64_t bytes; void* stream;
+  } v{a.l(), a.l(), a.l(), a.p(), a.i(), a.l(), a.p(), a.i(), a.d(), a.i(), a.p<float>(), a.p(), a.l(), a.p()};
+  if (!a) return nullptr;
+  return PyLong_FromLong(mpb_embedding_backward(v.N, v.V, v.D, v.d, v.dt, v.sr, v.ids, v.idt, v.scale, v.into, v.table,
+                                                v.scratch, (size_t)v.bytes, (mpb_stream_t)v.stream));
+}
+
 #define MPB_METHOD(name, doc) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, doc}
 
 PyMethodDef kMethods[] = {
@@ -394,6 +492,15 @@ PyMethodDef kMethods[] = {
     MPB_METHOD(dropout, "mpb_dropout"),
     MPB_METHOD(policy_loss, "mpb_policy_loss"),
     MPB_METHOD(policy_loss_scratch_bytes, "mpb_policy_loss_scratch_bytes"),
+    MPB_METHOD(linear_attention, "mpb_linear_attention"),
+    MPB_METHOD(linear_attention_backward, "mpb_linear_attention_backward"),
+    MPB_METHOD(linear_attention_step, "mpb_linear_attention_step"),
+    MPB_METHOD(linear_attention_scratch_bytes, "mpb_linear_attention_scratch_bytes"),
+    MPB_METHOD(distill_loss, "mpb_distill_loss"),
+    MPB_METHOD(distill_loss_scratch_bytes, "mpb_distill_loss_scratch_bytes"),
+    MPB_METHOD(embedding, "mpb_embedding"),
+    MPB_METHOD(embedding_backward, "mpb_embedding_backward"),
+    MPB_METHOD(embedding_backward_scratch_bytes, "mpb_embedding_backward_scratch_bytes"),
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -34,6 +34,7 @@
 #include "async_copy.cuh"
 #include "common.cuh"
 #include "internal.h"
+#include "logits.cuh"
 #include "musapy_b200.h"
 #include "rows.cuh"
 
@@ -87,31 +88,6 @@ MPB_D void token_terms(const PolicyArgs& p, const Token& token, float logp, floa
   }
 }
 
-// Tokens in the mask, the same value in every thread: counted before, or here,
-// 16 bytes at a time where the mask is aligned.
-MPB_D float tokens_in_mask(const PolicyArgs& p, float* red) {
-  if (!p.mask) return (float)p.N;
-  if (p.count) return *p.count;
-  int n = 0;
-  const int64_t words = (uintptr_t)p.mask % 16 == 0 ? p.N / 16 : 0;
-  auto set = [](uint32_t v) { return __popc((v | ((v & 0x7f7f7f7fu) + 0x7f7f7f7fu)) & 0x80808080u); };  // bytes that are not 0
-#pragma unroll 4
-  for (int64_t w = threadIdx.x; w < words; w += blockDim.x) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.mask) + w);
-    n += set(v.x) + set(v.y) + set(v.z) + set(v.w);
-  }
-  for (int64_t i = words * 16 + threadIdx.x; i < p.N; i += blockDim.x) n += p.mask[i] ? 1 : 0;
-  return block_sum((float)n, red);
-}
-
-MPB_D float block_max(float v, float* red) {
-  v = warp_max(v);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  const int lane = threadIdx.x & 31;
-  return warp_max(lane < (int)(blockDim.x >> 5) ? red[lane] : -INFINITY);
-}
-
 // A masked token: zeros.
 template <class T>
 MPB_D void write_masked(const PolicyArgs& p, int64_t i, int64_t from, int64_t to, int tid, int threads) {
@@ -135,100 +111,10 @@ MPB_D int64_t target_of(const PolicyArgs& p, int64_t i) {
   return p.targets64 ? ((const int64_t*)p.targets)[i] : ((const int32_t*)p.targets)[i];
 }
 
-// e^(z - base) of one value.
-MPB_D float exp_from(float z, float minus_base) { return ex2f((z + minus_base) * -kMinusLog2e); }
-
-// e^(z - base) of many. Near: 2^(z c + k) with c = log2 e and k = -base c, one
-// fused multiply-add each; k is rounded, which scales all of them alike, and
-// fix() is the factor that takes this out of them again. Far from zero, where
-// the rounding of k is no small number, the difference is taken first.
-constexpr float kNear = 65536.0f;  // k is off by at most 2^-8 below it
-template <bool NEAR>
-struct Exponent {
-  float base, k;
-  MPB_D explicit Exponent(float b) : base(b), k(b * kMinusLog2e) {}
-  MPB_D float fix() const { return NEAR ? ex2f(-fmaf(base, -kMinusLog2e, k)) : 1.0f; }
-  MPB_D float2 operator()(float2 z) const {
-    const float2 x = NEAR ? vfma(z, vset<2>(-kMinusLog2e), vset<2>(k))
-                          : vmul(vadd(z, vset<2>(-base)), vset<2>(-kMinusLog2e));
-    return make_float2(ex2f(x.x), ex2f(x.y));
-  }
-};
-// f with the form that goes with the base.
-template <class F>
-MPB_D void with_exponent(float base, F f) {
-  if (fabsf(base) <= kNear) f(Exponent<true>(base));
-  else f(Exponent<false>(base));
-}
-
-// 16 bytes of logits as pairs of floats.
-template <class T>
-struct Sixteen {
-  static constexpr int kElems = 16 / (int)sizeof(T), kPairs = kElems / 2;
-  union {
-    uint4 w;
-    T v[kElems];
-    typename Word<2 * sizeof(T)>::type pair[kPairs];
-  };
-  MPB_D explicit Sixteen(uint4 q) : w(q) {}
-  MPB_D float2 get(int i) const {
-    Pack<T, 2> p;
-    p.w = pair[i];
-    return unpack(p);
-  }
-  MPB_D void put(int i, float2 f) { pair[i] = pack<T>(f).w; }
-};
-
-// The pairwise larger of 16 bytes of elements, and the largest of them as float.
-template <class T>
-MPB_D uint4 larger(uint4 a, uint4 b) {
-  auto two = [](uint32_t x, uint32_t y) -> uint32_t {
-    if constexpr (std::is_same<T, float>::value) {
-      return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
-    } else if constexpr (std::is_same<T, __half>::value) {
-      const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&x), *reinterpret_cast<__half2*>(&y));
-      return *reinterpret_cast<const uint32_t*>(&m);
-    } else {
-      const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&x), *reinterpret_cast<__nv_bfloat162*>(&y));
-      return *reinterpret_cast<const uint32_t*>(&m);
-    }
-  };
-  return make_uint4(two(a.x, b.x), two(a.y, b.y), two(a.z, b.z), two(a.w, b.w));
-}
-template <class T>
-MPB_D float largest(uint4 a) {
-  const Sixteen<T> x(a);
-  float m = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < Sixteen<T>::kPairs; ++i) m = fmaxf(m, fmaxf(x.get(i).x, x.get(i).y));
-  return m;
-}
-// 16 bytes of -inf: in the place of words that a thread does not have.
-template <class T>
-MPB_D uint4 no_words() {
-  const uint32_t w = std::is_same<T, float>::value ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-  return make_uint4(w, w, w, w);
-}
-
-// The larger maximum, and the sum of exponentials taken from it. -inf with a
-// sum of zero is the empty set.
-struct Fold {
-  float top, sum;
-  MPB_D void join(float t, float s) {
-    const float m = fmaxf(top, t), b = m == -INFINITY ? 0.0f : m;
-    sum = sum * exp_from(top, -b) + s * exp_from(t, -b);
-    top = m;
-  }
-};
-
 constexpr int kRowThreads = 256;
 constexpr int kGroups = 4;  // in which a block's copies arrive
 constexpr int kBatch = 4;   // words a thread folds at once: one maximum, one rescaling of its sum
 constexpr int kMostBlocks = 8;
-
-MPB_D void copy_word16(uint32_t dst, const uint4* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 
 // Block `rank` of the row's cluster takes `per` 16-byte words of it. The
 // elements before the first aligned word and after the last, fewer than a word
@@ -289,7 +175,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_policy_row(PolicyArgs p, int
   }
   const bool valid = t >= 0 && t < p.V;
   const float zt = valid ? to_f(z[t]) : 0.0f;
-  const float count = p.grad ? tokens_in_mask(p, red[0]) : 1.0f;
+  const float count = p.grad ? tokens_in_mask(p.mask, p.N, p.count, red[0]) : 1.0f;
   auto fold_batch = [&](const uint4 (&v)[kBatch]) {
     uint4 most = v[0];
 #pragma unroll
@@ -400,7 +286,7 @@ __global__ void __launch_bounds__(kWarpRows * 32) k_policy_warp(PolicyArgs p) {
   constexpr int E = 16 / (int)sizeof(T);
   const int lane = threadIdx.x & 31;
   const int64_t i = (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5);
-  const float count = p.grad ? tokens_in_mask(p, red) : 1.0f;
+  const float count = p.grad ? tokens_in_mask(p.mask, p.N, p.count, red) : 1.0f;
   if (i >= p.N) return;
   const Token token(p, i);
   if (p.mask && !p.mask[i]) {
@@ -481,7 +367,7 @@ __global__ void __launch_bounds__(kThreads) k_policy_passes(PolicyArgs p) {
     write_masked<T>(p, i, 0, p.V, threadIdx.x, blockDim.x);
     return;
   }
-  const float count = tokens_in_mask(p, red[0]);
+  const float count = tokens_in_mask(p.mask, p.N, p.count, red[0]);
   float top = -INFINITY;
   for (int64_t j = threadIdx.x; j < p.V; j += kThreads) top = fmaxf(top, to_f(z[j]));
   top = block_max(top, red[1]);
@@ -512,7 +398,7 @@ __global__ void __launch_bounds__(kThreads) k_policy_passes(PolicyArgs p) {
 // The mean over the mask, in a fixed order.
 __global__ void __launch_bounds__(1024) k_policy_mean(PolicyArgs p) {
   __shared__ float red[2][32];
-  const float count = tokens_in_mask(p, red[0]);
+  const float count = tokens_in_mask(p.mask, p.N, p.count, red[0]);
   float v = 0.0f;
 #pragma unroll 4
   for (int64_t w = threadIdx.x; w < p.N / 4; w += 1024) {
@@ -527,7 +413,7 @@ __global__ void __launch_bounds__(1024) k_policy_mean(PolicyArgs p) {
 
 __global__ void __launch_bounds__(1024) k_policy_count(PolicyArgs p, float* count) {
   __shared__ float red[32];
-  const float n = tokens_in_mask(p, red);
+  const float n = tokens_in_mask(p.mask, p.N, p.count, red);
   if (threadIdx.x == 0) *count = n;
 }
 
