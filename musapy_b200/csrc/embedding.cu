@@ -11,8 +11,7 @@
 // the block that finishes last. A new table is written once, rows that no token names
 // as zeros; a gradient that is there already is added to, where tokens name it.
 //
-// Bound: memory. Up to kSmall tokens one block sorts them, in shared memory; more
-// are sorted by two kernels per digit.
+// Bound: memory. Up to kSmall tokens are sorted by one kernel, more by two for each digit.
 #include "common.cuh"
 #include "internal.h"
 #include "musapy_b200.h"
@@ -27,8 +26,8 @@ constexpr int kPart = 32;     // tokens of a row that are summed by one group of
 constexpr int kMostBits = 9;  // of a digit
 constexpr int kMostBins = 1 << kMostBits;
 constexpr int kTileTokens = 2048;
-constexpr int kSortThreads = 1024;
 constexpr int kSmall = 8192;
+constexpr int kSmallBytes = (kSmall + 32) * 8;
 
 MPB_D int64_t token_of(const void* tokens, int wide, int64_t n) {
   return wide ? ((const int64_t*)tokens)[n] : (int64_t)((const int32_t*)tokens)[n];
@@ -88,9 +87,15 @@ MPB_D int key_of(const Sorted& p, int64_t n) {
   return t >= 0 && t < p.V ? (int)t : p.V;
 }
 
-// Ranks of a warp's 32 keys of one digit among those before them in the warp; count: the warp's counters.
-MPB_D int warp_rank(uint16_t* count, int digit, bool on) {
-  const unsigned all = __ballot_sync(0xffffffffu, on), same = __match_any_sync(0xffffffffu, on ? digit : -1) & all;
+// Ranks of a warp's 32 keys of one digit among those before them in the warp; count: the warp's counters. Who has the
+// same digit is found by a vote for each of its bits (the instruction that matches whole words took 5 times as long).
+MPB_D int warp_rank(uint16_t* count, int digit, int bits, bool on) {
+  unsigned same = __ballot_sync(0xffffffffu, on);
+  for (int b = 0; b < bits; ++b) {
+    const bool set = digit >> b & 1;
+    const unsigned with = __ballot_sync(0xffffffffu, set);
+    same &= set ? with : ~with;
+  }
   const int lane = threadIdx.x & 31;
   int before = 0;
   if (on) before = count[digit];
@@ -124,74 +129,41 @@ MPB_D int block_scan(int v, int* red, int& total) {
   return before + x - v;
 }
 
-// At most kSmall tokens, by one block: each warp has a run of them, each thread eight.
-constexpr int kRounds = kSmall / kSortThreads;
-constexpr int kSortBytes = kSmall * 4 + kSmall * 2 + (kSortThreads / 32) * kMostBins * 2;
-
-__global__ void __launch_bounds__(kSortThreads) k_embed_sort(Sorted p, int bits, int passes) {
-  extern __shared__ __align__(16) int shared[];
-  __shared__ int red[32], base[kMostBins];
-  constexpr int kWarps = kSortThreads / 32;
-  int* keys = shared;
-  uint16_t* at = reinterpret_cast<uint16_t*>(keys + kSmall);
-  uint16_t* counts = at + kSmall;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = (int)p.N, bins = 1 << bits;
-  for (int64_t i = tid; i < p.n_counters; i += kSortThreads) p.counters[i] = 0;
-  int key[kRounds], from[kRounds], to[kRounds];
+// At most kSmall tokens: a token's place is the number of tokens that sort before it, counted against all of them: a
+// key and its index are one number, so that is a comparison for each. A block finds the places of 32 tokens, each of
+// its warps against an eighth of the keys; it takes all keys into shared memory. 4097 tokens: 6.1 us, where one
+// block sorting them by digits took 12.8. C: a number that holds key and index.
+template <class C>
+__global__ void __launch_bounds__(kThreads) k_embed_rank(Sorted p) {
+  extern __shared__ __align__(16) unsigned char shared[];
+  __shared__ int part[kThreads / 32][32];
+  C* all = reinterpret_cast<C*>(shared);
+  constexpr int kAtOnce = 16 / (int)sizeof(C), kWarps = kThreads / 32;
+  const int n = (int)p.N, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int run = ((n + kWarps - 1) / kWarps + kAtOnce - 1) / kAtOnce * kAtOnce;  // of keys, for a warp
+#pragma unroll 8
+  for (int i = tid; i < run * kWarps; i += kThreads) all[i] = i < n ? (C)key_of(p, i) * kSmall + i : ~(C)0;
+  if (blockIdx.x == 0)
+    for (int64_t i = tid; i < p.n_counters; i += kThreads) p.counters[i] = 0;
+  __syncthreads();
+  const int mine = blockIdx.x * 32 + lane;
+  const C own = mine < n ? all[mine] : 0;
+  int before = 0;
+  const uint4* w = reinterpret_cast<const uint4*>(all + warp * run);
+#pragma unroll 8
+  for (int i = 0; i < run / kAtOnce; ++i) {
+    union { uint4 q; C c[kAtOnce]; } x;
+    x.q = w[i];
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const int i = (warp * kRounds + r) * 32 + lane;
-    from[r] = i;
-    key[r] = i < n ? key_of(p, i) : 0;
+    for (int k = 0; k < kAtOnce; ++k) before += x.c[k] < own ? 1 : 0;
   }
-  for (int pass = 0; pass < passes; ++pass) {
-    for (int i = tid; i < kWarps * bins; i += kSortThreads) counts[i] = 0;
-    __syncthreads();
+  part[warp][lane] = before;
+  __syncthreads();
+  if (warp != 0 || mine >= n) return;
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      const int i = (warp * kRounds + r) * 32 + lane;
-      to[r] = warp_rank(counts + warp * bins, key[r] >> (pass * bits) & (bins - 1), i < n);
-    }
-    __syncthreads();
-    int total = 0, all;
-    if (tid < bins)
-      for (int w = 0; w < kWarps; ++w) {
-        const int c = counts[w * bins + tid];
-        counts[w * bins + tid] = (uint16_t)total;
-        total += c;
-      }
-    const int start = block_scan<kSortThreads>(total, red, all);
-    if (tid < bins) base[tid] = start;
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      const int i = (warp * kRounds + r) * 32 + lane;
-      if (i < n) {
-        const int digit = key[r] >> (pass * bits) & (bins - 1), o = to[r] + base[digit] + counts[warp * bins + digit];
-        keys[o] = key[r];
-        at[o] = (uint16_t)from[r];
-      }
-    }
-    __syncthreads();
-    if (pass + 1 < passes) {
-#pragma unroll
-      for (int r = 0; r < kRounds; ++r) {
-        const int i = (warp * kRounds + r) * 32 + lane;
-        key[r] = i < n ? keys[i] : 0;
-        from[r] = i < n ? at[i] : 0;
-      }
-      __syncthreads();
-    }
-  }
-  for (int i = tid; i < n; i += kSortThreads) {
-    const int k = keys[i];
-    p.keys[i] = k;
-    p.at[i] = at[i];
-    if (p.first && k < p.V) {
-      if (i == 0 || keys[i - 1] != k) p.first[k] = i;
-      if (i + 1 == n || keys[i + 1] != k) p.end[k] = i + 1;
-    }
-  }
+  for (int k = 1; k < kWarps; ++k) before += part[k][lane];
+  p.keys[before] = (int)(own / kSmall);
+  p.at[before] = mine;
 }
 
 // More tokens: a block per kTileTokens. The digits of a tile, counted; the first pass also clears what later kernels need.
@@ -201,8 +173,15 @@ __global__ void __launch_bounds__(kThreads) k_embed_count(Sorted p, const int* k
   for (int i = tid; i < bins; i += kThreads) bin[i] = 0;
   __syncthreads();
   const int64_t n0 = (int64_t)blockIdx.x * kTileTokens;
-  for (int i = tid; i < kTileTokens && n0 + i < p.N; i += kThreads)
-    atomicAdd(&bin[(keys ? keys[n0 + i] : key_of(p, n0 + i)) >> shift & (bins - 1)], 1);
+  int key[kTileTokens / kThreads];
+#pragma unroll
+  for (int k = 0; k < kTileTokens / kThreads; ++k) {
+    const int64_t i = n0 + tid + k * kThreads;
+    key[k] = i >= p.N ? -1 : keys ? keys[i] : key_of(p, i);
+  }
+#pragma unroll
+  for (int k = 0; k < kTileTokens / kThreads; ++k)
+    if (key[k] >= 0) atomicAdd(&bin[key[k] >> shift & (bins - 1)], 1);
   if (!keys) {
     const int64_t step = (int64_t)gridDim.x * kThreads, i0 = (int64_t)blockIdx.x * kThreads + tid;
     for (int64_t i = i0; i < p.n_counters; i += step) p.counters[i] = 0;
@@ -228,6 +207,7 @@ __global__ void __launch_bounds__(kThreads) k_embed_place(Sorted p, const int* k
     const int b = tid * (kMostBins / kThreads) + k;
     before[k] = total[k] = 0;
     if (b < bins)
+#pragma unroll 8
       for (unsigned t = 0; t < gridDim.x; ++t) {
         const int c = counts[(int64_t)t * bins + b];
         if (t < blockIdx.x) before[k] += c;
@@ -253,7 +233,7 @@ __global__ void __launch_bounds__(kThreads) k_embed_place(Sorted p, const int* k
 #pragma unroll
   for (int r = 0; r < kSteps; ++r) {
     const int64_t i = n0 + (warp * kSteps + r) * 32 + lane;
-    to[r] = warp_rank(mine + warp * bins, key[r] >> shift & (bins - 1), i < p.N);
+    to[r] = warp_rank(mine + warp * bins, key[r] >> shift & (bins - 1), bits, i < p.N);
   }
   __syncthreads();
   for (int b = tid; b < bins; b += kThreads) {
@@ -293,54 +273,79 @@ struct Sums {
   const int *keys, *at, *first, *end;
   float scale;
   float* table;
-  bool into;
+  bool add, by_list;  // to what is there; the rows are found as the lists' begins, not as all of the table's
   float* parts;   // sums of the parts of long lists, one row each
   int* counters;  // per place of a part and tile of columns: parts that are done
   int64_t part_blocks;
-  int tiles;      // of columns
+  int tiles;      // of columns, for a part
 };
 
-// acc += the E columns from `c` of the tokens sorted at [s, e), in their order.
+// kCols accesses of E columns, `lanes` apart from column word w on, summed over a list of tokens, in their
+// order (at: where the n of them stand); several rows are under way at once.
+constexpr int kCols = 4;
 template <class T, int E>
-MPB_D void sum_rows(const Sums& p, int s, int e, int64_t c, float (&acc)[E]) {
-  constexpr int kAhead = 8;
+MPB_D void sum_rows(const Sums& p, const int* at, int n, int64_t w, int lanes, float (&acc)[kCols][E]) {
+  constexpr int kAhead = E > 4 ? 2 : 4;
   using P = Pack<T, E>;
-  const T* x = (const T*)p.dout + c;
-  for (int i = s; i < e; i += kAhead) {
-    P v[kAhead];
+  const int64_t words = p.D / E;
+  const auto* x = reinterpret_cast<const typename P::W*>(p.dout);
+  const int64_t step = p.d_sr / E;
+#pragma unroll
+  for (int c = 0; c < kCols; ++c)
+#pragma unroll
+    for (int j = 0; j < E; ++j) acc[c][j] = 0.0f;
+  for (int i = 0; i < n; i += kAhead) {
+    P v[kAhead][kCols];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      if (i + k < e) v[k].w = *reinterpret_cast<const typename P::W*>(x + (int64_t)p.at[i + k] * p.d_sr);
+      if (i + k < n) {
+        const auto* row = x + (int64_t)at[i + k] * step;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+          if (w + c * lanes < words) v[k][c].w = row[w + c * lanes];
+      }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      if (i + k < e) {
+      if (i + k < n) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) acc[j] += to_f(v[k].v[j]);
+        for (int c = 0; c < kCols; ++c)
+#pragma unroll
+          for (int j = 0; j < E; ++j) acc[c][j] += to_f(v[k][c].v[j]);
       }
   }
 }
 
-template <int E>
-MPB_D void put_row(const Sums& p, int row, int64_t c, const float (&acc)[E]) {
-  float* to = p.table + (int64_t)row * p.D + c;
+// What the table's gradient holds already, or zeros.
+template <int E, bool ADD>
+MPB_D void old_row(const Sums& p, int row, int64_t c, float (&old)[E]) {
+  const float* from = p.table + (int64_t)row * p.D + c;
   if constexpr (E % 4 == 0) {
 #pragma unroll
     for (int j = 0; j < E; j += 4) {
-      float4 v = make_float4(acc[j] * p.scale, acc[j + 1] * p.scale, acc[j + 2] * p.scale, acc[j + 3] * p.scale);
-      float4* at = reinterpret_cast<float4*>(to + j);
-      if (p.into) {
-        const float4 o = *at;
-        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-      }
-      *at = v;
+      const float4 o = ADD ? *reinterpret_cast<const float4*>(from + j) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      old[j] = o.x, old[j + 1] = o.y, old[j + 2] = o.z, old[j + 3] = o.w;
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < E; ++j) to[j] = p.into ? to[j] + acc[j] * p.scale : acc[j] * p.scale;
+    for (int j = 0; j < E; ++j) old[j] = ADD ? from[j] : 0.0f;
+  }
+}
+template <int E, bool ADD>
+MPB_D void put_row(const Sums& p, int row, int64_t c, const float (&old)[E], const float (&acc)[E]) {
+  float* to = p.table + (int64_t)row * p.D + c;
+  float v[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) v[j] = ADD ? old[j] + acc[j] * p.scale : acc[j] * p.scale;
+  if constexpr (E % 4 == 0) {
+#pragma unroll
+    for (int j = 0; j < E; j += 4) *reinterpret_cast<float4*>(to + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j) to[j] = v[j];
   }
 }
 
-// The end of the list of row `key` that sorted place s belongs to, and its begin, looked for in growing steps.
+// The end of the list of row `key` that begins at s, looked for in growing steps.
 MPB_D int list_end(const Sums& p, int s, int key) {
   int64_t at = s, step = 1;  // keys[at] == key
   while (at + step < p.N && p.keys[at + step] == key) at += step, step <<= 1;
@@ -348,80 +353,101 @@ MPB_D int list_end(const Sums& p, int s, int key) {
     if (at + step < p.N && p.keys[at + step] == key) at += step;
   return (int)at + 1;
 }
-MPB_D int list_begin(const Sums& p, int s, int key) {
-  int64_t at = s, step = 1;
-  while (at - step >= 0 && p.keys[at - step] == key) at -= step, step <<= 1;
-  for (; step; step >>= 1)
-    if (at - step >= 0 && p.keys[at - step] == key) at -= step;
-  return (int)at;
+// How many places behind (way 1) or before (-1) sorted place s are of the same list: by the whole block, 256
+// places at a time, in growing steps where that is not the end of it.
+MPB_D int list_reach(const Sums& p, int s, int key, int way) {
+  auto same = [&](int64_t from, int64_t step) {
+    const int64_t i = s + way * (from + step * (threadIdx.x + 1));
+    return __syncthreads_count(i >= 0 && i < p.N && p.keys[i] == key);
+  };
+  int64_t step = 1;
+  int n;
+  while ((n = same(0, step)) == kThreads) step *= kThreads;
+  int64_t reach = n * step;
+  while (step > 1) {
+    step /= kThreads;
+    reach += same(reach, step) * step;
+  }
+  return (int)reach;
 }
 
 // Where the part that begins at sorted place i keeps its sum: a list longer than kPart begins, and one of its later parts
 // begins, at most once among kPart neighbouring places.
 MPB_D int64_t part_place(int i, bool begins) { return (int64_t)(i / kPart) * 2 + (begins ? 1 : 0); }
 
-// The first blocks take the parts of long lists, one each; the others the rows: of the whole table, or the lists' first
-// tokens. `lanes` threads (a power of two, a warp at least) take a tile of a row.
-template <class T, int E>
+// The first blocks take the parts of long lists, one tile of columns each; the others the rows: of the whole table, or
+// the lists' first tokens. `lanes` threads (a power of two, a warp at least) walk a row's columns.
+template <class T, int E, bool ADD>
 __global__ void __launch_bounds__(kThreads) k_embed_sums(Sums p, int lanes) {
+  const int64_t words = p.D / E;
+  float acc[kCols][E];
   if (blockIdx.x < p.part_blocks) {
     __shared__ bool last;
     const int tile = (int)(blockIdx.x % p.tiles);
     const int64_t place = blockIdx.x / p.tiles;
     const int w0 = (int)(place >> 1) * kPart, w1 = (int)min((int64_t)w0 + kPart, p.N), n = (int)p.N;
-    int i, key, s, e;
-    if (place & 1) {  // a long list that begins here reaches behind these places
-      if (w1 >= n) return;
-      key = p.keys[w1 - 1];
-      if (p.keys[w1] != key) return;
-      s = list_begin(p, w1 - 1, key);
-      if (s < w0) return;
-      i = s;
-    } else {  // the list that the first place is of
-      key = p.keys[w0];
-      s = list_begin(p, w0, key);
-      i = s + (w0 - s + kPart - 1) / kPart * kPart;
-      if (i == s || i >= w1 || p.keys[i] != key) return;
-    }
-    if (key >= p.V) return;
-    e = list_end(p, i, key);
+    // a long list that begins here reaches behind these places; the list that the first place is of
+    const bool begins = place & 1;
+    if (begins && w1 >= n) return;
+    const int key = p.keys[begins ? w1 - 1 : w0];
+    if (key >= p.V || (begins && p.keys[w1] != key)) return;
+    const int s = (begins ? w1 - 1 : w0) - list_reach(p, begins ? w1 - 1 : w0, key, -1);
+    const int i = begins ? s : s + (w0 - s + kPart - 1) / kPart * kPart;
+    if (begins ? s < w0 : i == s || i >= w1 || p.keys[i] != key) return;
+    const int e = i + 1 + list_reach(p, i, key, 1);
     if (e - s <= kPart) return;
-    const int64_t c0 = (int64_t)tile * kThreads * E, c = c0 + threadIdx.x * E;
-    const bool on = c < p.D;
-    float acc[E] = {};
-    if (on) {
-      sum_rows<T, E>(p, i, min(e, i + kPart), c, acc);
-      float* to = p.parts + place * p.D + c;
+    // each warp sums four of the part's rows, so that all of them are under way at once, and the warps' sums are added
+    // in their order
+    constexpr int kWarps = kThreads / 32, kEach = kPart / kWarps, kValues = 32 * kCols * E;
+    __shared__ int rows[kPart];
+    __shared__ float sums[kWarps][kValues];
+    const int have = min(e - i, kPart), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if ((int)threadIdx.x < have) rows[threadIdx.x] = p.at[i + threadIdx.x];
+    __syncthreads();
+    sum_rows<T, E>(p, rows + warp * kEach, min(have - warp * kEach, kEach), (int64_t)tile * 32 * kCols + lane, 32, acc);
 #pragma unroll
-      for (int j = 0; j < E; ++j) to[j] = acc[j];
-    }
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int j = 0; j < E; ++j) sums[warp][(c * E + j) * 32 + lane] = acc[c][j];
+    __syncthreads();
+    auto column = [&](int v) { return (((int64_t)tile * kCols + v / 32 / E) * 32 + v % 32) * E + v / 32 % E; };
+#pragma unroll
+    for (int v = threadIdx.x; v < kValues; v += kThreads)
+      if (column(v) < p.D) {
+        float x = sums[0][v];
+#pragma unroll
+        for (int k = 1; k < kWarps; ++k) x += sums[k][v];
+        p.parts[place * p.D + column(v)] = x;
+      }
     __threadfence();
     __syncthreads();
     const int parts = (e - s + kPart - 1) / kPart;
     if (threadIdx.x == 0) last = atomicAdd(&p.counters[part_place(s, true) / 2 * p.tiles + tile], 1) == parts - 1;
     __syncthreads();
-    if (!last || !on) return;
+    if (!last) return;
     __threadfence();
-#pragma unroll
-    for (int j = 0; j < E; ++j) acc[j] = 0.0f;
-#pragma unroll 4
-    for (int k = 0; k < parts; ++k) {
-      const float* from = p.parts + part_place(s + k * kPart, k == 0) * p.D + c;
-#pragma unroll
-      for (int j = 0; j < E; ++j) acc[j] += __ldcg(from + j);
+    for (int v = threadIdx.x; v < kValues; v += kThreads) {
+      const int64_t c = column(v);
+      if (c >= p.D) continue;
+      float* to = p.table + (int64_t)key * p.D + c;
+      const float old = ADD ? *to : 0.0f;
+      float x = 0.0f;
+#pragma unroll 8
+      for (int k = 0; k < parts; ++k) x += __ldcg(p.parts + part_place(s + k * kPart, k == 0) * p.D + c);
+      *to = ADD ? old + x * p.scale : x * p.scale;
     }
-    put_row<E>(p, key, c, acc);
     return;
   }
-  const int64_t block = blockIdx.x - p.part_blocks, item = block / p.tiles * (kThreads / lanes) + threadIdx.x / lanes;
-  const int tile = (int)(block % p.tiles);
+  const int64_t item = (blockIdx.x - p.part_blocks) * (kThreads / lanes) + threadIdx.x / lanes;
   int row, s, e;
-  if (p.into) {
+  if (p.by_list) {
     if (item >= p.N) return;
     s = (int)item;
     row = p.keys[s];
-    if (row >= p.V || (s > 0 && p.keys[s - 1] == row)) return;
-    e = list_end(p, s, row);
+    const int before = s > 0 ? p.keys[s - 1] : -1, after = s + 1 < p.N ? p.keys[s + 1] : -1;
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(p.at + s));
+    if (row >= p.V || before == row) return;
+    e = after == row ? list_end(p, s + 1, row) : s + 1;
   } else {
     if (item >= p.V) return;
     row = (int)item;
@@ -429,11 +455,16 @@ __global__ void __launch_bounds__(kThreads) k_embed_sums(Sums p, int lanes) {
     e = p.end[row];
   }
   if (e - s > kPart) return;
-  const int64_t c = ((int64_t)tile * lanes + (threadIdx.x & (lanes - 1))) * E;
-  if (c >= p.D) return;
-  float acc[E] = {};
-  sum_rows<T, E>(p, s, e, c, acc);
-  put_row<E>(p, row, c, acc);
+  for (int64_t w = threadIdx.x & (lanes - 1); w < words; w += (int64_t)kCols * lanes) {
+    float old[kCols][E];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+      if (w + c * lanes < words) old_row<E, ADD>(p, row, (w + c * lanes) * E, old[c]);
+    sum_rows<T, E>(p, p.at + s, e - s, w, lanes, acc);
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+      if (w + c * lanes < words) put_row<E, ADD>(p, row, (w + c * lanes) * E, old[c], acc[c]);
+  }
 }
 
 // ------------------------------------------------------------------- host
@@ -471,14 +502,14 @@ size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 struct Scratch {
   size_t keys, at, keys2, at2, counts, first, end, counters, parts, bytes;
   int64_t n_counters;
-  Scratch(int64_t N, int64_t V, int64_t D, bool into) {
+  Scratch(int64_t N, int64_t V, int64_t D, bool by_list) {
     const size_t n = round16((size_t)N * 4);
-    const int64_t windows = (N + kPart - 1) / kPart, col_tiles = (D + kThreads - 1) / kThreads;
+    const int64_t windows = (N + kPart - 1) / kPart, col_tiles = (D + 127) / 128;  // at most: a tile has 128 columns and more
     const bool small = N <= kSmall;
     keys = 0, at = n, keys2 = 2 * n, at2 = keys2 + (small ? 0 : n), counts = at2 + (small ? 0 : n);
     first = counts + (small ? 0 : round16((size_t)((N + kTileTokens - 1) / kTileTokens) * kMostBins * 4));
-    end = first + (into ? 0 : round16((size_t)V * 4));
-    counters = end + (into ? 0 : round16((size_t)V * 4));
+    end = first + (by_list ? 0 : round16((size_t)V * 4));
+    counters = end + (by_list ? 0 : round16((size_t)V * 4));
     n_counters = windows * col_tiles;
     parts = counters + round16((size_t)n_counters * 4);
     bytes = parts + (N > kPart ? (size_t)windows * 2 * D * 4 : 0);
@@ -486,14 +517,23 @@ struct Scratch {
 };
 
 int sort_tokens(Sorted& p, char* scratch, const Scratch& w, cudaStream_t s) {
-  const Digits g(p.V);
   if (p.N <= kSmall) {
-    if (p.first)
-      if (int rc = cuda_check(cudaMemsetAsync(p.first, 0, w.counters - w.first, s), "embedding_backward")) return rc;
-    if (int rc = allow_smem<k_embed_sort, kSortBytes>("embedding_backward")) return rc;
-    k_embed_sort<<<1, kSortThreads, kSortBytes, s>>>(p, g.bits, g.passes);
+    const unsigned blocks = (unsigned)((p.N + 31) / 32);
+    const int64_t most = (p.N + 31) / 32 * 32 + 32;  // keys with what fills up the warps' runs
+    if ((int64_t)(p.V + 1) * kSmall <= 0xffffffffLL) {
+      if (int rc = allow_smem<k_embed_rank<uint32_t>, kSmallBytes>("embedding_backward")) return rc;
+      k_embed_rank<uint32_t><<<blocks, kThreads, (size_t)most * 4, s>>>(p);
+    } else {
+      if (int rc = allow_smem<k_embed_rank<uint64_t>, kSmallBytes>("embedding_backward")) return rc;
+      k_embed_rank<uint64_t><<<blocks, kThreads, (size_t)most * 8, s>>>(p);
+    }
+    if (int rc = launch_check("embedding_backward")) return rc;
+    if (!p.first) return MPB_OK;
+    if (int rc = cuda_check(cudaMemsetAsync(p.first, 0, w.counters - w.first, s), "embedding_backward")) return rc;
+    k_embed_ends<<<(unsigned)((p.N + kThreads - 1) / kThreads), kThreads, 0, s>>>(p);
     return launch_check("embedding_backward");
   }
+  const Digits g(p.V);
   int *a_keys = p.keys, *a_at = p.at, *b_keys = (int*)(scratch + w.keys2), *b_at = (int*)(scratch + w.at2);
   const unsigned tiles = (unsigned)((p.N + kTileTokens - 1) / kTileTokens);
   int* counts = (int*)(scratch + w.counts);
@@ -512,15 +552,15 @@ int sort_tokens(Sorted& p, char* scratch, const Scratch& w, cudaStream_t s) {
 
 template <class T, int E>
 int launch_sums(Sums& p, cudaStream_t s) {
-  const int64_t words = (p.D + E - 1) / E;
-  const int lanes = lanes_for(words, 32);  // fewer than a block's only where they cover the row
-  p.tiles = (int)((words + kThreads - 1) / kThreads);
+  const int64_t words = p.D / E;
+  const int lanes = lanes_for((words + kCols - 1) / kCols, 32);
+  p.tiles = (int)((words + kCols * 32 - 1) / (kCols * 32));
   p.part_blocks = p.N > kPart ? (p.N + kPart - 1) / kPart * 2 * p.tiles : 0;
-  const int64_t items = p.into ? p.N : p.V, groups = kThreads / lanes;
-  const int64_t blocks = p.part_blocks + (items + groups - 1) / groups * p.tiles;
+  const int64_t items = p.by_list ? p.N : p.V, groups = kThreads / lanes;
+  const int64_t blocks = p.part_blocks + (items + groups - 1) / groups;
   if (blocks > 0x7fffffffLL) return fail(MPB_ERR_SHAPE, "embedding_backward: %lld blocks are too many for one call", (long long)blocks);
-  if (blocks == 0) return MPB_OK;
-  k_embed_sums<T, E><<<(unsigned)blocks, kThreads, 0, s>>>(p, lanes);
+  if (p.add) k_embed_sums<T, E, true><<<(unsigned)blocks, kThreads, 0, s>>>(p, lanes);
+  else k_embed_sums<T, E, false><<<(unsigned)blocks, kThreads, 0, s>>>(p, lanes);
   return launch_check("embedding_backward");
 }
 
@@ -530,6 +570,10 @@ int launch_gradient(Sums& p, cudaStream_t s) {
   const bool wide = ((uintptr_t)p.dout | (uintptr_t)p.table) % 16 == 0 && p.D % E == 0 && p.d_sr % E == 0;
   return wide ? launch_sums<T, E>(p, s) : launch_sums<T, 1>(p, s);
 }
+
+// A new table of more rows than tokens name is cleared first, and written again where tokens name it: half as many
+// tokens as rows at most write half of it twice. Of more tokens each row's list is looked up and written once.
+bool by_list(int64_t N, int64_t V, bool into) { return into || N <= V / 2; }
 
 }  // namespace
 }  // namespace mpb
@@ -558,7 +602,7 @@ int mpb_embedding(int64_t N, int64_t V, int64_t D, const void* table, int dtype,
 }
 
 size_t mpb_embedding_backward_scratch_bytes(int64_t N, int64_t V, int64_t D, int into) {
-  return N > 0 && V > 0 && D > 0 ? Scratch(N, V, D, into != 0).bytes : 0;
+  return N > 0 && V > 0 && D > 0 ? Scratch(N, V, D, by_list(N, V, into != 0)).bytes : 0;
 }
 
 int mpb_embedding_backward(int64_t N, int64_t V, int64_t D, const void* dout, int dtype, int64_t d_sr, const void* tokens,
@@ -576,16 +620,19 @@ int mpb_embedding_backward(int64_t N, int64_t V, int64_t D, const void* dout, in
   cudaStream_t s = (cudaStream_t)stream;
   if (!dtable || (N > 0 && (!dout || !tokens))) return fail(MPB_ERR_INVALID, "%s: null pointer", name);
   if (N == 0) return into ? MPB_OK : cuda_check(cudaMemsetAsync(dtable, 0, (size_t)V * D * 4, s), name);
-  const Scratch w(N, V, D, into != 0);
+  const bool listed = by_list(N, V, into != 0);
+  const Scratch w(N, V, D, listed);
   if (w.bytes > scratch_bytes || !scratch)
     return fail(MPB_ERR_SCRATCH, "%s: %zu bytes of scratch, %zu needed", name, scratch_bytes, w.bytes);
   if ((uintptr_t)scratch % 16 != 0) return fail(MPB_ERR_INVALID, "%s: scratch not 16-byte aligned", name);
   char* at = (char*)scratch;
   Sorted o = {N, (int)V, tokens, tokens_dtype == MPB_I64, (int*)(at + w.keys), (int*)(at + w.at),
-              into ? nullptr : (int*)(at + w.first), into ? nullptr : (int*)(at + w.end), (int*)(at + w.counters), w.n_counters};
+              listed ? nullptr : (int*)(at + w.first), listed ? nullptr : (int*)(at + w.end), (int*)(at + w.counters), w.n_counters};
+  if (listed && !into)
+    if (int rc = cuda_check(cudaMemsetAsync(dtable, 0, (size_t)V * D * 4, s), name)) return rc;
   if (int rc = sort_tokens(o, at, w, s)) return rc;
-  Sums p = {N, D, (int)V, dout, d_sr, o.keys, o.at, o.first, o.end, (float)scale, dtable, into != 0, (float*)(at + w.parts),
-            o.counters, 0, 1};
+  Sums p = {N, D, (int)V, dout, d_sr, o.keys, o.at, o.first, o.end, (float)scale, dtable, into != 0, listed,
+            (float*)(at + w.parts), o.counters, 0, 1};
   switch (dtype) {
     case MPB_F32: return launch_gradient<float>(p, s);
     case MPB_F16: return launch_gradient<__half>(p, s);
