@@ -296,15 +296,20 @@ int mpb_policy_loss(int64_t N, int64_t V, const void* logits, int dtype, int64_t
  *   S = e^log_decay S + k v',   o = scale S' q.
  * Writes o (B, T, H, DV) and, when state is not NULL, the last S (state0 when T == 0); state may
  * not overlap state0. A log-decay below -104 is a decay of zero: what came before has no part from there on.
- * Channels per head: 1 to 256. Values are finite: one that is not may reach every result of its chunk of 64 steps
+ * Channels per head: 1 to 256. Scratch: mpb_linear_attention_scratch_bytes; it is less where `aligned` says that q, k, v (and
+ * dout) are 16-byte aligned with strides that are positive multiples of 16 bytes, and has to be asked for so or not as the call's are. Values are finite: one that is not may reach every result of its chunk of 64 steps
  * and the later ones. */
 size_t mpb_linear_attention_scratch_bytes(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK, int64_t DV, int dtype,
-                                          int backward, int decay_by_head);
+                                          int backward, int decay_by_head, int aligned);
 int mpb_linear_attention(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK, int64_t DV, int dtype, const void* q,
                          int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh,
                          const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh, const float* log_decay, int64_t g_sb,
                          int64_t g_st, int64_t g_sh, const float* state0, double scale, void* o, float* state, void* scratch,
                          size_t scratch_bytes, mpb_stream_t stream);
+
+/* Synchronises `stream` and reads the status word that a call left in its scratch (NULL: it had none): MPB_OK, or
+ * MPB_ERR_TIMEOUT when a bounded wait between the warps of a block gave up (its results are incomplete). */
+int mpb_linear_attention_status(const void* scratch, mpb_stream_t stream);
 
 /* Gradients of mpb_linear_attention from dout (B, T, H, DV) and dstate (B, H, DK, DV) floats or NULL, that of the
  * last state. Writes dq and dk (B, T, Hq, DK, summed over the heads that share one), dv (B, T, H, DV), dlog_decay

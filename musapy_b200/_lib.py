@@ -99,6 +99,8 @@ def _load() -> ctypes.CDLL:
     L.mpb_cumsum_status.argtypes = [c_vp, c_vp]
     L.mpb_gated_scan_status.restype = ctypes.c_int
     L.mpb_gated_scan_status.argtypes = [c_vp, c_vp]
+    L.mpb_linear_attention_status.restype = ctypes.c_int
+    L.mpb_linear_attention_status.argtypes = [c_vp, c_vp]
     L.mpb_launch_count.restype = ctypes.c_ulonglong
     L.mpb_launch_count.argtypes = []
     L.mpb_shard_arg_combine.restype = ctypes.c_int

@@ -218,24 +218,6 @@ MPB_D void write_tile(O* dst, int64_t step, int rows, int cols, float (&acc)[8][
 }
 
 // ------------------------------------------------------------- states
-struct Shape {
-  int64_t B, T;
-  int H, share, DK, DV;      // share: heads that share one of q and k
-  int chunks, segments, per;  // per: chunks of a segment
-  int dkp, dvp;               // channels in the scratch, multiples of 16
-};
-struct Input {
-  const void* p;
-  int64_t sb, st, sh;
-  bool wide;  // 16-byte loads
-  template <class T>
-  MPB_D const T* at(int64_t b, int64_t t, int h) const { return (const T*)p + b * sb + t * st + h * sh; }
-};
-struct Decay {
-  const float* p;
-  int64_t sb, st, sh;
-};
-
 // The states at the chunks' borders: before each chunk (REV: behind each, of the gradient), as sums over the chunk's
 // segment alone; `first` is what the first segment begins with. One block has 64 x 64 of a head's state in registers
 // and walks a segment's chunks. since: the decay from the segment's begin to each chunk, ends: the segments' sums.
@@ -735,42 +717,78 @@ Shape make_shape(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK, int64_
   return d;
 }
 
-// The scratch of one direction's states.
+// The scratch of one direction's states: without `kept`, those of the segments alone.
 struct StateScratch {
   size_t at, since, ends, bytes;
-  explicit StateScratch(const Shape& d, size_t from) {
+  StateScratch(const Shape& d, size_t from, bool kept) {
     const size_t bh = (size_t)d.B * d.H, size = (size_t)d.dkp * d.dvp * 4;
     at = from;
-    since = at + bh * d.chunks * size;
+    since = at + (kept ? bh * d.chunks * size : 0);
     ends = since + round16(bh * d.chunks * 2 * 4);
     bytes = ends + (d.segments > 1 ? bh * d.segments * size : 0);
   }
 };
+constexpr size_t kStatusBytes = 16;  // the status word leads the scratch
 
-Input make_input(const void* p, int64_t sb, int64_t st, int64_t sh, size_t e) {
-  const bool wide = (uintptr_t)p % 16 == 0 && (sb * (int64_t)e) % 16 == 0 && (st * (int64_t)e) % 16 == 0 && (sh * (int64_t)e) % 16 == 0;
-  return {p, sb, st, sh, wide};
+// Whether the walk of whole rows may be taken, as far as the layout does not decide.
+bool may_walk(int dtype, int64_t DK, int64_t DV, bool aligned) { return aligned && dtype == MPB_BF16 && DK <= 128 && DV <= 128; }
+
+// The walk's segments: as many as give every SM a block. They cost a walk more over k and v.
+Shape walk_shape(Shape d) {
+  const int64_t heads = d.B * d.H;
+  int64_t want = heads > 0 ? 148 / heads : 1, most = d.chunks / 4;
+  if (want > most) want = most;
+  d.per = want > 1 ? (int)((d.chunks + want - 1) / want) : d.chunks;
+  d.segments = d.per > 0 ? (d.chunks + d.per - 1) / d.per : 1;
+  return d;
 }
 
-template <class T, bool REV>
-int run_states(States p, cudaStream_t s) {
-  constexpr int kStatesBytes = (kExact + RawPieces<T>::n) * kPlane * 2;
+Input make_input(const void* p, int64_t sb, int64_t st, int64_t sh, size_t e) {
+  return {p, sb, st, sh, (uintptr_t)p % 16 == 0 && (sb * (int64_t)e) % 16 == 0 && (st * (int64_t)e) % 16 == 0 && (sh * (int64_t)e) % 16 == 0};
+}
+
+int join_states(const States& p, bool rev, cudaStream_t s) {
   const Shape& d = p.d;
-  const int64_t tiles = (int64_t)((d.dkp + kTile - 1) / kTile) * ((d.dvp + kTile - 1) / kTile);
-  if (int rc = allow_smem<k_la_states<T, REV>, kStatesBytes>("linear_attention")) return rc;
-  k_la_states<T, REV><<<(unsigned)(d.B * d.H * d.segments * tiles), kThreads, kStatesBytes, s>>>(p);
-  if (int rc = launch_check("linear_attention")) return rc;
   if (d.segments == 1) return MPB_OK;
-  k_la_join<REV><<<(unsigned)((d.B * d.H * d.dkp * d.dvp + 255) / 256), 256, 0, s>>>(p);
+  const unsigned blocks = (unsigned)((d.B * d.H * d.dkp * d.dvp + 255) / 256);
+  if (rev) k_la_join<true><<<blocks, 256, 0, s>>>(p);
+  else k_la_join<false><<<blocks, 256, 0, s>>>(p);
   return launch_check("linear_attention");
 }
 
+// The states of p's chunks (p.at null: of its segments alone).
+template <class T, bool REV>
+int run_states(const States& p, bool walk, int* status, cudaStream_t s) {
+  constexpr int kStatesBytes = (kExact + RawPieces<T>::n) * kPlane * 2;
+  const Shape& d = p.d;
+  if (walk) {
+    const Walk w = {d, {}, p.x, p.y, p.g, p.first, nullptr, p.scale, nullptr, REV, p.at, p.since, p.ends, p.last, status};
+    if (int rc = walk_states(w, s)) return rc;
+  } else {
+    const int64_t tiles = (int64_t)((d.dkp + kTile - 1) / kTile) * ((d.dvp + kTile - 1) / kTile);
+    if (int rc = allow_smem<k_la_states<T, REV>, kStatesBytes>("linear_attention")) return rc;
+    k_la_states<T, REV><<<(unsigned)(d.B * d.H * d.segments * tiles), kThreads, kStatesBytes, s>>>(p);
+    if (int rc = launch_check("linear_attention")) return rc;
+  }
+  return join_states(p, REV, s);
+}
+
 template <class T>
-int run_forward(const Shape& d, const Input& q, const Input& k, const Input& v, const Decay& g, const float* first, float scale,
-                void* o, float* state, char* scratch, cudaStream_t s) {
-  const StateScratch w(d, 0);
-  States st = {d, k, v, g, first, 1.0f, (float*)(scratch + w.at), (float*)(scratch + w.since), (float*)(scratch + w.ends), state};
-  if (int rc = run_states<T, false>(st, s)) return rc;
+int run_forward(Shape d, const Input& q, const Input& k, const Input& v, const Decay& g, const float* first, float scale,
+                void* o, float* state, bool walk, char* scratch, cudaStream_t s) {
+  int* status = (int*)scratch;
+  if (walk) d = walk_shape(d);
+  const StateScratch w(d, kStatusBytes, !walk);
+  States st = {d, k, v, g, first, 1.0f, walk ? nullptr : (float*)(scratch + w.at), (float*)(scratch + w.since),
+               (float*)(scratch + w.ends), state};
+  if (walk) {
+    if (int rc = cuda_check(cudaMemsetAsync(status, 0, kStatusBytes, s), "linear_attention")) return rc;
+    if (d.segments > 1)
+      if (int rc = run_states<T, false>(st, true, status, s)) return rc;
+    const Walk p = {d, q, k, v, g, first, st.ends, scale, o, false, nullptr, nullptr, nullptr, d.segments > 1 ? nullptr : state, status};
+    return walk_outputs(p, s);
+  }
+  if (int rc = run_states<T, false>(st, false, status, s)) return rc;
   constexpr int PT = RawPieces<T>::n, PS = Keep<T>::S;
   constexpr int kOutputBytes = (2 * PT + (PT > PS ? PT : PS)) * kPlane * 2;
   Outputs out = {d, q, k, v, g, scale, {st.at, st.since, st.ends}, o};
@@ -783,9 +801,9 @@ int run_forward(const Shape& d, const Input& q, const Input& k, const Input& v, 
 struct GradScratch {
   size_t s, u, dq, dk, dg, bytes;
   GradScratch(const Shape& d, bool by_head) {
-    const StateScratch a(d, 0), b(d, a.bytes);
+    const StateScratch a(d, kStatusBytes, true), b(d, a.bytes, true);
     const size_t part = d.share > 1 ? (size_t)d.B * d.T * d.H * d.DK * 4 : 0;
-    s = 0, u = a.bytes, dq = round16(b.bytes), dk = dq + round16(part), dg = dk + round16(part);
+    s = kStatusBytes, u = a.bytes, dq = round16(b.bytes), dk = dq + round16(part), dg = dk + round16(part);
     bytes = dg + (by_head ? round16((size_t)d.B * d.chunks * d.H * 4) : 0);
   }
 };
@@ -800,15 +818,19 @@ int run_gradients(const Gradients& p, cudaStream_t s) {
 
 template <class T>
 int run_backward(Gradients p, const float* first, const float* dstate, void* dq, void* dk, float* dg, bool by_head, float* dfirst,
-                 char* scratch, cudaStream_t s) {
+                 bool walk, char* scratch, cudaStream_t s) {
+  if (walk) p.d = walk_shape(p.d);
   const Shape& d = p.d;
   const GradScratch w(d, by_head);
-  const StateScratch a(d, w.s), b(d, w.u);
+  const StateScratch a(d, w.s, true), b(d, w.u, true);
+  int* status = (int*)scratch;
+  if (walk)
+    if (int rc = cuda_check(cudaMemsetAsync(status, 0, kStatusBytes, s), "linear_attention_backward")) return rc;
   States st = {d, p.k, p.v, p.g, first, 1.0f, (float*)(scratch + a.at), (float*)(scratch + a.since), (float*)(scratch + a.ends), nullptr};
-  if (int rc = run_states<T, false>(st, s)) return rc;
+  if (int rc = run_states<T, false>(st, walk, status, s)) return rc;
   States ut = {d, p.q, p.g_o, p.g, dstate, p.scale, (float*)(scratch + b.at), (float*)(scratch + b.since), (float*)(scratch + b.ends),
                dfirst};
-  if (int rc = run_states<T, true>(ut, s)) return rc;
+  if (int rc = run_states<T, true>(ut, walk, status, s)) return rc;
   p.s = {st.at, st.since, st.ends}, p.u = {ut.at, ut.since, ut.ends};
   p.dg = by_head ? nullptr : dg, p.dg_chunk = by_head ? (float*)(scratch + w.dg) : nullptr;
   if (d.share > 1) {
@@ -869,10 +891,21 @@ using namespace mpb;
 extern "C" {
 
 size_t mpb_linear_attention_scratch_bytes(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK, int64_t DV, int dtype,
-                                          int backward, int decay_by_head) {
+                                          int backward, int decay_by_head, int aligned) {
   if (check_shape("linear_attention", B, T, H, Hq, DK, DV, dtype) || B * T == 0) return 0;
-  const Shape d = make_shape(B, T, H, Hq, DK, DV);
-  return backward ? GradScratch(d, decay_by_head != 0).bytes : StateScratch(d, 0).bytes;
+  Shape d = make_shape(B, T, H, Hq, DK, DV);
+  const bool walk = may_walk(dtype, DK, DV, aligned != 0);
+  if (walk) d = walk_shape(d);
+  return backward ? GradScratch(d, decay_by_head != 0).bytes : StateScratch(d, kStatusBytes, !walk).bytes;
+}
+
+int mpb_linear_attention_status(const void* scratch, mpb_stream_t stream) {
+  if (!scratch) return MPB_OK;
+  int status = MPB_OK;
+  if (int rc = cuda_check(cudaMemcpyAsync(&status, scratch, sizeof(int), cudaMemcpyDeviceToHost, (cudaStream_t)stream), "linear_attention"))
+    return rc;
+  if (int rc = cuda_check(cudaStreamSynchronize((cudaStream_t)stream), "linear_attention")) return rc;
+  return status == MPB_ERR_TIMEOUT ? fail(MPB_ERR_TIMEOUT, "linear_attention: a wait between its warps gave up") : MPB_OK;
 }
 
 int mpb_linear_attention(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK, int64_t DV, int dtype, const void* q,
@@ -891,16 +924,17 @@ int mpb_linear_attention(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK
     return cuda_check(cudaMemsetAsync(state, 0, state_bytes, s), name);
   }
   if (!q || !k || !v || !log_decay || !o) return fail(MPB_ERR_INVALID, "%s: null pointer", name);
-  if (int rc = check_scratch(name, mpb_linear_attention_scratch_bytes(B, T, H, Hq, DK, DV, dtype, 0, 0), scratch, scratch_bytes))
-    return rc;
   const Shape d = make_shape(B, T, H, Hq, DK, DV);
   const size_t e = bytes_of(dtype);
   const Input qi = make_input(q, q_sb, q_st, q_sh, e), ki = make_input(k, k_sb, k_st, k_sh, e), vi = make_input(v, v_sb, v_st, v_sh, e);
+  const bool walk = may_walk(dtype, DK, DV, true) && walk_takes(d, qi, ki, vi);
+  if (int rc = check_scratch(name, mpb_linear_attention_scratch_bytes(B, T, H, Hq, DK, DV, dtype, 0, 0, walk), scratch, scratch_bytes))
+    return rc;
   const Decay g = {log_decay, g_sb, g_st, g_sh};
   switch (dtype) {
-    case MPB_F32: return run_forward<float>(d, qi, ki, vi, g, state0, (float)scale, o, state, (char*)scratch, s);
-    case MPB_F16: return run_forward<__half>(d, qi, ki, vi, g, state0, (float)scale, o, state, (char*)scratch, s);
-    default: return run_forward<bf16>(d, qi, ki, vi, g, state0, (float)scale, o, state, (char*)scratch, s);
+    case MPB_F32: return run_forward<float>(d, qi, ki, vi, g, state0, (float)scale, o, state, walk, (char*)scratch, s);
+    case MPB_F16: return run_forward<__half>(d, qi, ki, vi, g, state0, (float)scale, o, state, walk, (char*)scratch, s);
+    default: return run_forward<bf16>(d, qi, ki, vi, g, state0, (float)scale, o, state, walk, (char*)scratch, s);
   }
 }
 
@@ -924,9 +958,6 @@ int mpb_linear_attention_backward(int64_t B, int64_t T, int64_t H, int64_t Hq, i
   }
   if (!dout || !q || !k || !v || !log_decay || !dq || !dk || !dv || !dlog_decay || !dstate0)
     return fail(MPB_ERR_INVALID, "%s: null pointer", name);
-  if (int rc = check_scratch(name, mpb_linear_attention_scratch_bytes(B, T, H, Hq, DK, DV, dtype, 1, decay_by_head), scratch,
-                             scratch_bytes))
-    return rc;
   const size_t e = bytes_of(dtype);
   Gradients p = {};
   p.d = make_shape(B, T, H, Hq, DK, DV);
@@ -934,11 +965,15 @@ int mpb_linear_attention_backward(int64_t B, int64_t T, int64_t H, int64_t Hq, i
   p.v = make_input(v, v_sb, v_st, v_sh, e), p.g_o = make_input(dout, do_sb, do_st, do_sh, e);
   p.g = {log_decay, g_sb, g_st, g_sh};
   p.scale = (float)scale, p.dv = dv;
+  const bool walk = may_walk(dtype, DK, DV, true) && walk_takes(p.d, p.q, p.k, p.v) && walk_takes(p.d, p.q, p.k, p.g_o);
+  if (int rc = check_scratch(name, mpb_linear_attention_scratch_bytes(B, T, H, Hq, DK, DV, dtype, 1, decay_by_head, walk), scratch,
+                             scratch_bytes))
+    return rc;
   const bool by = decay_by_head != 0;
   switch (dtype) {
-    case MPB_F32: return run_backward<float>(p, state0, dstate, dq, dk, dlog_decay, by, dstate0, (char*)scratch, s);
-    case MPB_F16: return run_backward<__half>(p, state0, dstate, dq, dk, dlog_decay, by, dstate0, (char*)scratch, s);
-    default: return run_backward<bf16>(p, state0, dstate, dq, dk, dlog_decay, by, dstate0, (char*)scratch, s);
+    case MPB_F32: return run_backward<float>(p, state0, dstate, dq, dk, dlog_decay, by, dstate0, walk, (char*)scratch, s);
+    case MPB_F16: return run_backward<__half>(p, state0, dstate, dq, dk, dlog_decay, by, dstate0, walk, (char*)scratch, s);
+    default: return run_backward<bf16>(p, state0, dstate, dq, dk, dlog_decay, by, dstate0, walk, (char*)scratch, s);
   }
 }
 

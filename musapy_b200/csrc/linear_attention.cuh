@@ -88,4 +88,39 @@ struct ChunkDecay {
   }
 };
 
+struct Shape {
+  int64_t B, T;
+  int H, share, DK, DV;      // share: heads that share one of q and k
+  int chunks, segments, per;  // per: chunks of a segment
+  int dkp, dvp;               // channels in the scratch, multiples of 16
+};
+struct Input {
+  const void* p;
+  int64_t sb, st, sh;
+  bool wide;  // 16-byte loads
+  template <class T>
+  MPB_D const T* at(int64_t b, int64_t t, int h) const { return (const T*)p + b * sb + t * st + h * sh; }
+};
+struct Decay {
+  const float* p;
+  int64_t sb, st, sh;
+};
+
+// The bf16 kernel of whole rows (linear_attention_walk.cu): one block per head of a sequence and segment.
+struct Walk {
+  Shape d;
+  Input q, k, v;       // without outputs q is unused: k and v, or the pair that the state is summed from
+  Decay g;
+  const float* first;  // the state before the first segment, (DK, DV) per head, or null
+  const float* starts; // the states before the other segments, padded; null without outputs: each begins from nothing
+  float scale;
+  void* o;
+  bool rev;
+  float *at, *since, *ends, *last;  // as k_la_states leaves them; null where not wanted
+  int* status;
+};
+bool walk_takes(const Shape& d, const Input& q, const Input& k, const Input& v);
+int walk_outputs(const Walk& p, cudaStream_t s);
+int walk_states(const Walk& p, cudaStream_t s);
+
 }  // namespace mpb

@@ -1,0 +1,531 @@
+// Linear attention of bf16 heads of up to 128 channels: a block walks a head's chunks (or those of one segment of
+// it) with the state on chip, so that q, k and v are read and o is written once. The formulas are those of
+// linear_attention.cu. Per chunk of 64 steps the tensor core makes
+//
+//   A = q k'           (steps x steps)        -> P = D A, rounded to bf16, back to shared memory
+//   E = (w k)' v       (channels x channels)  w_j = e^(G_C - G_j); w k as three bf16 numbers that sum to it
+//   X' = S' q', Y' = v' P'  (channels of v x steps),  o = scale (e^(G_i) X + Y)
+//
+// and the state's threads S <- e^(G_C) S + E in float, from which X takes S rounded once to bf16: like the rounding of P
+// it is half a step of the output's type, and the state itself keeps 32 bits. Only that sum ties a chunk to the
+// next; E, A and P of the next chunks are made ahead of it.
+//
+// Roles of the block's warps: 4 keep the state (in tensor memory, one row of channels per thread), 4 write
+// outputs, 4 weigh and split k, 2 make P, one copies (TMA, two chunks in shared memory), one issues the matrix
+// instructions, one makes the decays. They meet at mbarriers; every wait gives up after two seconds, sets the status
+// word and ends the block.
+//
+// Operands lie as the copies leave them, rows of 128 bytes in the 128-byte swizzle; what is needed transposed (k, v, S as
+// left operands, v as a right one) is read "along the other dim" by the tensor core. Every matrix
+// instruction has 128 rows: of operands with 64, the second half is whatever lies behind them in shared memory, and its
+// results are not read.
+#include <cuda.h>
+#include "async_copy.cuh"
+#include "common.cuh"
+#include "internal.h"
+#include "linear_attention.cuh"
+#include "rows.cuh"
+
+namespace mpb {
+namespace {
+
+using bf16 = __nv_bfloat16;
+
+constexpr int kThreads = 17 * 32;
+constexpr int kStages = 2;   // chunks of q, k, v in shared memory
+constexpr int kSlots = 4;    // chunks whose decays are there
+constexpr int kPieces = 3;   // of w k
+constexpr uint32_t kTmemColumns = 512;
+constexpr uint32_t kColA = 0, kColX = 64, kColY = 128, kColE = 192, kColS = 320;
+
+// ------------------------------------------------------- tensor core
+MPB_D void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+MPB_D void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+MPB_D void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+MPB_D void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+MPB_D void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+MPB_D void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+MPB_D void tmem_load(uint32_t (&r)[32], uint32_t at) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at));
+}
+MPB_D void tmem_store(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
+      "r"(at)
+      : "memory");
+}
+MPB_D void wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+MPB_D void wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A shared memory operand in the 128-byte swizzle: `group`, bytes between groups of eight rows of 128 bytes; `block`,
+// between blocks of 64 elements where the rows run along the other dim.
+MPB_D uint64_t operand(uint32_t at, uint32_t block, uint32_t group) {
+  return (uint64_t)((at >> 4) & 0x3fff) | (uint64_t)((block >> 4) & 0x3fff) << 16 | (uint64_t)((group >> 4) & 0x3fff) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// bf16 operands, float sums, 128 rows, n columns; ta, tb: an operand whose rows run along its own dim, not the summed one.
+constexpr uint32_t instruction(int n, bool ta, bool tb) {
+  return 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)ta << 15 | (uint32_t)tb << 16 | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+}
+
+MPB_D void tma_tile(uint32_t dst, const CUtensorMap* map, int x, int h, int t, int b, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(h), "r"(t), "r"(b), "r"(bar)
+      : "memory");
+}
+
+// ------------------------------------------------------------ layout
+enum Bar { kFull0, kFull1, kEmpty0, kEmpty1, kDec0, kDec1, kDec2, kDec3, kADone, kAFree, kPReady, kWReady, kEDone, kEFree, kSReady,
+           kXDone, kODone, kOFree, kFree0, kFree1, kFree2, kFree3, kEnd, kBars };
+
+template <int DK, int DV>
+struct Layout {
+  static constexpr int kBlock = 64 * 128;  // 64 steps of 64 channels
+  static constexpr int q = 0, k = q + DK / 64 * kBlock, v = k + DK / 64 * kBlock, kStage = v + DV / 64 * kBlock;
+  static constexpr int P = kStages * kStage, W = P + kBlock, S = W + kPieces * (DK / 64) * kBlock;
+  // S has two blocks of 64 columns in any case: a left operand has 128 rows, and may read the second
+  static constexpr int decays = S + 2 * DK * 128;
+  static constexpr int bars = decays + kSlots * ((int)sizeof(ChunkDecay) + 15) / 16 * 16, tmem = bars + kBars * 8;
+  static constexpr int bytes = tmem + 16 + 1024;  // the copies' rows want 1024-byte alignment
+};
+
+struct Maps {
+  CUtensorMap q, k, v;
+};
+
+template <int DK, int DV, bool OUT>
+__global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__ Maps maps, Walk p) {
+  using L = Layout<DK, DV>;
+  extern __shared__ unsigned char raw[];
+  const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u;
+  unsigned char* mem = raw + (smem - smem_u32(raw));
+  ChunkDecay* decays = reinterpret_cast<ChunkDecay*>(mem + L::decays);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Shape& d = p.d;
+  const int seg = (int)(blockIdx.x % d.segments);
+  const int64_t bh = blockIdx.x / d.segments;
+  const int h = (int)(bh % d.H), hq = h / d.share;
+  const int64_t b = bh / d.H;
+  const int c0 = seg * d.per, c1 = min(d.chunks, c0 + d.per), n_chunks = c1 - c0;
+  auto bar = [&](int i) { return smem + L::bars + 8 * i; };
+  auto chunk = [&](int n) { return p.rev ? c1 - 1 - n : c0 + n; };
+  bool ok = true;
+  // true where the phase of chunk n has come
+  auto wait = [&](int i, int n) {
+    if (ok) ok = mbar_wait(bar(i), (uint32_t)n & 1);
+    return ok;
+  };
+  auto wait_warp = [&](int i, int n) {
+    ok = __all_sync(0xffffffffu, wait(i, n));
+    return ok;
+  };
+  if (tid == 0) {
+    for (int i = 0; i < kBars; ++i) {
+      const int count = i >= kDec0 && i <= kDec3 ? 32 : i == kAFree || i == kPReady ? 64 : i == kWReady ? 128
+                        : i == kEFree || i == kSReady ? DK : i == kOFree ? DV
+                        : i >= kFree0 && i <= kFree3 ? DK + (OUT ? DV : 0) : 1;
+      mbar_init(bar(i), count);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 16) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem + L::tmem), "n"(kTmemColumns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(mem + L::tmem);
+  const uint32_t quarter = tmem + ((uint32_t)(warp & 3) * 32 << 16);
+  const int row = (warp & 3) * 32 + lane;
+  constexpr uint32_t kOther = L::kBlock;
+
+  if (warp < 4) {  // ------------------------------------------- the state
+    if (row < DK) {
+      const int64_t size = (int64_t)d.dkp * d.dvp;
+      const float* first = nullptr;
+      int pitch = 0;
+      bool have = false;
+      const bool begins = p.rev ? c1 == d.chunks : seg == 0;
+      if (begins) {
+        first = p.first + bh * d.DK * d.DV + (int64_t)row * d.DV, pitch = d.DV, have = p.first && row < d.DK;
+      } else if (p.starts) {
+        first = p.starts + (bh * d.segments + seg) * size + (int64_t)row * d.dvp, pitch = d.dvp, have = row < d.dkp;
+      }
+      unsigned char* s_row = mem + L::S + row * 128;
+      // 32 columns of S to shared memory, rounded
+      auto put = [&](int g, const uint32_t (&s)[32]) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint4 w;
+          w.x = pack<bf16>(make_float2(__uint_as_float(s[8 * c]), __uint_as_float(s[8 * c + 1]))).w;
+          w.y = pack<bf16>(make_float2(__uint_as_float(s[8 * c + 2]), __uint_as_float(s[8 * c + 3]))).w;
+          w.z = pack<bf16>(make_float2(__uint_as_float(s[8 * c + 4]), __uint_as_float(s[8 * c + 5]))).w;
+          w.w = pack<bf16>(make_float2(__uint_as_float(s[8 * c + 6]), __uint_as_float(s[8 * c + 7]))).w;
+          const int at = (g & 1) * 4 + c;
+          *reinterpret_cast<uint4*>(s_row + (g >> 1) * (DK * 128) + ((at ^ (row & 7)) << 4)) = w;
+        }
+      };
+#pragma unroll 1
+      for (int g = 0; g < DV / 32; ++g) {
+        uint32_t s[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s[i] = have && g * 32 + i < pitch ? __float_as_uint(first[g * 32 + i]) : 0u;
+        tmem_store(quarter + kColS + g * 32, s);
+        if (OUT) put(g, s);
+      }
+      wait_stores();
+      if (OUT) {
+        proxy_fence();
+        mbar_arrive(bar(kSReady));
+      }
+      float since = 1.0f;
+      for (int n = 0; n < n_chunks; ++n) {
+        const int c = chunk(n);
+        if (!wait_warp(kDec0 + n % kSlots, n / kSlots)) break;
+        const float all = decays[n % kSlots].all;
+        if (p.since && row == 0) p.since[bh * d.chunks + c] = since;
+        since *= all;
+        if (!wait_warp(kEDone, n)) break;
+        if (OUT && !wait_warp(kXDone, n)) break;
+        fence_after();
+        float* at = p.at ? p.at + (bh * d.chunks + c) * size + (int64_t)row * d.dvp : nullptr;
+#pragma unroll 1
+        for (int g = 0; g < DV / 32; ++g) {
+          uint32_t e[32], s[32];
+          tmem_load(e, quarter + kColE + g * 32);
+          tmem_load(s, quarter + kColS + g * 32);
+          wait_loads();
+          if (g == DV / 32 - 1) {
+            fence_before();
+            mbar_arrive(bar(kEFree));
+            mbar_arrive(bar(kFree0 + n % kSlots));
+          }
+          if (at && row < d.dkp) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              if (g * 32 + i < d.dvp)
+                *reinterpret_cast<uint4*>(at + g * 32 + i) = make_uint4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            s[i] = all == 0.0f ? e[i] : __float_as_uint(fmaf(all, __uint_as_float(s[i]), __uint_as_float(e[i])));
+          tmem_store(quarter + kColS + g * 32, s);
+          if (OUT) put(g, s);
+        }
+        wait_stores();
+        if (OUT) {
+          proxy_fence();
+          fence_before();
+          mbar_arrive(bar(kSReady));
+        }
+      }
+      if (ok) {
+        const bool whole = d.segments == 1;
+        float* to = whole ? (p.last ? p.last + bh * d.DK * d.DV + (int64_t)row * d.DV : nullptr)
+                          : (p.ends ? p.ends + (bh * d.segments + seg) * size + (int64_t)row * d.dvp : nullptr);
+        const int width = whole ? d.DV : d.dvp;
+        if (p.ends && !whole && row == 0) p.since[(bh + d.B * d.H) * d.chunks + seg] = since;
+#pragma unroll 1
+        for (int g = 0; g < DV / 32; ++g) {
+          uint32_t s[32];
+          tmem_load(s, quarter + kColS + g * 32);
+          wait_loads();
+          if (to && row < (whole ? d.DK : d.dkp)) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (g * 32 + i < width) to[g * 32 + i] = __uint_as_float(s[i]);
+          }
+        }
+      }
+    }
+  } else if (warp < 8) {  // ------------------------------------ outputs
+    if (OUT && row < DV) {
+      bf16* o = (bf16*)p.o + ((b * d.T) * d.H + h) * d.DV + row;
+      const int64_t step = (int64_t)d.H * d.DV;
+      const bool mine = row < d.DV;
+      for (int n = 0; n < n_chunks; ++n) {
+        const int64_t t0 = (int64_t)chunk(n) * kChunk;
+        const int steps = (int)min((int64_t)kChunk, d.T - t0);
+        if (!wait_warp(kDec0 + n % kSlots, n / kSlots) || !wait_warp(kODone, n)) break;
+        fence_after();
+        const float* into = decays[n % kSlots].into;
+#pragma unroll 1
+        for (int g = 0; g < 2; ++g) {
+          uint32_t x[32], y[32];
+          tmem_load(x, quarter + kColX + g * 32);
+          tmem_load(y, quarter + kColY + g * 32);
+          wait_loads();
+          float f[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float by = into[g * 32 + i];
+            f[i] = p.scale * (by != 0.0f ? fmaf(by, __uint_as_float(x[i]), __uint_as_float(y[i])) : __uint_as_float(y[i]));
+          }
+          if (g == 1) {
+            fence_before();
+            mbar_arrive(bar(kOFree));
+            mbar_arrive(bar(kFree0 + n % kSlots));
+          }
+          bf16* to = o + (t0 + g * 32) * step;
+          if (mine) {
+            if (steps == kChunk) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) to[i * step] = __float2bfloat16_rn(f[i]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (g * 32 + i < steps) to[i * step] = __float2bfloat16_rn(f[i]);
+            }
+          }
+        }
+      }
+    }
+  } else if (warp < 12) {  // ------------------------------ the weighed k
+    const int at = tid - 8 * 32;
+    for (int n = 0; n < n_chunks; ++n) {
+      if (!wait_warp(kDec0 + n % kSlots, n / kSlots) || !wait_warp(kFull0 + n % kStages, n / kStages)) break;
+      if (n > 0 && !wait_warp(kEDone, n - 1)) break;
+      const ChunkDecay& cd = decays[n % kSlots];
+      const unsigned char* from = mem + (n % kStages) * L::kStage + L::k;
+#pragma unroll
+      for (int i = 0; i < DK / 64 * kChunk * 8 / 128; ++i) {
+        const int word = at + i * 128, t = word / 8 % kChunk;
+        const float w = p.rev ? cd.into[t] * p.scale : cd.rest[t];
+        union { uint4 q; uint32_t pair[4]; } x, out[kPieces];
+        x.q = *reinterpret_cast<const uint4*>(from + word * 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float2 f = make_float2(__uint_as_float(x.pair[j] << 16), __uint_as_float(x.pair[j] & 0xffff0000u));
+          f = w != 0.0f ? vmul(f, vset<2>(w)) : vset<2>(0.0f);
+#pragma unroll
+          for (int k = 0; k < kPieces; ++k) {
+            out[k].pair[j] = pack<bf16>(f).w;
+            f = vadd(f, make_float2(-__uint_as_float(out[k].pair[j] << 16), -__uint_as_float(out[k].pair[j] & 0xffff0000u)));
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) *reinterpret_cast<uint4*>(mem + L::W + k * (DK / 64) * L::kBlock + word * 16) = out[k].q;
+      }
+      proxy_fence();
+      mbar_arrive(bar(kWReady));
+    }
+  } else if (warp < 14) {  // --------------------------------- the scores
+    if (OUT) {
+      unsigned char* to = mem + L::P + row * 128;
+      for (int n = 0; n < n_chunks; ++n) {
+        if (!wait_warp(kDec0 + n % kSlots, n / kSlots) || !wait_warp(kADone, n)) break;
+        fence_after();
+        const ChunkDecay& cd = decays[n % kSlots];
+        uint32_t a[2][32];
+        tmem_load(a[0], quarter + kColA);
+        tmem_load(a[1], quarter + kColA + 32);
+        wait_loads();
+        fence_before();
+        mbar_arrive(bar(kAFree));
+        const float hi = cd.hi[row], lo = cd.lo[row];
+        const int from = cd.from[row];
+        if (n > 0 && !wait_warp(kODone, n - 1)) break;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int j = c * 8 + i;
+            const float e = ex2f((hi - cd.hi[j]) + (lo - cd.lo[j]));
+            f[i] = j <= row && j >= from ? e * __uint_as_float(a[c >> 2][(c & 3) * 8 + i]) : 0.0f;
+          }
+          uint4 w;
+          w.x = pack<bf16>(make_float2(f[0], f[1])).w;
+          w.y = pack<bf16>(make_float2(f[2], f[3])).w;
+          w.z = pack<bf16>(make_float2(f[4], f[5])).w;
+          w.w = pack<bf16>(make_float2(f[6], f[7])).w;
+          *reinterpret_cast<uint4*>(to + ((c ^ (row & 7)) << 4)) = w;
+        }
+        proxy_fence();
+        mbar_arrive(bar(kPReady));
+      }
+    }
+  } else if (warp == 14) {  // -------------------------------- the copies
+    if (lane == 0) {
+      for (int n = 0; n < n_chunks; ++n) {
+        const int s = n % kStages;
+        if (n >= kStages && !wait(kEmpty0 + s, n / kStages - 1)) break;
+        const uint32_t at = smem + s * L::kStage;
+        const int t0 = chunk(n) * kChunk;
+        mbar_expect_tx(bar(kFull0 + s), L::kStage - (OUT ? 0 : L::k));
+        for (int i = 0; i < DK / 64; ++i) {
+          if (OUT) tma_tile(at + L::q + i * L::kBlock, &maps.q, i * 64, hq, t0, (int)b, bar(kFull0 + s));
+          tma_tile(at + L::k + i * L::kBlock, &maps.k, i * 64, hq, t0, (int)b, bar(kFull0 + s));
+        }
+        for (int i = 0; i < DV / 64; ++i) tma_tile(at + L::v + i * L::kBlock, &maps.v, i * 64, h, t0, (int)b, bar(kFull0 + s));
+      }
+    }
+  } else if (warp == 15) {  // ------------------- the matrix instructions
+    if (lane == 0) {
+      constexpr uint32_t kScores = instruction(64, false, false), kSum = instruction(DV, true, true), kOut = instruction(64, true, false);
+      auto scores = [&](int n) {
+        const uint32_t at = smem + (n % kStages) * L::kStage;
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i) {
+          const uint32_t o = (i / 4) * L::kBlock + (i % 4) * 32;
+          mma(tmem + kColA, operand(at + L::q + o, 16, 1024), operand(at + L::k + o, 16, 1024), kScores, i > 0);
+        }
+        commit(bar(kADone));
+      };
+      if (OUT && n_chunks > 0 && wait(kFull0, 0)) {
+        fence_after();
+        scores(0);
+      }
+      for (int n = 0; n < n_chunks; ++n) {
+        const uint32_t at = smem + (n % kStages) * L::kStage;
+        if (!wait(kWReady, n) || !wait(kFull0 + n % kStages, n / kStages)) break;
+        if (n > 0 && !wait(kEFree, n - 1)) break;
+        fence_after();
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k)  // the small pieces first
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            mma(tmem + kColE, operand(smem + L::W + (kPieces - 1 - k) * (DK / 64) * L::kBlock + i * 2048, kOther, 1024),
+                operand(at + L::v + i * 2048, kOther, 1024), kSum, k + i > 0);
+        commit(bar(kEDone));
+        if (!OUT) {
+          commit(bar(kEmpty0 + n % kStages));
+          continue;
+        }
+        if (n + 1 < n_chunks) {
+          if (!wait(kFull0 + (n + 1) % kStages, (n + 1) / kStages) || !wait(kAFree, n)) break;
+          fence_after();
+          scores(n + 1);
+        }
+        if (!wait(kSReady, n) || (n > 0 && !wait(kOFree, n - 1))) break;
+        fence_after();
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i)
+          mma(tmem + kColX, operand(smem + L::S + i * 2048, DK * 128, 1024),
+              operand(at + L::q + (i / 4) * L::kBlock + (i % 4) * 32, 16, 1024), kOut, i > 0);
+        commit(bar(kXDone));
+        if (!wait(kPReady, n)) break;
+        fence_after();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          mma(tmem + kColY, operand(at + L::v + i * 2048, kOther, 1024), operand(smem + L::P + i * 32, 16, 1024), kOut, i > 0);
+        commit(bar(kODone));
+        commit(bar(kEmpty0 + n % kStages));
+      }
+    }
+  } else {  // --------------------------------------------- the decays
+    const float* g = p.g.p + b * p.g.sb + h * p.g.sh;
+    for (int n = 0; n < n_chunks; ++n) {
+      const int64_t t0 = (int64_t)chunk(n) * kChunk;
+      if (n >= kSlots && !wait_warp(kFree0 + n % kSlots, n / kSlots - 1)) break;
+      decays[n % kSlots].fill(g + t0 * p.g.st, p.g.st, (int)min((int64_t)kChunk, d.T - t0));
+      mbar_arrive(bar(kDec0 + n % kSlots));
+    }
+  }
+  if (!ok && p.status) *p.status = MPB_ERR_TIMEOUT;
+  __syncwarp();
+  // a block that gave up: what it has under way ends before its memory does
+  const bool failed = __syncthreads_or(!ok);
+  if (failed && warp == 15 && lane == 0) {
+    commit(bar(kEnd));
+    mbar_wait(bar(kEnd), 0);
+    for (int s = 0; s < kStages; ++s) mbar_wait(bar(kFull0 + s), 0);
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 16)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemColumns) : "memory");
+}
+
+// ------------------------------------------------------------------- host
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encoder() {
+  static EncodeTiled fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
+      (void)cudaGetLastError();
+      f = nullptr;
+    }
+    return reinterpret_cast<EncodeTiled>(f);
+  }();
+  return fn;
+}
+
+// Boxes of 64 channels and 64 steps of one head of a (B, T, heads, D) array; zeros outside it.
+bool encode(CUtensorMap* m, const Input& x, int64_t B, int64_t T, int64_t heads, int64_t D) {
+  const EncodeTiled fn = encoder();
+  if (!fn) return false;
+  // a dim of one step has no stride of its own
+  auto bytes = [&](int64_t n, int64_t stride) { return (cuuint64_t)(n > 1 ? stride * 2 : (D * 2 + 15) / 16 * 16); };
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)T, (cuuint64_t)B};
+  const cuuint64_t strides[3] = {bytes(heads, x.sh), bytes(T, x.st), bytes(B, x.sb)};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)kChunk, 1}, each[4] = {1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(x.p), dims, strides, box, each,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DK, int DV, bool OUT>
+int launch(const Walk& p, cudaStream_t s) {
+  const Shape& d = p.d;
+  Maps maps;
+  const int64_t hq = d.H / d.share;
+  if ((OUT && !encode(&maps.q, p.q, d.B, d.T, hq, d.DK)) || !encode(&maps.k, p.k, d.B, d.T, hq, d.DK) ||
+      !encode(&maps.v, p.v, d.B, d.T, d.H, d.DV))
+    return fail(MPB_ERR_CUDA, "linear_attention: the copies' maps cannot be made");
+  constexpr int kWalkBytes = Layout<DK, DV>::bytes;
+  if (int rc = allow_smem<k_la_walk<DK, DV, OUT>, kWalkBytes>("linear_attention")) return rc;
+  k_la_walk<DK, DV, OUT><<<(unsigned)(d.B * d.H * d.segments), kThreads, kWalkBytes, s>>>(maps, p);
+  return launch_check("linear_attention");
+}
+
+template <bool OUT>
+int launch_for(const Walk& p, cudaStream_t s) {
+  const bool k = p.d.DK > 64, v = p.d.DV > 64;
+  return k ? (v ? launch<128, 128, OUT>(p, s) : launch<128, 64, OUT>(p, s))
+           : (v ? launch<64, 128, OUT>(p, s) : launch<64, 64, OUT>(p, s));
+}
+
+}  // namespace
+
+bool walk_takes(const Shape& d, const Input& q, const Input& k, const Input& v) {
+  if (d.DK > 128 || d.DV > 128 || d.T >= (1LL << 31) - kChunk || d.B >= (1LL << 31)) return false;
+  for (const Input* x : {&q, &k, &v}) {
+    if (!x->wide) return false;
+    const int64_t heads = x == &v ? d.H : d.H / d.share;
+    if ((d.B > 1 && x->sb <= 0) || (d.T > 1 && x->st <= 0) || (heads > 1 && x->sh <= 0)) return false;
+    if (x->sb >= (1LL << 38) || x->st >= (1LL << 38) || x->sh >= (1LL << 38)) return false;
+  }
+  return true;
+}
+int walk_outputs(const Walk& p, cudaStream_t s) { return launch_for<true>(p, s); }
+int walk_states(const Walk& p, cudaStream_t s) { return launch_for<false>(p, s); }
+
+}  // namespace mpb

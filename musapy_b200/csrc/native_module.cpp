@@ -377,10 +377,11 @@ PyObject* py_policy_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyObject* py_linear_attention_scratch_bytes(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  Args a(args, n, 9, "linear_attention_scratch_bytes");
-  struct { int64_t B, T, H, Hq, DK, DV; int dt, back, by; } v{a.l(), a.l(), a.l(), a.l(), a.l(), a.l(), a.i(), a.i(), a.i()};
+  Args a(args, n, 10, "linear_attention_scratch_bytes");
+  struct { int64_t B, T, H, Hq, DK, DV; int dt, back, by, aligned; } v{a.l(), a.l(), a.l(), a.l(), a.l(),
+                                                                       a.l(), a.i(), a.i(), a.i(), a.i()};
   if (!a) return nullptr;
-  return PyLong_FromSize_t(mpb_linear_attention_scratch_bytes(v.B, v.T, v.H, v.Hq, v.DK, v.DV, v.dt, v.back, v.by));
+  return PyLong_FromSize_t(mpb_linear_attention_scratch_bytes(v.B, v.T, v.H, v.Hq, v.DK, v.DV, v.dt, v.back, v.by, v.aligned));
 }
 
 PyObject* py_linear_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {

@@ -11,11 +11,11 @@ from typing import NamedTuple, Optional
 from . import dtypes as _dt
 from . import errors
 from . import streams as _streams
-from ._lib import NATIVE, check
+from ._lib import LIB, NATIVE, check
 from .array import Array
 from .blocks import (_array, _carve, _dense, _element, _floats, _new, _norm_input, _of, _prod, _ptr, _rows, _scratch, _sptr,
                      _unit_inner)
-from .ops import _alias, _check_out, _same_device, contiguous
+from .ops import _CHECK_SCAN_STATUS, _alias, _check_out, _same_device, contiguous
 
 _MOST_CHANNELS = 256  # of a head
 _MOST_TOP = 1024  # entries of a teacher's list
@@ -61,6 +61,24 @@ def _attention_inputs(name: str, q, k, v, log_decay, time: bool):
     return _unit_inner(q), _unit_inner(k), _unit_inner(v), gs, B, T, H, Hq, DK, DV, by_head
 
 
+def _aligned(*arrays) -> int:
+    """Are these 16-byte aligned, with strides that are positive multiples of 16 bytes (of the dims that have steps)?"""
+    for x in arrays:
+        unit = 16 // x._dtype.itemsize - 1
+        if x._ptr & 15:
+            return 0
+        for n, s in zip(x._shape[:-1], x._strides):
+            if s & unit or (n > 1 and s <= 0):
+                return 0
+    return 1
+
+
+def _attention_status(name: str, scratch, dev: int) -> None:
+    """With ``ops.set_scan_status_check(True)`` (it synchronises): did a wait inside the kernel give up?"""
+    if scratch is not None and _CHECK_SCAN_STATUS[0]:
+        check(LIB.mpb_linear_attention_status(scratch.data_ptr(), _streams.current_stream(dev).cuda_stream), name)
+
+
 def linear_attention(q, k, v, log_decay, state=None, scale=None, return_state=False, out=None):
     """Linear attention with a decay for each head: ``S[t] = exp(log_decay[t]) S[t-1] + k[t] v[t]'``,
     ``o[t] = scale S[t]' q[t]``.
@@ -91,11 +109,12 @@ def linear_attention(q, k, v, log_decay, state=None, scale=None, return_state=Fa
     last = _new(s, (B, H, DK, DV), _dt.float32, dev) if return_state else None
     if B:
         code = q._dtype.code
-        nbytes = NATIVE.linear_attention_scratch_bytes(B, T, H, Hq, DK, DV, code, 0, 0)
+        nbytes = NATIVE.linear_attention_scratch_bytes(B, T, H, Hq, DK, DV, code, 0, 0, _aligned(q, k, v))
         scratch = _scratch(nbytes, dev)
         check(NATIVE.linear_attention(B, T, H, Hq, DK, DV, code, q._ptr, *q._strides[:3], k._ptr, *k._strides[:3], v._ptr,
                                       *v._strides[:3], log_decay._ptr, *gs, _ptr(state), scale, o._ptr, _ptr(last),
                                       _sptr(scratch), nbytes, _streams.launch_on(s, name, *ins, o, last)), name)
+        _attention_status(name, scratch, dev)
     return (o, last) if return_state else o
 
 
@@ -121,13 +140,15 @@ def linear_attention_backward(do, q, k, v, log_decay, state=None, dstate=None, s
     dq, dk, dv = (_new(s, x._shape, x._dtype, dev) for x in (q, k, v))
     dg, dstate0 = _new(s, log_decay._shape, _dt.float32, dev), _new(s, sshape, _dt.float32, dev)
     code = q._dtype.code
-    nbytes = NATIVE.linear_attention_scratch_bytes(B, T, H, Hq, DK, DV, code, 1, int(by_head))
+    nbytes = NATIVE.linear_attention_scratch_bytes(B, T, H, Hq, DK, DV, code, 1, int(by_head),
+                                                   _aligned(do, q, k, v))
     scratch = _scratch(nbytes, dev)
     check(NATIVE.linear_attention_backward(
         B, T, H, Hq, DK, DV, code, do._ptr, *do._strides[:3], q._ptr, *q._strides[:3], k._ptr, *k._strides[:3], v._ptr,
         *v._strides[:3], log_decay._ptr, *gs, _ptr(state), _ptr(dstate), scale, dq._ptr, dk._ptr, dv._ptr, dg._ptr,
         int(by_head), dstate0._ptr, _sptr(scratch), nbytes,
         _streams.launch_on(s, name, *ins, dq, dk, dv, dg, dstate0)), name)
+    _attention_status(name, scratch, dev)
     return dq, dk, dv, dg, dstate0
 
 

@@ -168,8 +168,10 @@ def test_c_entry_points_return_status():
     from musapy_b200._lib import MPB_ERR_DTYPE, MPB_ERR_INVALID, MPB_ERR_SCRATCH, MPB_ERR_SHAPE, MPB_OK, NATIVE as N, last_error
 
     f32, f16, bf16, i32, i64 = 10, 9, 12, 3, 4
-    need = N.linear_attention_scratch_bytes(2, 70, 4, 2, 8, 6, bf16, 0, 0)
-    assert need > 0 and N.linear_attention_scratch_bytes(2, 70, 4, 3, 8, 6, bf16, 0, 0) == 0
+    # strides of 6 channels are no multiples of 16 bytes
+    need = N.linear_attention_scratch_bytes(2, 70, 4, 2, 8, 6, bf16, 0, 0, 0)
+    assert N.linear_attention_scratch_bytes(2, 70, 4, 2, 8, 8, bf16, 0, 0, 1) < need
+    assert need > 0 and N.linear_attention_scratch_bytes(2, 70, 4, 3, 8, 6, bf16, 0, 0, 1) == 0
     att = lambda **k: N.linear_attention(*{**dict(
         B=2, T=70, H=4, Hq=2, DK=8, DV=6, dt=bf16, q=16, a=1120, b=16, c=8, k=16, d=1120, e=16, f=8, v=16, g=1680, h=24, i=6,
         g_=16, j=280, l=4, m=1, s0=0, scale=1.0, o=16, s=0, sc=16, nb=need, st=0), **k}.values())
@@ -180,7 +182,7 @@ def test_c_entry_points_return_status():
         assert att(**{x: 0}) == MPB_ERR_INVALID
     assert att(nb=need - 1) == MPB_ERR_SCRATCH and att(sc=0) == MPB_ERR_SCRATCH and att(sc=24) == MPB_ERR_INVALID
     assert att(B=0, q=0, o=0) == MPB_OK and att(T=0, q=0, o=0) == MPB_OK
-    need = N.linear_attention_scratch_bytes(2, 70, 4, 2, 8, 6, f32, 1, 1)
+    need = N.linear_attention_scratch_bytes(2, 70, 4, 2, 8, 6, f32, 1, 1, 0)
     back = lambda **k: N.linear_attention_backward(*{**dict(
         B=2, T=70, H=4, Hq=2, DK=8, DV=6, dt=f32, do=16, x=1680, y=24, z=6, q=16, a=1120, b=16, c=8, k=16, d=1120, e=16, f=8, v=16,
         g=1680, h=24, i=6, g_=16, j=0, l=0, m=1, s0=0, ds=0, scale=1.0, dq=16, dk=16, dv=16, dg=16, by=1, ds0=16, sc=16, nb=need,
@@ -207,7 +209,7 @@ def test_c_entry_points_return_status():
     assert emb(N=-1) == MPB_ERR_SHAPE and emb(N=1 << 31) == MPB_ERR_SHAPE and emb(idt=f32) == MPB_ERR_DTYPE and emb(dt=i64) == MPB_ERR_DTYPE
     assert emb(t=0) == MPB_ERR_INVALID and emb(o=0) == MPB_ERR_INVALID and emb(N=0, ids=0) == MPB_OK and emb(D=0, o=0) == MPB_OK
     need = N.embedding_backward_scratch_bytes(4, 8, 3, 0)
-    assert need > N.embedding_backward_scratch_bytes(4, 8, 3, 1) > 0 and N.embedding_backward_scratch_bytes(0, 8, 3, 0) == 0
+    assert N.embedding_backward_scratch_bytes(6, 8, 3, 0) > N.embedding_backward_scratch_bytes(6, 8, 3, 1) > 0 and N.embedding_backward_scratch_bytes(0, 8, 3, 0) == 0
     grad = lambda **k: N.embedding_backward(*{**dict(N=4, V=8, D=3, d=16, dt=f32, sr=3, ids=16, idt=i32, scale=1.0, into=0, t=16,
                                                      sc=16, nb=need, st=0), **k}.values())
     assert grad(V=-1) == MPB_ERR_SHAPE and grad(N=1 << 31) == MPB_ERR_SHAPE and grad(V=1 << 31) == MPB_ERR_SHAPE
