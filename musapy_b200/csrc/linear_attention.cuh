@@ -33,7 +33,7 @@ MPB_D void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t
 // two large sums has to be right to float precision. A decay below
 // e^-104, which is zero in float (-inf among them), begins anew: sums restart there
 // and pairs across it have a decay of exactly zero.
-struct ChunkDecay {
+struct alignas(16) ChunkDecay {
   float hi[kChunk], lo[kChunk];
   int from[kChunk];                      // the last step at or before that begins anew, or -1
   float into[kChunk], rest[kChunk], weight[kChunk];  // from before the chunk to a step, from a step to the chunk's end

@@ -11,7 +11,7 @@
 // next; E, A and P of the next chunks are made ahead of it.
 //
 // Roles of the block's warps: 4 keep the state (in tensor memory, one row of channels per thread), 4 write
-// outputs, 4 weigh and split k, 2 make P, one copies (TMA, two chunks in shared memory), one issues the matrix
+// outputs, 4 weigh and split k, 4 make P, one copies (TMA, three chunks in shared memory), one issues the matrix
 // instructions, one makes the decays. They meet at mbarriers; every wait gives up after two seconds, sets the status
 // word and ends the block.
 //
@@ -31,10 +31,10 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 
-constexpr int kThreads = 17 * 32;
-constexpr int kStages = 2;   // chunks of q, k, v in shared memory
+constexpr int kThreads = 19 * 32;
+constexpr int kStages = 3;   // chunks of q, k, v in shared memory
 constexpr int kSlots = 4;    // chunks whose decays are there
-constexpr int kPieces = 3;   // of w k
+constexpr int kPieces = 3;   // of w k: the code takes them to be three
 constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kColA = 0, kColX = 64, kColY = 128, kColE = 192, kColS = 320;
 
@@ -46,12 +46,25 @@ MPB_D void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: 
 MPB_D void commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-MPB_D void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
-      : "memory");
+// An operand's descriptor in two halves: the lower one moves with the address, in units of 16 bytes.
+struct Operand {
+  uint32_t lo, hi;
+};
+template <bool ADD>
+MPB_D void mma(uint32_t d, Operand a, int a_off, Operand b, int b_off, uint32_t idesc) {
+  const uint32_t al = a.lo + (uint32_t)(a_off >> 4), bl = b.lo + (uint32_t)(b_off >> 4);
+  if (ADD)
+    asm volatile(
+        "{\n\t.reg .b64 da, db;\n\t.reg .pred p;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\tsetp.eq.u32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d),
+        "r"(al), "r"(a.hi), "r"(bl), "r"(b.hi), "r"(idesc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .b64 da, db;\n\t.reg .pred p;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\tsetp.ne.u32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d),
+        "r"(al), "r"(a.hi), "r"(bl), "r"(b.hi), "r"(idesc)
+        : "memory");
 }
 MPB_D void tmem_load(uint32_t (&r)[32], uint32_t at) {
   asm volatile(
@@ -78,9 +91,8 @@ MPB_D void wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "me
 
 // A shared memory operand in the 128-byte swizzle: `group`, bytes between groups of eight rows of 128 bytes; `block`,
 // between blocks of 64 elements where the rows run along the other dim.
-MPB_D uint64_t operand(uint32_t at, uint32_t block, uint32_t group) {
-  return (uint64_t)((at >> 4) & 0x3fff) | (uint64_t)((block >> 4) & 0x3fff) << 16 | (uint64_t)((group >> 4) & 0x3fff) << 32 |
-         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+MPB_D Operand operand(uint32_t at, uint32_t block, uint32_t group) {
+  return {((at >> 4) & 0x3fff) | (block >> 4) << 16, (group >> 4) | 1u << 14 | 2u << 29};
 }
 // bf16 operands, float sums, 128 rows, n columns; ta, tb: an operand whose rows run along its own dim, not the summed one.
 constexpr uint32_t instruction(int n, bool ta, bool tb) {
@@ -95,14 +107,15 @@ MPB_D void tma_tile(uint32_t dst, const CUtensorMap* map, int x, int h, int t, i
 }
 
 // ------------------------------------------------------------ layout
-enum Bar { kFull0, kFull1, kEmpty0, kEmpty1, kDec0, kDec1, kDec2, kDec3, kADone, kAFree, kPReady, kWReady, kEDone, kEFree, kSReady,
+enum Bar { kFull0, kFull1, kFull2, kEmpty0, kEmpty1, kEmpty2, kDec0, kDec1, kDec2, kDec3, kADone, kAFree, kPReady, kWReady, kEDone, kEFree, kSReady,
            kXDone, kODone, kOFree, kFree0, kFree1, kFree2, kFree3, kEnd, kBars };
 
 template <int DK, int DV>
 struct Layout {
   static constexpr int kBlock = 64 * 128;  // 64 steps of 64 channels
   static constexpr int q = 0, k = q + DK / 64 * kBlock, v = k + DK / 64 * kBlock, kStage = v + DV / 64 * kBlock;
-  static constexpr int P = kStages * kStage, W = P + kBlock, S = W + kPieces * (DK / 64) * kBlock;
+  // the first piece of w k takes the place of k
+  static constexpr int P = kStages * kStage, W = P + kBlock, S = W + (kPieces - 1) * (DK / 64) * kBlock;
   // S has two blocks of 64 columns in any case: a left operand has 128 rows, and may read the second
   static constexpr int decays = S + 2 * DK * 128;
   static constexpr int bars = decays + kSlots * ((int)sizeof(ChunkDecay) + 15) / 16 * 16, tmem = bars + kBars * 8;
@@ -141,14 +154,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
   };
   if (tid == 0) {
     for (int i = 0; i < kBars; ++i) {
-      const int count = i >= kDec0 && i <= kDec3 ? 32 : i == kAFree || i == kPReady ? 64 : i == kWReady ? 128
+      const int count = i >= kDec0 && i <= kDec3 ? 32 : i == kAFree || i == kPReady || i == kWReady ? 128
                         : i == kEFree || i == kSReady ? DK : i == kOFree ? DV
                         : i >= kFree0 && i <= kFree3 ? DK + (OUT ? DV : 0) : 1;
       mbar_init(bar(i), count);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 16) {
+  if (warp == 18) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem + L::tmem), "n"(kTmemColumns)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -280,7 +293,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
           float f[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const float by = into[g * 32 + i];
+            const float4 four = *reinterpret_cast<const float4*>(into + g * 32 + (i & ~3));
+            const float by = (i & 3) == 0 ? four.x : (i & 3) == 1 ? four.y : (i & 3) == 2 ? four.z : four.w;
             f[i] = p.scale * (by != 0.0f ? fmaf(by, __uint_as_float(x[i]), __uint_as_float(y[i])) : __uint_as_float(y[i]));
           }
           if (g == 1) {
@@ -304,65 +318,76 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
     }
   } else if (warp < 12) {  // ------------------------------ the weighed k
     const int at = tid - 8 * 32;
+    constexpr int kWords = DK / 64 * kChunk * 8 / 128;
     for (int n = 0; n < n_chunks; ++n) {
       if (!wait_warp(kDec0 + n % kSlots, n / kSlots) || !wait_warp(kFull0 + n % kStages, n / kStages)) break;
-      if (n > 0 && !wait_warp(kEDone, n - 1)) break;
       const ChunkDecay& cd = decays[n % kSlots];
-      const unsigned char* from = mem + (n % kStages) * L::kStage + L::k;
+      unsigned char* from = mem + (n % kStages) * L::kStage + L::k + at * 16;
+      unsigned char* to = mem + L::W + at * 16;
+      union Word { uint4 q; uint32_t pair[4]; };
+      Word x[kWords];
+      float w[4];
 #pragma unroll
-      for (int i = 0; i < DK / 64 * kChunk * 8 / 128; ++i) {
-        const int word = at + i * 128, t = word / 8 % kChunk;
-        const float w = p.rev ? cd.into[t] * p.scale : cd.rest[t];
-        union { uint4 q; uint32_t pair[4]; } x, out[kPieces];
-        x.q = *reinterpret_cast<const uint4*>(from + word * 16);
+      for (int i = 0; i < kWords; ++i) x[i].q = *reinterpret_cast<const uint4*>(from + i * 2048);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = p.rev ? cd.into[at / 8 + 16 * i] * p.scale : cd.rest[at / 8 + 16 * i];
+      // the pieces go where matrix instructions still read: of the chunk before, and the scores
+      if ((n > 0 && !wait_warp(kEDone, n - 1)) || (OUT && !wait_warp(kADone, n))) break;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        Word out[kPieces];
+        const float by = w[i % 4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float2 f = make_float2(__uint_as_float(x.pair[j] << 16), __uint_as_float(x.pair[j] & 0xffff0000u));
-          f = w != 0.0f ? vmul(f, vset<2>(w)) : vset<2>(0.0f);
+          float2 f = make_float2(__uint_as_float(x[i].pair[j] << 16), __uint_as_float(x[i].pair[j] & 0xffff0000u));
+          f = by != 0.0f ? vmul(f, vset<2>(by)) : vset<2>(0.0f);
 #pragma unroll
           for (int k = 0; k < kPieces; ++k) {
             out[k].pair[j] = pack<bf16>(f).w;
             f = vadd(f, make_float2(-__uint_as_float(out[k].pair[j] << 16), -__uint_as_float(out[k].pair[j] & 0xffff0000u)));
           }
         }
+        *reinterpret_cast<uint4*>(from + i * 2048) = out[0].q;
 #pragma unroll
-        for (int k = 0; k < kPieces; ++k) *reinterpret_cast<uint4*>(mem + L::W + k * (DK / 64) * L::kBlock + word * 16) = out[k].q;
+        for (int k = 1; k < kPieces; ++k) *reinterpret_cast<uint4*>(to + (k - 1) * (DK / 64) * L::kBlock + i * 2048) = out[k].q;
       }
       proxy_fence();
       mbar_arrive(bar(kWReady));
     }
-  } else if (warp < 14) {  // --------------------------------- the scores
+  } else if (warp == 12 || warp == 13 || warp == 16 || warp == 17) {  // the scores: 32 rows and 32 columns of a warp
     if (OUT) {
+      const int half = warp >> 4;  // of the columns
       unsigned char* to = mem + L::P + row * 128;
       for (int n = 0; n < n_chunks; ++n) {
         if (!wait_warp(kDec0 + n % kSlots, n / kSlots) || !wait_warp(kADone, n)) break;
         fence_after();
         const ChunkDecay& cd = decays[n % kSlots];
-        uint32_t a[2][32];
-        tmem_load(a[0], quarter + kColA);
-        tmem_load(a[1], quarter + kColA + 32);
-        wait_loads();
+        uint4 w[4] = {};
+        if ((warp & 3) >= half) {
+          uint32_t a[32];
+          tmem_load(a, quarter + kColA + half * 32);
+          const float hi = cd.hi[row], lo = cd.lo[row];
+          const int from = cd.from[row];
+          wait_loads();
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const int j = half * 32 + c * 4;
+            const float4 hj = *reinterpret_cast<const float4*>(cd.hi + j), lj = *reinterpret_cast<const float4*>(cd.lo + j);
+            const float e[4] = {ex2f((hi - hj.x) + (lo - lj.x)), ex2f((hi - hj.y) + (lo - lj.y)), ex2f((hi - hj.z) + (lo - lj.z)),
+                                ex2f((hi - hj.w) + (lo - lj.w))};
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = j + i <= row && j + i >= from ? e[i] * __uint_as_float(a[c * 4 + i]) : 0.0f;
+            const uint32_t x = pack<bf16>(make_float2(f[0], f[1])).w, y = pack<bf16>(make_float2(f[2], f[3])).w;
+            if (c & 1) w[c >> 1].z = x, w[c >> 1].w = y;
+            else w[c >> 1].x = x, w[c >> 1].y = y;
+          }
+        }
         fence_before();
         mbar_arrive(bar(kAFree));
-        const float hi = cd.hi[row], lo = cd.lo[row];
-        const int from = cd.from[row];
         if (n > 0 && !wait_warp(kODone, n - 1)) break;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          float f[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int j = c * 8 + i;
-            const float e = ex2f((hi - cd.hi[j]) + (lo - cd.lo[j]));
-            f[i] = j <= row && j >= from ? e * __uint_as_float(a[c >> 2][(c & 3) * 8 + i]) : 0.0f;
-          }
-          uint4 w;
-          w.x = pack<bf16>(make_float2(f[0], f[1])).w;
-          w.y = pack<bf16>(make_float2(f[2], f[3])).w;
-          w.z = pack<bf16>(make_float2(f[4], f[5])).w;
-          w.w = pack<bf16>(make_float2(f[6], f[7])).w;
-          *reinterpret_cast<uint4*>(to + ((c ^ (row & 7)) << 4)) = w;
-        }
+        for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(to + (((half * 4 + c) ^ (row & 7)) << 4)) = w[c];
         proxy_fence();
         mbar_arrive(bar(kPReady));
       }
@@ -385,13 +410,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
   } else if (warp == 15) {  // ------------------- the matrix instructions
     if (lane == 0) {
       constexpr uint32_t kScores = instruction(64, false, false), kSum = instruction(DV, true, true), kOut = instruction(64, true, false);
-      auto scores = [&](int n) {
-        const uint32_t at = smem + (n % kStages) * L::kStage;
+      const Operand q0 = operand(smem + L::q, 16, 1024), k0 = operand(smem + L::k, 16, 1024), kt0 = operand(smem + L::k, kOther, 1024),
+                    vt0 = operand(smem + L::v, kOther, 1024), w0 = operand(smem + L::W, kOther, 1024),
+                    s0 = operand(smem + L::S, DK * 128, 1024), p0 = operand(smem + L::P, 16, 1024);
+      auto in_stage = [&](Operand o, int s) { return Operand{o.lo + (uint32_t)(s * (L::kStage >> 4)), o.hi}; };
+      constexpr int kPiece = DK / 64 * L::kBlock;
+      auto scores = [&](int s) {
+        const Operand q = in_stage(q0, s), k = in_stage(k0, s);
+        mma<false>(tmem + kColA, q, 0, k, 0, kScores);
 #pragma unroll
-        for (int i = 0; i < DK / 16; ++i) {
-          const uint32_t o = (i / 4) * L::kBlock + (i % 4) * 32;
-          mma(tmem + kColA, operand(at + L::q + o, 16, 1024), operand(at + L::k + o, 16, 1024), kScores, i > 0);
-        }
+        for (int i = 1; i < DK / 16; ++i)
+          mma<true>(tmem + kColA, q, (i / 4) * L::kBlock + (i % 4) * 32, k, (i / 4) * L::kBlock + (i % 4) * 32, kScores);
         commit(bar(kADone));
       };
       if (OUT && n_chunks > 0 && wait(kFull0, 0)) {
@@ -399,40 +428,43 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         scores(0);
       }
       for (int n = 0; n < n_chunks; ++n) {
-        const uint32_t at = smem + (n % kStages) * L::kStage;
-        if (!wait(kWReady, n) || !wait(kFull0 + n % kStages, n / kStages)) break;
+        const int st = n % kStages, next = (n + 1) % kStages;
+        const Operand kt = in_stage(kt0, st), vt = in_stage(vt0, st);
+        if (!wait(kWReady, n) || !wait(kFull0 + st, n / kStages)) break;
         if (n > 0 && !wait(kEFree, n - 1)) break;
         fence_after();
+        // the small pieces first
+        mma<false>(tmem + kColE, w0, kPiece, vt, 0, kSum);
 #pragma unroll
-        for (int k = 0; k < kPieces; ++k)  // the small pieces first
+        for (int i = 1; i < 4; ++i) mma<true>(tmem + kColE, w0, kPiece + i * 2048, vt, i * 2048, kSum);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            mma(tmem + kColE, operand(smem + L::W + (kPieces - 1 - k) * (DK / 64) * L::kBlock + i * 2048, kOther, 1024),
-                operand(at + L::v + i * 2048, kOther, 1024), kSum, k + i > 0);
+        for (int i = 0; i < 4; ++i) mma<true>(tmem + kColE, w0, i * 2048, vt, i * 2048, kSum);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mma<true>(tmem + kColE, kt, i * 2048, vt, i * 2048, kSum);
         commit(bar(kEDone));
         if (!OUT) {
-          commit(bar(kEmpty0 + n % kStages));
+          commit(bar(kEmpty0 + st));
           continue;
         }
         if (n + 1 < n_chunks) {
-          if (!wait(kFull0 + (n + 1) % kStages, (n + 1) / kStages) || !wait(kAFree, n)) break;
+          if (!wait(kFull0 + next, (n + 1) / kStages) || !wait(kAFree, n)) break;
           fence_after();
-          scores(n + 1);
+          scores(next);
         }
         if (!wait(kSReady, n) || (n > 0 && !wait(kOFree, n - 1))) break;
         fence_after();
+        const Operand q = in_stage(q0, st);
+        mma<false>(tmem + kColX, s0, 0, q, 0, kOut);
 #pragma unroll
-        for (int i = 0; i < DK / 16; ++i)
-          mma(tmem + kColX, operand(smem + L::S + i * 2048, DK * 128, 1024),
-              operand(at + L::q + (i / 4) * L::kBlock + (i % 4) * 32, 16, 1024), kOut, i > 0);
+        for (int i = 1; i < DK / 16; ++i) mma<true>(tmem + kColX, s0, i * 2048, q, (i / 4) * L::kBlock + (i % 4) * 32, kOut);
         commit(bar(kXDone));
         if (!wait(kPReady, n)) break;
         fence_after();
+        mma<false>(tmem + kColY, vt, 0, p0, 0, kOut);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          mma(tmem + kColY, operand(at + L::v + i * 2048, kOther, 1024), operand(smem + L::P + i * 32, 16, 1024), kOut, i > 0);
+        for (int i = 1; i < 4; ++i) mma<true>(tmem + kColY, vt, i * 2048, p0, i * 32, kOut);
         commit(bar(kODone));
-        commit(bar(kEmpty0 + n % kStages));
+        commit(bar(kEmpty0 + st));
       }
     }
   } else {  // --------------------------------------------- the decays
@@ -456,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 16)
+  if (warp == 18)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemColumns) : "memory");
 }
 
