@@ -296,8 +296,8 @@ int mpb_policy_loss(int64_t N, int64_t V, const void* logits, int dtype, int64_t
  *   S = e^log_decay S + k v',   o = scale S' q.
  * Writes o (B, T, H, DV) and, when state is not NULL, the last S (state0 when T == 0); state may
  * not overlap state0. A log-decay below -104 is a decay of zero: what came before has no part from there on.
- * Channels per head: 1 to 256. Scratch: mpb_linear_attention_scratch_bytes; it is less where `aligned` says that q, k, v (and
- * dout) are 16-byte aligned with strides that are positive multiples of 16 bytes, and has to be asked for so or not as the call's are. Values are finite: one that is not may reach every result of its chunk of 64 steps
+ * Channels per head: 1 to 256. Scratch: mpb_linear_attention_scratch_bytes; it is less where `aligned` says that q, k, v and o
+ * (backward: q, k, v and dout) are 16-byte aligned with strides that are positive multiples of 16 bytes, and has to be asked for so or not as the call's are. Values are finite: one that is not may reach every result of its chunk of 64 steps
  * and the later ones. */
 size_t mpb_linear_attention_scratch_bytes(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK, int64_t DV, int dtype,
                                           int backward, int decay_by_head, int aligned);

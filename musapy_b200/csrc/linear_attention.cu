@@ -320,24 +320,45 @@ __global__ void __launch_bounds__(kThreads) k_la_states(States p) {
   }
 }
 
-// The segments' sums become the states before them, in place; the last one goes to `last`.
+// The segments' sums become the states before them, in place; the last one goes to `last`. A thread has four neighbouring
+// elements of one head's state, loads the sums of eight segments at once and then runs through them.
+constexpr int kJoinAhead = 8;
 template <bool REV>
-__global__ void __launch_bounds__(256) k_la_join(States p) {
+__global__ void __launch_bounds__(128) k_la_join(States p) {
   const Shape& d = p.d;
-  const int64_t size = (int64_t)d.dkp * d.dvp, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= d.B * d.H * size) return;
-  const int64_t bh = e / size, i = e - bh * size;
-  const float* decay = p.since + (bh + d.B * d.H) * d.chunks;
-  float s = 0.0f;
-  for (int n = 0; n < d.segments; ++n) {
-    const int seg = REV ? d.segments - 1 - n : n;
-    float* at = p.ends + (bh * d.segments + seg) * size + i;
-    const float own = *at, a = decay[seg];
-    *at = s;
-    s = n == 0 || a == 0.0f ? own : fmaf(a, s, own);
+  const int size = d.dkp * d.dvp, i = (blockIdx.x * 128 + threadIdx.x) * 4;
+  if (i >= size) return;
+  const int r = i / d.dvp, c = i % d.dvp;
+  for (int64_t bh = blockIdx.y; bh < d.B * d.H; bh += gridDim.y) {
+    const float* decay = p.since + (bh + d.B * d.H) * d.chunks;
+    float4* ends = reinterpret_cast<float4*>(p.ends + bh * d.segments * size + i);
+    auto seg = [&](int n) { return REV ? d.segments - 1 - n : n; };
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int n0 = 0; n0 < d.segments; n0 += kJoinAhead) {
+      float4 own[kJoinAhead];
+      float a[kJoinAhead];
+#pragma unroll
+      for (int k = 0; k < kJoinAhead; ++k)
+        if (n0 + k < d.segments) own[k] = ends[(int64_t)seg(n0 + k) * (size / 4)], a[k] = decay[seg(n0 + k)];
+#pragma unroll
+      for (int k = 0; k < kJoinAhead; ++k)
+        if (n0 + k < d.segments) {
+          ends[(int64_t)seg(n0 + k) * (size / 4)] = s;
+          if (n0 + k > 0 && a[k] != 0.0f) {
+            own[k].x = fmaf(a[k], s.x, own[k].x), own[k].y = fmaf(a[k], s.y, own[k].y);
+            own[k].z = fmaf(a[k], s.z, own[k].z), own[k].w = fmaf(a[k], s.w, own[k].w);
+          }
+          s = own[k];
+        }
+    }
+    if (p.last && r < d.DK) {
+      float* to = p.last + bh * d.DK * d.DV + (int64_t)r * d.DV + c;
+      if (c < d.DV) to[0] = s.x;
+      if (c + 1 < d.DV) to[1] = s.y;
+      if (c + 2 < d.DV) to[2] = s.z;
+      if (c + 3 < d.DV) to[3] = s.w;
+    }
   }
-  const int r = (int)(i / d.dvp), c = (int)(i % d.dvp);
-  if (p.last && r < d.DK && c < d.DV) p.last[bh * d.DK * d.DV + (int64_t)r * d.DV + c] = s;
 }
 
 struct StateSet {
@@ -655,7 +676,10 @@ struct Step {
 };
 
 constexpr int kStepThreads = 256;
-// A block updates the state of one head: a thread takes V neighbouring columns of every (256 / lanes)-th row.
+constexpr int kStepRows = 8;  // of the state that a thread has under way
+
+// A block updates the state of one head: a thread takes V neighbouring columns of every (256 / lanes)-th row. The state is
+// read and written once and not looked at again soon: evict-first, in both directions.
 template <class T, int V>
 __global__ void __launch_bounds__(kStepThreads) k_la_step(Step p) {
   __shared__ float qs[kMostChannels], ks[kMostChannels], part[kStepThreads * V];
@@ -663,7 +687,20 @@ __global__ void __launch_bounds__(kStepThreads) k_la_step(Step p) {
   const int h = (int)(bh % p.H), lanes = (p.DV + V - 1) / V, groups = kStepThreads / lanes;
   const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes, c = lane * V;
   const bool on = group < groups;
-  float* S = p.state + bh * p.DK * p.DV;
+  float* S = p.state + bh * p.DK * p.DV + c;
+  using W = typename Word<4 * V>::type;
+  union Cell { W w; float f[V]; };
+  auto load = [&](Cell (&x)[kStepRows], int r0) {
+#pragma unroll
+    for (int k = 0; k < kStepRows; ++k)
+      if (r0 + k * groups < p.DK) {
+        const W* at = reinterpret_cast<const W*>(S + (int64_t)(r0 + k * groups) * p.DV);
+        if constexpr (V == 4) x[k].w = ld_stream16(at);
+        else x[k].w = *at;
+      }
+  };
+  Cell x[kStepRows];
+  if (on) load(x, group);
   for (int i = threadIdx.x; i < p.DK; i += kStepThreads) {
     qs[i] = to_f(p.q.at<T>(b, 0, h / p.share)[i]) * p.scale;
     ks[i] = to_f(p.k.at<T>(b, 0, h / p.share)[i]);
@@ -675,17 +712,21 @@ __global__ void __launch_bounds__(kStepThreads) k_la_step(Step p) {
   for (int j = 0; j < V; ++j) v[j] = on && c + j < p.DV ? to_f(vp[c + j]) : 0.0f, o[j] = 0.0f;
   __syncthreads();
   if (on) {
-#pragma unroll 8
-    for (int r = group; r < p.DK; r += groups) {
-      using W = typename Word<4 * V>::type;
-      union { W w; float f[V]; } x;
-      x.w = *reinterpret_cast<const W*>(S + (int64_t)r * p.DV + c);
+    for (int r0 = group; r0 < p.DK; r0 += kStepRows * groups) {
+      if (r0 != group) load(x, r0);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        x.f[j] = fmaf(ks[r], v[j], a != 0.0f ? a * x.f[j] : 0.0f);
-        o[j] = fmaf(qs[r], x.f[j], o[j]);
+      for (int k = 0; k < kStepRows; ++k) {
+        const int r = r0 + k * groups;
+        if (r >= p.DK) break;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          x[k].f[j] = fmaf(ks[r], v[j], a != 0.0f ? a * x[k].f[j] : 0.0f);
+          o[j] = fmaf(qs[r], x[k].f[j], o[j]);
+        }
+        W* at = reinterpret_cast<W*>(S + (int64_t)r * p.DV);
+        if constexpr (V == 4) st_stream16(at, x[k].w);
+        else *at = x[k].w;
       }
-      *reinterpret_cast<W*>(S + (int64_t)r * p.DV + c) = x.w;
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) part[(group * lanes + lane) * V + j] = o[j];
@@ -731,7 +772,7 @@ struct StateScratch {
 constexpr size_t kStatusBytes = 16;  // the status word leads the scratch
 
 // Whether the walk of whole rows may be taken, as far as the layout does not decide.
-bool may_walk(int dtype, int64_t DK, int64_t DV, bool aligned) { return aligned && dtype == MPB_BF16 && DK <= 128 && DV <= 128; }
+bool may_walk(int dtype, int64_t DK, int64_t DV, bool aligned) { return aligned && dtype == MPB_BF16 && DK <= 128 && DV <= 128 && DV % 8 == 0; }
 
 // The walk's segments: as many as give every SM a block. They cost a walk more over k and v.
 Shape walk_shape(Shape d) {
@@ -750,9 +791,10 @@ Input make_input(const void* p, int64_t sb, int64_t st, int64_t sh, size_t e) {
 int join_states(const States& p, bool rev, cudaStream_t s) {
   const Shape& d = p.d;
   if (d.segments == 1) return MPB_OK;
-  const unsigned blocks = (unsigned)((d.B * d.H * d.dkp * d.dvp + 255) / 256);
-  if (rev) k_la_join<true><<<blocks, 256, 0, s>>>(p);
-  else k_la_join<false><<<blocks, 256, 0, s>>>(p);
+  const int64_t heads = d.B * d.H;
+  const dim3 blocks((unsigned)((d.dkp * d.dvp / 4 + 127) / 128), (unsigned)(heads < 65535 ? heads : 65535));
+  if (rev) k_la_join<true><<<blocks, 128, 0, s>>>(p);
+  else k_la_join<false><<<blocks, 128, 0, s>>>(p);
   return launch_check("linear_attention");
 }
 
@@ -927,7 +969,7 @@ int mpb_linear_attention(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK
   const Shape d = make_shape(B, T, H, Hq, DK, DV);
   const size_t e = bytes_of(dtype);
   const Input qi = make_input(q, q_sb, q_st, q_sh, e), ki = make_input(k, k_sb, k_st, k_sh, e), vi = make_input(v, v_sb, v_st, v_sh, e);
-  const bool walk = may_walk(dtype, DK, DV, true) && walk_takes(d, qi, ki, vi);
+  const bool walk = may_walk(dtype, DK, DV, (uintptr_t)o % 16 == 0) && walk_takes(d, qi, ki, vi);
   if (int rc = check_scratch(name, mpb_linear_attention_scratch_bytes(B, T, H, Hq, DK, DV, dtype, 0, 0, walk), scratch, scratch_bytes))
     return rc;
   const Decay g = {log_decay, g_sb, g_st, g_sh};

@@ -10,9 +10,9 @@
 // it is half a step of the output's type, and the state itself keeps 32 bits. Only that sum ties a chunk to the
 // next; E, A and P of the next chunks are made ahead of it.
 //
-// Roles of the block's warps: 4 keep the state (in tensor memory, one row of channels per thread), 4 write
-// outputs, 4 weigh and split k, 4 make P, one copies (TMA, three chunks in shared memory), one issues the matrix
-// instructions, one makes the decays. They meet at mbarriers; every wait gives up after two seconds, sets the status
+// Roles of the block's warps: 8 keep the state (in tensor memory, half a row of channels per thread), 4 write
+// outputs (where q was, for a copy to take them), 8 weigh and split k, 4 make P, one copies in (TMA, three chunks in
+// shared memory), one copies out, one issues the matrix instructions, one makes the decays. They meet at mbarriers; every wait gives up after some seconds, sets the status
 // word and ends the block.
 //
 // Operands lie as the copies leave them, rows of 128 bytes in the 128-byte swizzle; what is needed transposed (k, v, S as
@@ -31,12 +31,21 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 
-constexpr int kThreads = 19 * 32;
+constexpr int kThreads = 28 * 32;
 constexpr int kStages = 3;   // chunks of q, k, v in shared memory
 constexpr int kSlots = 4;    // chunks whose decays are there
 constexpr int kPieces = 3;   // of w k: the code takes them to be three
 constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kColA = 0, kColX = 64, kColY = 128, kColE = 192, kColS = 320;
+
+// A bounded wait in few instructions: there are many of them. A try itself waits for a while, so that 2^22 of
+// them are seconds.
+MPB_D bool mbar_wait_short(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < 1 << 22; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return false;
+}
 
 // ------------------------------------------------------- tensor core
 MPB_D void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
@@ -66,24 +75,23 @@ MPB_D void mma(uint32_t d, Operand a, int a_off, Operand b, int b_off, uint32_t 
         "r"(al), "r"(a.hi), "r"(bl), "r"(b.hi), "r"(idesc)
         : "memory");
 }
-MPB_D void tmem_load(uint32_t (&r)[32], uint32_t at) {
+MPB_D void tmem_load(uint32_t (&r)[16], uint32_t at) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(at));
 }
-MPB_D void tmem_store(uint32_t at, const uint32_t (&r)[32]) {
+MPB_D void tmem_load(uint32_t (&r)[8], uint32_t at) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(at));
+}
+MPB_D void tmem_store(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
       "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
-      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
-      "r"(at)
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(at)
       : "memory");
 }
 MPB_D void wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -106,9 +114,15 @@ MPB_D void tma_tile(uint32_t dst, const CUtensorMap* map, int x, int h, int t, i
       : "memory");
 }
 
+MPB_D void tma_write(const CUtensorMap* map, uint32_t src, int x, int h, int t, int b) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map), "r"(src), "r"(x),
+               "r"(h), "r"(t), "r"(b)
+               : "memory");
+}
+
 // ------------------------------------------------------------ layout
-enum Bar { kFull0, kFull1, kFull2, kEmpty0, kEmpty1, kEmpty2, kDec0, kDec1, kDec2, kDec3, kADone, kAFree, kPReady, kWReady, kEDone, kEFree, kSReady,
-           kXDone, kODone, kOFree, kFree0, kFree1, kFree2, kFree3, kEnd, kBars };
+enum Bar { kFull0, kFull1, kFull2, kEmpty0, kEmpty1, kEmpty2, kDec0, kDec1, kDec2, kDec3, kADone0, kADone1, kAFree, kPReady, kWReady, kEDone, kEFree, kSReady,
+           kXDone, kODone, kOFree, kOReady0, kOReady1, kOReady2, kFree0, kFree1, kFree2, kFree3, kEnd, kBars };
 
 template <int DK, int DV>
 struct Layout {
@@ -123,7 +137,7 @@ struct Layout {
 };
 
 struct Maps {
-  CUtensorMap q, k, v;
+  CUtensorMap q, k, v, o;
 };
 
 template <int DK, int DV, bool OUT>
@@ -145,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
   bool ok = true;
   // true where the phase of chunk n has come
   auto wait = [&](int i, int n) {
-    if (ok) ok = mbar_wait(bar(i), (uint32_t)n & 1);
+    if (ok) ok = mbar_wait_short(bar(i), (uint32_t)n & 1);
     return ok;
   };
   auto wait_warp = [&](int i, int n) {
@@ -154,14 +168,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
   };
   if (tid == 0) {
     for (int i = 0; i < kBars; ++i) {
-      const int count = i >= kDec0 && i <= kDec3 ? 32 : i == kAFree || i == kPReady || i == kWReady ? 128
-                        : i == kEFree || i == kSReady ? DK : i == kOFree ? DV
-                        : i >= kFree0 && i <= kFree3 ? DK + (OUT ? DV : 0) : 1;
+      const int count = i >= kDec0 && i <= kDec3 ? 32 : i == kAFree || i == kPReady ? 128 : i == kWReady ? 256
+                        : i == kEFree || i == kSReady ? 2 * DK : i == kOFree || (i >= kOReady0 && i <= kOReady2) ? DV
+                        : OUT && i >= kEmpty0 && i <= kEmpty2 ? 2
+                        : i >= kFree0 && i <= kFree3 ? 2 * DK + (OUT ? DV : 0) : 1;
       mbar_init(bar(i), count);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 18) {
+  if (warp == 26) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem + L::tmem), "n"(kTmemColumns)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -174,8 +189,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
   const int row = (warp & 3) * 32 + lane;
   constexpr uint32_t kOther = L::kBlock;
 
-  if (warp < 4) {  // ------------------------------------------- the state
+  if (warp < 8) {  // ------------------------------------------- the state
     if (row < DK) {
+      constexpr int kGroups = DV / 32;  // of 16 columns, of a thread: half of its row of the state
+      const int col0 = (warp >> 2) * (DV / 2);
       const int64_t size = (int64_t)d.dkp * d.dvp;
       const float* first = nullptr;
       int pitch = 0;
@@ -187,25 +204,30 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         first = p.starts + (bh * d.segments + seg) * size + (int64_t)row * d.dvp, pitch = d.dvp, have = row < d.dkp;
       }
       unsigned char* s_row = mem + L::S + row * 128;
-      // 32 columns of S to shared memory, rounded
-      auto put = [&](int g, const uint32_t (&s)[32]) {
+      const uint32_t s_tmem = quarter + kColS + col0, e_tmem = quarter + kColE + col0;
+      // 16 columns of S to shared memory, rounded
+      auto put = [&](int g, const uint32_t (&s)[16]) {
+        const int c = col0 + g * 16;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int k = 0; k < 2; ++k) {
           uint4 w;
-          w.x = pack<bf16>(make_float2(__uint_as_float(s[8 * c]), __uint_as_float(s[8 * c + 1]))).w;
-          w.y = pack<bf16>(make_float2(__uint_as_float(s[8 * c + 2]), __uint_as_float(s[8 * c + 3]))).w;
-          w.z = pack<bf16>(make_float2(__uint_as_float(s[8 * c + 4]), __uint_as_float(s[8 * c + 5]))).w;
-          w.w = pack<bf16>(make_float2(__uint_as_float(s[8 * c + 6]), __uint_as_float(s[8 * c + 7]))).w;
-          const int at = (g & 1) * 4 + c;
-          *reinterpret_cast<uint4*>(s_row + (g >> 1) * (DK * 128) + ((at ^ (row & 7)) << 4)) = w;
+          w.x = pack<bf16>(make_float2(__uint_as_float(s[8 * k]), __uint_as_float(s[8 * k + 1]))).w;
+          w.y = pack<bf16>(make_float2(__uint_as_float(s[8 * k + 2]), __uint_as_float(s[8 * k + 3]))).w;
+          w.z = pack<bf16>(make_float2(__uint_as_float(s[8 * k + 4]), __uint_as_float(s[8 * k + 5]))).w;
+          w.w = pack<bf16>(make_float2(__uint_as_float(s[8 * k + 6]), __uint_as_float(s[8 * k + 7]))).w;
+          const int at = c / 8 % 8 + k;
+          *reinterpret_cast<uint4*>(s_row + c / 64 * (DK * 128) + ((at ^ (row & 7)) << 4)) = w;
         }
       };
 #pragma unroll 1
-      for (int g = 0; g < DV / 32; ++g) {
-        uint32_t s[32];
+      for (int g = 0; g < kGroups; ++g) {
+        uint32_t s[16];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) s[i] = have && g * 32 + i < pitch ? __float_as_uint(first[g * 32 + i]) : 0u;
-        tmem_store(quarter + kColS + g * 32, s);
+        for (int i = 0; i < 16; ++i) {
+          const int c = col0 + g * 16 + i;
+          s[i] = have && c < pitch ? __float_as_uint(first[c]) : 0u;
+        }
+        tmem_store(s_tmem + g * 16, s);
         if (OUT) put(g, s);
       }
       wait_stores();
@@ -218,34 +240,39 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         const int c = chunk(n);
         if (!wait_warp(kDec0 + n % kSlots, n / kSlots)) break;
         const float all = decays[n % kSlots].all;
-        if (p.since && row == 0) p.since[bh * d.chunks + c] = since;
+        if (p.since && row == 0 && col0 == 0) p.since[bh * d.chunks + c] = since;
         since *= all;
         if (!wait_warp(kEDone, n)) break;
-        if (OUT && !wait_warp(kXDone, n)) break;
         fence_after();
-        float* at = p.at ? p.at + (bh * d.chunks + c) * size + (int64_t)row * d.dvp : nullptr;
-#pragma unroll 1
-        for (int g = 0; g < DV / 32; ++g) {
-          uint32_t e[32], s[32];
-          tmem_load(e, quarter + kColE + g * 32);
-          tmem_load(s, quarter + kColS + g * 32);
+        float* at = p.at ? p.at + (bh * d.chunks + c) * size + (int64_t)row * d.dvp + col0 : nullptr;
+        const int width = row < d.dkp ? d.dvp - col0 : 0;
+        uint32_t e[2][16], s[2][16];
+        tmem_load(e[0], e_tmem);
+        tmem_load(s[0], s_tmem);
+        if (OUT && !wait_warp(kXDone, n)) break;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          uint32_t(&eg)[16] = e[g & 1], (&sg)[16] = s[g & 1];
           wait_loads();
-          if (g == DV / 32 - 1) {
+          if (g + 1 < kGroups) {
+            tmem_load(e[g + 1 & 1], e_tmem + (g + 1) * 16);
+            tmem_load(s[g + 1 & 1], s_tmem + (g + 1) * 16);
+          } else {
             fence_before();
             mbar_arrive(bar(kEFree));
             mbar_arrive(bar(kFree0 + n % kSlots));
           }
-          if (at && row < d.dkp) {
+          if (!OUT && at) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              if (g * 32 + i < d.dvp)
-                *reinterpret_cast<uint4*>(at + g * 32 + i) = make_uint4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+            for (int i = 0; i < 16; i += 4)
+              if (g * 16 + i < width)
+                *reinterpret_cast<uint4*>(at + g * 16 + i) = make_uint4(sg[i], sg[i + 1], sg[i + 2], sg[i + 3]);
           }
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            s[i] = all == 0.0f ? e[i] : __float_as_uint(fmaf(all, __uint_as_float(s[i]), __uint_as_float(e[i])));
-          tmem_store(quarter + kColS + g * 32, s);
-          if (OUT) put(g, s);
+          for (int i = 0; i < 16; ++i)
+            sg[i] = all == 0.0f ? eg[i] : __float_as_uint(fmaf(all, __uint_as_float(sg[i]), __uint_as_float(eg[i])));
+          tmem_store(s_tmem + g * 16, sg);
+          if (OUT) put(g, sg);
         }
         wait_stores();
         if (OUT) {
@@ -258,114 +285,113 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         const bool whole = d.segments == 1;
         float* to = whole ? (p.last ? p.last + bh * d.DK * d.DV + (int64_t)row * d.DV : nullptr)
                           : (p.ends ? p.ends + (bh * d.segments + seg) * size + (int64_t)row * d.dvp : nullptr);
-        const int width = whole ? d.DV : d.dvp;
-        if (p.ends && !whole && row == 0) p.since[(bh + d.B * d.H) * d.chunks + seg] = since;
+        const int width = row < (whole ? d.DK : d.dkp) && to ? (whole ? d.DV : d.dvp) : 0;
+        if (p.ends && !whole && row == 0 && col0 == 0) p.since[(bh + d.B * d.H) * d.chunks + seg] = since;
 #pragma unroll 1
-        for (int g = 0; g < DV / 32; ++g) {
-          uint32_t s[32];
-          tmem_load(s, quarter + kColS + g * 32);
+        for (int g = 0; g < kGroups; ++g) {
+          uint32_t s[16];
+          tmem_load(s, s_tmem + g * 16);
           wait_loads();
-          if (to && row < (whole ? d.DK : d.dkp)) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (g * 32 + i < width) to[g * 32 + i] = __uint_as_float(s[i]);
-          }
+          for (int i = 0; i < 16; ++i)
+            if (col0 + g * 16 + i < width) to[col0 + g * 16 + i] = __uint_as_float(s[i]);
         }
       }
     }
-  } else if (warp < 8) {  // ------------------------------------ outputs
+  } else if (warp < 12) {  // ----------------------------------- outputs
     if (OUT && row < DV) {
-      bf16* o = (bf16*)p.o + ((b * d.T) * d.H + h) * d.DV + row;
-      const int64_t step = (int64_t)d.H * d.DV;
-      const bool mine = row < d.DV;
+      const float2 scale = vset<2>(p.scale);
       for (int n = 0; n < n_chunks; ++n) {
-        const int64_t t0 = (int64_t)chunk(n) * kChunk;
-        const int steps = (int)min((int64_t)kChunk, d.T - t0);
         if (!wait_warp(kDec0 + n % kSlots, n / kSlots) || !wait_warp(kODone, n)) break;
         fence_after();
         const float* into = decays[n % kSlots].into;
-#pragma unroll 1
-        for (int g = 0; g < 2; ++g) {
-          uint32_t x[32], y[32];
-          tmem_load(x, quarter + kColX + g * 32);
-          tmem_load(y, quarter + kColY + g * 32);
+        // the outputs take the place of q, laid out like it, and are copied from there
+        unsigned char* to = mem + (n % kStages) * L::kStage + row / 64 * L::kBlock + row % 8 * 2;
+        const int word = row / 8 % 8;
+        uint32_t two[32];  // outputs of two steps each
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          uint32_t x[8], y[8];
+          tmem_load(x, quarter + kColX + g * 8);
+          tmem_load(y, quarter + kColY + g * 8);
           wait_loads();
-          float f[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float4 four = *reinterpret_cast<const float4*>(into + g * 32 + (i & ~3));
-            const float by = (i & 3) == 0 ? four.x : (i & 3) == 1 ? four.y : (i & 3) == 2 ? four.z : four.w;
-            f[i] = p.scale * (by != 0.0f ? fmaf(by, __uint_as_float(x[i]), __uint_as_float(y[i])) : __uint_as_float(y[i]));
-          }
-          if (g == 1) {
-            fence_before();
-            mbar_arrive(bar(kOFree));
-            mbar_arrive(bar(kFree0 + n % kSlots));
-          }
-          bf16* to = o + (t0 + g * 32) * step;
-          if (mine) {
-            if (steps == kChunk) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) to[i * step] = __float2bfloat16_rn(f[i]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (g * 32 + i < steps) to[i * step] = __float2bfloat16_rn(f[i]);
-            }
+          for (int i = 0; i < 8; i += 2) {
+            const float2 by = *reinterpret_cast<const float2*>(into + g * 8 + i);
+            float2 v = make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+            // what a decay of zero has dropped may be anything
+            v.x = by.x != 0.0f ? v.x : 0.0f;
+            v.y = by.y != 0.0f ? v.y : 0.0f;
+            two[g * 4 + i / 2] = pack<bf16>(vmul(vfma(by, v, make_float2(__uint_as_float(y[i]), __uint_as_float(y[i + 1]))), scale)).w;
           }
         }
+        // more channels than q has: the place of k too, once the state's sum has been made from it
+        if (DV > DK && !wait_warp(kEDone, n)) break;
+        fence_before();
+        mbar_arrive(bar(kOFree));
+        mbar_arrive(bar(kFree0 + n % kSlots));
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const uint32_t x = two[i];
+          *reinterpret_cast<uint16_t*>(to + 2 * i * 128 + ((word ^ (2 * i & 7)) << 4)) = (uint16_t)x;
+          *reinterpret_cast<uint16_t*>(to + (2 * i + 1) * 128 + ((word ^ (2 * i + 1 & 7)) << 4)) = (uint16_t)(x >> 16);
+        }
+        proxy_fence();
+        mbar_arrive(bar(kOReady0 + n % kStages));
       }
     }
-  } else if (warp < 12) {  // ------------------------------ the weighed k
-    const int at = tid - 8 * 32;
-    constexpr int kWords = DK / 64 * kChunk * 8 / 128;
+  } else if (warp < 20) {  // ------------------------------ the weighed k
+    const int at = tid - 12 * 32;
+    constexpr int kWords = DK / 64 * kChunk * 8 / 256;
     for (int n = 0; n < n_chunks; ++n) {
       if (!wait_warp(kDec0 + n % kSlots, n / kSlots) || !wait_warp(kFull0 + n % kStages, n / kStages)) break;
       const ChunkDecay& cd = decays[n % kSlots];
       unsigned char* from = mem + (n % kStages) * L::kStage + L::k + at * 16;
       unsigned char* to = mem + L::W + at * 16;
       union Word { uint4 q; uint32_t pair[4]; };
-      Word x[kWords];
-      float w[4];
+      Word x[kPieces][kWords];
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) x[i].q = *reinterpret_cast<const uint4*>(from + i * 2048);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = p.rev ? cd.into[at / 8 + 16 * i] * p.scale : cd.rest[at / 8 + 16 * i];
-      // the pieces go where matrix instructions still read: of the chunk before, and the scores
-      if ((n > 0 && !wait_warp(kEDone, n - 1)) || (OUT && !wait_warp(kADone, n))) break;
+      for (int i = 0; i < kWords; ++i) x[0][i].q = *reinterpret_cast<const uint4*>(from + i * 4096);
 #pragma unroll
       for (int i = 0; i < kWords; ++i) {
-        Word out[kPieces];
-        const float by = w[i % 4];
+        const int t = (at / 8 + 32 * i) % kChunk;
+        const float by = p.rev ? cd.into[t] * p.scale : cd.rest[t];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float2 f = make_float2(__uint_as_float(x[i].pair[j] << 16), __uint_as_float(x[i].pair[j] & 0xffff0000u));
+          float2 f = make_float2(__uint_as_float(x[0][i].pair[j] << 16), __uint_as_float(x[0][i].pair[j] & 0xffff0000u));
           f = by != 0.0f ? vmul(f, vset<2>(by)) : vset<2>(0.0f);
 #pragma unroll
           for (int k = 0; k < kPieces; ++k) {
-            out[k].pair[j] = pack<bf16>(f).w;
-            f = vadd(f, make_float2(-__uint_as_float(out[k].pair[j] << 16), -__uint_as_float(out[k].pair[j] & 0xffff0000u)));
+            const uint32_t h2 = pack<bf16>(f).w;
+            x[k][i].pair[j] = h2;
+            f = vfma(make_float2(__uint_as_float(h2 << 16), __uint_as_float(h2 & 0xffff0000u)), vset<2>(-1.0f), f);
           }
         }
-        *reinterpret_cast<uint4*>(from + i * 2048) = out[0].q;
+      }
+      // the pieces go where matrix instructions still read: of the chunk before, and the scores
+      if ((n > 0 && !wait_warp(kEDone, n - 1)) || (OUT && !wait_warp(kADone0 + (n & 1), n / 2))) break;
 #pragma unroll
-        for (int k = 1; k < kPieces; ++k) *reinterpret_cast<uint4*>(to + (k - 1) * (DK / 64) * L::kBlock + i * 2048) = out[k].q;
+      for (int i = 0; i < kWords; ++i) {
+        *reinterpret_cast<uint4*>(from + i * 4096) = x[0][i].q;
+#pragma unroll
+        for (int k = 1; k < kPieces; ++k) *reinterpret_cast<uint4*>(to + (k - 1) * (DK / 64) * L::kBlock + i * 4096) = x[k][i].q;
       }
       proxy_fence();
       mbar_arrive(bar(kWReady));
     }
-  } else if (warp == 12 || warp == 13 || warp == 16 || warp == 17) {  // the scores: 32 rows and 32 columns of a warp
+  } else if ((warp & 3) < 2 && warp < 26) {  // the scores: 32 rows and 32 columns of a warp
     if (OUT) {
-      const int half = warp >> 4;  // of the columns
+      const int half = warp >= 24;  // of the columns
       unsigned char* to = mem + L::P + row * 128;
       for (int n = 0; n < n_chunks; ++n) {
-        if (!wait_warp(kDec0 + n % kSlots, n / kSlots) || !wait_warp(kADone, n)) break;
+        if (!wait_warp(kDec0 + n % kSlots, n / kSlots) || !wait_warp(kADone0 + (n & 1), n / 2)) break;
         fence_after();
         const ChunkDecay& cd = decays[n % kSlots];
         uint4 w[4] = {};
         if ((warp & 3) >= half) {
-          uint32_t a[32];
-          tmem_load(a, quarter + kColA + half * 32);
+          uint32_t a[2][16];
+          tmem_load(a[0], quarter + kColA + half * 32);
+          tmem_load(a[1], quarter + kColA + half * 32 + 16);
           const float hi = cd.hi[row], lo = cd.lo[row];
           const int from = cd.from[row];
           wait_loads();
@@ -377,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
                                 ex2f((hi - hj.w) + (lo - lj.w))};
             float f[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = j + i <= row && j + i >= from ? e[i] * __uint_as_float(a[c * 4 + i]) : 0.0f;
+            for (int i = 0; i < 4; ++i) f[i] = j + i <= row && j + i >= from ? e[i] * __uint_as_float(a[c >> 2][(c & 3) * 4 + i]) : 0.0f;
             const uint32_t x = pack<bf16>(make_float2(f[0], f[1])).w, y = pack<bf16>(make_float2(f[2], f[3])).w;
             if (c & 1) w[c >> 1].z = x, w[c >> 1].w = y;
             else w[c >> 1].x = x, w[c >> 1].y = y;
@@ -392,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         mbar_arrive(bar(kPReady));
       }
     }
-  } else if (warp == 14) {  // -------------------------------- the copies
+  } else if (warp == 22) {  // -------------------------------- the copies
     if (lane == 0) {
       for (int n = 0; n < n_chunks; ++n) {
         const int s = n % kStages;
@@ -407,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         for (int i = 0; i < DV / 64; ++i) tma_tile(at + L::v + i * L::kBlock, &maps.v, i * 64, h, t0, (int)b, bar(kFull0 + s));
       }
     }
-  } else if (warp == 15) {  // ------------------- the matrix instructions
+  } else if (warp == 23) {  // ------------------- the matrix instructions
     if (lane == 0) {
       constexpr uint32_t kScores = instruction(64, false, false), kSum = instruction(DV, true, true), kOut = instruction(64, true, false);
       const Operand q0 = operand(smem + L::q, 16, 1024), k0 = operand(smem + L::k, 16, 1024), kt0 = operand(smem + L::k, kOther, 1024),
@@ -415,21 +441,43 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
                     s0 = operand(smem + L::S, DK * 128, 1024), p0 = operand(smem + L::P, 16, 1024);
       auto in_stage = [&](Operand o, int s) { return Operand{o.lo + (uint32_t)(s * (L::kStage >> 4)), o.hi}; };
       constexpr int kPiece = DK / 64 * L::kBlock;
-      auto scores = [&](int s) {
+      auto scores = [&](int n, int s) {
         const Operand q = in_stage(q0, s), k = in_stage(k0, s);
         mma<false>(tmem + kColA, q, 0, k, 0, kScores);
 #pragma unroll
         for (int i = 1; i < DK / 16; ++i)
           mma<true>(tmem + kColA, q, (i / 4) * L::kBlock + (i % 4) * 32, k, (i / 4) * L::kBlock + (i % 4) * 32, kScores);
-        commit(bar(kADone));
+        commit(bar(kADone0 + (n & 1)));
       };
       if (OUT && n_chunks > 0 && wait(kFull0, 0)) {
         fence_after();
-        scores(0);
+        scores(0, 0);
       }
       for (int n = 0; n < n_chunks; ++n) {
         const int st = n % kStages, next = (n + 1) % kStages;
         const Operand kt = in_stage(kt0, st), vt = in_stage(vt0, st);
+        if (OUT) {
+          if (!wait(kSReady, n) || !wait(kFull0 + st, n / kStages) || (n > 0 && !wait(kOFree, n - 1))) break;
+          fence_after();
+          const Operand q = in_stage(q0, st);
+          mma<false>(tmem + kColX, s0, 0, q, 0, kOut);
+#pragma unroll
+          for (int i = 1; i < DK / 16; ++i) mma<true>(tmem + kColX, s0, i * 2048, q, (i / 4) * L::kBlock + (i % 4) * 32, kOut);
+          commit(bar(kXDone));
+        }
+        if (OUT) {
+          if (!wait(kPReady, n)) break;
+          fence_after();
+          mma<false>(tmem + kColY, vt, 0, p0, 0, kOut);
+#pragma unroll
+          for (int i = 1; i < 4; ++i) mma<true>(tmem + kColY, vt, i * 2048, p0, i * 32, kOut);
+          commit(bar(kODone));
+          if (n + 1 < n_chunks) {
+            if (!wait(kFull0 + next, (n + 1) / kStages) || !wait(kAFree, n)) break;
+            fence_after();
+            scores(n + 1, next);
+          }
+        }
         if (!wait(kWReady, n) || !wait(kFull0 + st, n / kStages)) break;
         if (n > 0 && !wait(kEFree, n - 1)) break;
         fence_after();
@@ -442,30 +490,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
 #pragma unroll
         for (int i = 0; i < 4; ++i) mma<true>(tmem + kColE, kt, i * 2048, vt, i * 2048, kSum);
         commit(bar(kEDone));
-        if (!OUT) {
-          commit(bar(kEmpty0 + st));
-          continue;
-        }
-        if (n + 1 < n_chunks) {
-          if (!wait(kFull0 + next, (n + 1) / kStages) || !wait(kAFree, n)) break;
-          fence_after();
-          scores(next);
-        }
-        if (!wait(kSReady, n) || (n > 0 && !wait(kOFree, n - 1))) break;
-        fence_after();
-        const Operand q = in_stage(q0, st);
-        mma<false>(tmem + kColX, s0, 0, q, 0, kOut);
-#pragma unroll
-        for (int i = 1; i < DK / 16; ++i) mma<true>(tmem + kColX, s0, i * 2048, q, (i / 4) * L::kBlock + (i % 4) * 32, kOut);
-        commit(bar(kXDone));
-        if (!wait(kPReady, n)) break;
-        fence_after();
-        mma<false>(tmem + kColY, vt, 0, p0, 0, kOut);
-#pragma unroll
-        for (int i = 1; i < 4; ++i) mma<true>(tmem + kColY, vt, i * 2048, p0, i * 32, kOut);
-        commit(bar(kODone));
         commit(bar(kEmpty0 + st));
       }
+    }
+  } else if (warp == 27) {  // ----------------------- the outputs' copies
+    if (OUT && lane == 0) {
+      for (int n = 0; n < n_chunks; ++n) {
+        if (!wait(kOReady0 + n % kStages, n / kStages)) break;
+        const uint32_t at = smem + (n % kStages) * L::kStage;
+        for (int i = 0; i < DV / 64; ++i)
+          if (i * 64 < d.DV) tma_write(&maps.o, at + i * L::kBlock, i * 64, h, chunk(n) * kChunk, (int)b);
+        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+        mbar_arrive(bar(kEmpty0 + n % kStages));
+      }
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
   } else {  // --------------------------------------------- the decays
     const float* g = p.g.p + b * p.g.sb + h * p.g.sh;
@@ -480,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
   __syncwarp();
   // a block that gave up: what it has under way ends before its memory does
   const bool failed = __syncthreads_or(!ok);
-  if (failed && warp == 15 && lane == 0) {
+  if (failed && warp == 23 && lane == 0) {
     commit(bar(kEnd));
     mbar_wait(bar(kEnd), 0);
     for (int s = 0; s < kStages; ++s) mbar_wait(bar(kFull0 + s), 0);
@@ -488,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 18)
+  if (warp == 26)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemColumns) : "memory");
 }
 
@@ -530,7 +568,8 @@ int launch(const Walk& p, cudaStream_t s) {
   Maps maps;
   const int64_t hq = d.H / d.share;
   if ((OUT && !encode(&maps.q, p.q, d.B, d.T, hq, d.DK)) || !encode(&maps.k, p.k, d.B, d.T, hq, d.DK) ||
-      !encode(&maps.v, p.v, d.B, d.T, d.H, d.DV))
+      !encode(&maps.v, p.v, d.B, d.T, d.H, d.DV) ||
+      (OUT && !encode(&maps.o, {p.o, d.T * d.H * d.DV, (int64_t)d.H * d.DV, d.DV, true}, d.B, d.T, d.H, d.DV)))
     return fail(MPB_ERR_CUDA, "linear_attention: the copies' maps cannot be made");
   constexpr int kWalkBytes = Layout<DK, DV>::bytes;
   if (int rc = allow_smem<k_la_walk<DK, DV, OUT>, kWalkBytes>("linear_attention")) return rc;
@@ -548,7 +587,7 @@ int launch_for(const Walk& p, cudaStream_t s) {
 }  // namespace
 
 bool walk_takes(const Shape& d, const Input& q, const Input& k, const Input& v) {
-  if (d.DK > 128 || d.DV > 128 || d.T >= (1LL << 31) - kChunk || d.B >= (1LL << 31)) return false;
+  if (d.DK > 128 || d.DV > 128 || d.T >= (1LL << 31) - kChunk || d.B >= (1LL << 31) ) return false;
   for (const Input* x : {&q, &k, &v}) {
     if (!x->wide) return false;
     const int64_t heads = x == &v ? d.H : d.H / d.share;

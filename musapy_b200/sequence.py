@@ -109,7 +109,8 @@ def linear_attention(q, k, v, log_decay, state=None, scale=None, return_state=Fa
     last = _new(s, (B, H, DK, DV), _dt.float32, dev) if return_state else None
     if B:
         code = q._dtype.code
-        nbytes = NATIVE.linear_attention_scratch_bytes(B, T, H, Hq, DK, DV, code, 0, 0, _aligned(q, k, v))
+        nbytes = NATIVE.linear_attention_scratch_bytes(B, T, H, Hq, DK, DV, code, 0, 0,
+                                                       _aligned(q, k, v) if o._ptr & 15 == 0 else 0)
         scratch = _scratch(nbytes, dev)
         check(NATIVE.linear_attention(B, T, H, Hq, DK, DV, code, q._ptr, *q._strides[:3], k._ptr, *k._strides[:3], v._ptr,
                                       *v._strides[:3], log_decay._ptr, *gs, _ptr(state), scale, o._ptr, _ptr(last),
