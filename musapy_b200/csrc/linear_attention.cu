@@ -141,13 +141,13 @@ MPB_D void load_state(bf16* dst, const StateTile& s, int64_t at, int dvp, int ro
 }
 
 // ----------------------------------------------------------- products
-// acc (16 x 8 NT of a warp) += A B over 64: A's rows from `m`, B's columns from 0. TA: A lies with its rows as columns,
+// acc (16 x 8 NT of a warp) += A B over 64: A's rows from `m`, B's columns from `n0`. TA: A lies with its rows as columns,
 // TB: B lies with the summed index as rows. Pieces pa, pb with pa + pb < L take part.
 template <int NT, bool TA, bool TB, int PA, int PB, int L>
-MPB_D void multiply(float (&acc)[NT][4], const bf16* A, int m, const bf16* B) {
+MPB_D void multiply(float (&acc)[NT][4], const bf16* A, int m, const bf16* B, int n0 = 0) {
   const int lane = threadIdx.x & 31, r = lane & 7, lo = (lane >> 3 & 1) * 8, hi = (lane >> 4) * 8;
   const uint32_t a_at = smem_addr(A) + 2 * (TA ? (hi + r) * kPitch + m + lo : (m + lo + r) * kPitch + hi);
-  const uint32_t b_at = smem_addr(B) + 2 * (TB ? (lo + r) * kPitch + hi : (hi + r) * kPitch + lo);
+  const uint32_t b_at = smem_addr(B) + 2 * (TB ? (lo + r) * kPitch + hi + n0 : (hi + r + n0) * kPitch + lo);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     uint32_t a[PA][4];
@@ -443,6 +443,35 @@ struct Gradients {
   float *dg, *dg_chunk;  // per step, or the sums of chunks
 };
 
+// The decays' gradients of a chunk, by one warp: each lane has two steps, of which `back` counts for the steps up to it and
+// `fore` for those behind; `through` is <U, S>.
+MPB_D void write_decay(const Gradients& p, const ChunkDecay& cd, int64_t b, int h, int c, int steps, const float (&back)[2],
+                       const float (&fore)[2], float through) {
+  const int lane = threadIdx.x & 31, t = 2 * lane;
+  float after = back[0] + back[1], before = fore[0] + fore[1];
+  const float own_a = after, own_b = before;
+  for (int o = 1; o < 32; o <<= 1) {
+    const float x = __shfl_down_sync(0xffffffffu, after, o), y = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane + o < 32) after += x;
+    if (lane >= o) before += y;
+  }
+  after -= own_a;
+  before -= own_b;
+  const float all_pass = cd.all != 0.0f ? cd.all * through : 0.0f;
+  float out[2] = {after + back[1] + back[0] + before + all_pass, after + back[1] + before + fore[0] + all_pass};
+  float sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (cd.resets(t + e)) out[e] = 0.0f;
+    if (t + e < steps) {
+      if (p.dg) p.dg[(b * p.d.T + (int64_t)c * kChunk + t + e) * p.d.H + h] = out[e];
+      sum += out[e];
+    }
+  }
+  sum = warp_sum(sum);
+  if (p.dg_chunk && lane == 0) p.dg_chunk[(b * p.d.chunks + c) * p.d.H + h] = sum;
+}
+
 template <class T, class O>
 __global__ void __launch_bounds__(kThreads) k_la_gradients(Gradients p) {
   extern __shared__ __align__(16) bf16 tiles[];
@@ -609,38 +638,227 @@ __global__ void __launch_bounds__(kThreads) k_la_gradients(Gradients p) {
   pass = warp_sum(pass);
   if (lane == 0) through[warp] = pass;
   __syncthreads();
-  // each lane has two steps: sums from a step on, and sums before it
-  if (warp == 0) {
-    const int t = 2 * lane;
-    float back[2], fore[2];
+  if (warp != 0) return;
+  float back[2], fore[2];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      back[e] = far_q[t + e] + (rows_m[t + e] - ((cols_m[0][t + e] + cols_m[1][t + e]) + (cols_m[2][t + e] + cols_m[3][t + e])));
-      fore[e] = far_k[t + e];
-    }
-    float after = back[0] + back[1], before = fore[0] + fore[1];
-    const float own_a = after, own_b = before;
-    for (int o = 1; o < 32; o <<= 1) {
-      const float x = __shfl_down_sync(0xffffffffu, after, o), y = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane + o < 32) after += x;
-      if (lane >= o) before += y;
-    }
-    after -= own_a;
-    before -= own_b;
-    const float all = cd.all, all_pass = all != 0.0f ? all * ((through[0] + through[1]) + (through[2] + through[3])) : 0.0f;
-    float out[2] = {after + back[1] + back[0] + before + all_pass, after + back[1] + before + fore[0] + all_pass};
-    float sum = 0.0f;
+  for (int e = 0; e < 2; ++e) {
+    const int t = 2 * lane + e;
+    back[e] = far_q[t] + (rows_m[t] - ((cols_m[0][t] + cols_m[1][t]) + (cols_m[2][t] + cols_m[3][t])));
+    fore[e] = far_k[t];
+  }
+  write_decay(p, cd, b, h, c, steps, back, fore, (through[0] + through[1]) + (through[2] + through[3]));
+}
+
+// The same for bf16 heads of up to 64 NK and 64 NV channels: all of the chunk's q, k, v and do stay in shared memory,
+// copied there at once, and the two states pass through it once, a tile of 64 x 64 at a time, the next one on its way to registers
+// meanwhile. Eight warps: 16 rows and half of a tile's columns each. 4 x 4096 x 16 heads of 128: BIG_HERE us, where the kernel above, which
+// loads a tile whenever it needs one, takes 1273.
+constexpr int kWideThreads = 256;
+
+// A tile of 64 x 64 by asynchronous copies, zeros outside.
+MPB_D void copy_tile(bf16* dst, const bf16* src, int64_t step, int rows, int cols) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      if (cd.resets(t + e)) out[e] = 0.0f;
-      if (t + e < steps) {
-        if (p.dg) p.dg[(b * d.T + t0 + t + e) * d.H + h] = out[e];
-        sum += out[e];
+  for (int k = 0; k < kChunk * kTile / 8 / kWideThreads; ++k) {
+    const int at = threadIdx.x + k * kWideThreads, r = at >> 3, c = (at & 7) * 8;
+    const int have = r < rows ? min(max(cols - c, 0), 8) * 2 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst + r * kPitch + c)),
+                 "l"(have ? src + r * step + c : src), "r"(have)
+                 : "memory");
+  }
+}
+
+template <int NK, int NV, class O>
+__global__ void __launch_bounds__(kWideThreads, 1) k_la_gradients_wide(Gradients p) {
+  extern __shared__ __align__(16) bf16 tiles[];
+  __shared__ ChunkDecay cd;
+  __shared__ float rows_m[2][kChunk], cols_m[4][kChunk], far_q[2][kChunk], far_k[2][kChunk], through[8];
+  bf16 *Q = tiles, *K = Q + NK * kPlane, *V = K + NK * kPlane, *G = V + NV * kPlane, *Z = G + NV * kPlane, *W = Z + kExact * kPlane;
+  bf16 *Pt = W + kExact * kPlane, *Rt = Pt + kPlane;
+  const Shape& d = p.d;
+  const int c = (int)(blockIdx.x % d.chunks), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int m = (warp & 3) * 16, side = warp >> 2, n0 = side * 32;
+  const int64_t bh = blockIdx.x / d.chunks;
+  const int h = (int)(bh % d.H), hq = h / d.share;
+  const int64_t b = bh / d.H, t0 = (int64_t)c * kChunk;
+  const int steps = (int)min((int64_t)kChunk, d.T - t0);
+  for (int i = 0; i < NK; ++i) {
+    copy_tile(Q + i * kPlane, p.q.at<bf16>(b, t0, hq) + i * kTile, p.q.st, steps, d.DK - i * kTile);
+    copy_tile(K + i * kPlane, p.k.at<bf16>(b, t0, hq) + i * kTile, p.k.st, steps, d.DK - i * kTile);
+  }
+  for (int i = 0; i < NV; ++i) {
+    copy_tile(V + i * kPlane, p.v.at<bf16>(b, t0, h) + i * kTile, p.v.st, steps, d.DV - i * kTile);
+    copy_tile(G + i * kPlane, p.g_o.at<bf16>(b, t0, h) + i * kTile, p.g_o.st, steps, d.DV - i * kTile);
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  // the states: a thread has 8 neighbouring columns of rows r and r + 32 of a tile
+  const StateTile s = p.s.of(d, bh, c, false), u = p.u.of(d, bh, c, true);
+  const int sr = threadIdx.x >> 3, sc = (threadIdx.x & 7) * 8;
+  float xs[2][8], xu[2][8];
+  auto fetch = [&](int tile) {
+    const int ik = tile / NV, iv = tile % NV;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int r = ik * kTile + sr + 32 * k, col = iv * kTile + sc;
+      const bool in = r < d.dkp && col < d.dvp;
+      const int64_t at = (int64_t)r * d.dvp + col;
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) {
+        const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f), a = in ? s.get(at + j) : zero, e = in ? u.get(at + j) : zero;
+        xs[k][j] = a.x, xs[k][j + 1] = a.y, xs[k][j + 2] = a.z, xs[k][j + 3] = a.w;
+        xu[k][j] = e.x, xu[k][j + 1] = e.y, xu[k][j + 2] = e.z, xu[k][j + 3] = e.w;
       }
     }
-    sum = warp_sum(sum);
-    if (p.dg_chunk && lane == 0) p.dg_chunk[(b * d.chunks + c) * d.H + h] = sum;
+  };
+  fetch(0);
+  if (threadIdx.x < 32) cd.fill(p.g.p + b * p.g.sb + t0 * p.g.st + h * p.g.sh, p.g.st, steps);
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  const int row = m + (lane >> 2), col = n0 + (lane & 3) * 2;
+  {
+    float P[4][4], R[4][4];
+    clear(P);
+    clear(R);
+#pragma unroll
+    for (int i = 0; i < NK; ++i) multiply<4, false, false, 1, 1, 1>(P, Q + i * kPlane, m, K + i * kPlane, n0);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) multiply<4, false, false, 1, 1, 1>(R, G + i * kPlane, m, V + i * kPlane, n0);
+    float rs[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      float cs[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const int r = row + 8 * a, j = n * 8 + col;
+        float pr[2], rr[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float by = cd.pair(r, j + e) * p.scale;
+          pr[e] = by * P[n][2 * a + e];
+          rr[e] = by * R[n][2 * a + e];
+          const float both = pr[e] * R[n][2 * a + e];
+          rs[a] += both;
+          cs[e] += both;
+        }
+        store_pair<1>(Pt, r, j, pr[0], pr[1]);
+        store_pair<1>(Rt, r, j, rr[0], rr[1]);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        for (int o = 4; o < 32; o <<= 1) cs[e] += __shfl_xor_sync(0xffffffffu, cs[e], o);
+        if (lane < 4) cols_m[warp & 3][n0 + n * 8 + lane * 2 + e] = cs[e];
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      rs[a] += __shfl_xor_sync(0xffffffffu, rs[a], 1);
+      rs[a] += __shfl_xor_sync(0xffffffffu, rs[a], 2);
+      if ((lane & 3) == 0) rows_m[side][row + 8 * a] = rs[a];
+    }
   }
+  auto weigh = [&](float (&acc)[4][4], const float* w, float by) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const float f = w[row + 8 * a] * by;
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) acc[n][2 * a + e] = f != 0.0f ? acc[n][2 * a + e] * f : 0.0f;
+    }
+  };
+  auto write = [&](auto* dst, int64_t step, int cols, float (&acc)[4][4]) {
+    using T = typename std::remove_pointer<decltype(dst)>::type;
+    const bool pairs = ((uintptr_t)dst / sizeof(T) | (uintptr_t)step) % 2 == 0;
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const int r = row + 8 * a, j = n * 8 + col;
+        if (r >= steps) continue;
+        T* to = dst + r * step + j;
+        if (pairs && j + 1 < cols) {
+          *reinterpret_cast<typename Word<2 * sizeof(T)>::type*>(to) = pack<T>(make_float2(acc[n][2 * a], acc[n][2 * a + 1])).w;
+        } else {
+          if (j < cols) to[0] = Cvt<T>::from(acc[n][2 * a]);
+          if (j + 1 < cols) to[1] = Cvt<T>::from(acc[n][2 * a + 1]);
+        }
+      }
+  };
+  auto dot = [&](float (&acc)[4][4], const bf16* x, float (&sum)[2]) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const uint32_t two = *reinterpret_cast<const uint32_t*>(x + (row + 8 * a) * kPitch + n * 8 + col);
+        sum[a] = fmaf(__uint_as_float(two << 16), acc[n][2 * a], sum[a]);
+        sum[a] = fmaf(__uint_as_float(two & 0xffff0000u), acc[n][2 * a + 1], sum[a]);
+      }
+  };
+  float fq[2] = {0.0f, 0.0f}, fk[2] = {0.0f, 0.0f}, pass = 0.0f, dv[NV][4][4];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) clear(dv[i]);
+#pragma unroll
+  for (int ik = 0; ik < NK; ++ik) {
+    float aq[4][4], ak[4][4];
+    clear(aq);
+    clear(ak);
+#pragma unroll
+    for (int iv = 0; iv < NV; ++iv) {
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pass = fmaf(xs[k][j], xu[k][j], pass);
+        store8<kExact>(Z + (sr + 32 * k) * kPitch + sc, xs[k]);
+        store8<kExact>(W + (sr + 32 * k) * kPitch + sc, xu[k]);
+      }
+      if (ik * NV + iv + 1 < NK * NV) fetch(ik * NV + iv + 1);
+      __syncthreads();
+      multiply<4, false, false, 1, kExact, kExact>(aq, G + iv * kPlane, m, Z, n0);
+      multiply<4, false, false, 1, kExact, kExact>(ak, V + iv * kPlane, m, W, n0);
+      multiply<4, false, true, 1, Keep<bf16>::S, Keep<bf16>::S>(dv[iv], K + ik * kPlane, m, W, n0);
+    }
+    weigh(aq, cd.into, p.scale);
+    weigh(ak, cd.rest, 1.0f);
+    dot(aq, Q + ik * kPlane, fq);
+    dot(ak, K + ik * kPlane, fk);
+    multiply<4, false, true, 1, 1, 1>(aq, Rt, m, K + ik * kPlane, n0);
+    multiply<4, true, true, 1, 1, 1>(ak, Rt, m, Q + ik * kPlane, n0);
+    const int64_t to = ((b * d.T + t0) * d.H + h) * d.DK + ik * kTile;
+    write((O*)p.dq + to, (int64_t)d.H * d.DK, d.DK - ik * kTile, aq);
+    write((O*)p.dk + to, (int64_t)d.H * d.DK, d.DK - ik * kTile, ak);
+  }
+#pragma unroll
+  for (int iv = 0; iv < NV; ++iv) {
+    weigh(dv[iv], cd.rest, 1.0f);
+    multiply<4, true, true, 1, 1, 1>(dv[iv], Pt, m, G + iv * kPlane, n0);
+    write((bf16*)p.dv + ((b * d.T + t0) * d.H + h) * d.DV + iv * kTile, (int64_t)d.H * d.DV, d.DV - iv * kTile, dv[iv]);
+  }
+#pragma unroll
+  for (int a = 0; a < 2; ++a) {
+    for (int o = 1; o < 4; o <<= 1) {
+      fq[a] += __shfl_xor_sync(0xffffffffu, fq[a], o);
+      fk[a] += __shfl_xor_sync(0xffffffffu, fk[a], o);
+    }
+    if ((lane & 3) == 0) {
+      far_q[side][row + 8 * a] = fq[a];
+      far_k[side][row + 8 * a] = fk[a];
+    }
+  }
+  pass = warp_sum(pass);
+  if (lane == 0) through[warp] = pass;
+  __syncthreads();
+  if (warp != 0) return;
+  float back[2], fore[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int t = 2 * lane + e;
+    back[e] = (far_q[0][t] + far_q[1][t]) +
+              ((rows_m[0][t] + rows_m[1][t]) - ((cols_m[0][t] + cols_m[1][t]) + (cols_m[2][t] + cols_m[3][t])));
+    fore[e] = far_k[0][t] + far_k[1][t];
+  }
+  float all_pass = 0.0f;
+  for (int k = 0; k < 8; ++k) all_pass += through[k];
+  write_decay(p, cd, b, h, c, steps, back, fore, all_pass);
 }
 
 // Sums over the heads that share one, in their order: (rows, heads, share, n) floats to (rows, heads, n).
@@ -741,7 +959,7 @@ __global__ void __launch_bounds__(kStepThreads) k_la_step(Step p) {
 }
 
 // ------------------------------------------------------------------- host
-size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+size_t round32(size_t n) { return (n + 31) / 32 * 32; }
 
 Shape make_shape(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK, int64_t DV) {
   Shape d = {};
@@ -765,11 +983,11 @@ struct StateScratch {
     const size_t bh = (size_t)d.B * d.H, size = (size_t)d.dkp * d.dvp * 4;
     at = from;
     since = at + (kept ? bh * d.chunks * size : 0);
-    ends = since + round16(bh * d.chunks * 2 * 4);
+    ends = since + round32(bh * d.chunks * 2 * 4);
     bytes = ends + (d.segments > 1 ? bh * d.segments * size : 0);
   }
 };
-constexpr size_t kStatusBytes = 16;  // the status word leads the scratch
+constexpr size_t kStatusBytes = 32;  // the status word leads the scratch
 
 // Whether the walk of whole rows may be taken, as far as the layout does not decide.
 bool may_walk(int dtype, int64_t DK, int64_t DV, bool aligned) { return aligned && dtype == MPB_BF16 && DK <= 128 && DV <= 128 && DV % 8 == 0; }
@@ -845,13 +1063,28 @@ struct GradScratch {
   GradScratch(const Shape& d, bool by_head) {
     const StateScratch a(d, kStatusBytes, true), b(d, a.bytes, true);
     const size_t part = d.share > 1 ? (size_t)d.B * d.T * d.H * d.DK * 4 : 0;
-    s = kStatusBytes, u = a.bytes, dq = round16(b.bytes), dk = dq + round16(part), dg = dk + round16(part);
-    bytes = dg + (by_head ? round16((size_t)d.B * d.chunks * d.H * 4) : 0);
+    s = kStatusBytes, u = a.bytes, dq = round32(b.bytes), dk = dq + round32(part), dg = dk + round32(part);
+    bytes = dg + (by_head ? round32((size_t)d.B * d.chunks * d.H * 4) : 0);
   }
 };
 
+template <int NK, int NV, class O>
+int run_wide(const Gradients& p, cudaStream_t s) {
+  constexpr int kWideBytes = (2 * NK + 2 * NV + 2 * kExact + 2) * kPlane * 2;
+  if (int rc = allow_smem<k_la_gradients_wide<NK, NV, O>, kWideBytes>("linear_attention_backward")) return rc;
+  k_la_gradients_wide<NK, NV, O><<<(unsigned)(p.d.B * p.d.H * p.d.chunks), kWideThreads, kWideBytes, s>>>(p);
+  return launch_check("linear_attention_backward");
+}
+
+// wide: bf16 heads of up to 128 channels, all inputs in 16-byte words.
 template <class T, class O>
-int run_gradients(const Gradients& p, cudaStream_t s) {
+int run_gradients(const Gradients& p, bool wide, cudaStream_t s) {
+  if constexpr (std::is_same<T, bf16>::value) {
+    if (wide) {
+      if (p.d.DK > 64) return p.d.DV > 64 ? run_wide<2, 2, O>(p, s) : run_wide<2, 1, O>(p, s);
+      return p.d.DV > 64 ? run_wide<1, 2, O>(p, s) : run_wide<1, 1, O>(p, s);
+    }
+  }
   constexpr int kGradBytes = (2 * RawPieces<T>::n + 2 * kExact + 2 * Keep<T>::P) * kPlane * 2;
   if (int rc = allow_smem<k_la_gradients<T, O>, kGradBytes>("linear_attention_backward")) return rc;
   k_la_gradients<T, O><<<(unsigned)(p.d.B * p.d.H * p.d.chunks), kThreads, kGradBytes, s>>>(p);
@@ -877,7 +1110,7 @@ int run_backward(Gradients p, const float* first, const float* dstate, void* dq,
   p.dg = by_head ? nullptr : dg, p.dg_chunk = by_head ? (float*)(scratch + w.dg) : nullptr;
   if (d.share > 1) {
     p.dq = scratch + w.dq, p.dk = scratch + w.dk;
-    if (int rc = run_gradients<T, float>(p, s)) return rc;
+    if (int rc = run_gradients<T, float>(p, walk, s)) return rc;
     const int64_t total = d.B * d.T * (d.H / d.share) * d.DK;
     const unsigned blocks = (unsigned)((total + 255) / 256);
     k_la_unshare<T><<<blocks, 256, 0, s>>>((const float*)p.dq, (T*)dq, total, d.share, d.DK);
@@ -885,7 +1118,7 @@ int run_backward(Gradients p, const float* first, const float* dstate, void* dq,
     if (int rc = launch_check("linear_attention_backward")) return rc;
   } else {
     p.dq = dq, p.dk = dk;
-    if (int rc = run_gradients<T, T>(p, s)) return rc;
+    if (int rc = run_gradients<T, T>(p, walk, s)) return rc;
   }
   if (by_head) {
     k_la_decay_sum<<<(unsigned)d.H, 256, 0, s>>>(p.dg_chunk, dg, d.B * d.chunks, d.H);

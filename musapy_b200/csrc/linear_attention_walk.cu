@@ -236,6 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         mbar_arrive(bar(kSReady));
       }
       float since = 1.0f;
+      const bool sectors = (uintptr_t)p.at % 32 == 0;  // 32 bytes of a thread's row in one store: a whole sector
       for (int n = 0; n < n_chunks; ++n) {
         const int c = chunk(n);
         if (!wait_warp(kDec0 + n % kSlots, n / kSlots)) break;
@@ -264,9 +265,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
           }
           if (!OUT && at) {
 #pragma unroll
-            for (int i = 0; i < 16; i += 4)
-              if (g * 16 + i < width)
-                *reinterpret_cast<uint4*>(at + g * 16 + i) = make_uint4(sg[i], sg[i + 1], sg[i + 2], sg[i + 3]);
+            for (int i = 0; i < 16; i += 8)
+              if (g * 16 + i < width) {
+                if (sectors) {
+                  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(at + g * 16 + i), "r"(sg[i]), "r"(sg[i + 1]),
+                               "r"(sg[i + 2]), "r"(sg[i + 3]), "r"(sg[i + 4]), "r"(sg[i + 5]), "r"(sg[i + 6]), "r"(sg[i + 7])
+                               : "memory");
+                } else {
+                  *reinterpret_cast<uint4*>(at + g * 16 + i) = make_uint4(sg[i], sg[i + 1], sg[i + 2], sg[i + 3]);
+                  *reinterpret_cast<uint4*>(at + g * 16 + i + 4) = make_uint4(sg[i + 4], sg[i + 5], sg[i + 6], sg[i + 7]);
+                }
+              }
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i)
