@@ -65,16 +65,29 @@ MPB_D float teacher_logit(const DistillArgs& p, int64_t at) {
   return to_f(((const __nv_bfloat16*)p.teacher)[at]);
 }
 
+MPB_D int64_t teacher_id(const DistillArgs& p, int64_t at) {
+  return p.ids64 ? ((const int64_t*)p.ids)[at] : ((const int32_t*)p.ids)[at];
+}
+
+// A thread's first entry, asked for before the row: behind the row's copies it would arrive last.
+struct FirstEntry {
+  float x;
+  int64_t id;
+  MPB_D FirstEntry(const DistillArgs& p, int64_t i) : x(-INFINITY), id(0) {
+    if ((int)threadIdx.x < p.K) x = teacher_logit(p, i * p.K + threadIdx.x), id = teacher_id(p, i * p.K + threadIdx.x);
+  }
+};
+
 // ids (-1: left out), and p: each entry's share. Every thread of the block takes part; red: two of 32 floats.
-MPB_D Teacher load_teacher(const DistillArgs& p, int64_t i, int* ids, float* share, float (*red)[32]) {
+MPB_D Teacher load_teacher(const DistillArgs& p, int64_t i, const FirstEntry& first, int* ids, float* share, float (*red)[32]) {
   const int tid = threadIdx.x, threads = blockDim.x;
   const float per = 1.0f / p.tau;
   Teacher t;
   float top = -INFINITY;
   bool bad = false, nan = false;
   for (int k = tid; k < p.K; k += threads) {
-    const float x = teacher_logit(p, i * p.K + k);
-    const int64_t id = p.ids64 ? ((const int64_t*)p.ids)[i * p.K + k] : ((const int32_t*)p.ids)[i * p.K + k];
+    const float x = k == tid ? first.x : teacher_logit(p, i * p.K + k);
+    const int64_t id = k == tid ? first.id : teacher_id(p, i * p.K + k);
     const bool in = x != -INFINITY, inside = id >= 0 && id < p.V;
     bad |= in && !inside;
     nan |= x != x;
@@ -163,6 +176,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_distill_row(DistillArgs p, i
     zero_row<T>(p, i, from < p.V ? from : p.V, to < p.V ? to : p.V, tid, threads);
     return;
   }
+  const FirstEntry first(p, i);
   // every block of the cluster runs (nothing is made visible by this)
   if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const uint4* src = reinterpret_cast<const uint4*>(z + head) + w0;
@@ -194,7 +208,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_distill_row(DistillArgs p, i
     f.sum = exp_from(end, -(end == -INFINITY ? 0.0f : end), c);
   }
   const float count = p.grad ? tokens_in_mask(p.mask, p.N, p.count, red[0]) : 1.0f;
-  const Teacher t = load_teacher(p, i, ids, share, red + 1);
+  const Teacher t = load_teacher(p, i, first, ids, share, red + 1);
   auto fold_batch = [&](const uint4 (&v)[kBatch]) {
     uint4 most = v[0];
 #pragma unroll
@@ -314,7 +328,7 @@ __global__ void __launch_bounds__(kPassThreads) k_distill_passes(DistillArgs p) 
   }
   const float c = -kMinusLog2e / p.tau;
   const float count = p.grad ? tokens_in_mask(p.mask, p.N, p.count, red[0]) : 1.0f;
-  const Teacher t = load_teacher(p, i, ids, share, red + 1);
+  const Teacher t = load_teacher(p, i, FirstEntry(p, i), ids, share, red + 1);
   float top = -INFINITY;
   for (int64_t j = threadIdx.x; j < p.V; j += kPassThreads) top = fmaxf(top, to_f(z[j]));
   top = block_max(top, red[3]);

@@ -282,8 +282,8 @@ struct Sums {
 
 // kCols accesses of E columns, `lanes` apart from column word w on, summed over a list of tokens, in their
 // order (at: where the n of them stand); several rows are under way at once.
-constexpr int kCols = 4;
-template <class T, int E>
+template <int E> constexpr int cols_of() { return E > 4 ? 2 : 4; }
+template <class T, int E, int kCols>
 MPB_D void sum_rows(const Sums& p, const int* at, int n, int64_t w, int lanes, float (&acc)[kCols][E]) {
   constexpr int kAhead = E > 4 ? 2 : 4;
   using P = Pack<T, E>;
@@ -379,6 +379,7 @@ MPB_D int64_t part_place(int i, bool begins) { return (int64_t)(i / kPart) * 2 +
 // the lists' first tokens. `lanes` threads (a power of two, a warp at least) walk a row's columns.
 template <class T, int E, bool ADD>
 __global__ void __launch_bounds__(kThreads) k_embed_sums(Sums p, int lanes) {
+  constexpr int kCols = cols_of<E>();
   const int64_t words = p.D / E;
   float acc[kCols][E];
   if (blockIdx.x < p.part_blocks) {
@@ -404,7 +405,7 @@ __global__ void __launch_bounds__(kThreads) k_embed_sums(Sums p, int lanes) {
     const int have = min(e - i, kPart), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if ((int)threadIdx.x < have) rows[threadIdx.x] = p.at[i + threadIdx.x];
     __syncthreads();
-    sum_rows<T, E>(p, rows + warp * kEach, min(have - warp * kEach, kEach), (int64_t)tile * 32 * kCols + lane, 32, acc);
+    sum_rows<T, E, kCols>(p, rows + warp * kEach, min(have - warp * kEach, kEach), (int64_t)tile * 32 * kCols + lane, 32, acc);
 #pragma unroll
     for (int c = 0; c < kCols; ++c)
 #pragma unroll
@@ -460,7 +461,7 @@ __global__ void __launch_bounds__(kThreads) k_embed_sums(Sums p, int lanes) {
 #pragma unroll
     for (int c = 0; c < kCols; ++c)
       if (w + c * lanes < words) old_row<E, ADD>(p, row, (w + c * lanes) * E, old[c]);
-    sum_rows<T, E>(p, p.at + s, e - s, w, lanes, acc);
+    sum_rows<T, E, kCols>(p, p.at + s, e - s, w, lanes, acc);
 #pragma unroll
     for (int c = 0; c < kCols; ++c)
       if (w + c * lanes < words) put_row<E, ADD>(p, row, (w + c * lanes) * E, old[c], acc[c]);
@@ -552,6 +553,7 @@ int sort_tokens(Sorted& p, char* scratch, const Scratch& w, cudaStream_t s) {
 
 template <class T, int E>
 int launch_sums(Sums& p, cudaStream_t s) {
+  constexpr int kCols = cols_of<E>();
   const int64_t words = p.D / E;
   const int lanes = lanes_for((words + kCols - 1) / kCols, 32);
   p.tiles = (int)((words + kCols * 32 - 1) / (kCols * 32));
