@@ -419,7 +419,7 @@ int launch_distill(DistillArgs& p, cudaStream_t s) {
       attr[0].val.clusterDim.x = (unsigned)blocks;
       attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
       cfg.attrs = attr;
-      cfg.numAttrs = 1;
+      cfg.numAttrs = blocks > 1 ? 1 : 0;
       if (int rc = launch_check_pdl(cudaLaunchKernelEx(&cfg, k_distill_row<T>, p, (int)per, blocks), "distill_loss"))
         return rc;
     } else {

@@ -208,9 +208,9 @@ def test_c_entry_points_return_status():
     emb = lambda **k: N.embedding(*{**dict(N=4, V=8, D=3, t=16, dt=f32, sr=3, ids=16, idt=i32, scale=1.0, o=16, st=0), **k}.values())
     assert emb(N=-1) == MPB_ERR_SHAPE and emb(N=1 << 31) == MPB_ERR_SHAPE and emb(idt=f32) == MPB_ERR_DTYPE and emb(dt=i64) == MPB_ERR_DTYPE
     assert emb(t=0) == MPB_ERR_INVALID and emb(o=0) == MPB_ERR_INVALID and emb(N=0, ids=0) == MPB_OK and emb(D=0, o=0) == MPB_OK
-    need = N.embedding_backward_scratch_bytes(4, 8, 3, 0)
-    assert N.embedding_backward_scratch_bytes(6, 8, 3, 0) > N.embedding_backward_scratch_bytes(6, 8, 3, 1) > 0 and N.embedding_backward_scratch_bytes(0, 8, 3, 0) == 0
-    grad = lambda **k: N.embedding_backward(*{**dict(N=4, V=8, D=3, d=16, dt=f32, sr=3, ids=16, idt=i32, scale=1.0, into=0, t=16,
+    need = N.embedding_backward_scratch_bytes(200, 8, 3, 0)
+    assert N.embedding_backward_scratch_bytes(200, 8, 3, 0) > N.embedding_backward_scratch_bytes(200, 8, 3, 1) > 0 and N.embedding_backward_scratch_bytes(0, 8, 3, 0) == 0
+    grad = lambda **k: N.embedding_backward(*{**dict(N=200, V=8, D=3, d=16, dt=f32, sr=3, ids=16, idt=i32, scale=1.0, into=0, t=16,
                                                      sc=16, nb=need, st=0), **k}.values())
     assert grad(V=-1) == MPB_ERR_SHAPE and grad(N=1 << 31) == MPB_ERR_SHAPE and grad(V=1 << 31) == MPB_ERR_SHAPE
     assert grad(idt=bf16) == MPB_ERR_DTYPE and grad(dt=11) == MPB_ERR_DTYPE and grad(d=0) == MPB_ERR_INVALID and grad(t=0) == MPB_ERR_INVALID
