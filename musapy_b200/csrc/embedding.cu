@@ -11,7 +11,10 @@
 // the block that finishes last. A new table is written once, rows that no token names
 // as zeros; a gradient that is there already is added to, where tokens name it.
 //
-// Bound: memory. Up to kSmall tokens are sorted by one kernel, more by two for each digit.
+// Bound: memory. Up to kFew tokens need no sort, up to kSmall are sorted by one kernel, more by two for each digit.
+// Lookup of 32768 rows of 4096 bf16: 82 us (6.5 TB/s); 64 rows 2.3 us on the GPU. Gradient of 32768 tokens of 32000 x 2048 from
+// bf16: 130 us, of which the sums 98 (4.1 TB/s; they wait on three loads in a row: the list, its tokens, their rows) and the sort 27; of 4097 of
+// 50257 x 769 float, added: 24 us on the GPU, sort 6, sums 18 (rows that begin at no 16-byte boundary go by single elements).
 #include "common.cuh"
 #include "internal.h"
 #include "musapy_b200.h"

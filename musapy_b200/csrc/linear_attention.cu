@@ -20,8 +20,19 @@
 //
 // Products run on the tensor cores with operands of bf16 and sums in float. A
 // bf16 input is one such operand; a float16 input is the sum of two, a float of three,
-// and so is what a float weight makes of an input (Pieces). Products of pieces whose
+// and so is what a float weight makes of an input. Products of pieces whose
 // place together is past the result's precision are left out.
+//
+// This file has the kernels of any type, layout and width up to 256: the states at the
+// chunks' borders (k_la_states, over segments that k_la_join joins), from which
+// all chunks' outputs (k_la_output) and gradients (k_la_gradients) follow side by side; the step;
+// and the gradients of bf16 heads of up to 128 channels (k_la_gradients_wide). bf16 rows of 16-byte words are walked by
+// linear_attention_walk.cu, without storing states going forward.
+//
+// Bound: forward and backward move 0.5 GB each way at most for what takes them hundreds of us; they wait on their own
+// tiles (synchronous loads, two barriers a tile, splits into pieces), at 8 warps per SM: gradients of 4 x 4096 x 16 heads of 128 bf16
+// 677 us (1.3 TB/s under the profiler, tensor cores 0.2), 1 x 19250 x 3 heads of 128 and 64 float, all of the backward pass, 705 us.
+// The step is bound by memory: 64 x 16 heads of 128 x 128, 134 MB, 24.6 us (5.5 TB/s).
 #include "common.cuh"
 #include "internal.h"
 #include "linear_attention.cuh"
@@ -149,8 +160,14 @@ MPB_D void multiply(float (&acc)[NT][4], const bf16* A, int m, const bf16* B, in
   const uint32_t a_at = smem_addr(A) + 2 * (TA ? (hi + r) * kPitch + m + lo : (m + lo + r) * kPitch + hi);
   const uint32_t b_at = smem_addr(B) + 2 * (TB ? (lo + r) * kPitch + hi + n0 : (hi + r + n0) * kPitch + lo);
   if constexpr (PA > 1 && PB > 1) {
-    // The tensor core cuts a sum where others round: the small products come first, of all steps, and only the large ones
-    // meet the sum at its size (float inputs: errors of 1.2e-6 with the pieces of each step together, 6e-7 so).
+    // The tensor core cuts a sum where others round: the small products come first, of all steps, only the large ones meet
+    // the sum at its size, and what is summed already is added outside. (Errors of float inputs: 1.2e-6 with the pieces of
+    // each step together, 6e-7 in this order, 3e-7 with the sum added outside.)
+    float sum[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[n][i] = 0.0f;
 #pragma unroll
     for (int l = L - 1; l >= 0; --l) {
 #pragma unroll
@@ -165,12 +182,16 @@ MPB_D void multiply(float (&acc)[NT][4], const bf16* A, int m, const bf16* B, in
           for (int n = 0; n < NT / 2; ++n) {
             uint32_t b[4];
             ldmatrix4<TB>(b, b_at + 2 * (q * kPlane + (TB ? 16 * k * kPitch + 16 * n : 16 * n * kPitch + 16 * k)));
-            mma_bf16(acc[2 * n], a, b[0], b[1]);
-            mma_bf16(acc[2 * n + 1], a, b[2], b[3]);
+            mma_bf16(sum[2 * n], a, b[0], b[1]);
+            mma_bf16(sum[2 * n + 1], a, b[2], b[3]);
           }
         }
       }
     }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[n][i] += sum[n][i];
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
