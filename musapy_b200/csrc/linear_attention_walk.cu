@@ -130,7 +130,7 @@ MPB_D void tma_write(const CUtensorMap* map, uint32_t src, int x, int h, int t, 
 
 // ------------------------------------------------------------ layout
 enum Bar { kFull0, kFull1, kFull2, kEmpty0, kEmpty1, kEmpty2, kDec0, kDec1, kDec2, kDec3, kADone0, kADone1, kAFree, kPReady, kWReady, kEDone, kEFree, kSReady,
-           kXDone, kODone, kOFree, kOReady0, kOReady1, kOReady2, kFree0, kFree1, kFree2, kFree3, kEnd, kBars };
+           kXDone, kODone, kOFree, kOReady0, kOReady1, kOReady2, kOEmpty, kFree0, kFree1, kFree2, kFree3, kEnd, kBars };
 
 template <int DK, int DV>
 struct Layout {
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
   if (tid == 0) {
     for (int i = 0; i < kBars; ++i) {
       const int count = i >= kDec0 && i <= kDec3 ? 32 : i == kAFree || i == kPReady ? 128 : i == kWReady ? 256
-                        : i == kEFree || i == kSReady ? 2 * DK : i == kOFree || (i >= kOReady0 && i <= kOReady2) ? DV
+                        : i == kEFree || i == kSReady || (!OUT && i == kOReady0) ? 2 * DK : i == kOFree || (i >= kOReady0 && i <= kOReady2) ? DV
                         : OUT && i >= kEmpty0 && i <= kEmpty2 ? 2
                         : i >= kFree0 && i <= kFree3 ? 2 * DK + (OUT ? DV : 0) : 1;
       mbar_init(bar(i), count);
@@ -244,7 +244,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         mbar_arrive(bar(kSReady));
       }
       float since = 1.0f;
-      const bool sectors = (uintptr_t)p.at % 32 == 0;  // 32 bytes of a thread's row in one store: a whole sector
+      // The state before each chunk leaves in float, by a copy of 32 columns each from where q would be, and S.
+      const bool keep = !OUT && p.at;
       for (int n = 0; n < n_chunks; ++n) {
         const int c = chunk(n);
         if (!wait_warp(kDec0 + n % kSlots, n / kSlots)) break;
@@ -253,8 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         since *= all;
         if (!wait_warp(kEDone, n)) break;
         fence_after();
-        float* at = p.at ? p.at + (bh * d.chunks + c) * size + (int64_t)row * d.dvp + col0 : nullptr;
-        const int width = row < d.dkp ? d.dvp - col0 : 0;
+        if (keep && n > 0 && !wait_warp(kOEmpty, n - 1)) break;
         uint32_t e[2][16], s[2][16];
         tmem_load(e[0], e_tmem);
         tmem_load(s[0], s_tmem);
@@ -271,19 +271,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
             mbar_arrive(bar(kEFree));
             mbar_arrive(bar(kFree0 + n % kSlots));
           }
-          if (!OUT && at) {
+          if (keep) {
+            const int c = col0 + g * 16;
+            unsigned char* to = mem + (c < 96 ? c / 32 * L::kStage + L::q : L::S) + row * 128;
 #pragma unroll
-            for (int i = 0; i < 16; i += 8)
-              if (g * 16 + i < width) {
-                if (sectors) {
-                  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(at + g * 16 + i), "r"(sg[i]), "r"(sg[i + 1]),
-                               "r"(sg[i + 2]), "r"(sg[i + 3]), "r"(sg[i + 4]), "r"(sg[i + 5]), "r"(sg[i + 6]), "r"(sg[i + 7])
-                               : "memory");
-                } else {
-                  *reinterpret_cast<uint4*>(at + g * 16 + i) = make_uint4(sg[i], sg[i + 1], sg[i + 2], sg[i + 3]);
-                  *reinterpret_cast<uint4*>(at + g * 16 + i + 4) = make_uint4(sg[i + 4], sg[i + 5], sg[i + 6], sg[i + 7]);
-                }
-              }
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint4*>(to + ((c / 4 % 8 + i ^ (row & 7)) << 4)) = make_uint4(sg[4 * i], sg[4 * i + 1], sg[4 * i + 2], sg[4 * i + 3]);
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -296,6 +289,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
           proxy_fence();
           fence_before();
           mbar_arrive(bar(kSReady));
+        } else if (keep) {
+          proxy_fence();
+          mbar_arrive(bar(kOReady0));
         }
       }
       if (ok) {
@@ -511,6 +507,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
       }
     }
   } else if (warp == 27) {  // ----------------------- the outputs' copies
+    if (!OUT && p.at && lane == 0) {
+      for (int n = 0; n < n_chunks; ++n) {
+        if (!wait(kOReady0, n)) break;
+        for (int i = 0; i < DV / 32; ++i)
+          if (i * 32 < d.dvp)
+            tma_write(&maps.o, smem + (i < 3 ? i * L::kStage + L::q : L::S), i * 32, 0, chunk(n), (int)bh);
+        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+        mbar_arrive(bar(kOEmpty));
+      }
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
     if (OUT && lane == 0) {
       for (int n = 0; n < n_chunks; ++n) {
         if (!wait(kOReady0 + n % kStages, n / kStages)) break;
@@ -579,6 +586,18 @@ bool encode(CUtensorMap* m, const Input& x, int64_t B, int64_t T, int64_t heads,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Boxes of 32 columns and all rows of a (heads, chunks, dkp, dvp) array of states in float.
+bool encode_states(CUtensorMap* m, const Walk& p, int rows) {
+  const EncodeTiled fn = encoder();
+  if (!fn) return false;
+  const Shape& d = p.d;
+  const cuuint64_t dims[4] = {(cuuint64_t)d.dvp, (cuuint64_t)d.dkp, (cuuint64_t)d.chunks, (cuuint64_t)(d.B * d.H)};
+  const cuuint64_t strides[3] = {(cuuint64_t)d.dvp * 4, (cuuint64_t)d.dkp * d.dvp * 4, (cuuint64_t)d.chunks * d.dkp * d.dvp * 4};
+  const cuuint32_t box[4] = {32, (cuuint32_t)rows, 1, 1}, each[4] = {1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.at, dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int DK, int DV, bool OUT>
 int launch(const Walk& p, cudaStream_t s) {
   const Shape& d = p.d;
@@ -586,7 +605,8 @@ int launch(const Walk& p, cudaStream_t s) {
   const int64_t hq = d.H / d.share;
   if ((OUT && !encode(&maps.q, p.q, d.B, d.T, hq, d.DK)) || !encode(&maps.k, p.k, d.B, d.T, hq, d.DK) ||
       !encode(&maps.v, p.v, d.B, d.T, d.H, d.DV) ||
-      (OUT && !encode(&maps.o, {p.o, d.T * d.H * d.DV, (int64_t)d.H * d.DV, d.DV, true}, d.B, d.T, d.H, d.DV)))
+      (OUT && !encode(&maps.o, {p.o, d.T * d.H * d.DV, (int64_t)d.H * d.DV, d.DV, true}, d.B, d.T, d.H, d.DV)) ||
+      (!OUT && p.at && !encode_states(&maps.o, p, DK)))
     return fail(MPB_ERR_CUDA, "linear_attention: the copies' maps cannot be made");
   constexpr int kWalkBytes = Layout<DK, DV>::bytes;
   if (int rc = allow_smem<k_la_walk<DK, DV, OUT>, kWalkBytes>("linear_attention")) return rc;
