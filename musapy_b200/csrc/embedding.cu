@@ -25,7 +25,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWords = 4;     // of a row that a thread has under way
-constexpr int kPart = 32;     // tokens of a row that are summed by one group of threads
+// Tokens of a row that are summed by one group of threads. Of 32768 tokens of 32000 x 2048 bf16, and of 4097 of 50257 x 769
+// float: 98 and 17.7 us for the sums at 32, 121 and 20.8 at 16, 161 and 27 at 8.
+constexpr int kPart = 32;
 constexpr int kMostBits = 9;  // of a digit
 constexpr int kMostBins = 1 << kMostBits;
 constexpr int kTileTokens = 2048;

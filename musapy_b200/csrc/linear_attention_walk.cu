@@ -16,7 +16,8 @@
 // word and ends the block.
 //
 // What it takes: 8 x 4096 x 16 heads of 128, 218 us (2.5 TB/s; 553 MB, 85 us at the copy rate; without this kernel 1441 us);
-// 1 x 32768 x 8 heads of 64 in 18 segments 125 us with the walk that finds their states. A chunk takes about 5500 cycles: the
+// 1 x 32768 x 8 heads of 64 in 18 segments 125 us with the walk that finds their states. Without outputs, the states of all chunks
+// kept in float, 4 x 4096 x 16 heads of 128 take 100 us (2.7 TB/s; by each thread's own stores 149). A chunk takes about 5500 cycles: the
 // tensor core has 32 instructions, each of which takes 73 cycles by itself whatever its columns up to 128 (its left operand's
 // 4 KB come at 64 bytes a cycle) and 90 to 110 beside the other warps' shared memory traffic; what passes from one chunk
 // to the next is E (12 instructions), the state's sum and X. Steps on the way: scores before their place is free 293 -> 224 us;
