@@ -274,6 +274,7 @@ struct States {
   const float* first;
   float scale;
   float *at, *since, *ends, *last;  // last: the final state, where one segment gives it
+  int* status = nullptr;            // cleared: nothing here waits
 };
 
 template <class T, bool REV>
@@ -294,6 +295,7 @@ __global__ void __launch_bounds__(kThreads) k_la_states(States p) {
   const int h = (int)(bh % d.H);
   const int64_t b = bh / d.H;
   const int c0 = seg * d.per, c1 = min(d.chunks, c0 + d.per);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.status = MPB_OK;
   const bool begins = REV ? c1 == d.chunks : seg == 0;
   const int64_t tile = (int64_t)ik * kTile * d.dvp + iv * kTile;
   const int rows = d.dkp - ik * kTile, cols = d.dvp - iv * kTile;
@@ -1073,7 +1075,9 @@ int run_states(const States& p, bool walk, int* status, cudaStream_t s) {
   } else {
     const int64_t tiles = (int64_t)((d.dkp + kTile - 1) / kTile) * ((d.dvp + kTile - 1) / kTile);
     if (int rc = allow_smem<k_la_states<T, REV>, kStatesBytes>("linear_attention")) return rc;
-    k_la_states<T, REV><<<(unsigned)(d.B * d.H * d.segments * tiles), kThreads, kStatesBytes, s>>>(p);
+    States q = p;
+    q.status = status;
+    k_la_states<T, REV><<<(unsigned)(d.B * d.H * d.segments * tiles), kThreads, kStatesBytes, s>>>(q);
     if (int rc = launch_check("linear_attention")) return rc;
   }
   return join_states(p, REV, s);

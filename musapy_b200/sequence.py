@@ -92,9 +92,9 @@ def linear_attention(q, k, v, log_decay, state=None, scale=None, return_state=Fa
     256. Returns o (B, T, H, DV) in v's dtype; with ``return_state`` also the last S in float32.
 
     S and every sum run in float32; the scores of float32, float16 and bfloat16 inputs are rounded to 24, 16 and 8 bits
-    before they meet v,
-    and so is the state of bfloat16 rows, copied for that, where it meets q. Inputs are finite: a value that is not may reach every result of its chunk of 64 steps and the
-    later ones. A prompt may be padded behind its end with log_decay 0 and k 0, which leaves the state as it was."""
+    before they meet v, and a copy of the state may be, of bfloat16 to 8 bits, where it meets q. Inputs are finite: a value
+    that is not may reach every result of its chunk of 64 steps and the later ones. A prompt may be padded behind its end
+    with log_decay 0 and k 0, which leaves the state as it was."""
     name = "linear_attention"
     q, k, v, gs, B, T, H, Hq, DK, DV, _ = _attention_inputs(name, q, k, v, log_decay, True)
     scale = DK ** -0.5 if scale is None else _number(name, "scale", scale)

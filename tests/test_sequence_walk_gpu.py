@@ -142,3 +142,20 @@ def test_in_graphs_and_on_streams_at_once(ms):
         torch.cuda.synchronize()
         for _, outs in graphs:
             assert all(torch.equal(a, b) for a, b in zip(w, outs))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_status_after_memory_that_was_another_calls(ms, dtype):
+    """Scratch that holds what a wait that gave up would leave, from whoever had the memory before."""
+    x = rand(1, 300, 2, 64, seed=1, dtype=dtype)
+    g = ms.from_torch(decays(1, 300, 2, seed=2))
+    ms.ops.set_scan_status_check(True)
+    try:
+        for _ in range(3):
+            used = [torch.full((n,), 6, dtype=torch.int32, device="cuda") for n in (256, 4096, 1 << 16, 1 << 18, 1 << 20, 1 << 22)]
+            del used
+            A = ms.from_torch
+            ms.linear_attention(A(x), A(x), A(x), g)
+            ms.linear_attention_backward(A(x), A(x), A(x), A(x), g)
+    finally:
+        ms.ops.set_scan_status_check(False)
