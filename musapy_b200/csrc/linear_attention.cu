@@ -20,7 +20,8 @@
 //
 // Products run on the tensor cores with operands of bf16 and sums in float. A
 // bf16 input is one such operand; a float16 input is the sum of two, a float of three,
-// and so is what a float weight makes of an input. Products of pieces whose
+// and so is what a float weight makes of an input. Scores and states that reach a 16-bit result alone are two
+// (16 bits: the result's own rounding is what remains). Products of pieces whose
 // place together is past the result's precision are left out.
 //
 // This file has the kernels of any type, layout and width up to 256: the states at the
@@ -53,10 +54,10 @@ template <> struct RawPieces<__half> { static constexpr int n = 2; };
 template <> struct RawPieces<float> { static constexpr int n = 3; };
 
 // What a product that only reaches a result of type T has to keep: the scores' pieces (P), the states' (S).
-// bf16: scores are rounded once to bf16, half a step like the result's own rounding; the states, whose
-// rounding would come on top, keep 16 bits. float16: 16 bits of both. float: 24.
+// 16-bit types: 16 bits of both, so that the result is off by its own rounding (with scores of 8 bits a bf16 result
+// was off by 2.35e-3 of its norm, where its rounding is 1.66e-3). float: 24.
 template <class T> struct Keep;
-template <> struct Keep<bf16> { static constexpr int P = 1, S = 2; };
+template <> struct Keep<bf16> { static constexpr int P = 2, S = 2; };
 template <> struct Keep<__half> { static constexpr int P = 2, S = 2; };
 template <> struct Keep<float> { static constexpr int P = 3, S = 3; };
 constexpr int kExact = 3;  // 24 bits: what reaches a result of 32 bits
@@ -527,7 +528,9 @@ __global__ void __launch_bounds__(kThreads) k_la_gradients(Gradients p) {
   __shared__ ChunkDecay cd;
   __shared__ float rows_m[kChunk], cols_m[4][kChunk], far_q[kChunk], far_k[kChunk], through[4];
   bf16 *X = tiles, *Y = X + PT * kPlane, *Z = Y + PT * kPlane, *W = Z + kExact * kPlane;
-  bf16 *Pt = W + kExact * kPlane, *Rt = Pt + PP * kPlane;
+  // the scores are used before U comes to W in three planes, those of the gradients beside it
+  bf16 *Pt = W, *Rt = W + kExact * kPlane;
+  static_assert(PP <= kExact, "the scores' planes fit those of U");
   const Shape& d = p.d;
   const int tk = (d.dkp + kTile - 1) / kTile, tv = (d.dvp + kTile - 1) / kTile;
   const int c = (int)(blockIdx.x % d.chunks), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m = warp * 16;
@@ -721,7 +724,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_la_gradients_wide(Gradients
   __shared__ ChunkDecay cd;
   __shared__ float rows_m[2][kChunk], cols_m[4][kChunk], far_q[2][kChunk], far_k[2][kChunk], through[8];
   bf16 *Q = tiles, *K = Q + NK * kPlane, *V = K + NK * kPlane, *G = V + NV * kPlane, *Z = G + NV * kPlane, *W = Z + kExact * kPlane;
-  bf16 *Pt = W + kExact * kPlane, *Rt = Pt + kPlane;
+  constexpr int PP = Keep<bf16>::P;
+  bf16 *Pt = W + kExact * kPlane, *Rt = Pt + PP * kPlane;
   const Shape& d = p.d;
   const int c = (int)(blockIdx.x % d.chunks), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int m = (warp & 3) * 16, side = warp >> 2, n0 = side * 32;
@@ -787,8 +791,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_la_gradients_wide(Gradients
           rs[a] += both;
           cs[e] += both;
         }
-        store_pair<1>(Pt, r, j, pr[0], pr[1]);
-        store_pair<1>(Rt, r, j, rr[0], rr[1]);
+        store_pair<PP>(Pt, r, j, pr[0], pr[1]);
+        store_pair<PP>(Rt, r, j, rr[0], rr[1]);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -869,8 +873,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_la_gradients_wide(Gradients
     weigh(ak, cd.rest, 1.0f);
     dot(aq, Q + ik * kPlane, fq);
     dot(ak, K + ik * kPlane, fk);
-    multiply<4, false, true, 1, 1, 1>(aq, Rt, m, K + ik * kPlane, n0);
-    multiply<4, true, true, 1, 1, 1>(ak, Rt, m, Q + ik * kPlane, n0);
+    multiply<4, false, true, PP, 1, PP>(aq, Rt, m, K + ik * kPlane, n0);
+    multiply<4, true, true, PP, 1, PP>(ak, Rt, m, Q + ik * kPlane, n0);
     const int64_t to = ((b * d.T + t0) * d.H + h) * d.DK + ik * kTile;
     write((O*)p.dq + to, (int64_t)d.H * d.DK, d.DK - ik * kTile, aq);
     write((O*)p.dk + to, (int64_t)d.H * d.DK, d.DK - ik * kTile, ak);
@@ -878,7 +882,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_la_gradients_wide(Gradients
 #pragma unroll
   for (int iv = 0; iv < NV; ++iv) {
     weigh(dv[iv], cd.rest, 1.0f);
-    multiply<4, true, true, 1, 1, 1>(dv[iv], Pt, m, G + iv * kPlane, n0);
+    multiply<4, true, true, PP, 1, PP>(dv[iv], Pt, m, G + iv * kPlane, n0);
     write((bf16*)p.dv + ((b * d.T + t0) * d.H + h) * d.DV + iv * kTile, (int64_t)d.H * d.DV, d.DV - iv * kTile, dv[iv]);
   }
 #pragma unroll
@@ -1120,7 +1124,7 @@ struct GradScratch {
 
 template <int NK, int NV, class O>
 int run_wide(const Gradients& p, cudaStream_t s) {
-  constexpr int kWideBytes = (2 * NK + 2 * NV + 2 * kExact + 2) * kPlane * 2;
+  constexpr int kWideBytes = (2 * NK + 2 * NV + 2 * kExact + 2 * Keep<bf16>::P) * kPlane * 2;
   if (int rc = allow_smem<k_la_gradients_wide<NK, NV, O>, kWideBytes>("linear_attention_backward")) return rc;
   k_la_gradients_wide<NK, NV, O><<<(unsigned)(p.d.B * p.d.H * p.d.chunks), kWideThreads, kWideBytes, s>>>(p);
   return launch_check("linear_attention_backward");
@@ -1135,7 +1139,7 @@ int run_gradients(const Gradients& p, bool wide, cudaStream_t s) {
       return p.d.DV > 64 ? run_wide<1, 2, O>(p, s) : run_wide<1, 1, O>(p, s);
     }
   }
-  constexpr int kGradBytes = (2 * RawPieces<T>::n + 2 * kExact + 2 * Keep<T>::P) * kPlane * 2;
+  constexpr int kGradBytes = (2 * RawPieces<T>::n + 2 * kExact + Keep<T>::P) * kPlane * 2;
   if (int rc = allow_smem<k_la_gradients<T, O>, kGradBytes>("linear_attention_backward")) return rc;
   k_la_gradients<T, O><<<(unsigned)(p.d.B * p.d.H * p.d.chunks), kThreads, kGradBytes, s>>>(p);
   return launch_check("linear_attention_backward");

@@ -2,27 +2,27 @@
 // it) with the state on chip, so that q, k and v are read and o is written once. The formulas are those of
 // linear_attention.cu. Per chunk of 64 steps the tensor core makes
 //
-//   A = q k'           (steps x steps)        -> P = D A, rounded to bf16, back to shared memory
+//   A = q k'           (steps x steps)        -> P = D A, as two bf16 numbers, back to shared memory
 //   E = (w k)' v       (channels x channels)  w_j = e^(G_C - G_j); w k as three bf16 numbers that sum to it
 //   X' = S' q', Y' = v' P'  (channels of v x steps),  o = scale (e^(G_i) X + Y)
 //
-// and the state's threads S <- e^(G_C) S + E in float, from which X takes S rounded once to bf16: like the rounding of P
-// it is half a step of the output's type, and the state itself keeps 32 bits. Only that sum ties a chunk to the
-// next; E, A and P of the next chunks are made ahead of it.
+// and the state's threads S <- e^(G_C) S + E in float, from which X takes S as two bf16 numbers. Two numbers keep 16 bits, so
+// that outputs are off by their own rounding (1.66e-3 of their norm; with P and S rounded once to bf16, 2.35e-3, in 211 us
+// instead of 266 for the first case below). The sum and X tie a chunk to the next.
 //
 // Roles of the block's warps: 8 keep the state (in tensor memory, half a row of channels per thread), 4 write
-// outputs (where q was, for a copy to take them), 8 weigh and split k, 4 make P, one copies in (TMA, three chunks in
+// outputs (where q was, for a copy to take them), 8 weigh and split k, 4 make P, one copies in (TMA, two or three chunks in
 // shared memory), one copies out, one issues the matrix instructions, one makes the decays. They meet at mbarriers; every wait gives up after some seconds, sets the status
 // word and ends the block.
 //
-// What it takes: 8 x 4096 x 16 heads of 128, 218 us (2.5 TB/s; 553 MB, 85 us at the copy rate; without this kernel 1441 us);
-// 1 x 32768 x 8 heads of 64 in 18 segments 125 us with the walk that finds their states. Without outputs, the states of all chunks
-// kept in float, 4 x 4096 x 16 heads of 128 take 100 us (2.7 TB/s; by each thread's own stores 149). A chunk takes about 5500 cycles: the
-// tensor core has 32 instructions, each of which takes 73 cycles by itself whatever its columns up to 128 (its left operand's
-// 4 KB come at 64 bytes a cycle) and 90 to 110 beside the other warps' shared memory traffic; what passes from one chunk
-// to the next is E (12 instructions), the state's sum and X. Steps on the way: scores before their place is free 293 -> 224 us;
-// outputs through shared memory and TMA instead of 2-byte stores 224 -> 218; q and k three chunks deep but v two, and the
-// order E, scores, X, Y 205 against 196 in the same run; two issuing warps 219.
+// What it takes: 8 x 4096 x 16 heads of 128, 266 us (2.1 TB/s; 553 MB, 85 us at the copy rate; without this kernel 1441 us);
+// 1 x 32768 x 8 heads of 64 in 18 segments 140 us with the walk that finds their states. Without outputs, the states of all chunks
+// kept in float, 4 x 4096 x 16 heads of 128 take 100 us (2.7 TB/s; by each thread's own stores 149). The
+// tensor core has 40 instructions a chunk, each of which takes 73 cycles by itself whatever its columns up to 128 (its left operand's
+// 4 KB come at 64 bytes a cycle), so that both pieces of P are one right operand of 128 columns; those of S, a left
+// operand, are two. From one chunk to the next pass X (16 instructions) and the state's sum, which Y and the next scores
+// overlap. Issue order E, X, Y, next scores: 279 us for the first case with the L2 flushed, 174 for its heads of 64; X, Y, next scores, E:
+// 298 and 206; X, E, Y, next scores: 279 and 180. Three chunks of 128 and 128 channels do not fit beside the pieces; there two are under way.
 //
 // Operands lie as the copies leave them, rows of 128 bytes in the 128-byte swizzle; what is needed transposed (k, v, S as
 // left operands, v as a right one) is read "along the other dim" by the tensor core. Every matrix
@@ -41,11 +41,11 @@ namespace {
 using bf16 = __nv_bfloat16;
 
 constexpr int kThreads = 28 * 32;
-constexpr int kStages = 3;   // chunks of q, k, v in shared memory
+constexpr int kMostStages = 3;  // chunks of q, k, v in shared memory
 constexpr int kSlots = 4;    // chunks whose decays are there
 constexpr int kPieces = 3;   // of w k: the code takes them to be three
 constexpr uint32_t kTmemColumns = 512;
-constexpr uint32_t kColA = 0, kColX = 64, kColY = 128, kColE = 192, kColS = 320;
+constexpr uint32_t kColA = 0, kColX = 64, kColY = 128, kColE = 256, kColS = 384;  // Y: of P's two pieces, side by side
 
 // A bounded wait in few instructions: there are many of them. A try itself waits for a while, so that 2^22 of
 // them are seconds.
@@ -129,18 +129,26 @@ MPB_D void tma_write(const CUtensorMap* map, uint32_t src, int x, int h, int t, 
                : "memory");
 }
 
+// Two floats as two bf16 numbers each: their rounding, and that of what it leaves.
+MPB_D void two_pieces(float2 f, uint32_t& high, uint32_t& low) {
+  high = pack<bf16>(f).w;
+  low = pack<bf16>(vfma(make_float2(__uint_as_float(high << 16), __uint_as_float(high & 0xffff0000u)), vset<2>(-1.0f), f)).w;
+}
+
 // ------------------------------------------------------------ layout
 enum Bar { kFull0, kFull1, kFull2, kEmpty0, kEmpty1, kEmpty2, kDec0, kDec1, kDec2, kDec3, kADone0, kADone1, kAFree, kPReady, kWReady, kEDone, kEFree, kSReady,
            kXDone, kODone, kOFree, kOReady0, kOReady1, kOReady2, kOEmpty, kFree0, kFree1, kFree2, kFree3, kEnd, kBars };
 
-template <int DK, int DV>
+template <int DK, int DV, bool OUT>
 struct Layout {
   static constexpr int kBlock = 64 * 128;  // 64 steps of 64 channels
-  static constexpr int q = 0, k = q + DK / 64 * kBlock, v = k + DK / 64 * kBlock, kStage = v + DV / 64 * kBlock;
-  // the first piece of w k takes the place of k
-  static constexpr int P = kStages * kStage, W = P + kBlock, S = W + (kPieces - 1) * (DK / 64) * kBlock;
-  // S has two blocks of 64 columns in any case: a left operand has 128 rows, and may read the second
-  static constexpr int decays = S + 2 * DK * 128;
+  static constexpr int q = 0, k = q + (OUT ? DK / 64 * kBlock : 0), v = k + DK / 64 * kBlock, kStage = v + DV / 64 * kBlock;
+  // three chunks of 128 and 128 channels do not fit beside the two pieces of S and P
+  static constexpr int kStages = OUT && DK + DV == 256 ? 2 : kMostStages;
+  // The first piece of w k takes the place of k. A left operand has 128 rows, and where it holds 64 the other half is read
+  // from what follows: S behind W, P behind S.
+  static constexpr int W = kStages * kStage, S = W + (kPieces - 1) * (DK / 64) * kBlock;
+  static constexpr int kPieceS = DV / 64 * DK * 128, P = S + 2 * kPieceS, decays = P + 2 * kBlock;
   static constexpr int bars = decays + kSlots * ((int)sizeof(ChunkDecay) + 15) / 16 * 16, tmem = bars + kBars * 8;
   static constexpr int bytes = tmem + 16 + 1024;  // the copies' rows want 1024-byte alignment
 };
@@ -151,7 +159,8 @@ struct Maps {
 
 template <int DK, int DV, bool OUT>
 __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__ Maps maps, Walk p) {
-  using L = Layout<DK, DV>;
+  using L = Layout<DK, DV, OUT>;
+  constexpr int kStages = L::kStages;
   extern __shared__ unsigned char raw[];
   const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u;
   unsigned char* mem = raw + (smem - smem_u32(raw));
@@ -214,18 +223,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
       }
       unsigned char* s_row = mem + L::S + row * 128;
       const uint32_t s_tmem = quarter + kColS + col0, e_tmem = quarter + kColE + col0;
-      // 16 columns of S to shared memory, rounded
+      // 16 columns of S to shared memory, as two bf16 numbers each: its rounding, and that of what it leaves
       auto put = [&](int g, const uint32_t (&s)[16]) {
         const int c = col0 + g * 16;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          uint4 w;
-          w.x = pack<bf16>(make_float2(__uint_as_float(s[8 * k]), __uint_as_float(s[8 * k + 1]))).w;
-          w.y = pack<bf16>(make_float2(__uint_as_float(s[8 * k + 2]), __uint_as_float(s[8 * k + 3]))).w;
-          w.z = pack<bf16>(make_float2(__uint_as_float(s[8 * k + 4]), __uint_as_float(s[8 * k + 5]))).w;
-          w.w = pack<bf16>(make_float2(__uint_as_float(s[8 * k + 6]), __uint_as_float(s[8 * k + 7]))).w;
-          const int at = c / 8 % 8 + k;
-          *reinterpret_cast<uint4*>(s_row + c / 64 * (DK * 128) + ((at ^ (row & 7)) << 4)) = w;
+          uint32_t high[4], low[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) two_pieces(make_float2(__uint_as_float(s[8 * k + 2 * j]), __uint_as_float(s[8 * k + 2 * j + 1])), high[j], low[j]);
+          unsigned char* to = s_row + c / 64 * (DK * 128) + ((c / 8 % 8 + k ^ (row & 7)) << 4);
+          *reinterpret_cast<uint4*>(to) = make_uint4(high[0], high[1], high[2], high[3]);
+          *reinterpret_cast<uint4*>(to + L::kPieceS) = make_uint4(low[0], low[1], low[2], low[3]);
         }
       };
 #pragma unroll 1
@@ -245,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         mbar_arrive(bar(kSReady));
       }
       float since = 1.0f;
-      // The state before each chunk leaves in float, by a copy of 32 columns each from where q would be, and S.
+      // The state before each chunk leaves in float, by a copy of 32 columns each from where S's pieces would be.
       const bool keep = !OUT && p.at;
       for (int n = 0; n < n_chunks; ++n) {
         const int c = chunk(n);
@@ -274,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
           }
           if (keep) {
             const int c = col0 + g * 16;
-            unsigned char* to = mem + (c < 96 ? c / 32 * L::kStage + L::q : L::S) + row * 128;
+            unsigned char* to = mem + L::S + c / 32 * (DK * 128) + row * 128;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               *reinterpret_cast<uint4*>(to + ((c / 4 % 8 + i ^ (row & 7)) << 4)) = make_uint4(sg[4 * i], sg[4 * i + 1], sg[4 * i + 2], sg[4 * i + 3]);
@@ -325,9 +333,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         uint32_t two[32];  // outputs of two steps each
 #pragma unroll
         for (int g = 0; g < 8; ++g) {
-          uint32_t x[8], y[8];
+          uint32_t x[8], y[8], z[8];
           tmem_load(x, quarter + kColX + g * 8);
           tmem_load(y, quarter + kColY + g * 8);
+          tmem_load(z, quarter + kColY + 64 + g * 8);
           wait_loads();
 #pragma unroll
           for (int i = 0; i < 8; i += 2) {
@@ -336,7 +345,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
             // what a decay of zero has dropped may be anything
             v.x = by.x != 0.0f ? v.x : 0.0f;
             v.y = by.y != 0.0f ? v.y : 0.0f;
-            two[g * 4 + i / 2] = pack<bf16>(vmul(vfma(by, v, make_float2(__uint_as_float(y[i]), __uint_as_float(y[i + 1]))), scale)).w;
+            const float2 near = vadd(make_float2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])),
+                                     make_float2(__uint_as_float(z[i]), __uint_as_float(z[i + 1])));
+            two[g * 4 + i / 2] = pack<bf16>(vmul(vfma(by, v, near), scale)).w;
           }
         }
         // more channels than q has: the place of k too, once the state's sum has been made from it
@@ -401,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         if (!wait_warp(kDec0 + n % kSlots, n / kSlots) || !wait_warp(kADone0 + (n & 1), n / 2)) break;
         fence_after();
         const ChunkDecay& cd = decays[n % kSlots];
-        uint4 w[4] = {};
+        uint4 w[4] = {}, z[4] = {};
         if ((warp & 3) >= half) {
           uint32_t a[2][16];
           tmem_load(a[0], quarter + kColA + half * 32);
@@ -418,16 +429,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
             float f[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) f[i] = j + i <= row && j + i >= from ? e[i] * __uint_as_float(a[c >> 2][(c & 3) * 4 + i]) : 0.0f;
-            const uint32_t x = pack<bf16>(make_float2(f[0], f[1])).w, y = pack<bf16>(make_float2(f[2], f[3])).w;
-            if (c & 1) w[c >> 1].z = x, w[c >> 1].w = y;
-            else w[c >> 1].x = x, w[c >> 1].y = y;
+            uint4 &high = w[c >> 1], &low = z[c >> 1];
+            if (c & 1) {
+              two_pieces(make_float2(f[0], f[1]), high.z, low.z);
+              two_pieces(make_float2(f[2], f[3]), high.w, low.w);
+            } else {
+              two_pieces(make_float2(f[0], f[1]), high.x, low.x);
+              two_pieces(make_float2(f[2], f[3]), high.y, low.y);
+            }
           }
         }
         fence_before();
         mbar_arrive(bar(kAFree));
         if (n > 0 && !wait_warp(kODone, n - 1)) break;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(to + (((half * 4 + c) ^ (row & 7)) << 4)) = w[c];
+        for (int c = 0; c < 4; ++c) {
+          unsigned char* at = to + (((half * 4 + c) ^ (row & 7)) << 4);
+          *reinterpret_cast<uint4*>(at) = w[c];
+          *reinterpret_cast<uint4*>(at + L::kBlock) = z[c];
+        }
         proxy_fence();
         mbar_arrive(bar(kPReady));
       }
@@ -439,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         if (n >= kStages && !wait(kEmpty0 + s, n / kStages - 1)) break;
         const uint32_t at = smem + s * L::kStage;
         const int t0 = chunk(n) * kChunk;
-        mbar_expect_tx(bar(kFull0 + s), L::kStage - (OUT ? 0 : L::k));
+        mbar_expect_tx(bar(kFull0 + s), L::kStage);
         for (int i = 0; i < DK / 64; ++i) {
           if (OUT) tma_tile(at + L::q + i * L::kBlock, &maps.q, i * 64, hq, t0, (int)b, bar(kFull0 + s));
           tma_tile(at + L::k + i * L::kBlock, &maps.k, i * 64, hq, t0, (int)b, bar(kFull0 + s));
@@ -449,7 +469,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
     }
   } else if (warp == 23) {  // ------------------- the matrix instructions
     if (lane == 0) {
-      constexpr uint32_t kScores = instruction(64, false, false), kSum = instruction(DV, true, true), kOut = instruction(64, true, false);
+      constexpr uint32_t kScores = instruction(64, false, false), kSum = instruction(DV, true, true), kOut = instruction(64, true, false),
+                         kOutTwo = instruction(128, true, false);
       const Operand q0 = operand(smem + L::q, 16, 1024), k0 = operand(smem + L::k, 16, 1024), kt0 = operand(smem + L::k, kOther, 1024),
                     vt0 = operand(smem + L::v, kOther, 1024), w0 = operand(smem + L::W, kOther, 1024),
                     s0 = operand(smem + L::S, DK * 128, 1024), p0 = operand(smem + L::P, 16, 1024);
@@ -470,28 +491,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
       for (int n = 0; n < n_chunks; ++n) {
         const int st = n % kStages, next = (n + 1) % kStages;
         const Operand kt = in_stage(kt0, st), vt = in_stage(vt0, st);
-        if (OUT) {
-          if (!wait(kSReady, n) || !wait(kFull0 + st, n / kStages) || (n > 0 && !wait(kOFree, n - 1))) break;
-          fence_after();
-          const Operand q = in_stage(q0, st);
-          mma<false>(tmem + kColX, s0, 0, q, 0, kOut);
-#pragma unroll
-          for (int i = 1; i < DK / 16; ++i) mma<true>(tmem + kColX, s0, i * 2048, q, (i / 4) * L::kBlock + (i % 4) * 32, kOut);
-          commit(bar(kXDone));
-        }
-        if (OUT) {
-          if (!wait(kPReady, n)) break;
-          fence_after();
-          mma<false>(tmem + kColY, vt, 0, p0, 0, kOut);
-#pragma unroll
-          for (int i = 1; i < 4; ++i) mma<true>(tmem + kColY, vt, i * 2048, p0, i * 32, kOut);
-          commit(bar(kODone));
-          if (n + 1 < n_chunks) {
-            if (!wait(kFull0 + next, (n + 1) / kStages) || !wait(kAFree, n)) break;
-            fence_after();
-            scores(n + 1, next);
-          }
-        }
+        // where the outputs take the place of k, they still wait for the sum before
+        if (OUT && DV > DK && n > 0 && !wait(kOFree, n - 1)) break;
         if (!wait(kWReady, n) || !wait(kFull0 + st, n / kStages)) break;
         if (n > 0 && !wait(kEFree, n - 1)) break;
         fence_after();
@@ -505,6 +506,30 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         for (int i = 0; i < 4; ++i) mma<true>(tmem + kColE, kt, i * 2048, vt, i * 2048, kSum);
         commit(bar(kEDone));
         commit(bar(kEmpty0 + st));
+        if (OUT) {
+          if (!wait(kSReady, n) || (n > 0 && !wait(kOFree, n - 1))) break;
+          fence_after();
+          const Operand q = in_stage(q0, st);
+          // the smaller piece first
+          mma<false>(tmem + kColX, s0, L::kPieceS, q, 0, kOut);
+#pragma unroll
+          for (int i = 1; i < DK / 16; ++i) mma<true>(tmem + kColX, s0, L::kPieceS + i * 2048, q, (i / 4) * L::kBlock + (i % 4) * 32, kOut);
+#pragma unroll
+          for (int i = 0; i < DK / 16; ++i) mma<true>(tmem + kColX, s0, i * 2048, q, (i / 4) * L::kBlock + (i % 4) * 32, kOut);
+          commit(bar(kXDone));
+          if (!wait(kPReady, n)) break;
+          fence_after();
+          // both pieces of P in one: 128 columns cost what 64 do
+          mma<false>(tmem + kColY, vt, 0, p0, 0, kOutTwo);
+#pragma unroll
+          for (int i = 1; i < 4; ++i) mma<true>(tmem + kColY, vt, i * 2048, p0, i * 32, kOutTwo);
+          commit(bar(kODone));
+          if (n + 1 < n_chunks) {
+            if (!wait(kFull0 + next, (n + 1) / kStages) || !wait(kAFree, n)) break;
+            fence_after();
+            scores(n + 1, next);
+          }
+        }
       }
     }
   } else if (warp == 27) {  // ----------------------- the outputs' copies
@@ -513,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         if (!wait(kOReady0, n)) break;
         for (int i = 0; i < DV / 32; ++i)
           if (i * 32 < d.dvp)
-            tma_write(&maps.o, smem + (i < 3 ? i * L::kStage + L::q : L::S), i * 32, 0, chunk(n), (int)bh);
+            tma_write(&maps.o, smem + L::S + i * (DK * 128), i * 32, 0, chunk(n), (int)bh);
         asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
         mbar_arrive(bar(kOEmpty));
       }
@@ -609,7 +634,7 @@ int launch(const Walk& p, cudaStream_t s) {
       (OUT && !encode(&maps.o, {p.o, d.T * d.H * d.DV, (int64_t)d.H * d.DV, d.DV, true}, d.B, d.T, d.H, d.DV)) ||
       (!OUT && p.at && !encode_states(&maps.o, p, DK)))
     return fail(MPB_ERR_CUDA, "linear_attention: the copies' maps cannot be made");
-  constexpr int kWalkBytes = Layout<DK, DV>::bytes;
+  constexpr int kWalkBytes = Layout<DK, DV, OUT>::bytes;
   if (int rc = allow_smem<k_la_walk<DK, DV, OUT>, kWalkBytes>("linear_attention")) return rc;
   k_la_walk<DK, DV, OUT><<<(unsigned)(d.B * d.H * d.segments), kThreads, kWalkBytes, s>>>(maps, p);
   return launch_check("linear_attention");

@@ -91,10 +91,9 @@ def linear_attention(q, k, v, log_decay, state=None, scale=None, return_state=Fa
     (B, H, DK, DV) float32, is S before the first step (zero when None). scale defaults to DK^-0.5. DK and DV are at most
     256. Returns o (B, T, H, DV) in v's dtype; with ``return_state`` also the last S in float32.
 
-    S and every sum run in float32; the scores of float32, float16 and bfloat16 inputs are rounded to 24, 16 and 8 bits
-    before they meet v, and a copy of the state may be, of bfloat16 to 8 bits, where it meets q. Inputs are finite: a value
-    that is not may reach every result of its chunk of 64 steps and the later ones. A prompt may be padded behind its end
-    with log_decay 0 and k 0, which leaves the state as it was."""
+    S and every sum run in float32; where the scores meet v, and the state meets q, they keep 24 bits (float32) or 16
+    (float16, bfloat16). Inputs are finite: a value that is not may reach every result of its chunk of 64 steps and the
+    later ones. A prompt may be padded behind its end with log_decay 0 and k 0, which leaves the state as it was."""
     name = "linear_attention"
     q, k, v, gs, B, T, H, Hq, DK, DV, _ = _attention_inputs(name, q, k, v, log_decay, True)
     scale = DK ** -0.5 if scale is None else _number(name, "scale", scale)
