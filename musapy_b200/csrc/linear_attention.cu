@@ -16,7 +16,9 @@
 //   dg_t = sum_(j<t<=i) M_ij + sum_(i>=t) a_i + sum_(j<t) b_j + e^(G_C) <U, S>
 //
 // with M = scale D (q k') (do v') and a_i = q_i dq_i, b_j = k_j dk_j of the terms
-// with S and U: what passes through step t, so that nothing large cancels.
+// with S and U: what passes through step t. Only that is added, nothing is taken away again, so that a strong decay's
+// gradient, as small as the decay, is right to float precision among large ones (row sums less column sums of M lost it whole
+// from log-decays of -16 on).
 //
 // Products run on the tensor cores with operands of bf16 and sums in float. A
 // bf16 input is one such operand; a float16 input is the sum of two, a float of three,
@@ -32,7 +34,7 @@
 //
 // Bound: forward and backward move 0.5 GB each way at most for what takes them hundreds of us; they wait on their own
 // tiles (synchronous loads, two barriers a tile, splits into pieces), at 8 warps per SM: gradients of 4 x 4096 x 16 heads of 128 bf16
-// 677 us (1.3 TB/s under the profiler, tensor cores 0.2), 1 x 19250 x 3 heads of 128 and 64 float, all of the backward pass, 705 us.
+// 726 us (tensor cores 0.2 of their time), 1 x 19250 x 3 heads of 128 and 64 float, all of the backward pass, 705 us.
 // The step is bound by memory: 64 x 16 heads of 128 x 128, 134 MB, 24.6 us (5.5 TB/s).
 #include "common.cuh"
 #include "internal.h"
@@ -492,22 +494,50 @@ struct Gradients {
   float *dg, *dg_chunk;  // per step, or the sums of chunks
 };
 
-// The decays' gradients of a chunk, by one warp: each lane has two steps, of which `back` counts for the steps up to it and
-// `fore` for those behind; `through` is <U, S>.
-MPB_D void write_decay(const Gradients& p, const ChunkDecay& cd, int64_t b, int h, int c, int steps, const float (&back)[2],
-                       const float (&fore)[2], float through) {
+// Sums of M (a chunk's pairs of steps) over the columns before column t, for a warp's rows from t on: what each pair of
+// steps passes through step t. each_row takes the next 8 columns of a thread's row, of which it has the two at t; before: the sum of
+// the columns before those.
+struct Passing {
+  float at[2] = {0.0f, 0.0f};
+  MPB_D void each_row(int row, int t, float m0, float m1, float& before) {
+    const int l = threadIdx.x & 3;
+    float run = m0 + m1;
+    float x = __shfl_up_sync(0xffffffffu, run, 1, 4);
+    if (l >= 1) run += x;
+    x = __shfl_up_sync(0xffffffffu, run, 2, 4);
+    if (l >= 2) run += x;
+    x = __shfl_up_sync(0xffffffffu, run, 1, 4);
+    const float first = before + (l ? x : 0.0f);
+    before += __shfl_sync(0xffffffffu, run, 3, 4);
+    if (row >= t) at[0] += first;
+    if (row >= t + 1) at[1] += first + m0;
+  }
+  // over the warp's rows; in every thread
+  MPB_D void join() {
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      for (int o = 4; o < 32; o <<= 1) at[e] += __shfl_xor_sync(0xffffffffu, at[e], o);
+  }
+};
+
+// The decays' gradients of a chunk, by one warp: each lane has two steps. near: what the chunk's pairs pass through them; `back`
+// counts for the steps up to it and `fore` for those behind; `through` is <U, S>.
+MPB_D void write_decay(const Gradients& p, const ChunkDecay& cd, int64_t b, int h, int c, int steps, const float (&near)[2],
+                       const float (&back)[2], const float (&fore)[2], float through) {
   const int lane = threadIdx.x & 31, t = 2 * lane;
   float after = back[0] + back[1], before = fore[0] + fore[1];
-  const float own_a = after, own_b = before;
   for (int o = 1; o < 32; o <<= 1) {
     const float x = __shfl_down_sync(0xffffffffu, after, o), y = __shfl_up_sync(0xffffffffu, before, o);
     if (lane + o < 32) after += x;
     if (lane >= o) before += y;
   }
-  after -= own_a;
-  before -= own_b;
+  // without its own: the neighbour's, not a difference
+  after = __shfl_down_sync(0xffffffffu, after, 1);
+  before = __shfl_up_sync(0xffffffffu, before, 1);
+  if (lane == 31) after = 0.0f;
+  if (lane == 0) before = 0.0f;
   const float all_pass = cd.all != 0.0f ? cd.all * through : 0.0f;
-  float out[2] = {after + back[1] + back[0] + before + all_pass, after + back[1] + before + fore[0] + all_pass};
+  float out[2] = {near[0] + (after + back[1] + back[0]) + before + all_pass, near[1] + (after + back[1]) + (before + fore[0]) + all_pass};
   float sum = 0.0f;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -526,7 +556,7 @@ __global__ void __launch_bounds__(kThreads) k_la_gradients(Gradients p) {
   extern __shared__ __align__(16) bf16 tiles[];
   constexpr int PT = RawPieces<T>::n, PP = Keep<T>::P, PS = Keep<T>::S;
   __shared__ ChunkDecay cd;
-  __shared__ float rows_m[kChunk], cols_m[4][kChunk], far_q[kChunk], far_k[kChunk], through[4];
+  __shared__ float passing[4][kChunk], far_q[kChunk], far_k[kChunk], through[4];
   bf16 *X = tiles, *Y = X + PT * kPlane, *Z = Y + PT * kPlane, *W = Z + kExact * kPlane;
   // the scores are used before U comes to W in three planes, those of the gradients beside it
   bf16 *Pt = W, *Rt = W + kExact * kPlane;
@@ -562,10 +592,10 @@ __global__ void __launch_bounds__(kThreads) k_la_gradients(Gradients p) {
     __syncthreads();
   }
   {
-    float rs[2] = {0.0f, 0.0f};
+    float before[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-      float cs[2] = {0.0f, 0.0f};
+      Passing pass;
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
         const int r = m + (lane >> 2) + 8 * a, j = n * 8 + (lane & 3) * 2;
@@ -575,24 +605,13 @@ __global__ void __launch_bounds__(kThreads) k_la_gradients(Gradients p) {
           const float by = cd.pair(r, j + e) * p.scale;
           pr[e] = by * P[n][2 * a + e];
           rr[e] = by * R[n][2 * a + e];
-          const float both = pr[e] * R[n][2 * a + e];
-          rs[a] += both;
-          cs[e] += both;
         }
+        pass.each_row(r, j, pr[0] * R[n][2 * a], pr[1] * R[n][2 * a + 1], before[a]);
         store_pair<PP>(Pt, r, j, pr[0], pr[1]);
         store_pair<PP>(Rt, r, j, rr[0], rr[1]);
       }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        for (int o = 4; o < 32; o <<= 1) cs[e] += __shfl_xor_sync(0xffffffffu, cs[e], o);
-        if (lane < 4) cols_m[warp][n * 8 + lane * 2 + e] = cs[e];
-      }
-    }
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      rs[a] += __shfl_xor_sync(0xffffffffu, rs[a], 1);
-      rs[a] += __shfl_xor_sync(0xffffffffu, rs[a], 2);
-      if ((lane & 3) == 0) rows_m[m + (lane >> 2) + 8 * a] = rs[a];
+      pass.join();
+      if (lane < 4) passing[warp][n * 8 + lane * 2] = pass.at[0], passing[warp][n * 8 + lane * 2 + 1] = pass.at[1];
     }
   }
   auto weigh = [&](float (&acc)[8][4], const float* w, float by) {
@@ -690,19 +709,20 @@ __global__ void __launch_bounds__(kThreads) k_la_gradients(Gradients p) {
   if (lane == 0) through[warp] = pass;
   __syncthreads();
   if (warp != 0) return;
-  float back[2], fore[2];
+  float near[2], back[2], fore[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int t = 2 * lane + e;
-    back[e] = far_q[t] + (rows_m[t] - ((cols_m[0][t] + cols_m[1][t]) + (cols_m[2][t] + cols_m[3][t])));
+    near[e] = (passing[0][t] + passing[1][t]) + (passing[2][t] + passing[3][t]);
+    back[e] = far_q[t];
     fore[e] = far_k[t];
   }
-  write_decay(p, cd, b, h, c, steps, back, fore, (through[0] + through[1]) + (through[2] + through[3]));
+  write_decay(p, cd, b, h, c, steps, near, back, fore, (through[0] + through[1]) + (through[2] + through[3]));
 }
 
 // The same for bf16 heads of up to 64 NK and 64 NV channels: all of the chunk's q, k, v and do stay in shared memory,
 // copied there at once, and the two states pass through it once, a tile of 64 x 64 at a time, the next one on its way to registers
-// meanwhile. Eight warps: 16 rows and half of a tile's columns each. 4 x 4096 x 16 heads of 128: 677 us, where the kernel above, which
+// meanwhile. Eight warps: 16 rows and half of a tile's columns each. 4 x 4096 x 16 heads of 128: 726 us, where the kernel above, which
 // loads a tile whenever it needs one, takes 1273.
 constexpr int kWideThreads = 256;
 
@@ -722,7 +742,7 @@ template <int NK, int NV, class O>
 __global__ void __launch_bounds__(kWideThreads, 1) k_la_gradients_wide(Gradients p) {
   extern __shared__ __align__(16) bf16 tiles[];
   __shared__ ChunkDecay cd;
-  __shared__ float rows_m[2][kChunk], cols_m[4][kChunk], far_q[2][kChunk], far_k[2][kChunk], through[8];
+  __shared__ float rows_m[kChunk], passing[4][kChunk], far_q[2][kChunk], far_k[2][kChunk], through[8];
   bf16 *Q = tiles, *K = Q + NK * kPlane, *V = K + NK * kPlane, *G = V + NV * kPlane, *Z = G + NV * kPlane, *W = Z + kExact * kPlane;
   constexpr int PP = Keep<bf16>::P;
   bf16 *Pt = W + kExact * kPlane, *Rt = Pt + PP * kPlane;
@@ -774,10 +794,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_la_gradients_wide(Gradients
     for (int i = 0; i < NK; ++i) multiply<4, false, false, 1, 1, 1>(P, Q + i * kPlane, m, K + i * kPlane, n0);
 #pragma unroll
     for (int i = 0; i < NV; ++i) multiply<4, false, false, 1, 1, 1>(R, G + i * kPlane, m, V + i * kPlane, n0);
-    float rs[2] = {0.0f, 0.0f};
+    float before[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-      float cs[2] = {0.0f, 0.0f};
+      Passing pass;
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
         const int r = row + 8 * a, j = n * 8 + col;
@@ -787,25 +807,17 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_la_gradients_wide(Gradients
           const float by = cd.pair(r, j + e) * p.scale;
           pr[e] = by * P[n][2 * a + e];
           rr[e] = by * R[n][2 * a + e];
-          const float both = pr[e] * R[n][2 * a + e];
-          rs[a] += both;
-          cs[e] += both;
         }
+        pass.each_row(r, j, pr[0] * R[n][2 * a], pr[1] * R[n][2 * a + 1], before[a]);
         store_pair<PP>(Pt, r, j, pr[0], pr[1]);
         store_pair<PP>(Rt, r, j, rr[0], rr[1]);
       }
+      pass.join();
+      if (lane < 4)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        for (int o = 4; o < 32; o <<= 1) cs[e] += __shfl_xor_sync(0xffffffffu, cs[e], o);
-        if (lane < 4) cols_m[warp & 3][n0 + n * 8 + lane * 2 + e] = cs[e];
-      }
+        for (int e = 0; e < 2; ++e) passing[warp & 3][n0 + n * 8 + lane * 2 + e] = pass.at[e];
     }
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      rs[a] += __shfl_xor_sync(0xffffffffu, rs[a], 1);
-      rs[a] += __shfl_xor_sync(0xffffffffu, rs[a], 2);
-      if ((lane & 3) == 0) rows_m[side][row + 8 * a] = rs[a];
-    }
+    if (side == 0 && (lane & 3) == 0) rows_m[row] = before[0], rows_m[row + 8] = before[1];
   }
   auto weigh = [&](float (&acc)[4][4], const float* w, float by) {
 #pragma unroll
@@ -900,17 +912,26 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_la_gradients_wide(Gradients
   if (lane == 0) through[warp] = pass;
   __syncthreads();
   if (warp != 0) return;
-  float back[2], fore[2];
+  float near[2], back[2], fore[2];
+  // the second half's steps: also what the first half's columns pass to the rows from there on
+  const float own = rows_m[2 * lane + 1];
+  float rest = rows_m[2 * lane] + own;
+  for (int o = 1; o < 32; o <<= 1) {
+    const float x = __shfl_down_sync(0xffffffffu, rest, o);
+    if (lane + o < 32) rest += x;
+  }
+  const float next = __shfl_down_sync(0xffffffffu, rest, 1);
+  const float half[2] = {lane >= 16 ? rest : 0.0f, lane >= 16 ? (lane < 31 ? next : 0.0f) + own : 0.0f};
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int t = 2 * lane + e;
-    back[e] = (far_q[0][t] + far_q[1][t]) +
-              ((rows_m[0][t] + rows_m[1][t]) - ((cols_m[0][t] + cols_m[1][t]) + (cols_m[2][t] + cols_m[3][t])));
+    near[e] = (passing[0][t] + passing[1][t]) + (passing[2][t] + passing[3][t]) + half[e];
+    back[e] = far_q[0][t] + far_q[1][t];
     fore[e] = far_k[0][t] + far_k[1][t];
   }
   float all_pass = 0.0f;
   for (int k = 0; k < 8; ++k) all_pass += through[k];
-  write_decay(p, cd, b, h, c, steps, back, fore, all_pass);
+  write_decay(p, cd, b, h, c, steps, near, back, fore, all_pass);
 }
 
 // Sums over the heads that share one, in their order: (rows, heads, share, n) floats to (rows, heads, n).
