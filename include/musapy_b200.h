@@ -311,6 +311,10 @@ int mpb_linear_attention(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK
  * MPB_ERR_TIMEOUT when a bounded wait between the warps of a block gave up (its results are incomplete). */
 int mpb_linear_attention_status(const void* scratch, mpb_stream_t stream);
 
+/* How long such a wait may take, in nanoseconds (in steps of 4000), in the calls from now on, of every thread: two seconds
+ * at most, and unless this says otherwise; 0 lets every wait give up at once, to test what follows. Returns the limit before. */
+int64_t mpb_linear_attention_wait_limit(int64_t ns);
+
 /* Gradients of mpb_linear_attention from dout (B, T, H, DV) and dstate (B, H, DK, DV) floats or NULL, that of the
  * last state. Writes dq and dk (B, T, Hq, DK, summed over the heads that share one), dv (B, T, H, DV), dlog_decay
  * (B, T, H) floats, or with decay_by_head (H) floats, summed over sequences and steps in a fixed order, and

@@ -101,6 +101,8 @@ def _load() -> ctypes.CDLL:
     L.mpb_gated_scan_status.argtypes = [c_vp, c_vp]
     L.mpb_linear_attention_status.restype = ctypes.c_int
     L.mpb_linear_attention_status.argtypes = [c_vp, c_vp]
+    L.mpb_linear_attention_wait_limit.restype = ctypes.c_int64
+    L.mpb_linear_attention_wait_limit.argtypes = [ctypes.c_int64]
     L.mpb_launch_count.restype = ctypes.c_ulonglong
     L.mpb_launch_count.argtypes = []
     L.mpb_shard_arg_combine.restype = ctypes.c_int

@@ -1258,6 +1258,10 @@ int mpb_linear_attention_status(const void* scratch, mpb_stream_t stream) {
   return status == MPB_ERR_TIMEOUT ? fail(MPB_ERR_TIMEOUT, "linear_attention: a wait between its warps gave up") : MPB_OK;
 }
 
+int64_t mpb_linear_attention_wait_limit(int64_t ns) {
+  return walk_wait_limit(ns < 0 ? 0 : ns > (int64_t)kMostWaitNs ? (int64_t)kMostWaitNs : ns);
+}
+
 int mpb_linear_attention(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK, int64_t DV, int dtype, const void* q,
                          int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh,
                          const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh, const float* log_decay, int64_t g_sb,

@@ -106,6 +106,8 @@ struct Decay {
   int64_t sb, st, sh;
 };
 
+constexpr uint32_t kMostWaitNs = 2000000000;  // of a wait between a block's warps
+
 // The bf16 kernel of whole rows (linear_attention_walk.cu): one block per head of a sequence and segment.
 struct Walk {
   Shape d;
@@ -118,9 +120,11 @@ struct Walk {
   bool rev;
   float *at, *since, *ends, *last;  // as k_la_states leaves them; null where not wanted
   int* status;
+  int tries = 0;  // of a wait between the block's warps: set by the two below
 };
+int64_t walk_wait_limit(int64_t ns);
 bool walk_takes(const Shape& d, const Input& q, const Input& k, const Input& v);
-int walk_outputs(const Walk& p, cudaStream_t s);
-int walk_states(const Walk& p, cudaStream_t s);
+int walk_outputs(Walk p, cudaStream_t s);
+int walk_states(Walk p, cudaStream_t s);
 
 }  // namespace mpb

@@ -8,15 +8,15 @@
 //
 // and the state's threads S <- e^(G_C) S + E in float, from which X takes S as two bf16 numbers. Two numbers keep 16 bits, so
 // that outputs are off by their own rounding (1.66e-3 of their norm; with P and S rounded once to bf16, 2.35e-3, in 211 us
-// instead of 266 for the first case below). The sum and X tie a chunk to the next.
+// instead of 263 for the first case below). The sum and X tie a chunk to the next.
 //
 // Roles of the block's warps: 8 keep the state (in tensor memory, half a row of channels per thread), 4 write
 // outputs (where q was, for a copy to take them), 8 weigh and split k, 4 make P, one copies in (TMA, two or three chunks in
-// shared memory), one copies out, one issues the matrix instructions, one makes the decays. They meet at mbarriers; every wait gives up after some seconds, sets the status
+// shared memory), one copies out, one issues the matrix instructions, one makes the decays. They meet at mbarriers; every wait gives up after two seconds, sets the status
 // word and ends the block.
 //
-// What it takes: 8 x 4096 x 16 heads of 128, 266 us (2.1 TB/s; 553 MB, 85 us at the copy rate; without this kernel 1441 us);
-// 1 x 32768 x 8 heads of 64 in 18 segments 140 us with the walk that finds their states. Without outputs, the states of all chunks
+// What it takes: 8 x 4096 x 16 heads of 128, 263 us (2.1 TB/s; 553 MB, 85 us at the copy rate; without this kernel 1441 us);
+// 1 x 32768 x 8 heads of 64 in 18 segments 148 us with the walk that finds their states. Without outputs, the states of all chunks
 // kept in float, 4 x 4096 x 16 heads of 128 take 100 us (2.7 TB/s; by each thread's own stores 149). The
 // tensor core has 40 instructions a chunk, each of which takes 73 cycles by itself whatever its columns up to 128 (its left operand's
 // 4 KB come at 64 bytes a cycle), so that both pieces of P are one right operand of 128 columns; those of S, a left
@@ -29,6 +29,7 @@
 // instruction has 128 rows: of operands with 64, the second half is whatever lies behind them in shared memory, and its
 // results are not read.
 #include <cuda.h>
+#include <atomic>
 #include "async_copy.cuh"
 #include "common.cuh"
 #include "internal.h"
@@ -47,11 +48,13 @@ constexpr int kPieces = 3;   // of w k: the code takes them to be three
 constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kColA = 0, kColX = 64, kColY = 128, kColE = 256, kColS = 384;  // Y: of P's two pieces, side by side
 
-// A bounded wait in few instructions: there are many of them. A try itself waits for a while, so that 2^22 of
-// them are seconds.
-MPB_D bool mbar_wait_short(uint32_t bar, uint32_t parity) {
+// A bounded wait in few instructions: there are many of them, and code in them that reads the clock, though it does not run,
+// took the first case above from 270 to 310 us. A try that fails has itself waited for 4 us (3.98 measured, by 1 to 896
+// threads at once), so that a number of tries is a time.
+constexpr uint32_t kTryNs = 4000;
+MPB_D bool mbar_wait_for(uint32_t bar, uint32_t parity, int tries) {
 #pragma unroll 1
-  for (int i = 0; i < 1 << 22; ++i)
+  for (int i = 0; i < tries; ++i)
     if (mbar_try_wait(bar, parity)) return true;
   return false;
 }
@@ -177,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
   bool ok = true;
   // true where the phase of chunk n has come
   auto wait = [&](int i, int n) {
-    if (ok) ok = mbar_wait_short(bar(i), (uint32_t)n & 1);
+    if (ok) ok = mbar_wait_for(bar(i), (uint32_t)n & 1, p.tries);
     return ok;
   };
   auto wait_warp = [&](int i, int n) {
@@ -267,7 +270,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         uint32_t e[2][16], s[2][16];
         tmem_load(e[0], e_tmem);
         tmem_load(s[0], s_tmem);
-        if (OUT && !wait_warp(kXDone, n)) break;
+        if (OUT && !wait_warp(kXDone, n)) {
+          wait_loads();
+          break;
+        }
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
           uint32_t(&eg)[16] = e[g & 1], (&sg)[16] = s[g & 1];
@@ -454,7 +460,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
     }
   } else if (warp == 22) {  // -------------------------------- the copies
     if (lane == 0) {
-      for (int n = 0; n < n_chunks; ++n) {
+      int n = 0;
+      for (; n < n_chunks; ++n) {
         const int s = n % kStages;
         if (n >= kStages && !wait(kEmpty0 + s, n / kStages - 1)) break;
         const uint32_t at = smem + s * L::kStage;
@@ -466,6 +473,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         }
         for (int i = 0; i < DV / 64; ++i) tma_tile(at + L::v + i * L::kBlock, &maps.v, i * 64, h, t0, (int)b, bar(kFull0 + s));
       }
+      // whatever the others did: the last copy into each place has landed before the block ends
+      for (int s = 0; s < kStages && s < n; ++s) mbar_wait(bar(kFull0 + s), (uint32_t)((n - 1 - s) / kStages) & 1);
     }
   } else if (warp == 23) {  // ------------------- the matrix instructions
     if (lane == 0) {
@@ -566,12 +575,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
   }
   if (!ok && p.status) *p.status = MPB_ERR_TIMEOUT;
   __syncwarp();
-  // a block that gave up: what it has under way ends before its memory does
-  const bool failed = __syncthreads_or(!ok);
-  if (failed && warp == 23 && lane == 0) {
-    commit(bar(kEnd));
-    mbar_wait(bar(kEnd), 0);
-    for (int s = 0; s < kStages; ++s) mbar_wait(bar(kFull0 + s), 0);
+  // A block that gave up: what it has under way ends before its memory does. The copies have been waited for by the warps
+  // that issued them.
+  if (__syncthreads_or(!ok)) {
+    wait_loads();
+    wait_stores();
+    if (warp == 23 && lane == 0) {
+      commit(bar(kEnd));
+      mbar_wait(bar(kEnd), 0);
+    }
   }
   fence_before();
   __syncthreads();
@@ -581,6 +593,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
 }
 
 // ------------------------------------------------------------------- host
+std::atomic<uint32_t> wait_limit{kMostWaitNs};
+
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -659,7 +673,14 @@ bool walk_takes(const Shape& d, const Input& q, const Input& k, const Input& v) 
   }
   return true;
 }
-int walk_outputs(const Walk& p, cudaStream_t s) { return launch_for<true>(p, s); }
-int walk_states(const Walk& p, cudaStream_t s) { return launch_for<false>(p, s); }
+int walk_outputs(Walk p, cudaStream_t s) {
+  p.tries = (int)((wait_limit.load() + kTryNs - 1) / kTryNs);
+  return launch_for<true>(p, s);
+}
+int walk_states(Walk p, cudaStream_t s) {
+  p.tries = (int)((wait_limit.load() + kTryNs - 1) / kTryNs);
+  return launch_for<false>(p, s);
+}
+int64_t walk_wait_limit(int64_t ns) { return wait_limit.exchange((uint32_t)ns); }
 
 }  // namespace mpb
