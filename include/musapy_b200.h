@@ -308,7 +308,8 @@ int mpb_linear_attention(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK
                          size_t scratch_bytes, mpb_stream_t stream);
 
 /* Synchronises `stream` and reads the status word that a call left in its scratch (NULL: it had none): MPB_OK, or
- * MPB_ERR_TIMEOUT when a bounded wait between the warps of a block gave up (its results are incomplete). */
+ * MPB_ERR_TIMEOUT when a bounded wait between the warps of a block gave up (its results, and what is made
+ * from its states, are NaN). */
 int mpb_linear_attention_status(const void* scratch, mpb_stream_t stream);
 
 /* How long such a wait may take, in nanoseconds (in steps of 4000), in the calls from now on, of every thread: two seconds

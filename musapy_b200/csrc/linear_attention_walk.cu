@@ -13,7 +13,7 @@
 // Roles of the block's warps: 8 keep the state (in tensor memory, half a row of channels per thread), 4 write
 // outputs (where q was, for a copy to take them), 8 weigh and split k, 4 make P, one copies in (TMA, two or three chunks in
 // shared memory), one copies out, one issues the matrix instructions, one makes the decays. They meet at mbarriers; every wait gives up after two seconds, sets the status
-// word and ends the block.
+// word and ends the block, whose results are NaN.
 //
 // What it takes: 8 x 4096 x 16 heads of 128, 263 us (2.1 TB/s; 553 MB, 85 us at the copy rate; without this kernel 1441 us);
 // 1 x 32768 x 8 heads of 64 in 18 segments 148 us with the walk that finds their states. Without outputs, the states of all chunks
@@ -160,8 +160,29 @@ struct Maps {
   CUtensorMap q, k, v, o;
 };
 
+// What a block leaves that gave up: NaN in the place of all its results, which also reaches what is made from its states.
+// (Not inlined: in the kernel's own text it took the first case above from 263 to 280 us.)
+template <bool OUT>
+__device__ __noinline__ void leave_nan(const Walk& p) {
+  const Shape& d = p.d;
+  const int seg = (int)(blockIdx.x % d.segments);
+  const int64_t bh = blockIdx.x / d.segments, size = (int64_t)d.dkp * d.dvp;
+  const int c0 = seg * d.per, c1 = min(d.chunks, c0 + d.per);
+  auto fill = [&](float* to, int64_t n) {
+    for (int64_t i = threadIdx.x; i < n; i += kThreads) to[i] = NAN;
+  };
+  if (OUT) {
+    const int64_t h = bh % d.H, b = bh / d.H, t1 = min((int64_t)c1 * kChunk, d.T);
+    for (int64_t t = (int64_t)c0 * kChunk + threadIdx.x / 32; t < t1; t += kThreads / 32)
+      for (int c = threadIdx.x % 32; c < d.DV; c += 32) ((bf16*)p.o)[((b * d.T + t) * d.H + h) * d.DV + c] = __float2bfloat16_rn(NAN);
+  }
+  if (!OUT && p.at) fill(p.at + (bh * d.chunks + c0) * size, (c1 - c0) * size);
+  if (d.segments > 1 && p.ends) fill(p.ends + (bh * d.segments + seg) * size, size);
+  if (d.segments == 1 && p.last) fill(p.last + bh * d.DK * d.DV, (int64_t)d.DK * d.DV);
+}
+
 template <int DK, int DV, bool OUT>
-__global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__ Maps maps, Walk p) {
+__global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__ Maps maps, const __grid_constant__ Walk p) {
   using L = Layout<DK, DV, OUT>;
   constexpr int kStages = L::kStages;
   extern __shared__ unsigned char raw[];
@@ -584,6 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
       commit(bar(kEnd));
       mbar_wait(bar(kEnd), 0);
     }
+    leave_nan<OUT>(p);
   }
   fence_before();
   __syncthreads();

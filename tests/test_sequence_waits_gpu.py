@@ -86,3 +86,31 @@ def test_the_limit_is_two_seconds_at_most(ms):
     for asked, kept in ((-5, 0), (1 << 40, TWO_SECONDS), (7, 7)):
         LIB.mpb_linear_attention_wait_limit(asked)
         assert LIB.mpb_linear_attention_wait_limit(TWO_SECONDS) == kept
+
+
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_what_a_block_that_gave_up_leaves_is_nan(ms, size):
+    x = inputs(*size)
+    with limit(0):
+        got = [*forward(ms, x), *backward(ms, x)]
+    assert all(y.isnan().all() for y in got)
+
+
+@pytest.mark.parametrize("size", SIZES, ids=str)
+@pytest.mark.parametrize("ns", [4000, 8000, 12000, 20000, 60000])
+def test_every_value_is_right_or_nan(ms, size, ns):
+    x = inputs(*size)
+    want = [*forward(ms, x), *backward(ms, x)]
+    for _ in range(3):
+        with limit(ns):
+            got = [*forward(ms, x), *backward(ms, x)]
+        assert all(((a == b) | a.isnan()).all() for a, b in zip(got, want))
+
+
+def test_rows_of_others_stay(ms):
+    """What a block that gave up fills is its own: nothing behind the outputs' last step."""
+    big = torch.full((1, 200, 2, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    x = inputs(64, 64, 70, 2)
+    with limit(0):
+        ms.linear_attention(*(ms.from_torch(t) for t in x[:5]), out=ms.from_torch(big[:, :70]))
+    assert big[:, :70].isnan().all() and (big[:, 70:] == 7.0).all()
