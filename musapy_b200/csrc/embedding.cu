@@ -11,7 +11,8 @@
 // the block that finishes last. A new table is written once, rows that no token names
 // as zeros; a gradient that is there already is added to, where tokens name it.
 //
-// Bound: memory. Up to kFew tokens need no sort, up to kSmall are sorted by one kernel, more by two for each digit.
+// Bound: memory. Up to kFew tokens need no sort, up to kSmall are sorted by one kernel, more by two for each digit, and three from
+// 2^18 on.
 // Lookup of 32768 rows of 4096 bf16: 82 us (6.5 TB/s); 64 rows 2.3 us on the GPU. Gradient of 32768 tokens of 32000 x 2048 from
 // bf16: 130 us, of which the sums 98 (4.1 TB/s; they wait on three loads in a row: the list, its tokens, their rows) and the sort 27; of 4097 of
 // 50257 x 769 float, added: 24 us on the GPU, sort 6, sums 18 (rows that begin at no 16-byte boundary go by single elements).
@@ -31,6 +32,9 @@ constexpr int kPart = 32;
 constexpr int kMostBits = 9;  // of a digit
 constexpr int kMostBins = 1 << kMostBits;
 constexpr int kTileTokens = 2048;
+// Tiles whose counts each block of the sort sums by itself: quadratic, where a scan of them is one more launch per digit. 32000 rows of
+// 8 from 128 tiles: 134 us, scanned 137; 256: 237 and 217; 8192: 20.7 and 7.5 ms.
+constexpr int kFewTiles = 128;
 constexpr int kSmall = 8192;
 constexpr int kSmallBytes = (kSmall + 32) * 8;
 
@@ -197,10 +201,40 @@ __global__ void __launch_bounds__(kThreads) k_embed_count(Sorted p, const int* k
   for (int i = tid; i < bins; i += kThreads) counts[(int64_t)blockIdx.x * bins + i] = bin[i];
 }
 
+// The counts of many tiles, per digit: in the place of each the sum of those before it, and the sum of all. A block takes 32
+// digits; each of its warps a run of tiles.
+constexpr int kStartWarps = 32;
+__global__ void __launch_bounds__(kStartWarps * 32) k_embed_starts(int* counts, int* totals, int tiles, int bins) {
+  constexpr int kAhead = 8;
+  __shared__ int sums[kStartWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x * 32 + lane;
+  const int run = (tiles + kStartWarps - 1) / kStartWarps, t0 = min(warp * run, tiles), t1 = min(t0 + run, tiles);
+  const bool on = b < bins;
+  int sum = 0;
+#pragma unroll 8
+  for (int t = t0; t < t1; ++t)
+    if (on) sum += counts[(int64_t)t * bins + b];
+  sums[warp][lane] = sum;
+  __syncthreads();
+  int before = 0;
+  for (int w = 0; w < warp; ++w) before += sums[w][lane];
+  if (!on) return;
+  if (warp == kStartWarps - 1) totals[b] = before + sum;
+  for (int t = t0; t < t1; t += kAhead) {
+    int c[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (t + k < t1) c[k] = counts[(int64_t)(t + k) * bins + b];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (t + k < t1) counts[(int64_t)(t + k) * bins + b] = before, before += c[k];
+  }
+}
+
 // A tile's tokens to their places: behind the smaller digits of all tiles, the same digit of the tiles before, and of
-// the tokens before in the tile.
+// the tokens before in the tile. The tiles' counts, of few tiles, are summed by every block; with totals they have been.
 __global__ void __launch_bounds__(kThreads) k_embed_place(Sorted p, const int* keys, const int* at, int* keys_to, int* at_to,
-                                                          const int* counts, int shift, int bits) {
+                                                          const int* counts, const int* totals, int shift, int bits) {
   constexpr int kWarps = kThreads / 32, kSteps = kTileTokens / kThreads;
   __shared__ int base[kMostBins], red[32];
   __shared__ uint16_t mine[kWarps * kMostBins];
@@ -211,7 +245,9 @@ __global__ void __launch_bounds__(kThreads) k_embed_place(Sorted p, const int* k
   for (int k = 0; k < kMostBins / kThreads; ++k) {
     const int b = tid * (kMostBins / kThreads) + k;
     before[k] = total[k] = 0;
-    if (b < bins)
+    if (b < bins && totals)
+      before[k] = counts[(int64_t)blockIdx.x * bins + b], total[k] = totals[b];
+    else if (b < bins)
 #pragma unroll 8
       for (unsigned t = 0; t < gridDim.x; ++t) {
         const int c = counts[(int64_t)t * bins + b];
@@ -549,14 +585,15 @@ struct Digits {
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
 struct Scratch {
-  size_t keys, at, keys2, at2, counts, first, end, counters, parts, bytes;
+  size_t keys, at, keys2, at2, counts, totals, first, end, counters, parts, bytes;
   int64_t n_counters;
   Scratch(int64_t N, int64_t V, int64_t D, bool by_list) {
     const size_t n = round16((size_t)N * 4);
     const int64_t windows = (N + kPart - 1) / kPart, col_tiles = (D + 127) / 128;  // at most: a tile has 128 columns and more
     const bool small = N <= kSmall;
     keys = 0, at = n, keys2 = 2 * n, at2 = keys2 + (small ? 0 : n), counts = at2 + (small ? 0 : n);
-    first = counts + (small ? 0 : round16((size_t)((N + kTileTokens - 1) / kTileTokens) * kMostBins * 4));
+    totals = counts + (small ? 0 : round16((size_t)((N + kTileTokens - 1) / kTileTokens) * kMostBins * 4));
+    first = totals + (small ? 0 : kMostBins * 4);
     end = first + (by_list ? 0 : round16((size_t)V * 4));
     counters = end + (by_list ? 0 : round16((size_t)V * 4));
     n_counters = windows * col_tiles;
@@ -585,12 +622,13 @@ int sort_tokens(Sorted& p, char* scratch, const Scratch& w, cudaStream_t s) {
   const Digits g(p.V);
   int *a_keys = p.keys, *a_at = p.at, *b_keys = (int*)(scratch + w.keys2), *b_at = (int*)(scratch + w.at2);
   const unsigned tiles = (unsigned)((p.N + kTileTokens - 1) / kTileTokens);
-  int* counts = (int*)(scratch + w.counts);
+  int *counts = (int*)(scratch + w.counts), *totals = tiles > kFewTiles ? (int*)(scratch + w.totals) : nullptr;
   if (g.passes % 2 == 0) std::swap(a_keys, b_keys), std::swap(a_at, b_at);  // the last pass writes to p.keys
   const int *from_keys = nullptr, *from_at = nullptr;
   for (int k = 0; k < g.passes; ++k) {
     k_embed_count<<<tiles, kThreads, 0, s>>>(p, from_keys, counts, k * g.bits, g.bits);
-    k_embed_place<<<tiles, kThreads, 0, s>>>(p, from_keys, from_at, a_keys, a_at, counts, k * g.bits, g.bits);
+    if (totals) k_embed_starts<<<((1u << g.bits) + 31) / 32, kStartWarps * 32, 0, s>>>(counts, totals, (int)tiles, 1 << g.bits);
+    k_embed_place<<<tiles, kThreads, 0, s>>>(p, from_keys, from_at, a_keys, a_at, counts, totals, k * g.bits, g.bits);
     if (int rc = launch_check("embedding_backward")) return rc;
     from_keys = a_keys, from_at = a_at;
     std::swap(a_keys, b_keys), std::swap(a_at, b_at);

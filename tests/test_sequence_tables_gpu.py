@@ -64,3 +64,28 @@ def test_rows_that_share_their_low_digits(ms):
     got = ms.embedding_backward(ms.from_torch(dout), ms.from_torch(t), rows=V).torch()
     want, slack = Q.embedding_gradient(dout.double(), t, V, 1.0)
     P.close(got, want, slack)
+
+
+@pytest.mark.parametrize("into", [False, True])
+@pytest.mark.parametrize("N", [128 * 2048, 128 * 2048 + 1, 1_500_001])
+def test_many_tokens(ms, N, into):
+    """Around the number of tiles from which their counts are scanned, and far above."""
+    check(ms, N, 32000, 2, into)
+
+
+def test_time_grows_with_the_tokens(ms):
+    """Four times the tokens take four times as long; where every block reads the counts of all it is sixteen (7.5 with the
+    rest of the call). Least times of some runs, six times allowed."""
+    def least(N):
+        t, dout = ms.from_torch(whole(0, 32000, N, seed=1)), ms.from_torch(torch.zeros(N, 8, device="cuda", dtype=torch.bfloat16))
+        times = []
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            ms.embedding_backward(dout, t, rows=32000)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    assert least(1 << 24) < 6 * least(1 << 22)
