@@ -34,7 +34,7 @@
 //
 // Bound: forward and backward move 0.5 GB each way at most for what takes them hundreds of us; they wait on their own
 // tiles (synchronous loads, two barriers a tile, splits into pieces), at 8 warps per SM: gradients of 4 x 4096 x 16 heads of 128 bf16
-// 726 us (tensor cores 0.2 of their time), 1 x 19250 x 3 heads of 128 and 64 float, all of the backward pass, 705 us.
+// 726 us (1.3 TB/s under the profiler, tensor cores 0.25), 1 x 19250 x 3 heads of 128 and 64 float, all of the backward pass, 733 us.
 // The step is bound by memory: 64 x 16 heads of 128 x 128, 134 MB, 24.6 us (5.5 TB/s).
 #include "common.cuh"
 #include "internal.h"
@@ -723,7 +723,7 @@ __global__ void __launch_bounds__(kThreads) k_la_gradients(Gradients p) {
 // The same for bf16 heads of up to 64 NK and 64 NV channels: all of the chunk's q, k, v and do stay in shared memory,
 // copied there at once, and the two states pass through it once, a tile of 64 x 64 at a time, the next one on its way to registers
 // meanwhile. Eight warps: 16 rows and half of a tile's columns each. 4 x 4096 x 16 heads of 128: 726 us, where the kernel above, which
-// loads a tile whenever it needs one, takes 1273.
+// loads a tile whenever it needs one, takes 1313.
 constexpr int kWideThreads = 256;
 
 // A tile of 64 x 64 by asynchronous copies, zeros outside.
@@ -1040,7 +1040,7 @@ Shape make_shape(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK, int64_
   d.dkp = (d.DK + 15) / 16 * 16, d.dvp = (d.DV + 15) / 16 * 16;
   d.chunks = (int)((T + kChunk - 1) / kChunk);
   // Few heads: a row's chunks are walked in segments side by side, down to single chunks, until about four blocks wait
-  // on each SM. (3 x 777 x 6 heads of 40 float16: 43 us a call, 55 with at least four chunks in a segment.)
+  // on each of 148 SMs. (3 x 777 x 6 heads of 40 float16: 43 us a call, 55 with at least four chunks in a segment.)
   const int64_t blocks = B * H * ((d.dkp + kTile - 1) / kTile) * ((d.dvp + kTile - 1) / kTile);
   int64_t want = 4 * 148 / (blocks > 0 ? blocks : 1), most = d.chunks;
   if (want > most) want = most;
@@ -1062,10 +1062,14 @@ struct StateScratch {
 };
 constexpr size_t kStatusBytes = 32;  // the status word leads the scratch
 
-// Whether the walk of whole rows may be taken, as far as the layout does not decide.
+// Whether the walk of whole rows may be taken, as far as the layout does not decide: of every length. Calls of 1, 128 and 512
+// steps of 64 heads of 128, forward: 13, 16 and 66 us, by the kernels of chunks 25, 44 and 111; backward: 58, 67 and 185,
+// and 92, 123 and 281. It loses where few heads have the four chunks from which rows are cut: 4 heads of 128, 256 steps forward 48 us, and 36.
 bool may_walk(int dtype, int64_t DK, int64_t DV, bool aligned) { return aligned && dtype == MPB_BF16 && DK <= 128 && DV <= 128 && DV % 8 == 0; }
 
-// The walk's segments: as many as give every SM a block. They cost a walk more over k and v.
+// The walk's segments: as many as give every SM (148) a block. They cost a walk more over k and v. Rows of 8192 steps of 128
+// channels, forward, 4, 37, 74 and 75 heads: 62, 243, 425 and 451 us; in one segment 416, 432, 449 and 449; in segments for two blocks per SM, which
+// run one after the other, 92, 267, 461 and 546.
 Shape walk_shape(Shape d) {
   const int64_t heads = d.B * d.H;
   int64_t want = heads > 0 ? 148 / heads : 1, most = d.chunks / 2;

@@ -15,7 +15,7 @@
 // shared memory), one copies out, one issues the matrix instructions, one makes the decays. They meet at mbarriers; every wait gives up after two seconds, sets the status
 // word and ends the block, whose results are NaN.
 //
-// What it takes: 8 x 4096 x 16 heads of 128, 263 us (2.1 TB/s; 553 MB, 85 us at the copy rate; without this kernel 1441 us);
+// What it takes: 8 x 4096 x 16 heads of 128, 263 us (2.1 TB/s; 553 MB, 85 us at the copy rate; without this kernel 1464 us);
 // 1 x 32768 x 8 heads of 64 in 18 segments 148 us with the walk that finds their states. Without outputs, the states of all chunks
 // kept in float, 4 x 4096 x 16 heads of 128 take 100 us (2.7 TB/s; by each thread's own stores 149). The
 // tensor core has 40 instructions a chunk, each of which takes 73 cycles by itself whatever its columns up to 128 (its left operand's

@@ -93,7 +93,10 @@ def linear_attention(q, k, v, log_decay, state=None, scale=None, return_state=Fa
 
     S and every sum run in float32; where the scores meet v, and the state meets q, they keep 24 bits (float32) or 16
     (float16, bfloat16). Inputs are finite: a value that is not may reach every result of its chunk of 64 steps and the
-    later ones. A prompt may be padded behind its end with log_decay 0 and k 0, which leaves the state as it was."""
+    later ones. A prompt may be padded behind its end with log_decay 0 and k 0, which leaves the state as it was.
+
+    bfloat16 heads of up to 128 channels (DV a multiple of 8) in rows of 16-byte words need little memory beside their
+    results; others hold the state at every 64th step meanwhile, T DK DV / 16 bytes per sequence and head."""
     name = "linear_attention"
     q, k, v, gs, B, T, H, Hq, DK, DV, _ = _attention_inputs(name, q, k, v, log_decay, True)
     scale = DK ** -0.5 if scale is None else _number(name, "scale", scale)
@@ -125,7 +128,9 @@ def linear_attention_backward(do, q, k, v, log_decay, state=None, dstate=None, s
     """Gradients of :func:`linear_attention`: ``(dq, dk, dv, dlog_decay, dstate0)`` from do, the gradient of its output,
     and dstate, that of its last state (float32, None for zero); the other arguments as the forward pass got them. dq and
     dk are summed over the heads that share one, dlog_decay, float32, has log_decay's shape (summed over sequences and
-    steps where that is (H,)), dstate0 is float32."""
+    steps where that is (H,)), dstate0 is float32. Meanwhile it holds the state and its gradient at every 64th step, T DK
+    DV / 8 bytes per sequence and head (1 GB for 8 sequences of 4096 steps, 16 heads of 128), and where heads share q and k,
+    dq and dk of each in float32."""
     name = "linear_attention_backward"
     q, k, v, gs, B, T, H, Hq, DK, DV, by_head = _attention_inputs(name, q, k, v, log_decay, True)
     scale = DK ** -0.5 if scale is None else _number(name, "scale", scale)
