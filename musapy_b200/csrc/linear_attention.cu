@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kThreads) k_la_states(States p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) S[k][j] = fmaf(all, S[k][j], E[k][j]);
     }
-    since *= all;
+    since = all == 0.0f ? 0.0f : since * all;  // one that overflowed is dropped too
     __syncthreads();
   }
   if (d.segments > 1) {

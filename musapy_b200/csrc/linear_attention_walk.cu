@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_la_walk(const __grid_constant__
         if (!wait_warp(kDec0 + n % kSlots, n / kSlots)) break;
         const float all = decays[n % kSlots].all;
         if (p.since && row == 0 && col0 == 0) p.since[bh * d.chunks + c] = since;
-        since *= all;
+        since = all == 0.0f ? 0.0f : since * all;  // one that overflowed is dropped too
         if (!wait_warp(kEDone, n)) break;
         fence_after();
         if (keep && n > 0 && !wait_warp(kOEmpty, n - 1)) break;

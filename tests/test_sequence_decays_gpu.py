@@ -73,3 +73,41 @@ def test_lengths(ms, path, T):
     q, k, v, do, state, dstate = inputs(*path, T=T)
     g = -5.0 - 10 * rand(1, T, 4, seed=4).abs()
     check(ms, q, k, v, g.clamp(min=-40), state, dstate, do)
+
+
+@pytest.mark.parametrize("dtype,D,before,fore,back", [("f32", 32, 0, (1540, 1900), (1540, 1900)),
+                                                      ("bf16", 64, 0, (1600, 2000), (1000, 1400)),
+                                                      ("bf16", 64, 1, (1540, 1900), (1540, 1900))])
+def test_states_that_overflowed_are_dropped(ms, dtype, D, before, fore, back):
+    """Decays above one that carry the state past the largest float, over chunks of one segment of a row, and a decay of zero
+    behind them: what follows is as if the row began there. Backward, the same for what comes before them."""
+    B, T, H = 1, 3000, 60
+    make = lambda seed: rand(B, T, H, D + 8 * before, seed=seed, dtype=dtype)[..., before:before + D]
+    q, k, v, do = (make(s) for s in (1, 2, 3, 7))
+    state, dstate = rand(B, H, D, D, seed=5), rand(B, H, D, D, seed=6)
+    A, n = ms.from_torch, 2 * (Q.roundings(T, D, D) * Q.EPS32 + Q.SCORES[q.dtype])
+
+    def grows(lo, hi, restart):
+        g = -0.05 * torch.ones(B, T, H, device="cuda")
+        g[:, lo:hi] = 0.5
+        g[:, restart] = -math.inf
+        return g
+
+    lo, at = fore
+    g = grows(lo, at, at)
+    o, last = [x.torch() for x in ms.linear_attention(A(q), A(k), A(v), A(g), A(state), return_state=True)]
+    w, wlast = [x.torch() for x in ms.linear_attention(*(A(x[:, at:]) for x in (q, k, v, g)), return_state=True)]
+    assert not o[:, at - 1].isfinite().all()  # it did overflow
+    mag = Q.attention(*(x[:, at:].double().abs() for x in (q, k, v)), g[:, at:].double(), None, D ** -0.5)
+    P.close(o[:, at:], w.double(), n * mag[0] + P.ROUND[o.dtype][0] * w.double().abs(), "o")
+    P.close(last, wlast.double(), n * mag[1], "state")
+    cut, hi = back
+    g = grows(cut, hi, cut)
+    got = [x.torch() for x in ms.linear_attention_backward(A(do), A(q), A(k), A(v), A(g), A(state), A(dstate))]
+    want = [x.torch() for x in ms.linear_attention_backward(*(A(x[:, :cut]) for x in (do, q, k, v, g)), A(state))]
+    assert not got[2][:, cut].isfinite().all()
+    mag = Q.attention_backward(*(x[:, :cut].double().abs() for x in (do, q, k, v)), g[:, :cut].double(), state.double().abs(), None,
+                               D ** -0.5)
+    for x, y, m, what in zip(got, want, mag, ("dq", "dk", "dv", "dlog_decay", "dstate0")):
+        x = x if what == "dstate0" else x[:, :cut]
+        P.close(x, y.double(), n * m + P.ROUND[x.dtype][0] * y.double().abs(), what)
