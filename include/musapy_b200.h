@@ -297,8 +297,11 @@ int mpb_policy_loss(int64_t N, int64_t V, const void* logits, int dtype, int64_t
  * Writes o (B, T, H, DV) and, when state is not NULL, the last S (state0 when T == 0); state may
  * not overlap state0. A log-decay below -104 is a decay of zero: what came before has no part from there on.
  * Channels per head: 1 to 256. Scratch: mpb_linear_attention_scratch_bytes; it is less where `aligned` says that q, k, v and o
- * (backward: q, k, v and dout) are 16-byte aligned with strides that are positive multiples of 16 bytes, and has to be asked for so or not as the call's are. Values are finite: one that is not may reach every result of its chunk of 64 steps
- * and the later ones. */
+ * (backward: q, k, v and dout) are 16-byte aligned with strides that are positive multiples of 16 bytes, and has to be asked
+ * for so or not as the call's are. Backward it holds the state and its gradient at every 64th step, T DK DV / 8 bytes per
+ * sequence and head; forward, but for aligned MPB_BF16 heads of up to 128 channels, the state. Values are finite: one that
+ * is not may reach every result of its chunk of 64 steps and the later ones. What decays leave below 2^-102 keeps fewer
+ * bits, and below 2^-126 none. */
 size_t mpb_linear_attention_scratch_bytes(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK, int64_t DV, int dtype,
                                           int backward, int decay_by_head, int aligned);
 int mpb_linear_attention(int64_t B, int64_t T, int64_t H, int64_t Hq, int64_t DK, int64_t DV, int dtype, const void* q,

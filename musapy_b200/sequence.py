@@ -92,8 +92,8 @@ def linear_attention(q, k, v, log_decay, state=None, scale=None, return_state=Fa
     256. Returns o (B, T, H, DV) in v's dtype; with ``return_state`` also the last S in float32.
 
     S and every sum run in float32; where the scores meet v, and the state meets q, they keep 24 bits (float32) or 16
-    (float16, bfloat16). Inputs are finite: a value that is not may reach every result of its chunk of 64 steps and the
-    later ones. A prompt may be padded behind its end with log_decay 0 and k 0, which leaves the state as it was.
+    (float16, bfloat16). What decays leave below 2^-102 keeps fewer bits, and below 2^-126 none, as the least floats do.
+    Inputs are finite: a value that is not may reach every result of its chunk of 64 steps and the later ones. A prompt may be padded behind its end with log_decay 0 and k 0, which leaves the state as it was.
 
     bfloat16 heads of up to 128 channels (DV a multiple of 8) in rows of 16-byte words need little memory beside their
     results; others hold the state at every 64th step meanwhile, T DK DV / 16 bytes per sequence and head."""
